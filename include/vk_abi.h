@@ -300,6 +300,109 @@ int vk_ivf_sync(vk_ivf_t* ivf, void* stream);
 int vk_ivf_assign_device(int device, const float* d_x, int64_t n, int d, const float* d_coarse, int nlist,
                          int32_t* d_list_of, void* stream);
 
+/* Paged key/value cache (no counterpart in the reference): the step of a retrieval user after the search. The keys
+ * and values of retrieved passages and of a model's own tokens live in fixed-size pages in DEVICE memory; a page
+ * table per sequence, made e.g. from a search's ids, lists the pages it reads (several sequences may list the same
+ * page). A sequence of length n occupies slots 0 .. n-1; slot s is entry s % page_size of page table[s / page_size].
+ *   vk_kv_append   writes new tokens' keys and values behind a sequence
+ *   vk_kv_attend   attention of a sequence's new tokens (one, a few or a chunk) over its slots and, on request, the
+ *                  attention weight that every slot gathered
+ *   vk_kv_evict    copies the slots that gathered most, and the latest ones, into other pages
+ * A cache (vk_kv_t) refers to the caller's pages and owns a small workspace that serves one call at a time: calls on
+ * different streams must be ordered by the caller, and the workspace grows on the first call that needs more (a
+ * warm-up call per shape before capturing a CUDA graph). All calls are asynchronous on `stream` (cudaStream_t as
+ * void*; NULL = the default stream). A page number outside [0, pages) or a length or offset outside its table is
+ * never followed: the affected slots read as absent and writes to them are skipped; vk_kv_sync waits and then reports
+ * it as VK_ERR_INVALID. */
+enum {
+    VK_KV_F16 = 0,
+    VK_KV_BF16 = 1
+};
+
+typedef struct {
+    int device;
+    int dtype;      /* VK_KV_F16 or VK_KV_BF16 */
+    int page_size;  /* slots per page: a power of two in [8, 1024] */
+    int kv_heads;
+    int head_dim;   /* a multiple of 8 in [8, 128] */
+    int64_t pages;
+    /* Element (page, slot, head, i) of the keys is k[page * k_stride[0] + slot * k_stride[1] + head * k_stride[2] + i],
+     * strides in elements: multiples of 8, base addresses 16-byte aligned. Values likewise. */
+    void* k;
+    int64_t k_stride[3];
+    void* v;
+    int64_t v_stride[3];
+} vk_kv_desc_t;
+
+/* The sequences of a call, in DEVICE memory: new tokens of sequence b are rows offsets[b] .. offsets[b + 1] - 1 of
+ * the call's tokens (offsets ascending, `tokens` rows in all), lens[b] its slots with the new tokens included, and
+ * table[b * table_stride + i] its i-th page, i < table_width. */
+typedef struct {
+    int batch;
+    int table_width;
+    int64_t table_stride;
+    int64_t tokens;
+    const int32_t* offsets; /* batch + 1; not read by vk_kv_evict */
+    const int32_t* table;
+    const int32_t* lens;
+} vk_kv_batch_t;
+
+typedef struct vk_kv vk_kv_t;
+int vk_kv_create(const vk_kv_desc_t* desc, vk_kv_t** out);
+int vk_kv_destroy(vk_kv_t* kv);
+/* Waits for the cache's work on `stream` and reports any kernel-side error (and clears it). */
+int vk_kv_sync(vk_kv_t* kv, void* stream);
+
+/* New token t of sequence b, of T, goes to slot lens[b] - T + t. Element (token, head, i) of the new keys is
+ * k[token * k_stride[0] + head * k_stride[1] + i] (strides in elements, multiples of 8; bases 16-byte aligned). */
+int vk_kv_append(vk_kv_t* kv, const vk_kv_batch_t* batch, const void* k, const int64_t* k_stride, const void* v,
+                 const int64_t* v_stride, void* stream);
+
+/* For token t (of T) and query head h of a sequence of n slots, with s_j = scale * q . k_j over the slots j < n, with
+ * `causal` only j <= n - T + t, of kv head h / (heads / kv_heads):
+ *   lse = log(sum_j exp(s_j)),  out = sum_j exp(s_j - lse) v_j;  no slot: out = 0, lse = -inf
+ *   scores[b][kv head][j] += sum over the sequence's tokens and the kv head's query heads of exp(s_j - lse)
+ * Products of 16-bit values are summed in 32 bits, softmax statistics and scores are 32-bit; weights are rounded to
+ * the cache's type before they meet the values. Slots j >= n hold anything (NaN too); the slots j < n have to be
+ * finite, those that the causal mask hides from some rows as well. Sums run in a fixed order that depends on the
+ * shapes alone: equal calls give equal bits. */
+typedef struct {
+    const void* q; /* [tokens][heads][head_dim], the cache's type */
+    int64_t q_stride[2];
+    void* out; /* the same shape and type */
+    int64_t out_stride[2];
+    float* lse;    /* [tokens][heads], contiguous; may be NULL */
+    float* scores; /* element (b, kv head, slot) at scores[b * scores_stride[0] + head * scores_stride[1] + slot],
+                      slots < scores_width; NULL: not gathered */
+    int64_t scores_stride[2];
+    int64_t scores_width;
+    int heads; /* a multiple of kv_heads, at most 128 times it */
+    int max_q; /* at least the largest number of new tokens of a sequence; 0 = unknown (`tokens` is assumed) */
+    int causal;
+    float scale;
+} vk_kv_attend_t;
+int vk_kv_attend(vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_attend_t* args, void* stream);
+
+/* For every sequence of n slots and every kv head: k = min(n, keep) slots are kept, the last r = min(recent, k) and, of
+ * the others, the k - r with the largest scores (ties to the lower slot; NaN counts as the lowest), in slot order.
+ * Their keys and values are copied to slots 0 .. k-1 of the sequence's pages in new_table, which no table of the call
+ * may read; kept[b][head][i] is the old slot of new slot i (-1 for i >= k), new_scores its score (0 for i >= k, up to
+ * scores_width) and new_lens[b] = k. Only slots < scores_width have a score; the others count as 0. */
+typedef struct {
+    const int32_t* new_table;
+    int64_t new_table_stride;
+    int new_table_width;
+    int keep;
+    int recent;
+    const float* scores; /* as in vk_kv_attend_t */
+    int64_t scores_stride[2];
+    int64_t scores_width;
+    float* new_scores; /* contiguous [batch][kv_heads][scores_width] */
+    int32_t* kept;     /* contiguous [batch][kv_heads][keep] */
+    int32_t* new_lens; /* [batch] */
+} vk_kv_evict_t;
+int vk_kv_evict(vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_evict_t* args, void* stream);
+
 /* No counterpart in the reference. A device-resident search that allocates nothing, for callers that must not
  * call cudaMalloc or cudaFree: code running where an allocation would synchronise the device and stall other
  * streams (latency-bound serving threads), or under an allocator the process has handed all memory to.

@@ -4,6 +4,7 @@ selection) on NVIDIA B200 (sm_100a), bit-identical to the reference CPU path of 
 The product is the native library veckern_b200/_native/libveckern_b200.so (C ABI: include/vk_abi.h; C++ API:
 include/veckern/gpu.hpp). This package is the Python host side over that ABI; it has no compute of its own.
 """
+from .kvcache import PagedCache  # noqa
 from .searcher import (NEIGHBOR_DTYPE, CoopSearch, DeviceInfo, IVFSearcher, LaunchShape, MultiPQSearcher,  # noqa
                        PQSearcher, ScanVariant, assign_lists,
                        Timings, Tuning,

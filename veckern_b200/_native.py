@@ -52,6 +52,35 @@ class LaunchShape(C.Structure):
                 ("vectors_per_step", C.c_int), ("blocks_per_sm", C.c_int), ("waves", C.c_double)]
 
 
+VK_KV_F16 = 0
+VK_KV_BF16 = 1
+
+
+class KvDesc(C.Structure):
+    _fields_ = [("device", C.c_int), ("dtype", C.c_int), ("page_size", C.c_int), ("kv_heads", C.c_int),
+                ("head_dim", C.c_int), ("pages", C.c_int64), ("k", C.c_void_p), ("k_stride", C.c_int64 * 3),
+                ("v", C.c_void_p), ("v_stride", C.c_int64 * 3)]
+
+
+class KvBatch(C.Structure):
+    _fields_ = [("batch", C.c_int), ("table_width", C.c_int), ("table_stride", C.c_int64), ("tokens", C.c_int64),
+                ("offsets", C.c_void_p), ("table", C.c_void_p), ("lens", C.c_void_p)]
+
+
+class KvAttend(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("q_stride", C.c_int64 * 2), ("out", C.c_void_p), ("out_stride", C.c_int64 * 2),
+                ("lse", C.c_void_p), ("scores", C.c_void_p), ("scores_stride", C.c_int64 * 2),
+                ("scores_width", C.c_int64), ("heads", C.c_int), ("max_q", C.c_int), ("causal", C.c_int),
+                ("scale", C.c_float)]
+
+
+class KvEvict(C.Structure):
+    _fields_ = [("new_table", C.c_void_p), ("new_table_stride", C.c_int64), ("new_table_width", C.c_int),
+                ("keep", C.c_int), ("recent", C.c_int), ("scores", C.c_void_p), ("scores_stride", C.c_int64 * 2),
+                ("scores_width", C.c_int64), ("new_scores", C.c_void_p), ("kept", C.c_void_p),
+                ("new_lens", C.c_void_p)]
+
+
 # (dist, id) pairs: the reference's Neighbor layout
 NEIGHBOR_DTYPE = np.dtype([("dist", "<f4"), ("id", "<i4")])
 
@@ -101,6 +130,12 @@ ABI = {
     "vk_coop_attach": (C.c_int, [_vp, C.c_int, _vp]),
     "vk_coop_destroy": (C.c_int, [_vp]),
     "vk_search_device_coop": (C.c_int, [_vp, _vp, C.c_uint32, _vp, _i64, C.c_int, C.POINTER(Tuning), _vp, _vp]),
+    "vk_kv_create": (C.c_int, [C.POINTER(KvDesc), C.POINTER(_vp)]),
+    "vk_kv_destroy": (C.c_int, [_vp]),
+    "vk_kv_sync": (C.c_int, [_vp, _vp]),
+    "vk_kv_append": (C.c_int, [_vp, _vp, _vp, C.POINTER(_i64), _vp, C.POINTER(_i64), _vp]),
+    "vk_kv_attend": (C.c_int, [_vp, _vp, _vp, _vp]),
+    "vk_kv_evict": (C.c_int, [_vp, _vp, _vp, _vp]),
     "vk_ivf_create": (C.c_int, [C.c_int, _vp, C.c_int, C.c_int, _vp, _i64, _vp, C.c_int, _vp, C.POINTER(_vp)]),
     "vk_ivf_destroy": (C.c_int, [_vp]),
     "vk_ivf_info": (C.c_int, [_vp, C.POINTER(_i64), C.POINTER(C.c_int), C.POINTER(_i64)]),

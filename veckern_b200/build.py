@@ -62,14 +62,15 @@ def build(verbose: bool = False, jobs: int | None = None) -> None:
     NATIVE.mkdir(exist_ok=True)
     gxx = _tool("g++")
     nvcc = _nvcc()
-    headers = _headers()
-    cu_srcs = [CSRC / "vk_abi.cu"] + sorted(CSRC.glob("scan_*.cu"))
+    all_headers = _headers()
+    headers = [h for h in all_headers if not h.name.startswith("kv_")]  # kv_*.cuh: only the kv_*.cu include them
+    cu_srcs = [CSRC / "vk_abi.cu"] + sorted(CSRC.glob("scan_*.cu")) + sorted(CSRC.glob("kv_*.cu"))
     jobs_list = []
     objs = []
     for src in cu_srcs:
         obj = OBJ / (src.stem + ".o")
         objs.append(obj)
-        if _stale(obj, [src] + headers):
+        if _stale(obj, [src] + (all_headers if src.name.startswith("kv_") else headers)):
             jobs_list.append([nvcc, *ARCH, "-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC",
                               "-ccbin", gxx, f"-I{INCLUDE}", f"-I{CSRC}", "-c", str(src), "-o", str(obj)])
     searcher = CSRC / "host" / "searcher.cpp"

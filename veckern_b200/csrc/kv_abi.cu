@@ -1,0 +1,248 @@
+// C ABI of the paged key/value cache (vk_kv_*): checks of arguments, the cache's handle, and the launches.
+#include <new>
+#include <type_traits>
+
+#include "kv_attend.cuh"
+#include "kv_move.cuh"
+#include "status.h"
+
+struct vk_kv {
+    vk_kv_desc_t desc{};
+    int page_shift = 0;
+    int sm_count = 0;
+    int* status = nullptr;
+    DevBuf<float> lse;
+    ~vk_kv() {
+        if (status) cudaFree(status);
+    }
+};
+
+namespace {
+
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+vk::KvPages pages_of(const vk_kv* kv) {
+    vk::KvPages c{};
+    c.k = static_cast<uint16_t*>(kv->desc.k);
+    c.v = static_cast<uint16_t*>(kv->desc.v);
+    for (int i = 0; i < 3; ++i) {
+        c.ks[i] = kv->desc.k_stride[i];
+        c.vs[i] = kv->desc.v_stride[i];
+    }
+    c.pages = kv->desc.pages;
+    c.page_shift = kv->page_shift;
+    c.heads = kv->desc.kv_heads;
+    c.dim = kv->desc.head_dim;
+    c.status = kv->status;
+    return c;
+}
+
+// Checks a call's handle and sequences; *out is the kernels' view of them.
+int check_batch(const vk_kv* kv, const vk_kv_batch_t* bt, bool offsets, vk::KvBatch* out) {
+    if (!kv) return fail(VK_ERR_INVALID, "cache must not be NULL");
+    if (!bt) return fail(VK_ERR_INVALID, "batch must not be NULL");
+    if (bt->batch < 0 || bt->batch > 65535) return fail(VK_ERR_INVALID, "batch must be in [0, 65535]");
+    if (bt->tokens < 0 || bt->tokens > INT32_MAX) return fail(VK_ERR_INVALID, "tokens must be in [0, 2^31)");
+    if (bt->table_width < 0 || bt->table_stride < 0 ||
+        ((int64_t)bt->table_width << kv->page_shift) > INT32_MAX - 1024)
+        return fail(VK_ERR_INVALID, "table_width must be >= 0 and cover less than 2^31 slots");
+    if (bt->batch > 0 && ((offsets && !bt->offsets) || !bt->lens || (bt->table_width > 0 && !bt->table)))
+        return fail(VK_ERR_INVALID, "offsets, lens and table must not be NULL");
+    out->offsets = bt->offsets;
+    out->table = bt->table;
+    out->lens = bt->lens;
+    out->table_stride = bt->table_stride;
+    out->tokens = bt->tokens;
+    out->batch = bt->batch;
+    out->width = bt->table_width;
+    return VK_OK;
+}
+
+int check_rows(const char* what, const void* p, const int64_t* stride) {
+    if (!p) return fail(VK_ERR_INVALID, "%s must not be NULL", what);
+    if (!aligned16(p)) return fail(VK_ERR_INVALID, "%s must be 16-byte aligned", what);
+    if (!stride || stride[0] < 0 || stride[1] < 0 || stride[0] % 8 || stride[1] % 8)
+        return fail(VK_ERR_INVALID, "%s: strides must be multiples of 8 elements", what);
+    return VK_OK;
+}
+
+template <typename T>
+int launch_attend(const vk::KvPages& c, const vk::KvBatch& bt, const vk::KvAttend& a, cudaStream_t st) {
+    vk::kv_attend_kernel<T><<<dim3((unsigned)bt.tokens, a.heads), 32 * vk::ROW_WARPS, 0, st>>>(c, bt, a);
+    VK_TRY_CUDA(cudaGetLastError());
+    const int64_t slots = (int64_t)bt.width << c.page_shift;
+    if (a.scores && slots > 0) {
+        vk::kv_weights_kernel<T><<<dim3((unsigned)ceil_div(slots, 8), c.heads, bt.batch), 256, 0, st>>>(c, bt, a);
+        VK_TRY_CUDA(cudaGetLastError());
+    }
+    return VK_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int vk_kv_create(const vk_kv_desc_t* d, vk_kv_t** out) {
+    if (!d || !out) return fail(VK_ERR_INVALID, "desc and out must not be NULL");
+    *out = nullptr;
+    if (d->dtype != VK_KV_F16 && d->dtype != VK_KV_BF16)
+        return fail(VK_ERR_INVALID, "dtype must be VK_KV_F16 or VK_KV_BF16");
+    if (d->page_size < 8 || d->page_size > 1024 || (d->page_size & (d->page_size - 1)))
+        return fail(VK_ERR_INVALID, "page_size must be a power of two in [8, 1024]");
+    if (d->head_dim < 8 || d->head_dim > 128 || d->head_dim % 8)
+        return fail(VK_ERR_INVALID, "head_dim must be a multiple of 8 in [8, 128]");
+    if (d->kv_heads < 1 || d->kv_heads > 65535) return fail(VK_ERR_INVALID, "kv_heads must be in [1, 65535]");
+    if (d->pages < 1 || d->pages > INT32_MAX) return fail(VK_ERR_INVALID, "pages must be in [1, 2^31)");
+    for (int side = 0; side < 2; ++side) {
+        const void* p = side ? d->v : d->k;
+        const int64_t* s = side ? d->v_stride : d->k_stride;
+        const char* what = side ? "v" : "k";
+        if (!p || !aligned16(p)) return fail(VK_ERR_INVALID, "%s must be a 16-byte aligned device address", what);
+        for (int i = 0; i < 3; ++i)
+            if (s[i] < 0 || s[i] % 8 || s[i] >= (int64_t(1) << 38))
+                return fail(VK_ERR_INVALID, "%s: strides must be multiples of 8 elements below 2^38", what);
+    }
+    DeviceGuard guard(d->device);
+    if (guard.err != cudaSuccess) return fail(VK_ERR_CUDA, "cudaSetDevice: %s", cudaGetErrorString(guard.err));
+    vk_kv* kv = new (std::nothrow) vk_kv;
+    if (!kv) return fail(VK_ERR_NOMEM, "out of host memory");
+    kv->desc = *d;
+    while ((1 << kv->page_shift) < d->page_size) ++kv->page_shift;
+    cudaError_t e = cudaDeviceGetAttribute(&kv->sm_count, cudaDevAttrMultiProcessorCount, d->device);
+    if (e == cudaSuccess) e = cudaMalloc(&kv->status, sizeof(int));
+    if (e == cudaSuccess) e = cudaMemset(kv->status, 0, sizeof(int));
+    if (e != cudaSuccess) {
+        delete kv;
+        return fail(e == cudaErrorMemoryAllocation ? VK_ERR_NOMEM : VK_ERR_CUDA, "vk_kv_create: %s",
+                    cudaGetErrorString(e));
+    }
+    *out = kv;
+    return VK_OK;
+}
+
+int vk_kv_destroy(vk_kv_t* kv) {
+    if (!kv) return VK_OK;
+    DeviceGuard guard(kv->desc.device);
+    delete kv;
+    return VK_OK;
+}
+
+int vk_kv_sync(vk_kv_t* kv, void* stream) {
+    if (!kv) return fail(VK_ERR_INVALID, "cache must not be NULL");
+    DeviceGuard guard(kv->desc.device);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    int status = 0;
+    VK_TRY_CUDA(cudaMemcpyAsync(&status, kv->status, sizeof(int), cudaMemcpyDeviceToHost, st));
+    VK_TRY_CUDA(cudaStreamSynchronize(st));
+    if (!status) return VK_OK;
+    VK_TRY_CUDA(cudaMemsetAsync(kv->status, 0, sizeof(int), st));
+    VK_TRY_CUDA(cudaStreamSynchronize(st));
+    if (status & (vk::ERR_WAIT_TIMEOUT | vk::ERR_DRAIN_TIMEOUT))
+        return fail(VK_ERR_DEVICE, "a bounded wait ran out in a cache kernel (status %d)", status);
+    return fail(VK_ERR_INVALID, "a page number, length or offset was out of range; the slots it names were left out");
+}
+
+int vk_kv_append(vk_kv_t* kv, const vk_kv_batch_t* batch, const void* k, const int64_t* k_stride, const void* v,
+                 const int64_t* v_stride, void* stream) {
+    vk::KvBatch bt{};
+    VK_TRY(check_batch(kv, batch, true, &bt));
+    if (bt.tokens == 0 || bt.batch == 0) return VK_OK;
+    VK_TRY(check_rows("k", k, k_stride));
+    VK_TRY(check_rows("v", v, v_stride));
+    DeviceGuard guard(kv->desc.device);
+    if (guard.err != cudaSuccess) return fail(VK_ERR_CUDA, "cudaSetDevice: %s", cudaGetErrorString(guard.err));
+    const int64_t threads = bt.tokens * kv->desc.kv_heads * (kv->desc.head_dim / 8);
+    const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(threads, 256), (int64_t)kv->sm_count * 32);
+    vk::kv_append_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(
+        pages_of(kv), bt, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), k_stride[0], k_stride[1],
+        v_stride[0], v_stride[1]);
+    VK_TRY_CUDA(cudaGetLastError());
+    return VK_OK;
+}
+
+int vk_kv_attend(vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_attend_t* args, void* stream) {
+    vk::KvBatch bt{};
+    VK_TRY(check_batch(kv, batch, true, &bt));
+    if (!args) return fail(VK_ERR_INVALID, "args must not be NULL");
+    const int g = kv->desc.kv_heads;
+    if (args->heads < g || args->heads % g || args->heads / g > 128)
+        return fail(VK_ERR_INVALID, "heads must be a multiple of kv_heads (%d), at most 128 times it", g);
+    if (args->max_q < 0) return fail(VK_ERR_INVALID, "max_q must be >= 0");
+    if (!(args->scale == args->scale) || args->scale - args->scale != 0.0f)
+        return fail(VK_ERR_INVALID, "scale must be finite");
+    if (args->scores && (args->scores_width < 0 || args->scores_stride[0] < 0 || args->scores_stride[1] < 0))
+        return fail(VK_ERR_INVALID, "scores: width and strides must be >= 0");
+    if (bt.tokens == 0 || bt.batch == 0) return VK_OK;
+    VK_TRY(check_rows("q", args->q, args->q_stride));
+    VK_TRY(check_rows("out", args->out, args->out_stride));
+    DeviceGuard guard(kv->desc.device);
+    if (guard.err != cudaSuccess) return fail(VK_ERR_CUDA, "cudaSetDevice: %s", cudaGetErrorString(guard.err));
+    vk::KvAttend a{};
+    a.q = static_cast<const uint16_t*>(args->q);
+    a.out = static_cast<uint16_t*>(args->out);
+    a.lse = args->lse;
+    a.scores = args->scores;
+    for (int i = 0; i < 2; ++i) {
+        a.qs[i] = args->q_stride[i];
+        a.os[i] = args->out_stride[i];
+        a.ss[i] = args->scores_stride[i];
+    }
+    a.scores_width = args->scores_width;
+    a.heads = args->heads;
+    a.group = args->heads / g;
+    a.max_q = args->max_q > 0 ? (int)std::min<int64_t>(args->max_q, bt.tokens) : (int)bt.tokens;
+    a.causal = args->causal != 0;
+    a.scale = args->scale;
+    if (!a.lse) {
+        VK_TRY(kv->lse.ensure((size_t)bt.tokens * a.heads));
+        a.lse = kv->lse.ptr;
+    }
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return kv->desc.dtype == VK_KV_F16 ? launch_attend<__half>(pages_of(kv), bt, a, st)
+                                       : launch_attend<__nv_bfloat16>(pages_of(kv), bt, a, st);
+}
+
+int vk_kv_evict(vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_evict_t* args, void* stream) {
+    vk::KvBatch bt{};
+    VK_TRY(check_batch(kv, batch, false, &bt));
+    if (!args) return fail(VK_ERR_INVALID, "args must not be NULL");
+    if (args->keep < 0 || args->recent < 0 || args->recent > args->keep)
+        return fail(VK_ERR_INVALID, "keep and recent must satisfy 0 <= recent <= keep");
+    if (args->new_table_width < 0 || args->new_table_stride < 0 ||
+        ((int64_t)args->new_table_width << kv->page_shift) > INT32_MAX - 1024)
+        return fail(VK_ERR_INVALID, "new_table_width must be >= 0 and cover less than 2^31 slots");
+    if (args->scores_width < 0 || args->scores_stride[0] < 0 || args->scores_stride[1] < 0)
+        return fail(VK_ERR_INVALID, "scores: width and strides must be >= 0");
+    if (bt.batch == 0) return VK_OK;
+    if ((args->scores_width > 0 && (!args->scores || !args->new_scores)) || !args->new_lens ||
+        (args->keep > 0 && (!args->kept || (args->new_table_width > 0 && !args->new_table))))
+        return fail(VK_ERR_INVALID, "scores, new_scores, kept, new_lens and new_table must not be NULL");
+    DeviceGuard guard(kv->desc.device);
+    if (guard.err != cudaSuccess) return fail(VK_ERR_CUDA, "cudaSetDevice: %s", cudaGetErrorString(guard.err));
+    vk::KvEvict e{};
+    e.new_table = args->new_table;
+    e.new_stride = args->new_table_stride;
+    e.new_width = args->new_table_width;
+    e.keep = args->keep;
+    e.recent = args->recent;
+    e.scores = args->scores;
+    e.ss[0] = args->scores_stride[0];
+    e.ss[1] = args->scores_stride[1];
+    e.width = args->scores_width;
+    e.new_scores = args->new_scores;
+    e.kept = args->kept;
+    e.new_lens = args->new_lens;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const vk::KvPages c = pages_of(kv);
+    vk::kv_select_kernel<<<dim3(c.heads, bt.batch), vk::SELECT_THREADS, 0, st>>>(c, bt, e);
+    VK_TRY_CUDA(cudaGetLastError());
+    if (e.keep > 0) {
+        const unsigned tiles = (unsigned)std::min<int64_t>(ceil_div((int64_t)e.keep * (c.dim / 8), 256), 4096);
+        vk::kv_compact_kernel<<<dim3(tiles, c.heads, bt.batch), 256, 0, st>>>(c, bt, e);
+        VK_TRY_CUDA(cudaGetLastError());
+    }
+    return VK_OK;
+}
+
+}  // extern "C"

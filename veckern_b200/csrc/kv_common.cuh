@@ -1,0 +1,105 @@
+// Shared by the kernels of the paged key/value cache: the views that they get by value, the sequences' bounds, and the
+// 16-bit types' conversions.
+//
+// What a call reads from device memory (offsets, lengths, page numbers) is never trusted: a sequence's bounds are
+// clamped to the call's sizes and a page number outside the cache is not followed. Both set ERR_LAYOUT.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "vk_device.cuh"
+
+namespace vk {
+
+struct KvPages {
+    uint16_t* k;  // elements of the cache's 16-bit type
+    uint16_t* v;
+    int64_t ks[3], vs[3];  // strides in elements: page, slot, head
+    int64_t pages;
+    int page_shift;  // page size = 1 << page_shift
+    int heads, dim;
+    int* status;
+};
+
+struct KvBatch {
+    const int32_t* offsets;
+    const int32_t* table;
+    const int32_t* lens;
+    int64_t table_stride;
+    int64_t tokens;
+    int batch;
+    int width;
+};
+
+struct KvSeq {
+    int64_t first;  // row of its first new token
+    int count;      // new tokens
+    int len;        // slots, new tokens included
+};
+
+__device__ __forceinline__ int kv_len(const KvPages& c, const KvBatch& bt, int b) {
+    const int64_t most = (int64_t)bt.width << c.page_shift;
+    int len = __ldg(bt.lens + b);
+    if (len < 0 || len > most) {
+        atomicOr(c.status, ERR_LAYOUT);
+        len = len < 0 ? 0 : (int)most;
+    }
+    return len;
+}
+
+__device__ __forceinline__ KvSeq kv_seq(const KvPages& c, const KvBatch& bt, int b) {
+    int64_t lo = __ldg(bt.offsets + b), hi = __ldg(bt.offsets + b + 1);
+    if (lo < 0 || hi < lo || hi > bt.tokens) {
+        atomicOr(c.status, ERR_LAYOUT);
+        lo = min(max(lo, int64_t(0)), bt.tokens);
+        hi = min(max(hi, lo), bt.tokens);
+    }
+    return {lo, (int)(hi - lo), kv_len(c, bt, b)};
+}
+
+// The page of a slot of sequence b (slot < its length), or -1.
+__device__ __forceinline__ int64_t kv_page(const KvPages& c, const int32_t* table, int slot) {
+    const int page = __ldg(table + (slot >> c.page_shift));
+    if ((uint64_t)(int64_t)page >= (uint64_t)c.pages) {
+        atomicOr(c.status, ERR_LAYOUT);
+        return -1;
+    }
+    return page;
+}
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T x) {
+    if constexpr (std::is_same_v<T, __half>) return __half2float(x);
+    else return __bfloat162float(x);
+}
+template <typename T>
+__device__ __forceinline__ T from_f32(float x) {
+    if constexpr (std::is_same_v<T, __half>) return __float2half_rn(x);
+    else return __float2bfloat16_rn(x);
+}
+
+// Sequence of a token row: the last b whose offset is at most it (offsets ascend; empty sequences share one).
+__device__ __forceinline__ int kv_find(const KvBatch& bt, int64_t row) {
+    int lo = 0, hi = bt.batch - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (__ldg(bt.offsets + mid) <= row) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+struct KvAttend {
+    const uint16_t* q;
+    uint16_t* out;
+    float* lse;     // [tokens][heads]
+    float* scores;  // may be null
+    int64_t qs[2], os[2], ss[2];
+    int64_t scores_width;
+    int heads, group;  // query heads; query heads per kv head
+    int max_q;
+    int causal;
+    float scale;
+};
+
+}  // namespace vk

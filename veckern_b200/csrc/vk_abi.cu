@@ -10,7 +10,6 @@
 #include <algorithm>
 #include <cstdlib>
 #include <cmath>
-#include <cstdarg>
 #include <cstdio>
 #include <cstring>
 #include <limits>
@@ -27,72 +26,9 @@
 #include "host/index_file.h"
 #include "kernels.cuh"
 #include "scan_dispatch.cuh"
+#include "status.h"
 
 namespace {
-
-thread_local std::string g_error;
-
-int fail(int code, const char* fmt, ...) {
-    char buf[1024];
-    va_list ap;
-    va_start(ap, fmt);
-    std::vsnprintf(buf, sizeof(buf), fmt, ap);
-    va_end(ap);
-    g_error = buf;
-    return code;
-}
-
-#define VK_TRY_CUDA(call)                                                                                  \
-    do {                                                                                                   \
-        const cudaError_t e_ = (call);                                                                     \
-        if (e_ != cudaSuccess) return fail(e_ == cudaErrorMemoryAllocation ? VK_ERR_NOMEM : VK_ERR_CUDA, \
-                                           "%s failed: %s", #call, cudaGetErrorString(e_));                \
-    } while (0)
-
-#define VK_TRY(call)                    \
-    do {                                \
-        const int r_ = (call);          \
-        if (r_ != VK_OK) return r_;     \
-    } while (0)
-
-// Restores the caller's current device on scope exit.
-struct DeviceGuard {
-    int prev = -1;
-    cudaError_t err = cudaSuccess;
-    explicit DeviceGuard(int dev) {
-        cudaGetDevice(&prev);
-        if (prev != dev) err = cudaSetDevice(dev);
-    }
-    ~DeviceGuard() {
-        int cur = -1;
-        cudaGetDevice(&cur);
-        if (prev >= 0 && cur != prev) cudaSetDevice(prev);
-    }
-};
-
-template <typename T>
-struct DevBuf {
-    T* ptr = nullptr;
-    size_t cap = 0;  // elements
-    ~DevBuf() { release(); }
-    void release() {
-        if (ptr) cudaFree(ptr);
-        ptr = nullptr;
-        cap = 0;
-    }
-    // Grows (never shrinks), like the reference's DeviceBuffer::ensure (src/cuda/searcher.cu:31-37).
-    int ensure(size_t count) {
-        if (count <= cap) return VK_OK;
-        release();
-        const cudaError_t e = cudaMalloc(&ptr, std::max<size_t>(count, 1) * sizeof(T));
-        if (e != cudaSuccess) {
-            ptr = nullptr;
-            return fail(VK_ERR_NOMEM, "cudaMalloc of %zu bytes failed: %s", count * sizeof(T), cudaGetErrorString(e));
-        }
-        cap = count;
-        return VK_OK;
-    }
-};
 
 constexpr size_t kL2WindowBytes = size_t(80) << 20;  // L2 share for one window's LUTs plus two chunks' codes
 constexpr int64_t kMaxRowsPerChunk = 1 << 20;       // L2 locality: a chunk's codes stay well inside the 126 MB L2
@@ -708,11 +644,11 @@ extern "C" {
 
 size_t vk_last_error(char* buf, size_t len) {
     if (buf && len > 0) {
-        const size_t n = std::min(len - 1, g_error.size());
-        std::memcpy(buf, g_error.data(), n);
+        const size_t n = std::min(len - 1, vk_status::g_error.size());
+        std::memcpy(buf, vk_status::g_error.data(), n);
         buf[n] = '\0';
     }
-    return g_error.size();
+    return vk_status::g_error.size();
 }
 
 void vk_tuning_default(vk_tuning_t* t) {

@@ -1,0 +1,195 @@
+"""Paged key/value cache over the C ABI (vk_kv_*, include/vk_abi.h): what a retrieval user's model does after the search.
+The keys and values of retrieved passages and of the model's own tokens live in fixed-size pages; a page table per
+sequence, made e.g. from a search's ids, says which pages it reads.
+
+    cache = PagedCache(k_pages, v_pages)                          # [pages, page_size, kv_heads, head_dim], f16 or bf16
+    cache.append(k, v, offsets, table, lens)                      # new tokens behind their sequences
+    out, lse = cache.attend(q, offsets, table, lens, scores=s)    # their attention over all slots
+    kept, lens, s = cache.evict(table, lens, new_table, keep, recent, s)
+
+All tensors are torch tensors on the cache's device. Sequence b of a call has the new tokens offsets[b]:offsets[b + 1]
+(int32, [batch + 1]), lens[b] slots with the new tokens included (int32, [batch]) and the pages table[b] (int32,
+[batch, width]; entries past its last slot are not read). Calls are asynchronous on `stream` (a torch.cuda.Stream or raw
+handle; default: the current stream); sync() waits and raises what the kernels found wrong. One cache serves one call at
+a time. No derivatives: a cache is for inference.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+from . import _native as N
+from ._native import check, lib
+
+_DTYPES = {"torch.float16": N.VK_KV_F16, "torch.bfloat16": N.VK_KV_BF16}
+
+
+def _want(t, name: str, dtype, ndim: int, device) -> None:
+    if t.dtype != dtype or t.dim() != ndim or t.device != device:
+        raise ValueError(f"{name} must be a {ndim}-dimensional {dtype} tensor on {device}, got {t.dim()}-dimensional "
+                         f"{t.dtype} on {t.device}")
+
+
+class PagedCache:
+    """k_pages and v_pages: [pages, page_size, kv_heads, head_dim], any strides that are multiples of 8 elements with
+    the last dimension contiguous (a [pages, kv_heads, page_size, head_dim] tensor is passed transposed). The cache
+    refers to the tensors, it does not copy them. page_size: a power of two in [8, 1024]; head_dim: a multiple of 8 up
+    to 128."""
+
+    def __init__(self, k_pages, v_pages):
+        import torch
+
+        self._torch = torch
+        self._h = C.c_void_p()
+        for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
+            if t.dim() != 4 or t.shape != k_pages.shape or t.dtype != k_pages.dtype or t.device != k_pages.device:
+                raise ValueError(f"{name} must be [pages, page_size, kv_heads, head_dim], k_pages and v_pages alike")
+            if not t.is_cuda:
+                raise ValueError(f"{name} must be on a GPU")
+            if t.stride(3) != 1:
+                raise ValueError(f"{name}: the last dimension must be contiguous")
+        if str(k_pages.dtype) not in _DTYPES:
+            raise ValueError("pages must be float16 or bfloat16")
+        self.k_pages, self.v_pages = k_pages, v_pages
+        self.pages, self.page_size, self.kv_heads, self.head_dim = k_pages.shape
+        self.dtype, self.device = k_pages.dtype, k_pages.device
+        d = N.KvDesc(device=self.device.index, dtype=_DTYPES[str(self.dtype)], page_size=self.page_size,
+                     kv_heads=self.kv_heads, head_dim=self.head_dim, pages=self.pages, k=k_pages.data_ptr(),
+                     k_stride=(C.c_int64 * 3)(*k_pages.stride()[:3]), v=v_pages.data_ptr(),
+                     v_stride=(C.c_int64 * 3)(*v_pages.stride()[:3]))
+        check(lib().vk_kv_create(C.byref(d), C.byref(self._h)), "vk_kv_create")
+        # argument structs, filled anew by every call
+        self._batch, self._attend, self._evict = N.KvBatch(), N.KvAttend(), N.KvEvict()
+        self._batch_ref, self._attend_ref, self._evict_ref = (C.byref(x) for x in
+                                                              (self._batch, self._attend, self._evict))
+
+    def _sequences(self, table, lens, offsets=None, tokens: int = 0) -> int:
+        i32, dev = self._torch.int32, self.device
+        _want(table, "table", i32, 2, dev)
+        _want(lens, "lens", i32, 1, dev)
+        n, width = table.shape
+        if lens.shape[0] != n or not lens.is_contiguous() or (width > 1 and table.stride(1) != 1):
+            raise ValueError("lens must be contiguous, one per row of table, and table's rows contiguous")
+        b = self._batch
+        if offsets is not None:
+            _want(offsets, "offsets", i32, 1, dev)
+            if offsets.shape[0] != n + 1 or not offsets.is_contiguous():
+                raise ValueError("offsets must be contiguous [batch + 1]")
+            b.offsets = offsets.data_ptr()
+        else:
+            b.offsets = None
+        b.batch, b.table_width, b.table_stride, b.tokens = n, width, table.stride(0), tokens
+        b.table, b.lens = table.data_ptr(), lens.data_ptr()
+        return n
+
+    def _rows(self, t, name: str, heads: int) -> None:
+        _want(t, name, self.dtype, 3, self.device)
+        if t.shape[1] != heads or t.shape[2] != self.head_dim or t.stride(2) != 1:
+            raise ValueError(f"{name} must be [tokens, {heads}, {self.head_dim}] with the last dimension contiguous")
+
+    def _stream(self, stream):
+        if stream is None:
+            return self._torch.cuda.current_stream(self.device).cuda_stream
+        return getattr(stream, "cuda_stream", stream)
+
+    def append(self, k, v, offsets, table, lens, *, stream=None) -> None:
+        """New token t of sequence b (of T) is written to slot lens[b] - T + t. k, v: [tokens, kv_heads, head_dim],
+        strides multiples of 8 elements (slices of one projection's output are fine)."""
+        self._rows(k, "k", self.kv_heads)
+        self._rows(v, "v", self.kv_heads)
+        if v.shape[0] != k.shape[0]:
+            raise ValueError("k and v must have the same number of tokens")
+        self._sequences(table, lens, offsets, k.shape[0])
+        ks, vs = (C.c_int64 * 2)(*k.stride()[:2]), (C.c_int64 * 2)(*v.stride()[:2])
+        check(lib().vk_kv_append(self._h, self._batch_ref, k.data_ptr(), ks, v.data_ptr(), vs, self._stream(stream)),
+              "append")
+
+    def attend(self, q, offsets, table, lens, *, causal: bool = True, scale: float | None = None, scores=None,
+               max_q: int = 0, out=None, lse=None, stream=None):
+        """Attention of new tokens q [tokens, heads, head_dim] over their sequences' slots: (out like q, lse [tokens,
+        heads] float32). Token t of T sees slots up to lens[b] - T + t when causal, all lens[b] otherwise; a row that
+        sees none gets zeros and -inf. scale defaults to head_dim ** -0.5. scores, [batch, kv_heads, width] float32
+        with the last dimension contiguous: the attention weights of a sequence's tokens and of a kv head's query
+        heads are added to its slots. max_q: an upper bound of a sequence's new tokens, where the caller knows it (a
+        decoding step: 1); it spares launches."""
+        torch = self._torch
+        if q.dim() != 3:
+            raise ValueError("q must be [tokens, heads, head_dim]")
+        tokens, heads = q.shape[0], q.shape[1]
+        self._rows(q, "q", heads)
+        n = self._sequences(table, lens, offsets, tokens)
+        if out is None:
+            out = torch.empty((tokens, heads, self.head_dim), dtype=self.dtype, device=self.device)
+        else:
+            self._rows(out, "out", heads)
+            if out.shape[0] != tokens:
+                raise ValueError("out must have q's shape")
+        if lse is None:
+            lse = torch.empty((tokens, heads), dtype=torch.float32, device=self.device)
+        else:
+            _want(lse, "lse", torch.float32, 2, self.device)
+            if lse.shape != (tokens, heads) or not lse.is_contiguous():
+                raise ValueError("lse must be contiguous [tokens, heads]")
+        a = self._attend
+        a.q, a.out, a.lse = q.data_ptr(), out.data_ptr(), lse.data_ptr()
+        a.q_stride[0], a.q_stride[1] = q.stride(0), q.stride(1)
+        a.out_stride[0], a.out_stride[1] = out.stride(0), out.stride(1)
+        a.scores = None
+        if scores is not None:
+            self._check_scores(scores, n)
+            a.scores, a.scores_width = scores.data_ptr(), scores.shape[2]
+            a.scores_stride[0], a.scores_stride[1] = scores.stride(0), scores.stride(1)
+        a.heads, a.max_q, a.causal = heads, max_q, causal
+        a.scale = self.head_dim ** -0.5 if scale is None else scale
+        check(lib().vk_kv_attend(self._h, self._batch_ref, self._attend_ref, self._stream(stream)), "attend")
+        return out, lse
+
+    def evict(self, table, lens, new_table, keep: int, recent: int, scores, *, stream=None):
+        """Cuts every sequence back to at most `keep` slots for each kv head: its last `recent` ones and, of the others,
+        those with the largest scores (ties to the lower slot), in slot order, copied to the pages of new_table (which
+        no sequence of the call reads). Returns (kept [batch, kv_heads, keep] int32: the old slots, -1 behind the last;
+        new lens [batch] int32; new scores like scores, contiguous, 0 behind the last)."""
+        torch = self._torch
+        n = self._sequences(table, lens)
+        self._check_scores(scores, n)
+        _want(new_table, "new_table", torch.int32, 2, self.device)
+        if new_table.shape[0] != n or (new_table.shape[1] > 1 and new_table.stride(1) != 1):
+            raise ValueError("new_table must have one row per sequence, rows contiguous")
+        if not 0 <= recent <= keep:
+            raise ValueError("keep and recent must satisfy 0 <= recent <= keep")
+        kept = torch.empty((n, self.kv_heads, keep), dtype=torch.int32, device=self.device)
+        new_lens = torch.empty((n,), dtype=torch.int32, device=self.device)
+        new_scores = torch.empty(scores.shape, dtype=torch.float32, device=self.device)
+        e = self._evict
+        e.new_table, e.new_table_stride, e.new_table_width = new_table.data_ptr(), new_table.stride(0), new_table.shape[1]
+        e.keep, e.recent = keep, recent
+        e.scores, e.scores_width = scores.data_ptr(), scores.shape[2]
+        e.scores_stride[0], e.scores_stride[1] = scores.stride(0), scores.stride(1)
+        e.new_scores, e.kept, e.new_lens = new_scores.data_ptr(), kept.data_ptr(), new_lens.data_ptr()
+        check(lib().vk_kv_evict(self._h, self._batch_ref, self._evict_ref, self._stream(stream)), "evict")
+        return kept, new_lens, new_scores
+
+    def _check_scores(self, scores, n: int) -> None:
+        _want(scores, "scores", self._torch.float32, 3, self.device)
+        if scores.shape[0] != n or scores.shape[1] != self.kv_heads or (scores.shape[2] > 1 and scores.stride(2) != 1):
+            raise ValueError(f"scores must be [batch, {self.kv_heads}, width] with the last dimension contiguous")
+
+    def sync(self, stream=None) -> None:
+        """Waits for the cache's work on the stream and raises VkError for anything its kernels found wrong."""
+        check(lib().vk_kv_sync(self._h, self._stream(stream)), "sync")
+
+    def close(self) -> None:
+        if self._h:
+            lib().vk_kv_destroy(self._h)
+            self._h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
