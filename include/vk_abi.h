@@ -308,12 +308,11 @@ int vk_ivf_assign_device(int device, const float* d_x, int64_t n, int d, const f
  *   vk_kv_attend   attention of a sequence's new tokens (one, a few or a chunk) over its slots and, on request, the
  *                  attention weight that every slot gathered
  *   vk_kv_evict    copies the slots that gathered most, and the latest ones, into other pages
- * A cache (vk_kv_t) refers to the caller's pages and owns a small workspace that serves one call at a time: calls on
- * different streams must be ordered by the caller, and the workspace grows on the first call that needs more (a
- * warm-up call per shape before capturing a CUDA graph). All calls are asynchronous on `stream` (cudaStream_t as
- * void*; NULL = the default stream). A page number outside [0, pages) or a length or offset outside its table is
- * never followed: the affected slots read as absent and writes to them are skipped; vk_kv_sync waits and then reports
- * it as VK_ERR_INVALID. */
+ * A cache (vk_kv_t) refers to the caller's pages and owns no other device memory than a status word: no call
+ * allocates, attention's working memory is the caller's (vk_kv_attend_workspace). All calls are asynchronous on `stream`
+ * (cudaStream_t as void*; NULL = the default stream) and may be captured into a CUDA graph. A page number outside
+ * [0, pages) or a length or offset outside its table is never followed: such a page reads as zeros and writes to it are
+ * skipped; vk_kv_sync waits and then reports it as VK_ERR_INVALID. */
 enum {
     VK_KV_F16 = 0,
     VK_KV_BF16 = 1
@@ -371,7 +370,7 @@ typedef struct {
     int64_t q_stride[2];
     void* out; /* the same shape and type */
     int64_t out_stride[2];
-    float* lse;    /* [tokens][heads], contiguous; may be NULL */
+    float* lse;    /* [tokens][heads], contiguous */
     float* scores; /* element (b, kv head, slot) at scores[b * scores_stride[0] + head * scores_stride[1] + slot],
                       slots < scores_width; NULL: not gathered */
     int64_t scores_stride[2];
@@ -380,7 +379,13 @@ typedef struct {
     int max_q; /* at least the largest number of new tokens of a sequence; 0 = unknown (`tokens` is assumed) */
     int causal;
     float scale;
+    void* workspace; /* DEVICE, 256-byte aligned, at least vk_kv_attend_workspace bytes; free again when the call's work
+                        on the stream is done, its contents are nothing that a later call needs */
+    size_t workspace_bytes;
 } vk_kv_attend_t;
+/* Bytes of working memory that vk_kv_attend needs for these sizes (pointers in batch and args are not read, except
+ * whether args->scores is NULL). */
+int vk_kv_attend_workspace(const vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_attend_t* args, size_t* bytes);
 int vk_kv_attend(vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_attend_t* args, void* stream);
 
 /* For every sequence of n slots and every kv head: k = min(n, keep) slots are kept, the last r = min(recent, k) and, of

@@ -71,7 +71,7 @@ class KvAttend(C.Structure):
     _fields_ = [("q", C.c_void_p), ("q_stride", C.c_int64 * 2), ("out", C.c_void_p), ("out_stride", C.c_int64 * 2),
                 ("lse", C.c_void_p), ("scores", C.c_void_p), ("scores_stride", C.c_int64 * 2),
                 ("scores_width", C.c_int64), ("heads", C.c_int), ("max_q", C.c_int), ("causal", C.c_int),
-                ("scale", C.c_float)]
+                ("scale", C.c_float), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
 class KvEvict(C.Structure):
@@ -135,6 +135,7 @@ ABI = {
     "vk_kv_sync": (C.c_int, [_vp, _vp]),
     "vk_kv_append": (C.c_int, [_vp, _vp, _vp, C.POINTER(_i64), _vp, C.POINTER(_i64), _vp]),
     "vk_kv_attend": (C.c_int, [_vp, _vp, _vp, _vp]),
+    "vk_kv_attend_workspace": (C.c_int, [_vp, _vp, _vp, C.POINTER(C.c_size_t)]),
     "vk_kv_evict": (C.c_int, [_vp, _vp, _vp, _vp]),
     "vk_ivf_create": (C.c_int, [C.c_int, _vp, C.c_int, C.c_int, _vp, _i64, _vp, C.c_int, _vp, C.POINTER(_vp)]),
     "vk_ivf_destroy": (C.c_int, [_vp]),

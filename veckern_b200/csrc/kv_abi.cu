@@ -2,6 +2,8 @@
 #include <new>
 #include <type_traits>
 
+#include <cudaTypedefs.h>
+
 #include "kv_attend.cuh"
 #include "kv_move.cuh"
 #include "status.h"
@@ -11,7 +13,7 @@ struct vk_kv {
     int page_shift = 0;
     int sm_count = 0;
     int* status = nullptr;
-    DevBuf<float> lse;
+    CUtensorMap map_k, map_v;
     ~vk_kv() {
         if (status) cudaFree(status);
     }
@@ -67,16 +69,140 @@ int check_rows(const char* what, const void* p, const int64_t* stride) {
     return VK_OK;
 }
 
-template <typename T>
-int launch_attend(const vk::KvPages& c, const vk::KvBatch& bt, const vk::KvAttend& a, cudaStream_t st) {
-    vk::kv_attend_kernel<T><<<dim3((unsigned)bt.tokens, a.heads), 32 * vk::ROW_WARPS, 0, st>>>(c, bt, a);
+size_t align256(size_t x) { return (x + 255) / 256 * 256; }
+
+// How a call's attention is laid out: which kernels may have work, their CTAs, and the workspace.
+struct AttendPlan {
+    bool step, chunk;
+    int rows;  // of the step path: 8 or 16
+    int step_ctas;
+    size_t o, ml, at, s, bytes;  // offsets
+};
+
+AttendPlan plan_attend(const vk_kv* kv, const vk::KvBatch& bt, int group, int max_q, bool scores) {
+    AttendPlan p{};
+    const int64_t rows = (int64_t)max_q * group;
+    p.chunk = rows > vk::STEP_ROWS;
+    p.step = group <= vk::STEP_ROWS && !(bt.batch == 1 && bt.tokens * group > vk::STEP_ROWS);
+    p.rows = std::min<int64_t>(rows, vk::STEP_ROWS) <= 8 ? 8 : 16;
+    p.step_ctas = 2 * kv->sm_count;
+    const int dp = kv->desc.head_dim <= 64 ? 64 : 128;
+    const int64_t slots = (int64_t)bt.width << kv->page_shift;
+    const size_t parts = 2 * (size_t)p.step_ctas;
+    p.ml = p.o + align256(parts * vk::STEP_ROWS * dp * sizeof(float));
+    p.at = p.ml + align256(parts * vk::STEP_ROWS * sizeof(float2));
+    p.s = p.at + align256(parts * sizeof(int4));
+    p.bytes = p.s + (scores && p.step ? align256((size_t)bt.batch * kv->desc.kv_heads * slots * p.rows * sizeof(float)) : 0);
+    return p;
+}
+
+// Launches fn so that it may start while the kernel before it on the stream ends; it waits for that one's results itself.
+template <class... Args>
+int launch_behind(void (*fn)(Args...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args... args) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    VK_TRY_CUDA(cudaLaunchKernelEx(&cfg, fn, args...));
+    return VK_OK;
+}
+
+template <typename T, int DP, int R, bool SCORES>
+int launch_step_as(const vk_kv* kv, const vk::KvPages& c, const vk::KvBatch& bt, const vk::KvAttend& a,
+                   const vk::KvParts& parts, int ctas, cudaStream_t st) {
+    const auto fn = &vk::kv_step_kernel<T, DP, R, SCORES>;
+    constexpr int smem = vk::step_smem<DP>();
+    VK_TRY_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    fn<<<ctas, vk::STEP_THREADS, smem, st>>>(kv->map_k, kv->map_v, c, bt, a, parts);
     VK_TRY_CUDA(cudaGetLastError());
-    const int64_t slots = (int64_t)bt.width << c.page_shift;
-    if (a.scores && slots > 0) {
-        vk::kv_weights_kernel<T><<<dim3((unsigned)ceil_div(slots, 8), c.heads, bt.batch), 256, 0, st>>>(c, bt, a);
-        VK_TRY_CUDA(cudaGetLastError());
+    VK_TRY(launch_behind(&vk::kv_join_kernel<T, DP, vk::STEP_ROWS, 16>, dim3(2 * ctas), 512, 0, st, c, bt, a, parts, ctas,
+                         vk::STEP_ROWS));
+    if constexpr (SCORES) {
+        const int64_t width = std::min(parts.s_slots, a.scores_width);
+        if (width > 0)
+            VK_TRY(launch_behind(&vk::kv_step_weights_kernel<R>,
+                                 dim3((unsigned)std::min<int64_t>(ceil_div(width, 256), 4096), c.heads, bt.batch), 256, 0, st,
+                                 c, bt, a, parts));
     }
     return VK_OK;
+}
+
+template <typename T, int DP>
+int launch_step(const vk_kv* kv, const vk::KvPages& c, const vk::KvBatch& bt, const vk::KvAttend& a,
+                const vk::KvParts& parts, const AttendPlan& p, cudaStream_t st) {
+    if (p.rows == 8)
+        return a.scores ? launch_step_as<T, DP, 8, true>(kv, c, bt, a, parts, p.step_ctas, st)
+                        : launch_step_as<T, DP, 8, false>(kv, c, bt, a, parts, p.step_ctas, st);
+    return a.scores ? launch_step_as<T, DP, 16, true>(kv, c, bt, a, parts, p.step_ctas, st)
+                    : launch_step_as<T, DP, 16, false>(kv, c, bt, a, parts, p.step_ctas, st);
+}
+
+template <typename T>
+int launch_attend(const vk_kv* kv, const vk::KvBatch& bt, const vk::KvAttend& a, void* workspace, const AttendPlan& p,
+                  cudaStream_t st) {
+    const vk::KvPages c = pages_of(kv);
+    uint8_t* w = static_cast<uint8_t*>(workspace);
+    vk::KvParts parts{};
+    parts.o = reinterpret_cast<float*>(w + p.o);
+    parts.ml = reinterpret_cast<float2*>(w + p.ml);
+    parts.at = reinterpret_cast<int4*>(w + p.at);
+    parts.s = reinterpret_cast<float*>(w + p.s);
+    parts.s_slots = (int64_t)bt.width << kv->page_shift;
+    if (p.step) VK_TRY((c.dim <= 64 ? launch_step<T, 64>(kv, c, bt, a, parts, p, st)
+                                    : launch_step<T, 128>(kv, c, bt, a, parts, p, st)));
+    if (p.chunk) {
+        vk::kv_attend_kernel<T><<<dim3((unsigned)bt.tokens, a.heads), 32 * vk::ROW_WARPS, 0, st>>>(c, bt, a);
+        VK_TRY_CUDA(cudaGetLastError());
+        const int64_t slots = (int64_t)bt.width << c.page_shift;
+        if (a.scores && slots > 0) {
+            vk::kv_weights_kernel<T><<<dim3((unsigned)ceil_div(slots, 8), c.heads, bt.batch), 256, 0, st>>>(c, bt, a);
+            VK_TRY_CUDA(cudaGetLastError());
+        }
+    }
+    return VK_OK;
+}
+
+// The tensor map of the keys' or values' pages: (element, slot, head, page), boxes of 64 elements of up to 64 slots.
+int encode_map(const vk_kv_desc_t& d, void* base, const int64_t* stride, CUtensorMap* map) {
+    static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+    if (!encode) {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        VK_TRY_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found));
+        if (!fn || found != cudaDriverEntryPointSuccess)
+            return fail(VK_ERR_UNSUPPORTED, "the driver has no cuTensorMapEncodeTiled");
+        encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    }
+    const cuuint64_t dims[4] = {(cuuint64_t)d.head_dim, (cuuint64_t)d.page_size, (cuuint64_t)d.kv_heads,
+                                (cuuint64_t)d.pages};
+    // a dimension of one entry is never stepped along: any valid stride does
+    const cuuint64_t strides[3] = {(cuuint64_t)stride[1] * 2, d.kv_heads > 1 ? (cuuint64_t)stride[2] * 2 : 16,
+                                   d.pages > 1 ? (cuuint64_t)stride[0] * 2 : 16};
+    const cuuint32_t box[4] = {64, (cuuint32_t)std::min(d.page_size, vk::STEP_TILE), 1, 1}, step[4] = {1, 1, 1, 1};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, base, dims, strides, box, step,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(VK_ERR_INVALID, "the pages' sizes and strides do not make a tensor map (%d)", (int)r);
+    return VK_OK;
+}
+
+// Checks what attention's launches and its workspace's size depend on.
+int check_attend(const vk_kv* kv, const vk_kv_attend_t* args) {
+    if (!args) return fail(VK_ERR_INVALID, "args must not be NULL");
+    const int g = kv->desc.kv_heads;
+    if (args->heads < g || args->heads % g || args->heads / g > 128)
+        return fail(VK_ERR_INVALID, "heads must be a multiple of kv_heads (%d), at most 128 times it", g);
+    if (args->max_q < 0) return fail(VK_ERR_INVALID, "max_q must be >= 0");
+    return VK_OK;
+}
+int max_q_of(const vk_kv_attend_t* args, int64_t tokens) {
+    return args->max_q > 0 ? (int)std::min<int64_t>(args->max_q, tokens) : (int)tokens;
 }
 
 }  // namespace
@@ -116,6 +242,12 @@ int vk_kv_create(const vk_kv_desc_t* d, vk_kv_t** out) {
         delete kv;
         return fail(e == cudaErrorMemoryAllocation ? VK_ERR_NOMEM : VK_ERR_CUDA, "vk_kv_create: %s",
                     cudaGetErrorString(e));
+    }
+    int r = encode_map(*d, d->k, d->k_stride, &kv->map_k);
+    if (r == VK_OK) r = encode_map(*d, d->v, d->v_stride, &kv->map_v);
+    if (r != VK_OK) {
+        delete kv;
+        return r;
     }
     *out = kv;
     return VK_OK;
@@ -164,11 +296,8 @@ int vk_kv_append(vk_kv_t* kv, const vk_kv_batch_t* batch, const void* k, const i
 int vk_kv_attend(vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_attend_t* args, void* stream) {
     vk::KvBatch bt{};
     VK_TRY(check_batch(kv, batch, true, &bt));
-    if (!args) return fail(VK_ERR_INVALID, "args must not be NULL");
+    VK_TRY(check_attend(kv, args));
     const int g = kv->desc.kv_heads;
-    if (args->heads < g || args->heads % g || args->heads / g > 128)
-        return fail(VK_ERR_INVALID, "heads must be a multiple of kv_heads (%d), at most 128 times it", g);
-    if (args->max_q < 0) return fail(VK_ERR_INVALID, "max_q must be >= 0");
     if (!(args->scale == args->scale) || args->scale - args->scale != 0.0f)
         return fail(VK_ERR_INVALID, "scale must be finite");
     if (args->scores && (args->scores_width < 0 || args->scores_stride[0] < 0 || args->scores_stride[1] < 0))
@@ -176,6 +305,7 @@ int vk_kv_attend(vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_attend_t* 
     if (bt.tokens == 0 || bt.batch == 0) return VK_OK;
     VK_TRY(check_rows("q", args->q, args->q_stride));
     VK_TRY(check_rows("out", args->out, args->out_stride));
+    if (!args->lse) return fail(VK_ERR_INVALID, "lse must not be NULL");
     DeviceGuard guard(kv->desc.device);
     if (guard.err != cudaSuccess) return fail(VK_ERR_CUDA, "cudaSetDevice: %s", cudaGetErrorString(guard.err));
     vk::KvAttend a{};
@@ -191,16 +321,28 @@ int vk_kv_attend(vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_attend_t* 
     a.scores_width = args->scores_width;
     a.heads = args->heads;
     a.group = args->heads / g;
-    a.max_q = args->max_q > 0 ? (int)std::min<int64_t>(args->max_q, bt.tokens) : (int)bt.tokens;
+    a.max_q = max_q_of(args, bt.tokens);
     a.causal = args->causal != 0;
     a.scale = args->scale;
-    if (!a.lse) {
-        VK_TRY(kv->lse.ensure((size_t)bt.tokens * a.heads));
-        a.lse = kv->lse.ptr;
-    }
+    const AttendPlan plan = plan_attend(kv, bt, a.group, a.max_q, a.scores != nullptr);
+    if (args->workspace_bytes < plan.bytes || !args->workspace || reinterpret_cast<uintptr_t>(args->workspace) % 256)
+        return fail(VK_ERR_INVALID, "workspace must be 256-byte aligned and hold %zu bytes (vk_kv_attend_workspace)",
+                    plan.bytes);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return kv->desc.dtype == VK_KV_F16 ? launch_attend<__half>(pages_of(kv), bt, a, st)
-                                       : launch_attend<__nv_bfloat16>(pages_of(kv), bt, a, st);
+    return kv->desc.dtype == VK_KV_F16 ? launch_attend<__half>(kv, bt, a, args->workspace, plan, st)
+                                       : launch_attend<__nv_bfloat16>(kv, bt, a, args->workspace, plan, st);
+}
+
+int vk_kv_attend_workspace(const vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_attend_t* args, size_t* bytes) {
+    vk::KvBatch bt{};
+    if (!kv || !batch || !bytes) return fail(VK_ERR_INVALID, "cache, batch and bytes must not be NULL");
+    vk_kv_batch_t sizes = *batch;  // pointers are not read
+    static const int32_t none = 0;
+    sizes.offsets = sizes.table = sizes.lens = &none;
+    VK_TRY(check_batch(kv, &sizes, true, &bt));
+    VK_TRY(check_attend(kv, args));
+    *bytes = plan_attend(kv, bt, args->heads / kv->desc.kv_heads, max_q_of(args, bt.tokens), args->scores != nullptr).bytes;
+    return VK_OK;
 }
 
 int vk_kv_evict(vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_evict_t* args, void* stream) {

@@ -1,6 +1,6 @@
 // Attention over the paged cache, one block per (new token, query head).
 #pragma once
-#include "kv_common.cuh"
+#include "kv_step.cuh"
 
 namespace vk {
 
@@ -28,7 +28,7 @@ __global__ void __launch_bounds__(32 * ROW_WARPS) kv_attend_kernel(KvPages c, Kv
     const int h = blockIdx.y, kvh = h / a.group, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int b = kv_find(bt, tok);
     const KvSeq s = kv_seq(c, bt, b);
-    if (tok < s.first || tok >= s.first + s.count) return;
+    if (tok < s.first || tok >= s.first + s.count || step_takes(s, a.group)) return;
     const int32_t* table = bt.table + b * bt.table_stride;
     const int end = a.causal ? max(0, s.len - s.count + (int)(tok - s.first) + 1) : s.len;
     float q[4], o[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
@@ -67,7 +67,7 @@ template <typename T>
 __global__ void __launch_bounds__(256) kv_weights_kernel(KvPages c, KvBatch bt, KvAttend a) {
     const int b = blockIdx.z, kvh = blockIdx.y, j = blockIdx.x * 8 + (threadIdx.x >> 5);
     const KvSeq s = kv_seq(c, bt, b);
-    if (j >= s.len || j >= a.scores_width) return;
+    if (j >= s.len || j >= a.scores_width || step_takes(s, a.group)) return;
     const int64_t page = kv_page(c, bt.table + b * bt.table_stride, j);
     if (page < 0) return;
     float k[4], sum = 0.f;

@@ -1,0 +1,507 @@
+// Attention of a sequence's few new tokens over the paged cache (at most 16 rows = tokens x query heads of a kv head:
+// decoding steps, drafted tokens), and the join of split sequences.
+//
+// Every slot's key and value (4 x head_dim bytes per kv head) is read once and meets at most 16 rows, so the kernel is
+// bound by memory. One CTA per 64-slot tile would leave SMs idle on short batches and unbalanced on ragged ones:
+// instead all (sequence, kv head, tile) units are laid end to end and every CTA takes an equal, contiguous share. A
+// sequence's head that a CTA holds whole is finished in place; one that is cut leaves parts (unnormalised sums with
+// their maximum and total) that the join kernel adds up in order, so results do not depend on timing.
+//
+// Inside a CTA one warp keeps a ring of tiles filled by TMA (one box per page and 64 head elements, in the 128-byte
+// swizzle that ldmatrix reads without conflicts); four warps take 16 slots of each tile, with their own running maximum
+// and sum, on mma.sync m16n8k16: at 16 rows the tensor work is under a fifth of its rate while memory is saturated, and
+// the operands stay in registers from the scores to the values, which tcgen05's 128-row tiles would not allow.
+#pragma once
+#include <cuda.h>
+
+#include "kv_common.cuh"
+
+namespace vk {
+
+constexpr int STEP_TILE = 64;  // slots of a tile
+constexpr int STEP_ROWS = 16;  // most rows of a sequence's kv head
+constexpr int STEP_WARPS = 4;  // consumers; one more warp loads
+constexpr int STEP_THREADS = 32 * (STEP_WARPS + 1);
+constexpr int STEP_RING = 96 * 1024;  // bytes in flight per CTA; two CTAs share an SM
+constexpr long long KV_WAIT_BUDGET = 4000000000LL;  // cycles: about two seconds
+
+// Parts of split sequences. CTA i leaves at most two: part 2i of the first (sequence, head) of its share, part 2i + 1 of
+// the last. The parts of one follow each other in the order of the CTAs.
+enum : int { PART_NONE = 0, PART_HELD = 1, PART_FIRST = 2, PART_LAST = 4 };
+struct KvParts {
+    float* o;     // [part][rows][padded head size], unnormalised
+    float2* ml;   // [part][rows]: maximum (base 2) and sum
+    int4* at;     // [part]: sequence, kv head, row tile, PART_ flags
+    float* s;     // [sequence][kv head][slot][R]: scaled scores (base 2) of the step path, for the weights
+    int64_t s_slots;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// A 2-d box of a page (box slots x 64 elements of one head) into shared memory.
+__device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int d, int slot, int head, int page,
+                                         uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(d), "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// Bounded waits of one thread or warp: after the first that runs out, the later ones return at once, so that the CTA
+// unwinds; what it computes then is void and the status word says so.
+struct KvWait {
+    int* status;
+    bool dead = false;
+    __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t parity) {
+        if (!dead && !mbar_wait_bounded(bar, parity, KV_WAIT_BUDGET)) {
+            dead = true;
+            atomicOr(status, ERR_WAIT_TIMEOUT);
+        }
+    }
+};
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same_v<T, __half>)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two values rounded to the 16-bit type, the first in the low half.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+    uint32_t r;
+    if constexpr (std::is_same_v<T, __half>) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// The share of one CTA: a walk over units laid end to end, sequence by sequence. Count(s) is the number of units of a
+// sequence; the caller splits a sequence's units into its heads and tiles.
+struct KvShare {
+    int b;         // sequence of the next unit
+    int64_t off;   // unit within it
+    int64_t left;  // units of this CTA
+};
+
+template <int THREADS, class Count>
+__device__ __forceinline__ KvShare kv_share(const KvPages& c, const KvBatch& bt, int64_t* scratch, Count&& count) {
+    // scratch: THREADS / 32 + 4 values of shared memory. Thread t sums a contiguous range of the sequences.
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    constexpr int WARPS = THREADS / 32;
+    const int each = (bt.batch + THREADS - 1) / THREADS;
+    const int b0 = min(bt.batch, t * each), b1 = min(bt.batch, b0 + each);
+    int64_t sum = 0;
+    for (int b = b0; b < b1; ++b) sum += count(kv_seq(c, bt, b));
+    int64_t incl = sum;
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t x = __shfl_up_sync(FULL, incl, o);
+        if (lane >= o) incl += x;
+    }
+    if (lane == 31) scratch[warp] = incl;
+    __syncthreads();
+    int64_t before = 0, total = 0;
+    for (int w = 0; w < WARPS; ++w) {
+        if (w < warp) before += scratch[w];
+        total += scratch[w];
+    }
+    // No empty share between two others: the parts of a split sequence lie at consecutive CTAs.
+    const int64_t ctas = min((int64_t)gridDim.x, total), i = min((int64_t)blockIdx.x, ctas);
+    const int64_t first = ctas ? total * i / ctas : 0, last = ctas ? total * min(i + 1, ctas) / ctas : 0;
+    before += incl - sum;
+    if (first >= before && first < before + sum) {
+        int64_t off = first - before;
+        int b = b0;
+        for (;; ++b) {
+            const int64_t n = count(kv_seq(c, bt, b));
+            if (off < n) break;
+            off -= n;
+        }
+        scratch[WARPS] = b;
+        scratch[WARPS + 1] = off;
+    }
+    __syncthreads();
+    return {(int)scratch[WARPS], scratch[WARPS + 1], last - first};
+}
+
+// Lowest slot that some row does not see: n for every row, or the first row's limit under the causal mask.
+__device__ __forceinline__ int row_limit(const KvSeq& s, int causal, int token) {
+    return causal ? s.len - s.count + token + 1 : s.len;
+}
+
+__device__ __forceinline__ bool step_takes(const KvSeq& s, int group) {
+    return s.count > 0 && s.count * (int64_t)group <= STEP_ROWS;
+}
+
+template <int DP>
+constexpr int STEP_STAGE = STEP_TILE * DP * 2 * 2;  // bytes of a tile's keys and values
+template <int DP>
+constexpr int step_smem() {
+    return STEP_RING + STEP_WARPS * 8 * DP * 4 + STEP_WARPS * STEP_ROWS * 8 + 256;
+}
+
+// DP: head size padded to 64 or 128 (the boxes' columns past the head read as zero). R: rows rounded up to 8 or 16; of
+// m16n8k16's rows the upper eight are not worked on when R is 8.
+template <typename T, int DP, int R, bool SCORES>
+__global__ void __launch_bounds__(STEP_THREADS, 2)
+    kv_step_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, KvPages c,
+                   KvBatch bt, KvAttend a, KvParts parts) {
+    constexpr int STAGE = STEP_STAGE<DP>, STAGES = STEP_RING / STAGE, HALVES = DP / 64, KS = DP / 16;
+    extern __shared__ __align__(1024) uint8_t ring[];  // the swizzle goes by address bits: 1024-byte aligned
+    float* sum_o = reinterpret_cast<float*>(ring + STEP_RING);                              // [warp][8][DP]
+    float2* sum_ml = reinterpret_cast<float2*>(sum_o + STEP_WARPS * 8 * DP);                // [warp][16]
+    uint64_t* full = reinterpret_cast<uint64_t*>(sum_ml + STEP_WARPS * STEP_ROWS);
+    uint64_t* empty = full + STAGES;
+    int64_t* scratch = reinterpret_cast<int64_t*>(empty + STAGES);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; ++i) {
+            mbar_init(full + i, 1);
+            mbar_init(empty + i, STEP_WARPS);
+        }
+        fence_mbar_init();
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    auto tiles_of = [&](const KvSeq& s) { return max(1, (s.len + STEP_TILE - 1) / STEP_TILE); };
+    auto units_of = [&](const KvSeq& s) -> int64_t {
+        return step_takes(s, a.group) ? (int64_t)tiles_of(s) * c.heads : 0;
+    };
+    KvShare share = kv_share<STEP_THREADS>(c, bt, scratch, units_of);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (threadIdx.x < 2) parts.at[2 * blockIdx.x + threadIdx.x].w = PART_NONE;
+    __syncthreads();
+    KvWait wait{c.status};
+    int stage = 0;
+    uint32_t phase = 0;
+    const int box_shift = min(c.page_shift, 6), boxes = STEP_TILE >> box_shift;
+    bool first_segment = true;
+    int loaded = 0;
+    while (share.left > 0) {
+        const KvSeq s = kv_seq(c, bt, share.b);
+        const int tiles = tiles_of(s);
+        if (!step_takes(s, a.group) || share.off >= (int64_t)tiles * c.heads) {
+            ++share.b;
+            share.off = 0;
+            continue;
+        }
+        const int head = (int)(share.off / tiles), t0 = (int)(share.off % tiles);
+        const int count = (int)min((int64_t)(tiles - t0), share.left);
+        share.off += count;
+        share.left -= count;
+        const int32_t* table = bt.table + share.b * bt.table_stride;
+        if (warp == STEP_WARPS) {
+            // Loads: lane = (key or value, half of the head, page of the tile).
+            const int per = boxes * HALVES, i = lane % boxes, half = lane / boxes % HALVES, side = lane / per;
+            for (int t = t0; t < t0 + count; ++t) {
+                const int slot = t * STEP_TILE + (i << box_shift);
+                const bool live = lane < 2 * per && slot < s.len;
+                int page = 0;
+                if (live) {
+                    page = (int)kv_page(c, table, slot);
+                    if (page < 0) page = (int)c.pages;  // past the map: reads as zero
+                }
+                const int n = __popc(__ballot_sync(FULL, live));
+                wait(empty + stage, phase ^ 1);
+                if (lane == 0) mbar_arrive_expect_tx(full + stage, n * (128 << box_shift));
+                __syncwarp();
+                if (live)
+                    tma_page(ring + stage * STAGE + (side * HALVES + half) * (STEP_TILE * 128) + (i << box_shift) * 128,
+                             side ? &map_v : &map_k, half * 64, slot & ((1 << c.page_shift) - 1), head, page,
+                             full + stage);
+                ++loaded;
+                if (++stage == STAGES) stage = 0, phase ^= 1;
+            }
+        } else {
+            const int g = lane >> 2, q2 = (lane & 3) * 2, rows = s.count * a.group;
+            uint32_t q[KS][4];
+            int lim[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int r = g + 8 * u;
+                const bool live = r < rows && (u == 0 || R == 16);
+                lim[u] = live ? row_limit(s, a.causal, r / a.group) : 0;
+                const uint16_t* row = a.q + (s.first + (live ? r / a.group : 0)) * a.qs[0] +
+                                      (head * a.group + (live ? r % a.group : 0)) * a.qs[1];
+#pragma unroll
+                for (int k = 0; k < KS; ++k)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const int d = 16 * k + 8 * e + q2;
+                        q[k][u + 2 * e] = live && d < c.dim ? __ldg(reinterpret_cast<const unsigned int*>(row + d)) : 0u;
+                    }
+            }
+            const float scale = a.scale * 1.4426950408889634f;
+            const int open = min(s.len, row_limit(s, a.causal, 0));  // slots that every row sees
+            float o[DP / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+            for (int t = t0; t < t0 + count; ++t) {
+                const int slot0 = t * STEP_TILE + warp * 16;
+                wait(full + stage, phase);
+                if (slot0 < s.len) {
+                    const uint32_t base = smem_u32(ring + stage * STAGE);
+                    const bool ends = slot0 + 16 > s.len;
+                    if (ends) {  // the page's slots past the sequence hold anything: their values must not meet a zero
+                        uint8_t* v = ring + stage * STAGE + HALVES * (STEP_TILE * 128);
+                        for (int i = (s.len - slot0) * 8 + lane; i < 16 * 8; i += 32)
+#pragma unroll
+                            for (int hf = 0; hf < HALVES; ++hf)
+                                *reinterpret_cast<uint4*>(v + hf * (STEP_TILE * 128) + warp * 2048 + i * 16) =
+                                    make_uint4(0u, 0u, 0u, 0u);
+                        __syncwarp();
+                    }
+                    float x[2][4] = {};
+#pragma unroll
+                    for (int k = 0; k < KS; ++k) {
+                        // matrices: slots 0-7 and 8-15, each with elements 0-7 and 8-15 of this step's 16
+                        const int slot = warp * 16 + (lane & 7) + ((lane >> 4) << 3), ch = (k & 3) * 2 + ((lane >> 3) & 1);
+                        uint32_t b[4];
+                        ldsm4(base + (k >> 2) * (STEP_TILE * 128) + slot * 128 + ((ch ^ (slot & 7)) << 4), b);
+                        mma16<T>(x[0], q[k], b[0], b[1]);
+                        mma16<T>(x[1], q[k], b[2], b[3]);
+                    }
+                    const bool masked = slot0 + 16 > open;
+#pragma unroll
+                    for (int u = 0; u < (R == 16 ? 2 : 1); ++u) {
+                        float top = -INFINITY;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float& y = x[e >> 1][2 * u + (e & 1)];
+                            y *= scale;
+                            if (masked && slot0 + (e >> 1) * 8 + q2 + (e & 1) >= lim[u]) y = -INFINITY;
+                            top = fmaxf(top, y);
+                        }
+                        if constexpr (SCORES) {
+                            float* sp = parts.s + (((int64_t)share.b * c.heads + head) * parts.s_slots + slot0 + q2) * R +
+                                        g + 8 * u;
+                            // a slot past the sequence may lie past the workspace's last slot: only its own are written
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int j = (e >> 1) * 8 + (e & 1);
+                                if (slot0 + q2 + j < s.len) sp[(int64_t)j * R] = x[e >> 1][2 * u + (e & 1)];
+                            }
+                        }
+                        top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
+                        top = fmaxf(top, __shfl_xor_sync(FULL, top, 2));
+                        const float next = fmaxf(m[u], top);
+                        const float ref = next == -INFINITY ? 0.f : next;
+                        if (__any_sync(FULL, next != m[u])) {
+                            const float f = ex2(m[u] - ref);
+                            l[u] *= f;
+#pragma unroll
+                            for (int i = 0; i < DP / 8; ++i) {
+                                o[i][2 * u] *= f;
+                                o[i][2 * u + 1] *= f;
+                            }
+                            m[u] = next;
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float& y = x[e >> 1][2 * u + (e & 1)];
+                            y = ex2(y - ref);
+                            l[u] += y;
+                        }
+                    }
+                    // the accumulator's layout of the weights is the operand's: 16 rows x 16 slots
+                    const uint32_t p[4] = {pack2<T>(x[0][0], x[0][1]), R == 16 ? pack2<T>(x[0][2], x[0][3]) : 0u,
+                                           pack2<T>(x[1][0], x[1][1]), R == 16 ? pack2<T>(x[1][2], x[1][3]) : 0u};
+#pragma unroll
+                    for (int i = 0; i < DP / 16; ++i) {
+                        const int slot = warp * 16 + (lane & 15), ch = (i & 3) * 2 + (lane >> 4);
+                        uint32_t b[4];
+                        ldsm4t(base + (HALVES + (i >> 2)) * (STEP_TILE * 128) + slot * 128 + ((ch ^ (slot & 7)) << 4), b);
+                        mma16<T>(o[2 * i], p, b[0], b[1]);
+                        mma16<T>(o[2 * i + 1], p, b[2], b[3]);
+                    }
+                    if (ends) fence_proxy_async_smem();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(empty + stage);
+                if (++stage == STAGES) stage = 0, phase ^= 1;
+            }
+            // Join the four warps, eight rows at a time.
+            const bool whole = count == tiles;
+            const int part = 2 * blockIdx.x + (first_segment ? 0 : 1);
+#pragma unroll
+            for (int u = 0; u < R / 8; ++u) {
+                l[u] += __shfl_xor_sync(FULL, l[u], 1);
+                l[u] += __shfl_xor_sync(FULL, l[u], 2);
+                if ((lane & 3) == 0) sum_ml[warp * STEP_ROWS + 8 * u + g] = make_float2(m[u], l[u]);
+            }
+#pragma unroll
+            for (int u = 0; u < R / 8; ++u) {
+#pragma unroll
+                for (int i = 0; i < DP / 8; ++i)
+                    *reinterpret_cast<float2*>(sum_o + (warp * 8 + g) * DP + 8 * i + q2) =
+                        make_float2(o[i][2 * u], o[i][2 * u + 1]);
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                for (int i = threadIdx.x; i < 8 * (DP / 8); i += 32 * STEP_WARPS) {
+                    const int r8 = i / (DP / 8), r = 8 * u + r8, d = i % (DP / 8) * 8;
+                    if (r >= rows) continue;
+                    float top = -INFINITY, total = 0.f, v[8] = {};
+#pragma unroll
+                    for (int w = 0; w < STEP_WARPS; ++w) top = fmaxf(top, sum_ml[w * STEP_ROWS + r].x);
+#pragma unroll
+                    for (int w = 0; w < STEP_WARPS; ++w) {
+                        const float2 ml = sum_ml[w * STEP_ROWS + r];
+                        const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+                        total += f * ml.y;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] += f * sum_o[(w * 8 + r8) * DP + d + e];
+                    }
+                    if (whole) {
+                        const int64_t tok = s.first + r / a.group;
+                        const int h = head * a.group + r % a.group;
+                        const float inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
+                        if (d < c.dim)
+                            *reinterpret_cast<uint4*>(a.out + tok * a.os[0] + h * a.os[1] + d) =
+                                make_uint4(pack2<T>(v[0] * inv, v[1] * inv), pack2<T>(v[2] * inv, v[3] * inv),
+                                           pack2<T>(v[4] * inv, v[5] * inv), pack2<T>(v[6] * inv, v[7] * inv));
+                        if (d == 0) a.lse[tok * a.heads + h] = (top + log2f(total)) * 0.6931471805599453f;
+                    } else {
+                        float4* po = reinterpret_cast<float4*>(parts.o + ((int64_t)part * STEP_ROWS + r) * DP + d);
+                        po[0] = make_float4(v[0], v[1], v[2], v[3]);
+                        po[1] = make_float4(v[4], v[5], v[6], v[7]);
+                        if (d == 0) parts.ml[(int64_t)part * STEP_ROWS + r] = make_float2(top, total);
+                    }
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+            }
+            if (!whole && threadIdx.x == 0)
+                parts.at[part] = make_int4(share.b, head, 0,
+                                           PART_HELD | (t0 == 0 ? PART_FIRST : 0) | (t0 + count == tiles ? PART_LAST : 0));
+        }
+        first_segment = false;
+    }
+    // A wait that ran out may have left copies in flight into this CTA's memory: see them land before it ends.
+    if (warp == STEP_WARPS && wait.dead && lane == 0)
+        for (int i = 0; i < STAGES; ++i) {
+            const int fills = loaded / STAGES + (i < loaded % STAGES);
+            if (fills && !mbar_wait_bounded(full + i, (fills - 1) & 1, 2 * KV_WAIT_BUDGET))
+                atomicOr(c.status, ERR_DRAIN_TIMEOUT);
+        }
+}
+
+// Adds up the parts of split (sequence, kv head, row tile)s. Block x starts at part x if that is a first one; the others
+// of it are the first parts of the CTAs that follow. One warp per row.
+template <typename T, int DP, int ROWS, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) kv_join_kernel(KvPages c, KvBatch bt, KvAttend a, KvParts parts, int ctas,
+                                                             int tile_tokens) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int4 at = parts.at[blockIdx.x];
+    if (!(at.w & PART_FIRST)) return;
+    const int lane = threadIdx.x & 31;
+    const KvSeq s = kv_seq(c, bt, at.x);
+    const int cta = blockIdx.x / 2;
+    int last = cta;
+    if (!(at.w & PART_LAST)) {
+        for (;;) {  // the CTAs that follow, 32 at a time, up to the one with the last part
+            const int i = last + 1 + lane;
+            const unsigned ends = __ballot_sync(FULL, i >= ctas || (parts.at[2 * i].w & PART_LAST));
+            if (ends) {
+                last += __ffs(ends);
+                break;
+            }
+            last += 32;
+        }
+        last = min(last, ctas - 1);
+    }
+    auto part_of = [&](int i) -> int64_t { return i == 0 ? (int64_t)blockIdx.x : 2 * (int64_t)(cta + i); };
+    const int n = last - cta + 1;
+    const int rows = min(ROWS, (s.count - at.z * tile_tokens) * a.group);
+    const int used = tile_tokens * a.group;
+    for (int r = blockIdx.y * WARPS + (threadIdx.x >> 5); r < min(rows, used); r += WARPS * gridDim.y) {
+        float top = -INFINITY;
+        for (int i = lane; i < n; i += 32) top = fmaxf(top, parts.ml[part_of(i) * ROWS + r].x);
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
+        float total = 0.f;
+        constexpr int PER = DP / 32;  // elements of a lane
+        float v[PER] = {};
+#pragma unroll 8
+        for (int i = 0; i < n; ++i) {
+            const int64_t p = part_of(i) * ROWS + r;
+            const float2 ml = parts.ml[p];
+            const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+            total += f * ml.y;
+            alignas(16) float po[PER];
+            if constexpr (PER == 4) *reinterpret_cast<float4*>(po) = reinterpret_cast<const float4*>(parts.o + p * DP)[lane];
+            else *reinterpret_cast<float2*>(po) = reinterpret_cast<const float2*>(parts.o + p * DP)[lane];
+#pragma unroll
+            for (int e = 0; e < PER; ++e) v[e] += f * po[e];
+        }
+        const int64_t tok = s.first + at.z * tile_tokens + r / a.group;
+        const int h = at.y * a.group + r % a.group;
+        const float inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
+        uint16_t* out = a.out + tok * a.os[0] + h * a.os[1] + lane * PER;
+        if (lane * PER < c.dim) {
+#pragma unroll
+            for (int e = 0; e < PER; e += 2) *reinterpret_cast<uint32_t*>(out + e) = pack2<T>(v[e] * inv, v[e + 1] * inv);
+        }
+        if (lane == 0) a.lse[tok * a.heads + h] = (top + log2f(total)) * 0.6931471805599453f;
+    }
+}
+
+// Weights that the rows of the step path gave each slot, from the scores that the step kernel left; one thread per slot.
+template <int R>
+__global__ void __launch_bounds__(256) kv_step_weights_kernel(KvPages c, KvBatch bt, KvAttend a, KvParts parts) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    __shared__ float s_lse[R];
+    const int b = blockIdx.z, head = blockIdx.y;
+    const KvSeq s = kv_seq(c, bt, b);
+    if (!step_takes(s, a.group)) return;
+    const int rows = s.count * a.group;
+    if (threadIdx.x < R) {
+        const int r = threadIdx.x;
+        float x = INFINITY;  // no row, or one that saw nothing: weight 0
+        if (r < rows) {
+            const float v = a.lse[(s.first + r / a.group) * a.heads + head * a.group + r % a.group];
+            x = v == -INFINITY ? INFINITY : v * 1.4426950408889634f;
+        }
+        s_lse[r] = x;
+    }
+    __syncthreads();
+    const int64_t end = min((int64_t)s.len, a.scores_width);
+    for (int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x; j < end; j += (int64_t)gridDim.x * 256) {
+        const float4* sp = reinterpret_cast<const float4*>(parts.s + (((int64_t)b * c.heads + head) * parts.s_slots + j) * R);
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < R / 4; ++i) {
+            const float4 x = __ldg(sp + i);
+            if (4 * i < rows) sum += ex2(x.x - s_lse[4 * i]);
+            if (4 * i + 1 < rows) sum += ex2(x.y - s_lse[4 * i + 1]);
+            if (4 * i + 2 < rows) sum += ex2(x.z - s_lse[4 * i + 2]);
+            if (4 * i + 3 < rows) sum += ex2(x.w - s_lse[4 * i + 3]);
+        }
+        a.scores[b * a.ss[0] + head * a.ss[1] + j] += sum;
+    }
+}
+
+}  // namespace vk

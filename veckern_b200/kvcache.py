@@ -57,6 +57,7 @@ class PagedCache:
                      k_stride=(C.c_int64 * 3)(*k_pages.stride()[:3]), v=v_pages.data_ptr(),
                      v_stride=(C.c_int64 * 3)(*v_pages.stride()[:3]))
         check(lib().vk_kv_create(C.byref(d), C.byref(self._h)), "vk_kv_create")
+        self._workspaces = {}  # bytes by sizes
         # argument structs, filled anew by every call
         self._batch, self._attend, self._evict = N.KvBatch(), N.KvAttend(), N.KvEvict()
         self._batch_ref, self._attend_ref, self._evict_ref = (C.byref(x) for x in
@@ -140,6 +141,16 @@ class PagedCache:
             a.scores_stride[0], a.scores_stride[1] = scores.stride(0), scores.stride(1)
         a.heads, a.max_q, a.causal = heads, max_q, causal
         a.scale = self.head_dim ** -0.5 if scale is None else scale
+        sizes = (n, self._batch.table_width, tokens, heads, max_q, scores is not None)
+        need = self._workspaces.get(sizes)
+        if need is None:
+            size = C.c_size_t()
+            check(lib().vk_kv_attend_workspace(self._h, self._batch_ref, self._attend_ref, C.byref(size)), "attend")
+            if len(self._workspaces) >= 4096:
+                self._workspaces.clear()
+            need = self._workspaces[sizes] = size.value
+        work = torch.empty((need,), dtype=torch.uint8, device=self.device)
+        a.workspace, a.workspace_bytes = work.data_ptr(), need
         check(lib().vk_kv_attend(self._h, self._batch_ref, self._attend_ref, self._stream(stream)), "attend")
         return out, lse
 
