@@ -75,7 +75,7 @@ size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 struct AttendPlan {
     bool step, chunk;
     int rows;  // of the step path: 8 or 16
-    int step_ctas;
+    int step_ctas, chunk_ctas;
     size_t o, ml, at, s, bytes;  // offsets
 };
 
@@ -86,11 +86,15 @@ AttendPlan plan_attend(const vk_kv* kv, const vk::KvBatch& bt, int group, int ma
     p.step = group <= vk::STEP_ROWS && !(bt.batch == 1 && bt.tokens * group > vk::STEP_ROWS);
     p.rows = std::min<int64_t>(rows, vk::STEP_ROWS) <= 8 ? 8 : 16;
     p.step_ctas = 2 * kv->sm_count;
+    p.chunk_ctas = kv->sm_count;
     const int dp = kv->desc.head_dim <= 64 ? 64 : 128;
     const int64_t slots = (int64_t)bt.width << kv->page_shift;
-    const size_t parts = 2 * (size_t)p.step_ctas;
-    p.ml = p.o + align256(parts * vk::STEP_ROWS * dp * sizeof(float));
-    p.at = p.ml + align256(parts * vk::STEP_ROWS * sizeof(float2));
+    // the two paths run one after the other on the stream: they share the parts' room
+    const size_t parts = 2 * (size_t)std::max(p.step ? p.step_ctas : 0, p.chunk ? p.chunk_ctas : 0);
+    const size_t rows_of_parts = std::max(p.step ? 2 * (size_t)p.step_ctas * vk::STEP_ROWS : 0,
+                                          p.chunk ? 2 * (size_t)p.chunk_ctas * vk::CHUNK_PART_ROWS : 0);
+    p.ml = p.o + align256(rows_of_parts * dp * sizeof(float));
+    p.at = p.ml + align256(rows_of_parts * sizeof(float2));
     p.s = p.at + align256(parts * sizeof(int4));
     p.bytes = p.s + (scores && p.step ? align256((size_t)bt.batch * kv->desc.kv_heads * slots * p.rows * sizeof(float)) : 0);
     return p;
@@ -121,7 +125,7 @@ int launch_step_as(const vk_kv* kv, const vk::KvPages& c, const vk::KvBatch& bt,
     VK_TRY_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     fn<<<ctas, vk::STEP_THREADS, smem, st>>>(kv->map_k, kv->map_v, c, bt, a, parts);
     VK_TRY_CUDA(cudaGetLastError());
-    VK_TRY(launch_behind(&vk::kv_join_kernel<T, DP, vk::STEP_ROWS, 16>, dim3(2 * ctas), 512, 0, st, c, bt, a, parts, ctas,
+    VK_TRY(launch_behind(&vk::kv_join_kernel<T, DP, vk::STEP_ROWS, vk::STEP_ROWS, 16>, dim3(2 * ctas), 512, 0, st, c, bt, a, parts, ctas,
                          vk::STEP_ROWS));
     if constexpr (SCORES) {
         const int64_t width = std::min(parts.s_slots, a.scores_width);
@@ -143,6 +147,65 @@ int launch_step(const vk_kv* kv, const vk::KvPages& c, const vk::KvBatch& bt, co
                     : launch_step_as<T, DP, 16, false>(kv, c, bt, a, parts, p.step_ctas, st);
 }
 
+int encoder(PFN_cuTensorMapEncodeTiled_v12000* out) {
+    static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+    if (!encode) {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        VK_TRY_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found));
+        if (!fn || found != cudaDriverEntryPointSuccess)
+            return fail(VK_ERR_UNSUPPORTED, "the driver has no cuTensorMapEncodeTiled");
+        encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    }
+    *out = encode;
+    return VK_OK;
+}
+
+// The tensor map of the keys' or values' pages: (element, slot, head, page), boxes of 64 elements of up to 64 slots.
+int encode_map(const vk_kv_desc_t& d, void* base, const int64_t* stride, CUtensorMap* map) {
+    PFN_cuTensorMapEncodeTiled_v12000 encode;
+    VK_TRY(encoder(&encode));
+    const cuuint64_t dims[4] = {(cuuint64_t)d.head_dim, (cuuint64_t)d.page_size, (cuuint64_t)d.kv_heads,
+                                (cuuint64_t)d.pages};
+    // a dimension of one entry is never stepped along: any valid stride does
+    const cuuint64_t strides[3] = {(cuuint64_t)stride[1] * 2, d.kv_heads > 1 ? (cuuint64_t)stride[2] * 2 : 16,
+                                   d.pages > 1 ? (cuuint64_t)stride[0] * 2 : 16};
+    const cuuint32_t box[4] = {64, (cuuint32_t)std::min(d.page_size, vk::STEP_TILE), 1, 1}, step[4] = {1, 1, 1, 1};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, base, dims, strides, box, step,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(VK_ERR_INVALID, "the pages' sizes and strides do not make a tensor map (%d)", (int)r);
+    return VK_OK;
+}
+
+// The tensor map of a chunk's query rows: (element, head, token), boxes of one row tile's tokens and kv head.
+int encode_rows(const vk::KvAttend& a, int dim, int64_t tokens, CUtensorMap* map) {
+    PFN_cuTensorMapEncodeTiled_v12000 encode;
+    VK_TRY(encoder(&encode));
+    const cuuint64_t dims[3] = {(cuuint64_t)dim, (cuuint64_t)a.heads, (cuuint64_t)tokens};
+    const cuuint64_t strides[2] = {a.heads > 1 ? (cuuint64_t)a.qs[1] * 2 : 16, tokens > 1 ? (cuuint64_t)a.qs[0] * 2 : 16};
+    const cuuint32_t box[3] = {64, (cuuint32_t)a.group, (cuuint32_t)(vk::CHUNK_ROWS / a.group)}, step[3] = {1, 1, 1};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 3, const_cast<uint16_t*>(a.q), dims, strides, box, step,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(VK_ERR_INVALID, "q's sizes and strides do not make a tensor map (%d)", (int)r);
+    return VK_OK;
+}
+
+template <typename T, int DP>
+int launch_chunk(const vk_kv* kv, const vk::KvPages& c, const vk::KvBatch& bt, const vk::KvAttend& a,
+                 const vk::KvParts& parts, const AttendPlan& p, cudaStream_t st) {
+    CUtensorMap map_q;
+    VK_TRY(encode_rows(a, c.dim, bt.tokens, &map_q));
+    const auto fn = &vk::kv_chunk_kernel<T, DP>;
+    constexpr int smem = vk::chunk_smem<DP>();
+    VK_TRY_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    fn<<<p.chunk_ctas, vk::CHUNK_THREADS, smem, st>>>(map_q, kv->map_k, kv->map_v, c, bt, a, parts);
+    VK_TRY_CUDA(cudaGetLastError());
+    return launch_behind(&vk::kv_join_kernel<T, DP, vk::CHUNK_PART_ROWS, vk::CHUNK_ROWS, 16>, dim3(2 * p.chunk_ctas, 4), 512,
+                         0, st, c, bt, a, parts, p.chunk_ctas, vk::CHUNK_ROWS / a.group);
+}
+
 template <typename T>
 int launch_attend(const vk_kv* kv, const vk::KvBatch& bt, const vk::KvAttend& a, void* workspace, const AttendPlan& p,
                   cudaStream_t st) {
@@ -157,38 +220,14 @@ int launch_attend(const vk_kv* kv, const vk::KvBatch& bt, const vk::KvAttend& a,
     if (p.step) VK_TRY((c.dim <= 64 ? launch_step<T, 64>(kv, c, bt, a, parts, p, st)
                                     : launch_step<T, 128>(kv, c, bt, a, parts, p, st)));
     if (p.chunk) {
-        vk::kv_attend_kernel<T><<<dim3((unsigned)bt.tokens, a.heads), 32 * vk::ROW_WARPS, 0, st>>>(c, bt, a);
-        VK_TRY_CUDA(cudaGetLastError());
+        VK_TRY((c.dim <= 64 ? launch_chunk<T, 64>(kv, c, bt, a, parts, p, st)
+                            : launch_chunk<T, 128>(kv, c, bt, a, parts, p, st)));
         const int64_t slots = (int64_t)bt.width << c.page_shift;
         if (a.scores && slots > 0) {
             vk::kv_weights_kernel<T><<<dim3((unsigned)ceil_div(slots, 8), c.heads, bt.batch), 256, 0, st>>>(c, bt, a);
             VK_TRY_CUDA(cudaGetLastError());
         }
     }
-    return VK_OK;
-}
-
-// The tensor map of the keys' or values' pages: (element, slot, head, page), boxes of 64 elements of up to 64 slots.
-int encode_map(const vk_kv_desc_t& d, void* base, const int64_t* stride, CUtensorMap* map) {
-    static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
-    if (!encode) {
-        void* fn = nullptr;
-        cudaDriverEntryPointQueryResult found;
-        VK_TRY_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found));
-        if (!fn || found != cudaDriverEntryPointSuccess)
-            return fail(VK_ERR_UNSUPPORTED, "the driver has no cuTensorMapEncodeTiled");
-        encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-    }
-    const cuuint64_t dims[4] = {(cuuint64_t)d.head_dim, (cuuint64_t)d.page_size, (cuuint64_t)d.kv_heads,
-                                (cuuint64_t)d.pages};
-    // a dimension of one entry is never stepped along: any valid stride does
-    const cuuint64_t strides[3] = {(cuuint64_t)stride[1] * 2, d.kv_heads > 1 ? (cuuint64_t)stride[2] * 2 : 16,
-                                   d.pages > 1 ? (cuuint64_t)stride[0] * 2 : 16};
-    const cuuint32_t box[4] = {64, (cuuint32_t)std::min(d.page_size, vk::STEP_TILE), 1, 1}, step[4] = {1, 1, 1, 1};
-    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, base, dims, strides, box, step,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return fail(VK_ERR_INVALID, "the pages' sizes and strides do not make a tensor map (%d)", (int)r);
     return VK_OK;
 }
 

@@ -410,8 +410,9 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
 }
 
 // Adds up the parts of split (sequence, kv head, row tile)s. Block x starts at part x if that is a first one; the others
-// of it are the first parts of the CTAs that follow. One warp per row.
-template <typename T, int DP, int ROWS, int WARPS>
+// of it are the first parts of the CTAs that follow. One warp per row; a part's rows are tiles of TILE rows, of
+// tile_tokens tokens each.
+template <typename T, int DP, int ROWS, int TILE, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS) kv_join_kernel(KvPages c, KvBatch bt, KvAttend a, KvParts parts, int ctas,
                                                              int tile_tokens) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -436,9 +437,9 @@ __global__ void __launch_bounds__(32 * WARPS) kv_join_kernel(KvPages c, KvBatch 
     }
     auto part_of = [&](int i) -> int64_t { return i == 0 ? (int64_t)blockIdx.x : 2 * (int64_t)(cta + i); };
     const int n = last - cta + 1;
-    const int rows = min(ROWS, (s.count - at.z * tile_tokens) * a.group);
-    const int used = tile_tokens * a.group;
-    for (int r = blockIdx.y * WARPS + (threadIdx.x >> 5); r < min(rows, used); r += WARPS * gridDim.y) {
+    for (int r = blockIdx.y * WARPS + (threadIdx.x >> 5); r < ROWS; r += WARPS * gridDim.y) {
+        const int in = r % TILE, token = (at.z * (ROWS / TILE) + r / TILE) * tile_tokens + in / a.group;
+        if (in >= tile_tokens * a.group || token >= s.count) continue;
         float top = -INFINITY;
         for (int i = lane; i < n; i += 32) top = fmaxf(top, parts.ml[part_of(i) * ROWS + r].x);
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
@@ -457,8 +458,8 @@ __global__ void __launch_bounds__(32 * WARPS) kv_join_kernel(KvPages c, KvBatch 
 #pragma unroll
             for (int e = 0; e < PER; ++e) v[e] += f * po[e];
         }
-        const int64_t tok = s.first + at.z * tile_tokens + r / a.group;
-        const int h = at.y * a.group + r % a.group;
+        const int64_t tok = s.first + token;
+        const int h = at.y * a.group + in % a.group;
         const float inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
         uint16_t* out = a.out + tok * a.os[0] + h * a.os[1] + lane * PER;
         if (lane * PER < c.dim) {
