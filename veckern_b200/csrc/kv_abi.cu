@@ -4,8 +4,8 @@
 
 #include <cudaTypedefs.h>
 
-#include "kv_attend.cuh"
 #include "kv_move.cuh"
+#include "kv_weights.cuh"
 #include "status.h"
 
 struct vk_kv {
@@ -202,8 +202,15 @@ int launch_chunk(const vk_kv* kv, const vk::KvPages& c, const vk::KvBatch& bt, c
     VK_TRY_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     fn<<<p.chunk_ctas, vk::CHUNK_THREADS, smem, st>>>(map_q, kv->map_k, kv->map_v, c, bt, a, parts);
     VK_TRY_CUDA(cudaGetLastError());
-    return launch_behind(&vk::kv_join_kernel<T, DP, vk::CHUNK_PART_ROWS, vk::CHUNK_ROWS, 16>, dim3(2 * p.chunk_ctas, 4), 512,
-                         0, st, c, bt, a, parts, p.chunk_ctas, vk::CHUNK_ROWS / a.group);
+    VK_TRY(launch_behind(&vk::kv_join_kernel<T, DP, vk::CHUNK_PART_ROWS, vk::CHUNK_ROWS, 16>, dim3(2 * p.chunk_ctas, 4), 512,
+                         0, st, c, bt, a, parts, p.chunk_ctas, vk::CHUNK_ROWS / a.group));
+    if (!a.scores || a.scores_width == 0) return VK_OK;
+    const auto weights = &vk::kv_weights_kernel<T, DP>;
+    constexpr int weights_smem = vk::weights_smem<DP>();
+    VK_TRY_CUDA(cudaFuncSetAttribute(weights, cudaFuncAttributeMaxDynamicSharedMemorySize, weights_smem));
+    VK_TRY(launch_behind(weights, dim3(p.chunk_ctas), vk::CHUNK_THREADS, weights_smem, st, map_q, kv->map_k, c, bt, a, parts));
+    return launch_behind(&vk::kv_weights_join_kernel, dim3(2 * p.chunk_ctas), vk::WEIGHTS_PAIR, 0, st, c, bt, a, parts,
+                         p.chunk_ctas);
 }
 
 template <typename T>
@@ -222,11 +229,6 @@ int launch_attend(const vk_kv* kv, const vk::KvBatch& bt, const vk::KvAttend& a,
     if (p.chunk) {
         VK_TRY((c.dim <= 64 ? launch_chunk<T, 64>(kv, c, bt, a, parts, p, st)
                             : launch_chunk<T, 128>(kv, c, bt, a, parts, p, st)));
-        const int64_t slots = (int64_t)bt.width << c.page_shift;
-        if (a.scores && slots > 0) {
-            vk::kv_weights_kernel<T><<<dim3((unsigned)ceil_div(slots, 8), c.heads, bt.batch), 256, 0, st>>>(c, bt, a);
-            VK_TRY_CUDA(cudaGetLastError());
-        }
     }
     return VK_OK;
 }

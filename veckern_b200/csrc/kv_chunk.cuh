@@ -34,6 +34,15 @@ constexpr int chunk_smem() {
     return CHUNK_Q<DP> + CHUNK_RING<DP> * CHUNK_SLOT<DP> + 512;
 }
 
+// A row tile's box of the queries (64 elements of a kv head's query heads, for a tile's tokens) into shared memory.
+__device__ __forceinline__ void tma_rows(void* dst, const CUtensorMap* map, int d, int head, int token, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(d), "r"(head), "r"(token), "r"(smem_u32(bar))
+        : "memory");
+}
+
 // ---- tcgen05
 __device__ __forceinline__ uint64_t umma_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
     // 128-byte swizzle (2 << 61), descriptor version 1; byte offsets in units of 16
@@ -255,12 +264,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                     mbar_arrive_expect_tx(q_full, n * HALVES * shape.tokens * a.group * 128);
                     for (int i = 0; i < n; ++i)
                         for (int h = 0; h < HALVES; ++h)
-                            asm volatile(
-                                "cp.async.bulk.tensor.3d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
-                                "%4}], [%5];" ::"r"(smem_u32(smem_q + (i * HALVES + h) * (CHUNK_ROWS * 128))),
-                                "l"(&map_q), "r"(h * 64), "r"(g.head * a.group),
-                                "r"((int)g.s.first + g.token0 + i * shape.tokens), "r"(smem_u32(q_full))
-                                : "memory");
+                            tma_rows(smem_q + (i * HALVES + h) * (CHUNK_ROWS * 128), &map_q, h * 64, g.head * a.group,
+                                     (int)g.s.first + g.token0 + i * shape.tokens, q_full);
                 }
                 q_phase ^= 1;
                 const int32_t* table = bt.table + g.b * bt.table_stride;

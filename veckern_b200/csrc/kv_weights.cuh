@@ -1,0 +1,341 @@
+// Weights that the rows of a chunk gave each slot: scores[slot] += sum over rows of exp(s - lse of the row).
+//
+// The attention kernel cannot add them up itself, since a row's total is only known at its end; what it would have to
+// keep (rows x slots) is larger than what it takes to compute the products again. Here the slots are the accumulator's
+// lanes: S^T = K Q^T puts a slot's products with 128 rows into one thread's columns, so that its weights are summed in
+// registers, without a shuffle or an atomic, and every row's lse is read by all threads alike from shared memory.
+//
+// A unit is a pair of slot tiles (2 x 128, one per warpgroup) against one row tile. Units run row tile by row tile within
+// a pair, the pair's keys stay in shared memory and the rows stream; the units of all (sequence, kv head, pair)s are laid
+// end to end and shared out equally. A pair that is cut leaves parts, added up in order by kv_weights_join_kernel.
+//
+// Bound: one exponential per (row, slot), 16 a clock and SM on the special function units (1,024 cycles per 128 x 128
+// tile against 512 for its product at a head size of 128).
+#pragma once
+#include "kv_chunk.cuh"
+
+namespace vk {
+
+constexpr int WEIGHTS_PAIR = 2 * CHUNK_SLOTS;  // slots of a pair
+template <int DP>
+constexpr int WEIGHTS_RING = 4;  // row tiles in flight
+template <int DP>
+constexpr int weights_smem() {
+    return (2 + WEIGHTS_RING<DP>) * CHUNK_SLOT<DP> + 2 * 2 * 128 * 4 + 512;
+}
+
+struct WeightsShape {
+    int group, causal;
+    int tokens;  // of a row tile
+    int64_t width;
+    __device__ __forceinline__ bool takes(const KvSeq& s) const {
+        return s.count > 0 && s.len > 0 && !step_takes(s, group);
+    }
+    __device__ __forceinline__ int pairs(const KvSeq& s) const {
+        return (int)((min((int64_t)s.len, width) + WEIGHTS_PAIR - 1) / WEIGHTS_PAIR);
+    }
+    __device__ __forceinline__ int row_tiles(const KvSeq& s) const { return (s.count + tokens - 1) / tokens; }
+    // the first row tile with a row that sees the pair's first slot
+    __device__ __forceinline__ int first(const KvSeq& s, int pair) const {
+        const int64_t x = (int64_t)pair * WEIGHTS_PAIR - (s.len - s.count);
+        return causal && x > 0 ? (int)(x / tokens) : 0;
+    }
+    // units of the pairs before `pair`
+    __device__ __forceinline__ int64_t before(const KvSeq& s, int pair) const {
+        int64_t sum = (int64_t)pair * row_tiles(s);
+        if (causal) {
+            const int64_t a = (int64_t)s.len - s.count;
+            const int64_t p0 = a < 0 ? 0 : min((int64_t)pair, (a + WEIGHTS_PAIR - 1) / WEIGHTS_PAIR);
+            sum -= floor_sum(pair - p0, tokens, WEIGHTS_PAIR, p0 * WEIGHTS_PAIR - a);
+        }
+        return sum;
+    }
+};
+
+// A CTA's next segment: consecutive row tiles of one (sequence, kv head, pair).
+struct WeightsSegment {
+    KvSeq s;
+    int b, head, pair, q0, count;
+    bool whole_from, whole_to;  // begins at the pair's first unit; ends at its last
+    bool both;                  // the second tile has slots
+};
+struct WeightsWalk {
+    const KvPages& c;
+    const KvBatch& bt;
+    const WeightsShape& shape;
+    KvShare share;
+    int head, pair, skip;
+    bool located;
+    __device__ __forceinline__ bool next(WeightsSegment* g) {
+        if (share.left <= 0) return false;
+        KvSeq s = kv_seq(c, bt, share.b);
+        while (!shape.takes(s) || head >= c.heads) {
+            s = kv_seq(c, bt, ++share.b);
+            head = pair = skip = 0;
+        }
+        const int all = shape.pairs(s);
+        if (!located) {
+            const int64_t per = shape.before(s, all);
+            head = (int)(share.off / per);
+            const int64_t off = share.off % per;
+            int lo = 0, hi = all - 1;
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (shape.before(s, mid) <= off) lo = mid;
+                else hi = mid - 1;
+            }
+            pair = lo;
+            skip = (int)(off - shape.before(s, lo));
+            located = true;
+        }
+        const int tiles = shape.row_tiles(s) - shape.first(s, pair);
+        g->s = s;
+        g->b = share.b;
+        g->head = head;
+        g->pair = pair;
+        g->q0 = shape.first(s, pair) + skip;
+        g->count = (int)min((int64_t)(tiles - skip), share.left);
+        g->whole_from = skip == 0;
+        g->whole_to = skip + g->count == tiles;
+        g->both = min((int64_t)s.len, shape.width) > (int64_t)pair * WEIGHTS_PAIR + CHUNK_SLOTS;
+        share.left -= g->count;
+        skip = 0;
+        if (++pair == all) pair = 0, ++head;
+        return true;
+    }
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(CHUNK_THREADS, 1)
+    kv_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, KvPages c,
+                      KvBatch bt, KvAttend a, KvParts parts) {
+    constexpr int HALVES = DP / 64, KS = DP / 16, RING = WEIGHTS_RING<DP>, SLOT = CHUNK_SLOT<DP>;
+    extern __shared__ __align__(1024) uint8_t ring[];  // the swizzle goes by address bits: 1024-byte aligned
+    uint8_t* smem_k = ring + RING * SLOT;              // the pair's two tiles
+    float* s_lse = reinterpret_cast<float*>(smem_k + 2 * SLOT);  // [warpgroup][2][128]
+    uint64_t* q_full = reinterpret_cast<uint64_t*>(s_lse + 2 * 2 * 128);
+    uint64_t* q_empty = q_full + RING;
+    uint64_t* k_full = q_empty + RING;
+    uint64_t* k_empty = k_full + 1;
+    uint64_t* s_full = k_empty + 1;  // [warpgroup][2]
+    uint64_t* s_empty = s_full + 4;
+    int64_t* scratch = reinterpret_cast<int64_t*>(s_empty + 4);
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(scratch + CHUNK_THREADS / 32 + 2);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < RING; ++i) {
+            mbar_init(q_full + i, 1);
+            mbar_init(q_empty + i, 1);
+        }
+        mbar_init(k_full, 1);
+        mbar_init(k_empty, 1);
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(s_full + i, 1);
+            mbar_init(s_empty + i, 128);
+        }
+        fence_mbar_init();
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_at))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // query rows past a tile's tokens are never loaded: their products must not be NaN
+    for (int i = threadIdx.x; i < RING * SLOT / 16; i += CHUNK_THREADS)
+        reinterpret_cast<uint4*>(ring)[i] = make_uint4(0u, 0u, 0u, 0u);
+    fence_proxy_async_smem();
+    tmem_fence_before();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const WeightsShape shape{a.group, a.causal, CHUNK_ROWS / a.group, a.scores_width};
+    KvShare share = kv_share<CHUNK_THREADS>(c, bt, scratch, [&](const KvSeq& s) -> int64_t {
+        return shape.takes(s) ? shape.before(s, shape.pairs(s)) * c.heads : 0;
+    });
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (threadIdx.x < 2) parts.at[2 * blockIdx.x + threadIdx.x].w = PART_NONE;
+    __syncthreads();
+    tmem_fence_after();
+    const uint32_t tm = *tmem_at;
+    KvWait wait{c.status};
+    WeightsWalk walk{c, bt, shape, share, 0, 0, 0, false};
+    WeightsSegment g;
+    if (warp == 9) {
+        int slot = 0, loaded = 0;
+        uint32_t phase = 0, k_phase = 0;
+        const int box_shift = min(c.page_shift, 6), boxes = CHUNK_SLOTS >> box_shift;
+        while (walk.next(&g)) {
+            const int32_t* table = bt.table + g.b * bt.table_stride;
+            const int i = lane % boxes, half = lane / boxes;
+            wait(k_empty, k_phase ^ 1);
+            int pages[2];
+            int n = 0;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int at = g.pair * WEIGHTS_PAIR + u * CHUNK_SLOTS + (i << box_shift);
+                const bool live = half < HALVES && at < g.s.len && (u == 0 || g.both);
+                pages[u] = -1;
+                if (live) {
+                    pages[u] = (int)kv_page(c, table, at);
+                    if (pages[u] < 0) pages[u] = (int)c.pages;  // past the map: reads as zero
+                }
+                n += __popc(__ballot_sync(FULL, live));
+            }
+            if (lane == 0) mbar_arrive_expect_tx(k_full, n * (128 << box_shift));
+            __syncwarp();
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+                if (pages[u] >= 0)
+                    tma_page(smem_k + u * SLOT + half * (CHUNK_SLOTS * 128) + (i << box_shift) * 128, &map_k, half * 64,
+                             (u * CHUNK_SLOTS + (i << box_shift) + g.pair * WEIGHTS_PAIR) & ((1 << c.page_shift) - 1), g.head,
+                             pages[u], k_full);
+            k_phase ^= 1;
+            for (int q = g.q0; q < g.q0 + g.count; ++q) {
+                wait(q_empty + slot, phase ^ 1);
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(q_full + slot, HALVES * shape.tokens * a.group * 128);
+                    for (int h = 0; h < HALVES; ++h)
+                        tma_rows(ring + slot * SLOT + h * (CHUNK_ROWS * 128), &map_q, h * 64, g.head * a.group,
+                                 (int)g.s.first + q * shape.tokens, q_full + slot);
+                }
+                __syncwarp();
+                ++loaded;
+                if (++slot == RING) slot = 0, phase ^= 1;
+            }
+        }
+        // A wait that ran out may have left copies in flight into this CTA's memory: see them land before it ends.
+        if (wait.dead && lane == 0) {
+            for (int i = 0; i < RING; ++i) {
+                const int fills = loaded / RING + (i < loaded % RING);
+                if (fills && !mbar_wait_bounded(q_full + i, (fills - 1) & 1, 2 * KV_WAIT_BUDGET))
+                    atomicOr(c.status, ERR_DRAIN_TIMEOUT);
+            }
+            if (loaded && !mbar_wait_bounded(k_full, k_phase ^ 1, 2 * KV_WAIT_BUDGET)) atomicOr(c.status, ERR_DRAIN_TIMEOUT);
+        }
+    } else if (warp == 8) {
+        const uint32_t idesc = umma_idesc<T>(CHUNK_ROWS, false, a.scale < 0.f);
+        int slot = 0, buf = 0;
+        uint32_t phase = 0, k_phase = 0, buf_phase[2] = {0, 0};  // of the first or second warpgroup's buffers
+        int used[2] = {0, 0};
+        while (walk.next(&g)) {
+            wait(k_full, k_phase);
+            k_phase ^= 1;
+            for (int q = 0; q < g.count; ++q) {
+                wait(q_full + slot, phase);
+                for (int i = 0; i < (g.both ? 2 : 1); ++i) {
+                    buf = used[i] & 1;
+                    buf_phase[i] = (used[i] >> 1) & 1;
+                    ++used[i];
+                    wait(s_empty + 2 * i + buf, buf_phase[i] ^ 1);
+                    tmem_fence_after();
+                    if (lane == 0) {
+                        const uint32_t k = smem_u32(smem_k) + i * SLOT, rows = smem_u32(ring) + slot * SLOT;
+#pragma unroll
+                        for (int e = 0; e < KS; ++e) {
+                            const uint32_t off = (e >> 2) * (CHUNK_ROWS * 128) + (e & 3) * 32;
+                            umma_ss(tm + (2 * i + buf) * 128, umma_desc(k + off, 16, 1024), umma_desc(rows + off, 16, 1024),
+                                    idesc, e > 0);
+                        }
+                        umma_commit(s_full + 2 * i + buf);
+                    }
+                    __syncwarp();
+                }
+                if (lane == 0) umma_commit(q_empty + slot);
+                __syncwarp();
+                if (++slot == RING) slot = 0, phase ^= 1;
+            }
+            if (lane == 0) umma_commit(k_empty);
+            __syncwarp();
+        }
+    } else if (warp < 8) {
+        const int i = warp >> 2, r = (warp & 3) * 32 + lane;
+        const uint32_t lanes = tm + ((uint32_t)((warp & 3) * 32) << 16) + i * 256;
+        float* lse = s_lse + i * 256;
+        const float scale = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-37f);
+        int used = 0;
+        bool first_segment = true;
+        while (walk.next(&g)) {
+            if (i == 0 || g.both) {
+                const int j = g.pair * WEIGHTS_PAIR + i * CHUNK_SLOTS + r;
+                // row r of tile q: its token and head, and its lse in base 2; no row, or one that saw nothing, has weight 0
+                auto lse_of = [&](int q) {
+                    const int token = q * shape.tokens + r / a.group;
+                    if (r >= shape.tokens * a.group || token >= g.s.count) return INFINITY;
+                    const float v = __ldg(a.lse + (g.s.first + token) * a.heads + g.head * a.group + r % a.group);
+                    return v == -INFINITY ? INFINITY : v * 1.4426950408889634f;
+                };
+                float sum = 0.f, next = lse_of(g.q0);
+                for (int q = g.q0; q < g.q0 + g.count; ++q) {
+                    const int buf = used & 1;
+                    const uint32_t phase = (used >> 1) & 1;
+                    ++used;
+                    lse[buf * 128 + r] = next;
+                    if (q + 1 < g.q0 + g.count) next = lse_of(q + 1);
+                    asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+                    wait(s_full + 2 * i + buf, phase);
+                    tmem_fence_after();
+                    float x[CHUNK_ROWS];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) tmem_ld32(lanes + buf * 128 + 32 * e, x + 32 * e);
+                    tmem_wait_ld();
+                    tmem_fence_before();
+                    mbar_arrive(s_empty + 2 * i + buf);
+                    // rows that see this slot: from `from` on; the tile's rows end at `to`
+                    const int to = min(shape.tokens, g.s.count - q * shape.tokens) * a.group;
+                    const int from = a.causal ? max(0, j - (g.s.len - g.s.count) - q * shape.tokens) * a.group : 0;
+                    if (__any_sync(FULL, from > 0) || to < shape.tokens * a.group) {
+#pragma unroll
+                        for (int e = 0; e < CHUNK_ROWS; ++e) x[e] = e >= from && e < to ? x[e] : -INFINITY;
+                    }
+                    float part[4] = {0.f, 0.f, 0.f, 0.f};
+                    const float4* l4 = reinterpret_cast<const float4*>(lse + buf * 128);
+#pragma unroll
+                    for (int e = 0; e < CHUNK_ROWS / 4; ++e) {
+                        const float4 y = l4[e];
+                        part[0] += ex2(fmaf(x[4 * e], scale, -y.x));
+                        part[1] += ex2(fmaf(x[4 * e + 1], scale, -y.y));
+                        part[2] += ex2(fmaf(x[4 * e + 2], scale, -y.z));
+                        part[3] += ex2(fmaf(x[4 * e + 3], scale, -y.w));
+                    }
+                    sum += (part[0] + part[1]) + (part[2] + part[3]);
+                }
+                if (j < min((int64_t)g.s.len, a.scores_width)) {
+                    if (g.whole_from && g.whole_to) {
+                        a.scores[g.b * a.ss[0] + g.head * a.ss[1] + j] += sum;
+                    } else {
+                        const int part = 2 * blockIdx.x + (first_segment ? 0 : 1);
+                        parts.o[(int64_t)part * WEIGHTS_PAIR + i * CHUNK_SLOTS + r] = sum;
+                    }
+                }
+                if (threadIdx.x == 0 && !(g.whole_from && g.whole_to))
+                    parts.at[2 * blockIdx.x + (first_segment ? 0 : 1)] =
+                        make_int4(g.b, g.head, g.pair,
+                                  PART_HELD | (g.whole_from ? PART_FIRST : 0) | (g.whole_to ? PART_LAST : 0));
+            }
+            first_segment = false;
+        }
+    }
+    __syncthreads();
+    if (warp == 8) {
+        tmem_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm) : "memory");
+    }
+}
+
+// Adds up the parts of cut pairs, one thread per slot; as kv_join_kernel.
+__global__ void __launch_bounds__(WEIGHTS_PAIR) kv_weights_join_kernel(KvPages c, KvBatch bt, KvAttend a, KvParts parts,
+                                                                       int ctas) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int4 at = parts.at[blockIdx.x];
+    if (!(at.w & PART_FIRST)) return;
+    const KvSeq s = kv_seq(c, bt, at.x);
+    const int64_t j = (int64_t)at.z * WEIGHTS_PAIR + threadIdx.x;
+    if (j >= s.len || j >= a.scores_width) return;
+    float sum = parts.o[(int64_t)blockIdx.x * WEIGHTS_PAIR + threadIdx.x];
+    bool last = at.w & PART_LAST;
+    for (int cta = blockIdx.x / 2 + 1; !last && cta < ctas; ++cta) {
+        last = parts.at[2 * cta].w & PART_LAST;
+        sum += parts.o[(int64_t)2 * cta * WEIGHTS_PAIR + threadIdx.x];
+    }
+    a.scores[at.x * a.ss[0] + at.y * a.ss[1] + j] += sum;
+}
+
+}  // namespace vk
