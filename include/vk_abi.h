@@ -379,10 +379,12 @@ typedef struct {
     int max_q; /* at least the largest number of new tokens of a sequence; 0 = unknown (`tokens` is assumed) */
     int causal;
     float scale;
-    void* workspace; /* DEVICE, 256-byte aligned, at least vk_kv_attend_workspace bytes; free again when the call's work
-                        on the stream is done, its contents are nothing that a later call needs */
+    void* workspace; /* DEVICE, 256-byte aligned, at least vk_kv_attend_workspace bytes, for one call at a time (the
+                        calls of one stream may share it, of several caches too). Its first VK_KV_WORKSPACE_ZEROED
+                        bytes have to be zero; a call leaves them zero, unless vk_kv_sync reports VK_ERR_DEVICE */
     size_t workspace_bytes;
 } vk_kv_attend_t;
+#define VK_KV_WORKSPACE_ZEROED 8192
 /* Bytes of working memory that vk_kv_attend needs for these sizes (pointers in batch and args are not read, except
  * whether args->scores is NULL). */
 int vk_kv_attend_workspace(const vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_attend_t* args, size_t* bytes);

@@ -76,7 +76,7 @@ struct AttendPlan {
     bool step, chunk;
     int rows;  // of the step path: 8 or 16
     int step_ctas, chunk_ctas;
-    size_t o, ml, at, s, bytes;  // offsets
+    size_t ready, o, ml, s, bytes;  // offsets
 };
 
 AttendPlan plan_attend(const vk_kv* kv, const vk::KvBatch& bt, int group, int max_q, bool scores) {
@@ -89,13 +89,13 @@ AttendPlan plan_attend(const vk_kv* kv, const vk::KvBatch& bt, int group, int ma
     p.chunk_ctas = kv->sm_count;
     const int dp = kv->desc.head_dim <= 64 ? 64 : 128;
     const int64_t slots = (int64_t)bt.width << kv->page_shift;
-    // the two paths run one after the other on the stream: they share the parts' room
-    const size_t parts = 2 * (size_t)std::max(p.step ? p.step_ctas : 0, p.chunk ? p.chunk_ctas : 0);
-    const size_t rows_of_parts = std::max(p.step ? 2 * (size_t)p.step_ctas * vk::STEP_ROWS : 0,
-                                          p.chunk ? 2 * (size_t)p.chunk_ctas * vk::CHUNK_PART_ROWS : 0);
+    // The two paths run one after the other on the stream: they share the parts' room. What has to be zero before a call
+    // lies at the start, whatever the sizes.
+    const size_t rows_of_parts = std::max(p.step ? (size_t)p.step_ctas * vk::STEP_ROWS : 0,
+                                          p.chunk ? 2 * (size_t)p.chunk_ctas * vk::CHUNK_ROWS : 0);
+    p.o = VK_KV_WORKSPACE_ZEROED;
     p.ml = p.o + align256(rows_of_parts * dp * sizeof(float));
-    p.at = p.ml + align256(rows_of_parts * sizeof(float2));
-    p.s = p.at + align256(parts * sizeof(int4));
+    p.s = p.ml + align256(rows_of_parts * sizeof(float2));
     p.bytes = p.s + (scores && p.step ? align256((size_t)bt.batch * kv->desc.kv_heads * slots * p.rows * sizeof(float)) : 0);
     return p;
 }
@@ -125,8 +125,6 @@ int launch_step_as(const vk_kv* kv, const vk::KvPages& c, const vk::KvBatch& bt,
     VK_TRY_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     fn<<<ctas, vk::STEP_THREADS, smem, st>>>(kv->map_k, kv->map_v, c, bt, a, parts);
     VK_TRY_CUDA(cudaGetLastError());
-    VK_TRY(launch_behind(&vk::kv_join_kernel<T, DP, vk::STEP_ROWS, vk::STEP_ROWS, 16>, dim3(2 * ctas), 512, 0, st, c, bt, a, parts, ctas,
-                         vk::STEP_ROWS));
     if constexpr (SCORES) {
         const int64_t width = std::min(parts.s_slots, a.scores_width);
         if (width > 0)
@@ -202,15 +200,11 @@ int launch_chunk(const vk_kv* kv, const vk::KvPages& c, const vk::KvBatch& bt, c
     VK_TRY_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     fn<<<p.chunk_ctas, vk::CHUNK_THREADS, smem, st>>>(map_q, kv->map_k, kv->map_v, c, bt, a, parts);
     VK_TRY_CUDA(cudaGetLastError());
-    VK_TRY(launch_behind(&vk::kv_join_kernel<T, DP, vk::CHUNK_PART_ROWS, vk::CHUNK_ROWS, 16>, dim3(2 * p.chunk_ctas, 4), 512,
-                         0, st, c, bt, a, parts, p.chunk_ctas, vk::CHUNK_ROWS / a.group));
     if (!a.scores || a.scores_width == 0) return VK_OK;
     const auto weights = &vk::kv_weights_kernel<T, DP>;
     constexpr int weights_smem = vk::weights_smem<DP>();
     VK_TRY_CUDA(cudaFuncSetAttribute(weights, cudaFuncAttributeMaxDynamicSharedMemorySize, weights_smem));
-    VK_TRY(launch_behind(weights, dim3(p.chunk_ctas), vk::CHUNK_THREADS, weights_smem, st, map_q, kv->map_k, c, bt, a, parts));
-    return launch_behind(&vk::kv_weights_join_kernel, dim3(2 * p.chunk_ctas), vk::WEIGHTS_PAIR, 0, st, c, bt, a, parts,
-                         p.chunk_ctas);
+    return launch_behind(weights, dim3(p.chunk_ctas), vk::CHUNK_THREADS, weights_smem, st, map_q, kv->map_k, c, bt, a, parts);
 }
 
 template <typename T>
@@ -219,9 +213,9 @@ int launch_attend(const vk_kv* kv, const vk::KvBatch& bt, const vk::KvAttend& a,
     const vk::KvPages c = pages_of(kv);
     uint8_t* w = static_cast<uint8_t*>(workspace);
     vk::KvParts parts{};
+    parts.ready = reinterpret_cast<uint32_t*>(w + p.ready);
     parts.o = reinterpret_cast<float*>(w + p.o);
     parts.ml = reinterpret_cast<float2*>(w + p.ml);
-    parts.at = reinterpret_cast<int4*>(w + p.at);
     parts.s = reinterpret_cast<float*>(w + p.s);
     parts.s_slots = (int64_t)bt.width << kv->page_shift;
     if (p.step) VK_TRY((c.dim <= 64 ? launch_step<T, 64>(kv, c, bt, a, parts, p, st)

@@ -1,19 +1,20 @@
 // Attention of a chunk of new tokens over the paged cache on the 5th-generation tensor cores.
 //
 // A kv head's rows (tokens x its query heads, token by token) come in tiles of 128, the tensor memory's lanes: with 5
-// query heads to a kv head a tile holds 25 tokens, 125 rows. A unit of work is a pair of row tiles against 128 slots; the
-// units of all (sequence, kv head, pair)s are laid end to end and every CTA takes an equal share, so that neither the
-// causal mask nor ragged lengths nor few rows over a long cache leave SMs idle; cut pairs are joined from parts
-// (kv_join_kernel).
+// query heads to a kv head a tile holds 25 tokens, 125 rows. A unit of work is a pair of row tiles against 128 slots or,
+// where a sequence's last pair has one tile only, that tile against 2 x 128 slots; the units of all (sequence, kv head,
+// pair)s are laid end to end and every CTA takes an equal share, so that neither the causal mask nor ragged lengths nor
+// few rows over a long cache leave SMs idle; cut pairs are finished from parts as in the step kernel.
 //
-// Per unit and row tile: scores S = Q K^T (tcgen05.mma, both operands in shared memory) into tensor memory; a warpgroup,
-// one row per thread, takes the maximum, exponentials and their sum, and puts the weights P as 16-bit values where S was;
+// Per unit and tile: scores S = Q K^T (tcgen05.mma, both operands in shared memory) into tensor memory; a warpgroup, one
+// row per thread, takes the maximum, exponentials and their sum, and puts the weights P as 16-bit values where S was;
 // O += P V with P from tensor memory. While one tile's warpgroup works, the tensor cores do the other tile's products.
 // O stays in tensor memory; it is rescaled only when a row's maximum has grown by more than 2^8 since the reference that
 // its weights use, which the sums allow (weights up to 256 in 16 bits keep their relative precision).
 //
-// Bound: 4 x 128 x 128 x head size operations per tile and unit on the tensor cores, and 128 x 128 exponentials on the
-// 16-a-clock special function units, which is the same time (1,024 cycles) at a head size of 128.
+// Bound: 4 x 128 x 128 x head size operations per tile and unit on the tensor cores (1,024 cycles at a head size of 128),
+// their operands from shared memory (8 KB per 64-cycle product of S: all of its 128 bytes a clock), and 128 x 128
+// exponentials: 1,024 cycles on the special function units, which is why a part of them is computed by a polynomial.
 #pragma once
 #include "kv_step.cuh"
 
@@ -22,16 +23,17 @@ namespace vk {
 constexpr int CHUNK_ROWS = 128;                 // rows of a tile
 constexpr int CHUNK_SLOTS = 128;                // slots of a unit
 constexpr int CHUNK_THREADS = 384;              // two softmax warpgroups; one with the MMA warp and the loading warp
-constexpr int CHUNK_PART_ROWS = 2 * CHUNK_ROWS;
 template <int DP>
 constexpr int CHUNK_Q = 2 * CHUNK_ROWS * DP * 2;   // bytes of the two query tiles
 template <int DP>
 constexpr int CHUNK_SLOT = CHUNK_SLOTS * DP * 2;   // bytes of a tile of keys or values
 template <int DP>
 constexpr int CHUNK_RING = DP == 128 ? 5 : 10;     // tiles in flight, keys and values alternating
+// Pairs of exponentials of every 8 that the polynomial takes.
+constexpr int CHUNK_POLY = 2;
 template <int DP>
 constexpr int chunk_smem() {
-    return CHUNK_Q<DP> + CHUNK_RING<DP> * CHUNK_SLOT<DP> + 512;
+    return CHUNK_Q<DP> + CHUNK_RING<DP> * CHUNK_SLOT<DP> + CHUNK_ROWS * 8 + 512;
 }
 
 // A row tile's box of the queries (64 elements of a kv head's query heads, for a tile's tokens) into shared memory.
@@ -44,10 +46,13 @@ __device__ __forceinline__ void tma_rows(void* dst, const CUtensorMap* map, int 
 }
 
 // ---- tcgen05
-__device__ __forceinline__ uint64_t umma_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
-    // 128-byte swizzle (2 << 61), descriptor version 1; byte offsets in units of 16
-    return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(stride >> 4) << 32 |
-           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+// A descriptor's low word holds the operand's address and leading offset in units of 16 bytes, so that the next step's
+// operand is one 32-bit addition away; the high word is constant. The thread that issues the products is alone with
+// them: with whole descriptors made per product it was the kernel's bound.
+__device__ __forceinline__ uint32_t umma_low(uint32_t addr, uint32_t lead) { return addr >> 4 | (lead >> 4) << 16; }
+__device__ __forceinline__ uint64_t umma_desc(uint32_t low) {
+    // 8-row groups 1,024 bytes apart, descriptor version 1, 128-byte swizzle
+    return (uint64_t)(1024u >> 4 | 1u << 14 | 2u << 29) << 32 | low;
 }
 template <typename T>
 __device__ __forceinline__ uint32_t umma_idesc(int n, bool b_by_rows, bool negate) {
@@ -99,6 +104,50 @@ __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t* x) {
         : "memory");
 }
 
+// ---- two 32-bit values at a time
+struct Pair {
+    unsigned long long v;
+};
+__device__ __forceinline__ Pair pair_of(float x, float y) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(x), "f"(y));
+    return p;
+}
+__device__ __forceinline__ float2 floats(Pair p) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p.v));
+    return f;
+}
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+    Pair p;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
+    return p;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair p;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return p;
+}
+// 2^x without the special function units, x at most 127: x = j + f with j whole and |f| <= 1/2 (adding and taking away
+// 1.5 x 2^23 rounds to whole), 2^f by the degree-5 polynomial of least largest relative error on [-1/2, 1/2] (Remez
+// exchange; 2.1e-7 in 32-bit arithmetic, as the hardware's approximation), j added to the exponent. Below -126: 2^-126.
+__device__ __forceinline__ float2 exp2_poly(Pair x) {
+    float2 y = floats(x);
+    const Pair t = pair_of(fmaxf(y.x, -126.f), fmaxf(y.y, -126.f));
+    const Pair big = pair_of(12582912.f, 12582912.f), minus = pair_of(-12582912.f, -12582912.f);
+    const Pair z = t + big, j = z + minus, f = fma2(j, pair_of(-1.f, -1.f), t);
+    Pair p = pair_of(1.32764725e-3f, 1.32764725e-3f);
+    p = fma2(p, f, pair_of(9.67554096e-3f, 9.67554096e-3f));
+    p = fma2(p, f, pair_of(5.55071309e-2f, 5.55071309e-2f));
+    p = fma2(p, f, pair_of(2.40221202e-1f, 2.40221202e-1f));
+    p = fma2(p, f, pair_of(6.93146944e-1f, 6.93146944e-1f));
+    p = fma2(p, f, pair_of(1.00000012f, 1.00000012f));
+    const float2 r = floats(p), w = floats(z);
+    // z's low bits hold j (in two's complement); shifting leaves them where the exponent is
+    return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(w.x) << 23)),
+                       __int_as_float(__float_as_int(r.y) + (__float_as_int(w.y) << 23)));
+}
+
 // ---- the order of units
 // sum of floor((a i + b) / m) over 0 <= i < n, by Euclid's steps on (m, a); a, b >= 0
 __device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
@@ -123,30 +172,37 @@ struct ChunkShape {
     int tokens;  // of a row tile
     __device__ __forceinline__ bool takes(const KvSeq& s) const { return s.count > 0 && !step_takes(s, group); }
     __device__ __forceinline__ int pairs(const KvSeq& s) const { return (s.count + 2 * tokens - 1) / (2 * tokens); }
+    // a sequence's last pair may have one tile only
+    __device__ __forceinline__ bool lone(const KvSeq& s, int pair) const { return s.count <= (2 * pair + 1) * tokens; }
     // slots that the pair's last row sees
     __device__ __forceinline__ int limit(const KvSeq& s, int pair) const {
         return causal ? max(0, s.len - s.count + min(s.count, (pair + 1) * 2 * tokens)) : s.len;
     }
-    __device__ __forceinline__ int tiles(const KvSeq& s, int pair) const {
-        return max(1, (limit(s, pair) + CHUNK_SLOTS - 1) / CHUNK_SLOTS);
+    __device__ __forceinline__ int units(const KvSeq& s, int pair) const {
+        const int n = lone(s, pair) ? 2 * CHUNK_SLOTS : CHUNK_SLOTS;
+        return max(1, (limit(s, pair) + n - 1) / n);
     }
     // units of the pairs before `pair`
     __device__ __forceinline__ int64_t before(const KvSeq& s, int pair) const {
-        if (!causal) return (int64_t)pair * tiles(s, 0);
         const int all = pairs(s), n = min(pair, all - 1), per = 2 * tokens;
         const int64_t a = (int64_t)s.len - s.count;
-        const int one = a > CHUNK_SLOTS ? 0 : (int)min((int64_t)n, (CHUNK_SLOTS - a) / per);  // pairs of one unit
-        const int64_t sum = one + floor_sum(n - one, CHUNK_SLOTS, per, a + (int64_t)(one + 1) * per + CHUNK_SLOTS - 1);
-        return pair < all ? sum : sum + tiles(s, all - 1);
+        int64_t sum;
+        if (!causal) {
+            sum = (int64_t)n * max(1, (s.len + CHUNK_SLOTS - 1) / CHUNK_SLOTS);
+        } else {
+            const int one = a > CHUNK_SLOTS ? 0 : (int)min((int64_t)n, (CHUNK_SLOTS - a) / per);  // pairs of one unit
+            sum = one + floor_sum(n - one, CHUNK_SLOTS, per, a + (int64_t)(one + 1) * per + CHUNK_SLOTS - 1);
+        }
+        return pair < all ? sum : sum + units(s, all - 1);
     }
 };
 
 // A CTA's next segment: consecutive units of one (sequence, kv head, pair).
 struct ChunkSegment {
     KvSeq s;
-    int b, head, pair, t0, count, tiles;
+    int b, head, t0, count, units;
     int token0;  // of the pair's first row
-    bool both;   // the second tile has rows
+    bool lone;
 };
 struct ChunkWalk {
     const KvPages& c;
@@ -180,12 +236,11 @@ struct ChunkWalk {
         g->s = s;
         g->b = share.b;
         g->head = head;
-        g->pair = pair;
         g->t0 = t0;
-        g->tiles = shape.tiles(s, pair);
-        g->count = (int)min((int64_t)(g->tiles - t0), share.left);
+        g->units = shape.units(s, pair);
+        g->count = (int)min((int64_t)(g->units - t0), share.left);
         g->token0 = pair * 2 * shape.tokens;
-        g->both = s.count > g->token0 + shape.tokens;
+        g->lone = shape.lone(s, pair);
         share.left -= g->count;
         t0 = 0;
         if (++pair == all) pair = 0, ++head;
@@ -201,13 +256,14 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     constexpr uint32_t TM_S = 0, TM_O = 256;  // columns: S (and P) of the two tiles, O of the two
     extern __shared__ __align__(1024) uint8_t ring[];  // the swizzle goes by address bits: 1024-byte aligned
     uint8_t* smem_q = ring + RING * SLOT;
-    uint64_t* kv_full = reinterpret_cast<uint64_t*>(smem_q + CHUNK_Q<DP>);
+    float2* lone_ml = reinterpret_cast<float2*>(smem_q + CHUNK_Q<DP>);  // of a lone tile's second warpgroup
+    uint64_t* kv_full = reinterpret_cast<uint64_t*>(lone_ml + CHUNK_ROWS);
     uint64_t* kv_empty = kv_full + RING;
     uint64_t* q_full = kv_empty + RING;
     uint64_t* q_empty = q_full + 1;
-    uint64_t* s_full = q_empty + 1;  // [2]
-    uint64_t* p_full = s_full + 2;
-    uint64_t* o_full = p_full + 2;
+    uint64_t* s_full = q_empty + 1;  // [tile]
+    uint64_t* p_full = s_full + 2;   // [tile][half of the slots]
+    uint64_t* o_full = p_full + 4;
     int64_t* scratch = reinterpret_cast<int64_t*>(o_full + 2);  // THREADS / 32 + 2
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(scratch + CHUNK_THREADS / 32 + 2);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -220,7 +276,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         mbar_init(q_empty, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(s_full + i, 1);
-            mbar_init(p_full + i, 128);
+            mbar_init(p_full + 2 * i, 128);
+            mbar_init(p_full + 2 * i + 1, 128);
             mbar_init(o_full + i, 1);
         }
         fence_mbar_init();
@@ -241,257 +298,310 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         return shape.takes(s) ? shape.before(s, shape.pairs(s)) * c.heads : 0;
     });
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (threadIdx.x < 2) parts.at[2 * blockIdx.x + threadIdx.x].w = PART_NONE;
-    __syncthreads();
     tmem_fence_after();
     const uint32_t tm = *tmem_at;
     KvWait wait{c.status};
     ChunkWalk walk{c, bt, shape, share, 0, 0, 0, false};
     ChunkSegment g;
-    int slot = 0;  // of the ring
-    uint32_t phase = 0;
-    const int box_shift = min(c.page_shift, 6);
     // 384 threads start with 168 registers: 2 x 128 x 216 + 128 x 72 is the same sum
     if (warp >= 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        // The ring's n-th fill; a segment's tiles come as keys, values, keys, values.
+        int fill = 0;
+        auto at = [&](int n) { return n % RING; };
+        auto parity = [&](int n) -> uint32_t { return n / RING & 1; };
         if (warp == 9) {
-            int loaded = 0;
             uint32_t q_phase = 0;
+            const int box_shift = min(c.page_shift, 6);
+            const int boxes = CHUNK_SLOTS >> box_shift, i = lane % boxes, half = lane / boxes;
             while (walk.next(&g)) {
                 wait(q_empty, q_phase ^ 1);
-                if (lane == 0) {
-                    const int n = g.both ? 2 : 1;
-                    mbar_arrive_expect_tx(q_full, n * HALVES * shape.tokens * a.group * 128);
-                    for (int i = 0; i < n; ++i)
-                        for (int h = 0; h < HALVES; ++h)
-                            tma_rows(smem_q + (i * HALVES + h) * (CHUNK_ROWS * 128), &map_q, h * 64, g.head * a.group,
-                                     (int)g.s.first + g.token0 + i * shape.tokens, q_full);
-                }
                 q_phase ^= 1;
+                if (lane == 0) {
+                    const int n = g.lone ? 1 : 2;
+                    mbar_arrive_expect_tx(q_full, n * HALVES * shape.tokens * a.group * 128);
+                    for (int k = 0; k < n; ++k)
+                        for (int h = 0; h < HALVES; ++h)
+                            tma_rows(smem_q + (k * HALVES + h) * (CHUNK_ROWS * 128), &map_q, h * 64, g.head * a.group,
+                                     (int)g.s.first + g.token0 + k * shape.tokens, q_full);
+                }
                 const int32_t* table = bt.table + g.b * bt.table_stride;
-                const int boxes = CHUNK_SLOTS >> box_shift, i = lane % boxes, half = lane / boxes;
-                for (int t = g.t0; t < g.t0 + g.count; ++t) {
-                    const int at = t * CHUNK_SLOTS + (i << box_shift);
-                    const bool live = half < HALVES && at < g.s.len;
+                const int per = g.lone ? 2 : 1;
+                for (int t = g.t0 * per; t < (g.t0 + g.count) * per; ++t) {
+                    const int first = t * CHUNK_SLOTS + (i << box_shift);
+                    const bool live = half < HALVES && first < g.s.len;
                     int page = 0;
                     if (live) {
-                        page = (int)kv_page(c, table, at);
+                        page = (int)kv_page(c, table, first);
                         if (page < 0) page = (int)c.pages;  // past the map: reads as zero
                     }
                     const int n = __popc(__ballot_sync(FULL, live));
-                    for (int side = 0; side < 2; ++side) {
-                        wait(kv_empty + slot, phase ^ 1);
+                    for (int side = 0; side < 2; ++side, ++fill) {
+                        const int slot = at(fill);
+                        wait(kv_empty + slot, parity(fill) ^ 1);
                         if (lane == 0) mbar_arrive_expect_tx(kv_full + slot, n * (128 << box_shift));
                         __syncwarp();
                         if (live)
                             tma_page(ring + slot * SLOT + half * (CHUNK_SLOTS * 128) + (i << box_shift) * 128,
-                                     side ? &map_v : &map_k, half * 64, at & ((1 << c.page_shift) - 1), g.head, page,
+                                     side ? &map_v : &map_k, half * 64, first & ((1 << c.page_shift) - 1), g.head, page,
                                      kv_full + slot);
-                        ++loaded;
-                        if (++slot == RING) slot = 0, phase ^= 1;
                     }
                 }
             }
             // A wait that ran out may have left copies in flight into this CTA's memory: see them land before it ends.
             if (wait.dead && lane == 0)
-                for (int i = 0; i < RING; ++i) {
-                    const int fills = loaded / RING + (i < loaded % RING);
-                    if (fills && !mbar_wait_bounded(kv_full + i, (fills - 1) & 1, 2 * KV_WAIT_BUDGET))
+                for (int k = max(0, fill - RING); k < fill; ++k)
+                    if (!mbar_wait_bounded(kv_full + at(k), parity(k), 2 * KV_WAIT_BUDGET))
                         atomicOr(c.status, ERR_DRAIN_TIMEOUT);
-                }
         } else if (warp == 8) {
-            uint32_t q_phase = 0, p_phase[2] = {0, 0};
+            uint32_t q_phase = 0, p_phase = 0;  // p_phase: bit per tile
+            const int ks = (c.dim + 15) / 16;   // steps of 16 elements; the padding's products are left out
+            const uint32_t idesc_s = umma_idesc<T>(CHUNK_SLOTS, false, a.scale < 0.f);
+            const uint32_t idesc_o = umma_idesc<T>(ks * 16, true, false);
+            const uint32_t q_low = umma_low(smem_u32(smem_q), 16), k_low = umma_low(smem_u32(ring), 16);
+            const uint32_t v_low = umma_low(smem_u32(ring), CHUNK_SLOTS * 128);
             while (walk.next(&g)) {
-                const uint32_t idesc_s = umma_idesc<T>(CHUNK_SLOTS, false, a.scale < 0.f);
-                const uint32_t idesc_o = umma_idesc<T>(DP, true, false);
-                auto scores = [&](int i) {  // S_i = Q_i K^T, K in the current ring slot
+                const int step = g.lone ? 4 : 2;
+                // keys of tile i's part of unit u of this segment, and its values the fill after it
+                auto key_fill = [&](int u, int i) { return fill + u * step + (g.lone ? 2 * i : 0); };
+                auto scores = [&](int u, int i) {  // S_i = Q_i K^T
+                    const int n = key_fill(u, i), slot = at(n);
+                    wait(kv_full + slot, parity(n));
+                    tmem_fence_after();
                     if (lane == 0) {
-                        const uint32_t q = smem_u32(smem_q) + i * HALVES * (CHUNK_ROWS * 128), k = smem_u32(ring + slot * SLOT);
+                        const uint32_t q = q_low + (g.lone ? 0 : i * HALVES * (CHUNK_ROWS * 8)), k = k_low + slot * (SLOT / 16);
 #pragma unroll
                         for (int e = 0; e < KS; ++e) {
-                            const uint32_t off = (e >> 2) * (CHUNK_ROWS * 128) + (e & 3) * 32;
-                            umma_ss(tm + TM_S + i * 128, umma_desc(q + off, 16, 1024), umma_desc(k + off, 16, 1024), idesc_s,
-                                    e > 0);
+                            const uint32_t off = (e >> 2) * (CHUNK_ROWS * 8) + (e & 3) * 2;
+                            if (e < ks) umma_ss(tm + TM_S + i * 128, umma_desc(q + off), umma_desc(k + off), idesc_s, e > 0);
                         }
                         umma_commit(s_full + i);
+                        if (g.lone || i == 1) umma_commit(kv_empty + slot);
                     }
                     __syncwarp();
-                };
-                auto advance = [&] {
-                    if (++slot == RING) slot = 0, phase ^= 1;
                 };
                 wait(q_full, q_phase);
                 q_phase ^= 1;
-                wait(kv_full + slot, phase);
-                tmem_fence_after();
-                scores(0);
-                if (g.both) scores(1);
-                if (lane == 0) {
-                    umma_commit(kv_empty + slot);
-                    if (g.count == 1) umma_commit(q_empty);
-                }
-                __syncwarp();
-                advance();
-                for (int t = g.t0; t < g.t0 + g.count; ++t) {
-                    // values of tile t in the current slot, keys of tile t + 1 in the next one
-                    const int v_slot = slot;
-                    const int held = min(CHUNK_SLOTS, g.s.len - t * CHUNK_SLOTS);  // slots of the sequence in this tile
-                    wait(kv_full + slot, phase);
-                    if (held < CHUNK_SLOTS && (held & 15) && held > 0) {
-                        // The page's slots past the sequence hold anything: none may meet a weight of zero. The product stops
-                        // at the 16 slots that hold the last one; their rest is cleared.
-                        for (int r = held; r < (held + 15) / 16 * 16; ++r)
-                            if (lane < 8 * HALVES)
-                                *reinterpret_cast<uint4*>(ring + v_slot * SLOT + (lane >> 3) * (CHUNK_SLOTS * 128) + r * 128 +
-                                                          (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                    }
-                    const int steps = max(1, (min(held, CHUNK_SLOTS) + 15) / 16);
-                    const bool more = t + 1 < g.t0 + g.count;
-                    advance();
-                    for (int i = 0; i < (g.both ? 2 : 1); ++i) {
-                        wait(p_full + i, p_phase[i]);
-                        p_phase[i] ^= 1;
-                        tmem_fence_after();
-                        if (lane == 0 && held > 0) {
-                            const uint32_t v = smem_u32(ring + v_slot * SLOT);
-                            for (int e = 0; e < steps; ++e)
-                                umma_ts(tm + TM_O + i * 128, tm + TM_S + i * 128 + e * 8,
-                                        umma_desc(v + e * 2048, CHUNK_SLOTS * 128, 1024), idesc_o, t > g.t0 || e > 0);
+                scores(0, 0);
+                scores(0, 1);
+                if (g.count == 1 && lane == 0) umma_commit(q_empty);
+                for (int u = 0; u < g.count; ++u) {
+#pragma unroll 1
+                    for (int i = 0; i < 2; ++i) {
+                        const int n = key_fill(u, i) + 1, slot = at(n);
+                        // slots of the sequence in this tile
+                        const int held = g.s.len - (g.lone ? 2 * (g.t0 + u) + i : g.t0 + u) * CHUNK_SLOTS;
+                        wait(kv_full + slot, parity(n));
+                        if (held > 0 && held < CHUNK_SLOTS && (held & 15) && (g.lone || i == 0)) {
+                            // The page's slots past the sequence hold anything: none may meet a weight of zero. The
+                            // product stops at the 16 slots that hold the last one; their rest is cleared.
+                            for (int r = held; r < (held + 15) / 16 * 16; ++r)
+                                if (lane < 8 * HALVES)
+                                    *reinterpret_cast<uint4*>(ring + slot * SLOT + (lane >> 3) * (CHUNK_SLOTS * 128) +
+                                                              r * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                            fence_proxy_async_smem();
+                            __syncwarp();
                         }
-                        __syncwarp();
-                        if (more) {
-                            if (i == 0) {
-                                wait(kv_full + slot, phase);
-                                tmem_fence_after();
-                            }
-                            scores(i);
-                        } else if (lane == 0) {
-                            umma_commit(o_full + i);
+                        const uint32_t v = v_low + slot * (SLOT / 16), p = tm + TM_S + i * 128, o = tm + TM_O + i * 128;
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            wait(p_full + 2 * i + half, p_phase >> i & 1);
+                            tmem_fence_after();
+                            if (lane == 0)
+#pragma unroll
+                                for (int e = 4 * half; e < 4 * half + 4; ++e)
+                                    if (16 * e < held) umma_ts(o, p + e * 8, umma_desc(v + e * 128), idesc_o, u > 0 || e > 0);
+                            __syncwarp();
                         }
+                        p_phase ^= 1u << i;
+                        if (lane == 0 && (g.lone || i == 1)) umma_commit(kv_empty + slot);
+                        if (u + 1 < g.count) scores(u + 1, i);
+                        else if (lane == 0) umma_commit(o_full + i);
                     }
-                    if (lane == 0) umma_commit(kv_empty + v_slot);
-                    if (more) {
-                        if (lane == 0) {
-                            umma_commit(kv_empty + slot);
-                            if (t + 2 == g.t0 + g.count) umma_commit(q_empty);
-                        }
-                        advance();
-                    }
+                    if (u + 2 == g.count && lane == 0) umma_commit(q_empty);
                     __syncwarp();
                 }
+                fill += g.count * step;
             }
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        const int i = warp >> 2, r = (warp & 3) * 32 + lane;  // tile and row
+        const uint32_t lanes = tm + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t tm_s = lanes + TM_S + i * 128, tm_o = lanes + TM_O + i * 128;
+        // base 2; a scale of zero keeps -inf what it is
+        const float scale = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-37f);
         uint32_t s_phase = 0, o_phase = 0;
-        bool first_segment = true;
         while (walk.next(&g)) {
-            const int i = warp >> 2, r = (warp & 3) * 32 + lane;
-            const uint32_t lanes = tm + ((uint32_t)((warp & 3) * 32) << 16);
-            const uint32_t tm_s = lanes + TM_S + i * 128, tm_o = lanes + TM_O + i * 128;
-            const int token = g.token0 + i * shape.tokens + r / a.group;
+            const int token1 = g.token0 + (g.lone ? 0 : i * shape.tokens);  // of the tile's first row
+            const int token = token1 + r / a.group;
             const bool live = r < shape.tokens * a.group && token < g.s.count;
             const int lim = live ? max(0, row_limit(g.s, a.causal, token)) : 0;
-            const int open = max(0, min(g.s.len, row_limit(g.s, a.causal, g.token0 + i * shape.tokens)));  // every row sees these
-            // base 2; a scale of zero keeps -inf what it is
-            const float scale = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-37f);
+            const int open = max(0, min(g.s.len, row_limit(g.s, a.causal, token1)));  // slots that every row sees
             float m = -INFINITY, l = 0.f;
-            if (i == 0 || g.both) {
-                for (int t = g.t0; t < g.t0 + g.count; ++t) {
-                    float x[CHUNK_SLOTS];
-                    wait(s_full + i, s_phase);
-                    s_phase ^= 1;
-                    tmem_fence_after();
+            for (int t = g.t0; t < g.t0 + g.count; ++t) {
+                const int slot0 = (g.lone ? 2 * t + i : t) * CHUNK_SLOTS;
+                float x[CHUNK_SLOTS];
+                wait(s_full + i, s_phase);
+                s_phase ^= 1;
+                tmem_fence_after();
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) tmem_ld32(tm_s + 32 * e, x + 32 * e);
-                    tmem_wait_ld();
-                    if ((t + 1) * CHUNK_SLOTS > open) {
-                        const int see = lim - t * CHUNK_SLOTS;
+                for (int e = 0; e < 4; ++e) tmem_ld32(tm_s + 32 * e, x + 32 * e);
+                tmem_wait_ld();
+                const bool masked = slot0 + CHUNK_SLOTS > open;
+                if (masked) {
+                    const int see = lim - slot0;
 #pragma unroll
-                        for (int e = 0; e < CHUNK_SLOTS; ++e) x[e] = e < see ? x[e] : -INFINITY;
-                    }
-                    float top4[4] = {x[0], x[1], x[2], x[3]};
+                    for (int e = 0; e < CHUNK_SLOTS; ++e) x[e] = e < see ? x[e] : -INFINITY;
+                }
+                float top4[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-                    for (int e = 4; e < CHUNK_SLOTS; ++e) top4[e & 3] = fmaxf(top4[e & 3], x[e]);
-                    const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
-                    const bool grow = (top - m) * scale > 8.f;  // m = -inf: unless all is masked
-                    if (t == g.t0) {
-                        m = top;
-                    } else if (__any_sync(FULL, grow)) {
-                        const float f = grow ? (m == -INFINITY ? 0.f : ex2((m - top) * scale)) : 1.f;
-                        if (grow) m = top;
-                        l *= f;
+                for (int e = 4; e < CHUNK_SLOTS; e += 4)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) top4[k] = fmaxf(top4[k], x[e + k]);
+                const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
+                const bool grow = (top - m) * scale > 8.f;  // m = -inf: unless all is masked
+                if (t == g.t0) {
+                    m = top;
+                } else if (__any_sync(FULL, grow)) {
+                    const float f = grow ? part_factor(m * scale, top * scale) : 1.f;
+                    if (grow) m = top;
+                    l *= f;
 #pragma unroll 1
-                        for (int e = 0; e < DP; e += 32) {
-                            float o[32];
-                            tmem_ld32(tm_o + e, o);
-                            tmem_wait_ld();
-                            uint32_t w[32];
+                    for (int e = 0; e < c.dim; e += 32) {
+                        float o[32];
+                        tmem_ld32(tm_o + e, o);
+                        tmem_wait_ld();
+                        uint32_t w[32];
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) w[k] = __float_as_uint(o[k] * f);
-                            tmem_st32(tm_o + e, w);
-                        }
+                        for (int k = 0; k < 32; ++k) w[k] = __float_as_uint(o[k] * f);
+                        tmem_st32(tm_o + e, w);
                     }
-                    const float ref = m == -INFINITY ? 0.f : m * scale;
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                    uint32_t p[CHUNK_SLOTS / 2];
+                }
+                const float ref = m == -INFINITY ? 0.f : m * scale;
+                const Pair scale2 = pair_of(scale, scale), ref2 = pair_of(-ref, -ref);
+                Pair sum0 = pair_of(0.f, 0.f), sum1 = sum0;
 #pragma unroll
-                    for (int e = 0; e < CHUNK_SLOTS; e += 2) {
-                        const float y0 = ex2(fmaf(x[e], scale, -ref)), y1 = ex2(fmaf(x[e + 1], scale, -ref));
-                        sum[e & 3] += y0;
-                        sum[(e & 3) + 1] += y1;
-                        p[e / 2] = pack2<T>(y0, y1);
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t p[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const int k = 64 * half + 2 * e;
+                        const Pair y = fma2(pair_of(x[k], x[k + 1]), scale2, ref2);
+                        float2 w = floats(y);
+                        // masked slots need the hardware's 2^-inf = 0
+                        if (e % 8 < CHUNK_POLY && !masked) w = exp2_poly(y);
+                        else w = make_float2(ex2(w.x), ex2(w.y));
+                        if (e & 1) sum1 = sum1 + pair_of(w.x, w.y);
+                        else sum0 = sum0 + pair_of(w.x, w.y);
+                        p[e] = pack2<T>(w.x, w.y);
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    tmem_st32(tm_s, p);
-                    tmem_st32(tm_s + 32, p + 32);
+                    tmem_st32(tm_s + 32 * half, p);
                     tmem_wait_st();
                     tmem_fence_before();
-                    mbar_arrive(p_full + i);
+                    mbar_arrive(p_full + 2 * i + half);
                 }
-                wait(o_full + i, o_phase);
-                o_phase ^= 1;
+                const float2 sum = floats(sum0 + sum1);
+                l += sum.x + sum.y;
+            }
+            wait(o_full + i, o_phase);
+            o_phase ^= 1;
+            tmem_fence_after();
+            // base 2 from here on. A tile past the sequence met no product: its O holds anything.
+            float top = m == -INFINITY ? -INFINITY : m * scale, total = l, f0 = 1.f, f1 = 0.f;
+            const float top0 = top;
+            if (g.lone) {  // the first warpgroup joins the two
+                if (i == 1) {
+                    lone_ml[r] = make_float2(top, total);
+                    tmem_fence_before();
+                    asm volatile("bar.sync 3, 256;" ::: "memory");
+                    asm volatile("bar.sync 3, 256;" ::: "memory");  // read
+                    continue;
+                }
+                asm volatile("bar.sync 3, 256;" ::: "memory");
                 tmem_fence_after();
-                const bool whole = g.count == g.tiles;
-                const bool none = g.t0 * CHUNK_SLOTS >= g.s.len;  // no product was made: O holds anything
-                const int64_t part = 2 * (int64_t)blockIdx.x + (first_segment ? 0 : 1);
-                const int h = g.head * a.group + r % a.group;
-                const int64_t tok = g.s.first + token;
-                const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;
+                const float2 ml = lone_ml[r];
+                top = fmaxf(top, ml.x);
+                f0 = part_factor(top0, top);
+                f1 = part_factor(ml.x, top);
+                total = total * f0 + ml.y * f1;
+            }
+            const bool none0 = (int64_t)g.t0 * (g.lone ? 2 : 1) * CHUNK_SLOTS >= g.s.len;
+            const bool none1 = !g.lone || (2 * (int64_t)g.t0 + 1) * CHUNK_SLOTS >= g.s.len;
+            const bool leaves = g.t0 > 0;                                                       // a part for an earlier CTA
+            const int follow = leaves ? 0 : walk.share.followers(g.units - g.count);  // CTAs with the rest of this one
+            auto part_of = [&](int k) -> int64_t { return 2 * (int64_t)(blockIdx.x + k) + i; };
+            if (follow) {
+                for (int k = r; k < follow; k += 128) part_await(parts, (int)part_of(1 + k), wait);
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+                const float mine = top;
+                for (int k = 0; k < follow; ++k) top = fmaxf(top, __ldcg(parts.ml + part_of(1 + k) * CHUNK_ROWS + r).x);
+                const float f = part_factor(mine, top);
+                f0 *= f;
+                f1 *= f;
+                total *= f;
+                for (int k = 0; k < follow; ++k) {
+                    const float2 ml = __ldcg(parts.ml + part_of(1 + k) * CHUNK_ROWS + r);
+                    total += ml.y * part_factor(ml.x, top);
+                }
+            }
+            const int h = g.head * a.group + r % a.group;
+            const int64_t tok = g.s.first + token;
+            const float inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
 #pragma unroll 1
-                for (int e = 0; e < DP; e += 32) {
-                    float o[32];
-                    tmem_ld32(tm_o + e, o);
+            for (int e = 0; e < c.dim; e += 32) {
+                float o[32];
+                tmem_ld32(tm_o + e, o);
+                tmem_wait_ld();
+#pragma unroll
+                for (int k = 0; k < 32; ++k) o[k] = none0 ? 0.f : o[k] * f0;
+                if (!none1) {
+                    float o1[32];
+                    tmem_ld32(tm_o + 128 + e, o1);
                     tmem_wait_ld();
-                    if (none)
 #pragma unroll
-                        for (int k = 0; k < 32; ++k) o[k] = 0.f;
-                    if (live && whole) {
-                        uint4* out = reinterpret_cast<uint4*>(a.out + tok * a.os[0] + h * a.os[1] + e);
+                    for (int k = 0; k < 32; ++k) o[k] += o1[k] * f1;
+                }
+                // parts: [four columns][row], so that a warp's accesses are contiguous
+                for (int k = 0; k < follow; ++k) {
+                    const int64_t part = part_of(1 + k);
+                    const float f = part_factor(__ldcg(parts.ml + part * CHUNK_ROWS + r).x, top);
+                    const float4* po = reinterpret_cast<const float4*>(parts.o) + (part * (DP / 4) + e / 4) * CHUNK_ROWS + r;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            if (e + 8 * k < c.dim)
-                                out[k] = make_uint4(pack2<T>(o[8 * k] * inv, o[8 * k + 1] * inv),
-                                                    pack2<T>(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
-                                                    pack2<T>(o[8 * k + 4] * inv, o[8 * k + 5] * inv),
-                                                    pack2<T>(o[8 * k + 6] * inv, o[8 * k + 7] * inv));
-                    } else if (live) {
-                        float4* po = reinterpret_cast<float4*>(parts.o + (part * CHUNK_PART_ROWS + i * CHUNK_ROWS + r) * DP + e);
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) po[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+                    for (int w = 0; w < 8; ++w) {
+                        const float4 y = __ldcg(po + w * CHUNK_ROWS);
+                        o[4 * w] += y.x * f, o[4 * w + 1] += y.y * f, o[4 * w + 2] += y.z * f, o[4 * w + 3] += y.w * f;
                     }
                 }
-                const float top = m == -INFINITY ? -INFINITY : m * scale;
-                if (live && whole) a.lse[tok * a.heads + h] = (top + log2f(l)) * 0.6931471805599453f;
-                else if (live) parts.ml[part * CHUNK_PART_ROWS + i * CHUNK_ROWS + r] = make_float2(top, l);
-                if (!whole && threadIdx.x == 0)
-                    parts.at[part] = make_int4(g.b, g.head, g.pair, PART_HELD | (g.t0 == 0 ? PART_FIRST : 0) |
-                                                                        (g.t0 + g.count == g.tiles ? PART_LAST : 0));
-                tmem_fence_before();
+                if (leaves) {
+                    float4* po = reinterpret_cast<float4*>(parts.o) + (part_of(0) * (DP / 4) + e / 4) * CHUNK_ROWS + r;
+#pragma unroll
+                    for (int w = 0; w < 8; ++w)
+                        po[w * CHUNK_ROWS] = make_float4(o[4 * w], o[4 * w + 1], o[4 * w + 2], o[4 * w + 3]);
+                } else if (live) {
+                    uint4* out = reinterpret_cast<uint4*>(a.out + tok * a.os[0] + h * a.os[1] + e);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (e + 8 * k < c.dim)
+                            out[k] = make_uint4(pack2<T>(o[8 * k] * inv, o[8 * k + 1] * inv),
+                                                pack2<T>(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
+                                                pack2<T>(o[8 * k + 4] * inv, o[8 * k + 5] * inv),
+                                                pack2<T>(o[8 * k + 6] * inv, o[8 * k + 7] * inv));
+                }
             }
-            first_segment = false;
+            tmem_fence_before();
+            if (g.lone) asm volatile("bar.sync 3, 256;" ::: "memory");
+            if (leaves) {
+                parts.ml[part_of(0) * CHUNK_ROWS + r] = make_float2(top, total);
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+                if (r == 0) part_publish(parts, (int)part_of(0));
+            } else {
+                if (live) a.lse[tok * a.heads + h] = (top + log2f(total)) * 0.6931471805599453f;
+                if (follow) {
+                    asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+                    for (int k = r; k < follow; k += 128) parts.ready[part_of(1 + k)] = 0;
+                }
+            }
         }
     }
     __syncthreads();

@@ -1,11 +1,12 @@
 // Attention of a sequence's few new tokens over the paged cache (at most 16 rows = tokens x query heads of a kv head:
-// decoding steps, drafted tokens), and the join of split sequences.
+// decoding steps, drafted tokens), and how a call's work is shared out.
 //
 // Every slot's key and value (4 x head_dim bytes per kv head) is read once and meets at most 16 rows, so the kernel is
 // bound by memory. One CTA per 64-slot tile would leave SMs idle on short batches and unbalanced on ragged ones:
 // instead all (sequence, kv head, tile) units are laid end to end and every CTA takes an equal, contiguous share. A
-// sequence's head that a CTA holds whole is finished in place; one that is cut leaves parts (unnormalised sums with
-// their maximum and total) that the join kernel adds up in order, so results do not depend on timing.
+// sequence's head that a CTA holds whole is finished in place. One that is cut is finished by the CTA that holds its
+// beginning, which comes to it last and finds the parts of the CTAs that follow (unnormalised sums with their maximum
+// and total; they come to theirs first) in the workspace. It adds them up in order: results do not depend on timing.
 //
 // Inside a CTA one warp keeps a ring of tiles filled by TMA (one box per page and 64 head elements, in the 128-byte
 // swizzle that ldmatrix reads without conflicts); four warps take 16 slots of each tile, with their own running maximum
@@ -25,14 +26,14 @@ constexpr int STEP_THREADS = 32 * (STEP_WARPS + 1);
 constexpr int STEP_RING = 96 * 1024;  // bytes in flight per CTA; two CTAs share an SM
 constexpr long long KV_WAIT_BUDGET = 4000000000LL;  // cycles: about two seconds
 
-// Parts of split sequences. CTA i leaves at most two: part 2i of the first (sequence, head) of its share, part 2i + 1 of
-// the last. The parts of one follow each other in the order of the CTAs.
-enum : int { PART_NONE = 0, PART_HELD = 1, PART_FIRST = 2, PART_LAST = 4 };
+// What a call keeps in its workspace. A CTA leaves at most one part of each of its row tiles: of its first segment, when
+// that does not begin its (sequence, kv head, rows); ready[part] tells the CTA that waits for it and is zero again when
+// the call is done.
 struct KvParts {
-    float* o;     // [part][rows][padded head size], unnormalised
-    float2* ml;   // [part][rows]: maximum (base 2) and sum
-    int4* at;     // [part]: sequence, kv head, row tile, PART_ flags
-    float* s;     // [sequence][kv head][slot][R]: scaled scores (base 2) of the step path, for the weights
+    uint32_t* ready;
+    float* o;    // [part]: unnormalised sums
+    float2* ml;  // [part][row]: maximum (base 2) and sum
+    float* s;    // [sequence][kv head][slot][R]: scaled scores (base 2) of the step path, for the weights
     int64_t s_slots;
 };
 
@@ -68,6 +69,26 @@ struct KvWait {
         }
     }
 };
+
+// Part `i` is written (by threads that a barrier has joined since): tell the CTA that adds it up.
+__device__ __forceinline__ void part_publish(const KvParts& parts, int i) {
+    __threadfence();
+    asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(parts.ready + i), "r"(1u) : "memory");
+}
+// Waits, with a limit, for part i. Its CTA comes to it before anything else and waits for nobody to make it.
+__device__ __forceinline__ void part_await(const KvParts& parts, int i, KvWait& wait) {
+    uint32_t there = 0;
+    const long long t0 = clock64();
+    while (!wait.dead) {
+        asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(there) : "l"(parts.ready + i) : "memory");
+        if (there) break;
+        if (clock64() - t0 > KV_WAIT_BUDGET) {
+            wait.dead = true;
+            atomicOr(wait.status, ERR_WAIT_TIMEOUT);
+        }
+    }
+}
+__device__ __forceinline__ float part_factor(float m, float top) { return m == -INFINITY ? 0.f : ex2(m - top); }
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -106,9 +127,19 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // The share of one CTA: a walk over units laid end to end, sequence by sequence. Count(s) is the number of units of a
 // sequence; the caller splits a sequence's units into its heads and tiles.
 struct KvShare {
-    int b;         // sequence of the next unit
-    int64_t off;   // unit within it
-    int64_t left;  // units of this CTA
+    int b;        // sequence of the next unit
+    int64_t off;  // unit within it
+    int64_t left;  // units of this CTA that are not taken yet
+    int64_t total;
+    int ctas;  // CTAs with a share; none of these is empty
+    // CTAs that hold the next `rest` units after this CTA's share
+    __device__ __forceinline__ int followers(int64_t rest) const {
+        const int me = blockIdx.x + 1;
+        const int64_t end = total * me / ctas + rest;
+        int n = 0;
+        while (me + n < ctas && total * (me + n) / ctas < end) ++n;
+        return n;
+    }
 };
 
 template <int THREADS, class Count>
@@ -132,7 +163,6 @@ __device__ __forceinline__ KvShare kv_share(const KvPages& c, const KvBatch& bt,
         if (w < warp) before += scratch[w];
         total += scratch[w];
     }
-    // No empty share between two others: the parts of a split sequence lie at consecutive CTAs.
     const int64_t ctas = min((int64_t)gridDim.x, total), i = min((int64_t)blockIdx.x, ctas);
     const int64_t first = ctas ? total * i / ctas : 0, last = ctas ? total * min(i + 1, ctas) / ctas : 0;
     before += incl - sum;
@@ -148,7 +178,7 @@ __device__ __forceinline__ KvShare kv_share(const KvPages& c, const KvBatch& bt,
         scratch[WARPS + 1] = off;
     }
     __syncthreads();
-    return {(int)scratch[WARPS], scratch[WARPS + 1], last - first};
+    return {(int)scratch[WARPS], scratch[WARPS + 1], last - first, total, (int)ctas};
 }
 
 // Lowest slot that some row does not see: n for every row, or the first row's limit under the causal mask.
@@ -195,13 +225,10 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
     };
     KvShare share = kv_share<STEP_THREADS>(c, bt, scratch, units_of);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (threadIdx.x < 2) parts.at[2 * blockIdx.x + threadIdx.x].w = PART_NONE;
-    __syncthreads();
     KvWait wait{c.status};
     int stage = 0;
     uint32_t phase = 0;
     const int box_shift = min(c.page_shift, 6), boxes = STEP_TILE >> box_shift;
-    bool first_segment = true;
     int loaded = 0;
     while (share.left > 0) {
         const KvSeq s = kv_seq(c, bt, share.b);
@@ -347,8 +374,9 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
                 if (++stage == STAGES) stage = 0, phase ^= 1;
             }
             // Join the four warps, eight rows at a time.
-            const bool whole = count == tiles;
-            const int part = 2 * blockIdx.x + (first_segment ? 0 : 1);
+            const bool leaves = t0 > 0;                                             // a part for an earlier CTA
+            const int follow = leaves ? 0 : share.followers(tiles - count);  // CTAs with the rest of this one
+            for (int i = threadIdx.x; i < follow; i += 32 * STEP_WARPS) part_await(parts, blockIdx.x + 1 + i, wait);
 #pragma unroll
             for (int u = 0; u < R / 8; ++u) {
                 l[u] += __shfl_xor_sync(FULL, l[u], 1);
@@ -376,29 +404,40 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
 #pragma unroll
                         for (int e = 0; e < 8; ++e) v[e] += f * sum_o[(w * 8 + r8) * DP + d + e];
                     }
-                    if (whole) {
-                        const int64_t tok = s.first + r / a.group;
-                        const int h = head * a.group + r % a.group;
-                        const float inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
-                        if (d < c.dim)
-                            *reinterpret_cast<uint4*>(a.out + tok * a.os[0] + h * a.os[1] + d) =
-                                make_uint4(pack2<T>(v[0] * inv, v[1] * inv), pack2<T>(v[2] * inv, v[3] * inv),
-                                           pack2<T>(v[4] * inv, v[5] * inv), pack2<T>(v[6] * inv, v[7] * inv));
-                        if (d == 0) a.lse[tok * a.heads + h] = (top + log2f(total)) * 0.6931471805599453f;
-                    } else {
-                        float4* po = reinterpret_cast<float4*>(parts.o + ((int64_t)part * STEP_ROWS + r) * DP + d);
+                    if (leaves) {
+                        float4* po = reinterpret_cast<float4*>(parts.o + ((int64_t)blockIdx.x * STEP_ROWS + r) * DP + d);
                         po[0] = make_float4(v[0], v[1], v[2], v[3]);
                         po[1] = make_float4(v[4], v[5], v[6], v[7]);
-                        if (d == 0) parts.ml[(int64_t)part * STEP_ROWS + r] = make_float2(top, total);
+                        if (d == 0) parts.ml[(int64_t)blockIdx.x * STEP_ROWS + r] = make_float2(top, total);
+                        continue;
                     }
+#pragma unroll 4
+                    for (int k = 0; k < follow; ++k) {
+                        const int64_t p = (int64_t)(blockIdx.x + 1 + k) * STEP_ROWS + r;
+                        const float2 ml = __ldcg(parts.ml + p);
+                        const float4* po = reinterpret_cast<const float4*>(parts.o + p * DP + d);
+                        const float4 x = __ldcg(po), y = __ldcg(po + 1);
+                        const float next = fmaxf(top, ml.x), f = part_factor(top, next), h = part_factor(ml.x, next);
+                        total = total * f + ml.y * h;
+                        v[0] = v[0] * f + x.x * h, v[1] = v[1] * f + x.y * h, v[2] = v[2] * f + x.z * h;
+                        v[3] = v[3] * f + x.w * h, v[4] = v[4] * f + y.x * h, v[5] = v[5] * f + y.y * h;
+                        v[6] = v[6] * f + y.z * h, v[7] = v[7] * f + y.w * h;
+                        top = next;
+                    }
+                    const int64_t tok = s.first + r / a.group;
+                    const int h = head * a.group + r % a.group;
+                    const float inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
+                    if (d < c.dim)
+                        *reinterpret_cast<uint4*>(a.out + tok * a.os[0] + h * a.os[1] + d) =
+                            make_uint4(pack2<T>(v[0] * inv, v[1] * inv), pack2<T>(v[2] * inv, v[3] * inv),
+                                       pack2<T>(v[4] * inv, v[5] * inv), pack2<T>(v[6] * inv, v[7] * inv));
+                    if (d == 0) a.lse[tok * a.heads + h] = (top + log2f(total)) * 0.6931471805599453f;
                 }
                 asm volatile("bar.sync 1, 128;" ::: "memory");
             }
-            if (!whole && threadIdx.x == 0)
-                parts.at[part] = make_int4(share.b, head, 0,
-                                           PART_HELD | (t0 == 0 ? PART_FIRST : 0) | (t0 + count == tiles ? PART_LAST : 0));
+            if (leaves && threadIdx.x == 0) part_publish(parts, blockIdx.x);
+            for (int i = threadIdx.x; i < follow; i += 32 * STEP_WARPS) parts.ready[blockIdx.x + 1 + i] = 0;
         }
-        first_segment = false;
     }
     // A wait that ran out may have left copies in flight into this CTA's memory: see them land before it ends.
     if (warp == STEP_WARPS && wait.dead && lane == 0)
@@ -407,67 +446,6 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
             if (fills && !mbar_wait_bounded(full + i, (fills - 1) & 1, 2 * KV_WAIT_BUDGET))
                 atomicOr(c.status, ERR_DRAIN_TIMEOUT);
         }
-}
-
-// Adds up the parts of split (sequence, kv head, row tile)s. Block x starts at part x if that is a first one; the others
-// of it are the first parts of the CTAs that follow. One warp per row; a part's rows are tiles of TILE rows, of
-// tile_tokens tokens each.
-template <typename T, int DP, int ROWS, int TILE, int WARPS>
-__global__ void __launch_bounds__(32 * WARPS) kv_join_kernel(KvPages c, KvBatch bt, KvAttend a, KvParts parts, int ctas,
-                                                             int tile_tokens) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int4 at = parts.at[blockIdx.x];
-    if (!(at.w & PART_FIRST)) return;
-    const int lane = threadIdx.x & 31;
-    const KvSeq s = kv_seq(c, bt, at.x);
-    const int cta = blockIdx.x / 2;
-    int last = cta;
-    if (!(at.w & PART_LAST)) {
-        for (;;) {  // the CTAs that follow, 32 at a time, up to the one with the last part
-            const int i = last + 1 + lane;
-            const unsigned ends = __ballot_sync(FULL, i >= ctas || (parts.at[2 * i].w & PART_LAST));
-            if (ends) {
-                last += __ffs(ends);
-                break;
-            }
-            last += 32;
-        }
-        last = min(last, ctas - 1);
-    }
-    auto part_of = [&](int i) -> int64_t { return i == 0 ? (int64_t)blockIdx.x : 2 * (int64_t)(cta + i); };
-    const int n = last - cta + 1;
-    for (int r = blockIdx.y * WARPS + (threadIdx.x >> 5); r < ROWS; r += WARPS * gridDim.y) {
-        const int in = r % TILE, token = (at.z * (ROWS / TILE) + r / TILE) * tile_tokens + in / a.group;
-        if (in >= tile_tokens * a.group || token >= s.count) continue;
-        float top = -INFINITY;
-        for (int i = lane; i < n; i += 32) top = fmaxf(top, parts.ml[part_of(i) * ROWS + r].x);
-        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL, top, o));
-        float total = 0.f;
-        constexpr int PER = DP / 32;  // elements of a lane
-        float v[PER] = {};
-#pragma unroll 8
-        for (int i = 0; i < n; ++i) {
-            const int64_t p = part_of(i) * ROWS + r;
-            const float2 ml = parts.ml[p];
-            const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
-            total += f * ml.y;
-            alignas(16) float po[PER];
-            if constexpr (PER == 4) *reinterpret_cast<float4*>(po) = reinterpret_cast<const float4*>(parts.o + p * DP)[lane];
-            else *reinterpret_cast<float2*>(po) = reinterpret_cast<const float2*>(parts.o + p * DP)[lane];
-#pragma unroll
-            for (int e = 0; e < PER; ++e) v[e] += f * po[e];
-        }
-        const int64_t tok = s.first + token;
-        const int h = at.y * a.group + in % a.group;
-        const float inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
-        uint16_t* out = a.out + tok * a.os[0] + h * a.os[1] + lane * PER;
-        if (lane * PER < c.dim) {
-#pragma unroll
-            for (int e = 0; e < PER; e += 2) *reinterpret_cast<uint32_t*>(out + e) = pack2<T>(v[e] * inv, v[e + 1] * inv);
-        }
-        if (lane == 0) a.lse[tok * a.heads + h] = (top + log2f(total)) * 0.6931471805599453f;
-    }
 }
 
 // Weights that the rows of the step path gave each slot, from the scores that the step kernel left; one thread per slot.

@@ -7,7 +7,7 @@
 //
 // A unit is a pair of slot tiles (2 x 128, one per warpgroup) against one row tile. Units run row tile by row tile within
 // a pair, the pair's keys stay in shared memory and the rows stream; the units of all (sequence, kv head, pair)s are laid
-// end to end and shared out equally. A pair that is cut leaves parts, added up in order by kv_weights_join_kernel.
+// end to end and shared out equally, and cut pairs are finished from parts, as in the step kernel.
 //
 // Bound: one exponential per (row, slot), 16 a clock and SM on the special function units (1,024 cycles per 128 x 128
 // tile against 512 for its product at a head size of 128).
@@ -56,7 +56,8 @@ struct WeightsShape {
 struct WeightsSegment {
     KvSeq s;
     int b, head, pair, q0, count;
-    bool whole_from, whole_to;  // begins at the pair's first unit; ends at its last
+    bool leaves;                // begins behind the pair's first unit
+    int rest;                   // units of the pair behind it
     bool both;                  // the second tile has slots
 };
 struct WeightsWalk {
@@ -95,8 +96,8 @@ struct WeightsWalk {
         g->pair = pair;
         g->q0 = shape.first(s, pair) + skip;
         g->count = (int)min((int64_t)(tiles - skip), share.left);
-        g->whole_from = skip == 0;
-        g->whole_to = skip + g->count == tiles;
+        g->leaves = skip > 0;
+        g->rest = tiles - skip - g->count;
         g->both = min((int64_t)s.len, shape.width) > (int64_t)pair * WEIGHTS_PAIR + CHUNK_SLOTS;
         share.left -= g->count;
         skip = 0;
@@ -151,8 +152,6 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         return shape.takes(s) ? shape.before(s, shape.pairs(s)) * c.heads : 0;
     });
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (threadIdx.x < 2) parts.at[2 * blockIdx.x + threadIdx.x].w = PART_NONE;
-    __syncthreads();
     tmem_fence_after();
     const uint32_t tm = *tmem_at;
     KvWait wait{c.status};
@@ -212,6 +211,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         }
     } else if (warp == 8) {
         const uint32_t idesc = umma_idesc<T>(CHUNK_ROWS, false, a.scale < 0.f);
+        const uint32_t k_low = umma_low(smem_u32(smem_k), 16), q_low = umma_low(smem_u32(ring), 16);
         int slot = 0, buf = 0;
         uint32_t phase = 0, k_phase = 0, buf_phase[2] = {0, 0};  // of the first or second warpgroup's buffers
         int used[2] = {0, 0};
@@ -227,12 +227,11 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                     wait(s_empty + 2 * i + buf, buf_phase[i] ^ 1);
                     tmem_fence_after();
                     if (lane == 0) {
-                        const uint32_t k = smem_u32(smem_k) + i * SLOT, rows = smem_u32(ring) + slot * SLOT;
+                        const uint32_t k = k_low + i * (SLOT / 16), rows = q_low + slot * (SLOT / 16);
 #pragma unroll
                         for (int e = 0; e < KS; ++e) {
-                            const uint32_t off = (e >> 2) * (CHUNK_ROWS * 128) + (e & 3) * 32;
-                            umma_ss(tm + (2 * i + buf) * 128, umma_desc(k + off, 16, 1024), umma_desc(rows + off, 16, 1024),
-                                    idesc, e > 0);
+                            const uint32_t off = (e >> 2) * (CHUNK_ROWS * 8) + (e & 3) * 2;
+                            umma_ss(tm + (2 * i + buf) * 128, umma_desc(k + off), umma_desc(rows + off), idesc, e > 0);
                         }
                         umma_commit(s_full + 2 * i + buf);
                     }
@@ -251,7 +250,6 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         float* lse = s_lse + i * 256;
         const float scale = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-37f);
         int used = 0;
-        bool first_segment = true;
         while (walk.next(&g)) {
             if (i == 0 || g.both) {
                 const int j = g.pair * WEIGHTS_PAIR + i * CHUNK_SLOTS + r;
@@ -297,20 +295,22 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                     }
                     sum += (part[0] + part[1]) + (part[2] + part[3]);
                 }
-                if (j < min((int64_t)g.s.len, a.scores_width)) {
-                    if (g.whole_from && g.whole_to) {
-                        a.scores[g.b * a.ss[0] + g.head * a.ss[1] + j] += sum;
-                    } else {
-                        const int part = 2 * blockIdx.x + (first_segment ? 0 : 1);
-                        parts.o[(int64_t)part * WEIGHTS_PAIR + i * CHUNK_SLOTS + r] = sum;
+                const int part = 2 * blockIdx.x + i;
+                if (g.leaves) {
+                    parts.o[(int64_t)part * CHUNK_SLOTS + r] = sum;
+                    asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+                    if (r == 0) part_publish(parts, part);
+                } else {
+                    const int follow = walk.share.followers(g.rest);
+                    if (follow) {
+                        for (int k = r; k < follow; k += 128) part_await(parts, part + 2 + 2 * k, wait);
+                        asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+                        for (int k = 0; k < follow; ++k) sum += __ldcg(parts.o + (int64_t)(part + 2 + 2 * k) * CHUNK_SLOTS + r);
+                        for (int k = r; k < follow; k += 128) parts.ready[part + 2 + 2 * k] = 0;
                     }
+                    if (j < min((int64_t)g.s.len, a.scores_width)) a.scores[g.b * a.ss[0] + g.head * a.ss[1] + j] += sum;
                 }
-                if (threadIdx.x == 0 && !(g.whole_from && g.whole_to))
-                    parts.at[2 * blockIdx.x + (first_segment ? 0 : 1)] =
-                        make_int4(g.b, g.head, g.pair,
-                                  PART_HELD | (g.whole_from ? PART_FIRST : 0) | (g.whole_to ? PART_LAST : 0));
             }
-            first_segment = false;
         }
     }
     __syncthreads();
@@ -318,24 +318,6 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         tmem_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm) : "memory");
     }
-}
-
-// Adds up the parts of cut pairs, one thread per slot; as kv_join_kernel.
-__global__ void __launch_bounds__(WEIGHTS_PAIR) kv_weights_join_kernel(KvPages c, KvBatch bt, KvAttend a, KvParts parts,
-                                                                       int ctas) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int4 at = parts.at[blockIdx.x];
-    if (!(at.w & PART_FIRST)) return;
-    const KvSeq s = kv_seq(c, bt, at.x);
-    const int64_t j = (int64_t)at.z * WEIGHTS_PAIR + threadIdx.x;
-    if (j >= s.len || j >= a.scores_width) return;
-    float sum = parts.o[(int64_t)blockIdx.x * WEIGHTS_PAIR + threadIdx.x];
-    bool last = at.w & PART_LAST;
-    for (int cta = blockIdx.x / 2 + 1; !last && cta < ctas; ++cta) {
-        last = parts.at[2 * cta].w & PART_LAST;
-        sum += parts.o[(int64_t)2 * cta * WEIGHTS_PAIR + threadIdx.x];
-    }
-    a.scores[at.x * a.ss[0] + at.y * a.ss[1] + j] += sum;
 }
 
 }  // namespace vk

@@ -10,15 +10,36 @@ sequence, made e.g. from a search's ids, says which pages it reads.
 All tensors are torch tensors on the cache's device. Sequence b of a call has the new tokens offsets[b]:offsets[b + 1]
 (int32, [batch + 1]), lens[b] slots with the new tokens included (int32, [batch]) and the pages table[b] (int32,
 [batch, width]; entries past its last slot are not read). Calls are asynchronous on `stream` (a torch.cuda.Stream or raw
-handle; default: the current stream); sync() waits and raises what the kernels found wrong. One cache serves one call at
-a time. No derivatives: a cache is for inference.
+handle; default: the current stream); sync() waits and raises what the kernels found wrong. The calls
+of one stream share their working memory. No derivatives: a cache is for inference.
 """
 from __future__ import annotations
 
 import ctypes as C
 
 from . import _native as N
-from ._native import check, lib
+from ._native import VkError, check, lib
+
+# Attention's working memory by (device, stream): the calls of a stream share one tensor, which grows and whose start is
+# zero between calls. Tensors that were outgrown are kept: a captured graph may hold their addresses.
+_WORK: dict = {}
+_OUTGROWN: list = []
+_ZEROED = 8192  # VK_KV_WORKSPACE_ZEROED
+
+
+def _workspace(torch, device, stream: int, need: int):
+    key = (device.index, stream)
+    work = _WORK.get(key)
+    if work is None or work.numel() < need:
+        if work is not None:
+            _OUTGROWN.append(work)
+            need = max(need, work.numel() * 3 // 2)
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+            work = torch.empty((need,), dtype=torch.uint8, device=device)
+            work[:_ZEROED].zero_()
+        _WORK[key] = work
+    return work
+
 
 _DTYPES = {"torch.float16": N.VK_KV_F16, "torch.bfloat16": N.VK_KV_BF16}
 
@@ -57,7 +78,7 @@ class PagedCache:
                      k_stride=(C.c_int64 * 3)(*k_pages.stride()[:3]), v=v_pages.data_ptr(),
                      v_stride=(C.c_int64 * 3)(*v_pages.stride()[:3]))
         check(lib().vk_kv_create(C.byref(d), C.byref(self._h)), "vk_kv_create")
-        self._workspaces = {}  # bytes by sizes
+        self._sizes = {}  # bytes of attention's working memory by what they depend on
         # argument structs, filled anew by every call
         self._batch, self._attend, self._evict = N.KvBatch(), N.KvAttend(), N.KvEvict()
         self._batch_ref, self._attend_ref, self._evict_ref = (C.byref(x) for x in
@@ -89,7 +110,7 @@ class PagedCache:
 
     def _stream(self, stream):
         if stream is None:
-            return self._torch.cuda.current_stream(self.device).cuda_stream
+            return self._torch._C._cuda_getCurrentRawStream(self.device.index)
         return getattr(stream, "cuda_stream", stream)
 
     def append(self, k, v, offsets, table, lens, *, stream=None) -> None:
@@ -142,16 +163,17 @@ class PagedCache:
         a.heads, a.max_q, a.causal = heads, max_q, causal
         a.scale = self.head_dim ** -0.5 if scale is None else scale
         sizes = (n, self._batch.table_width, tokens, heads, max_q, scores is not None)
-        need = self._workspaces.get(sizes)
+        need = self._sizes.get(sizes)
         if need is None:
             size = C.c_size_t()
             check(lib().vk_kv_attend_workspace(self._h, self._batch_ref, self._attend_ref, C.byref(size)), "attend")
-            if len(self._workspaces) >= 4096:
-                self._workspaces.clear()
-            need = self._workspaces[sizes] = size.value
-        work = torch.empty((need,), dtype=torch.uint8, device=self.device)
-        a.workspace, a.workspace_bytes = work.data_ptr(), need
-        check(lib().vk_kv_attend(self._h, self._batch_ref, self._attend_ref, self._stream(stream)), "attend")
+            if len(self._sizes) >= 4096:
+                self._sizes.clear()
+            need = self._sizes[sizes] = size.value
+        s = self._stream(stream)
+        work = _workspace(torch, self.device, s, need)
+        a.workspace, a.workspace_bytes = work.data_ptr(), work.numel()
+        check(lib().vk_kv_attend(self._h, self._batch_ref, self._attend_ref, s), "attend")
         return out, lse
 
     def evict(self, table, lens, new_table, keep: int, recent: int, scores, *, stream=None):
@@ -186,7 +208,13 @@ class PagedCache:
 
     def sync(self, stream=None) -> None:
         """Waits for the cache's work on the stream and raises VkError for anything its kernels found wrong."""
-        check(lib().vk_kv_sync(self._h, self._stream(stream)), "sync")
+        s = self._stream(stream)
+        try:
+            check(lib().vk_kv_sync(self._h, s), "sync")
+        except VkError as e:
+            if e.code == N.VK_ERR_DEVICE:  # an aborted call may have left the working memory's start in any state
+                _WORK.pop((self.device.index, s), None)
+            raise
 
     def close(self) -> None:
         if self._h:
