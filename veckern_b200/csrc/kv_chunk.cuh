@@ -470,6 +470,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 #pragma unroll 1
                     for (int e = 0; e < c.dim; e += 32) {
                         float o[32];
+                        __syncwarp();
                         tmem_ld32(tm_o + e, o);
                         tmem_wait_ld();
                         uint32_t w[32];
@@ -496,6 +497,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                         else sum0 = sum0 + pair_of(w.x, w.y);
                         p[e] = pack2<T>(w.x, w.y);
                     }
+                    __syncwarp();
                     tmem_st32(tm_s + 32 * half, p);
                     tmem_wait_st();
                     tmem_fence_before();
@@ -551,6 +553,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 #pragma unroll 1
             for (int e = 0; e < c.dim; e += 32) {
                 float o[32];
+                __syncwarp();  // lanes without a row come from another path
                 tmem_ld32(tm_o + e, o);
                 tmem_wait_ld();
 #pragma unroll
@@ -606,6 +609,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     }
     __syncthreads();
     if (warp == 8) {
+        __syncwarp();
         tmem_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm) : "memory");
     }

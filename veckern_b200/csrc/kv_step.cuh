@@ -58,7 +58,8 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 }
 
 // Bounded waits of one thread or warp: after the first that runs out, the later ones return at once, so that the CTA
-// unwinds; what it computes then is void and the status word says so.
+// unwinds; what it computes then is void and the status word says so. Called by whole warps, which leave it together: what
+// follows is often an instruction that all lanes have to execute as one.
 struct KvWait {
     int* status;
     bool dead = false;
@@ -67,6 +68,7 @@ struct KvWait {
             dead = true;
             atomicOr(status, ERR_WAIT_TIMEOUT);
         }
+        __syncwarp();
     }
 };
 

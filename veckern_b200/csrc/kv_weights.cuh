@@ -315,6 +315,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     }
     __syncthreads();
     if (warp == 8) {
+        __syncwarp();
         tmem_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm) : "memory");
     }
