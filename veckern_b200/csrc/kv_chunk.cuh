@@ -47,12 +47,19 @@ __device__ __forceinline__ void tma_rows(void* dst, const CUtensorMap* map, int 
 
 // ---- tcgen05
 // A descriptor's low word holds the operand's address and leading offset in units of 16 bytes, so that the next step's
-// operand is one 32-bit addition away; the high word is constant. The thread that issues the products is alone with
-// them: with whole descriptors made per product it was the kernel's bound.
+// operand is one 32-bit addition away; the high word is constant: 8-row groups 1,024 bytes apart, descriptor version 1,
+// 128-byte swizzle.
+//
+// The instructions below are reached by a whole warp and take effect for the lane that `me` is nonzero in. Issued inside
+// a branch of that lane instead, every operand was moved from the lane's to the warp's registers anew, about 100 cycles
+// per product: the warp that issues them was the kernel's bound (4,096 tokens over 16,384 slots, 32 heads over 8:
+// 1,105 us then, 770 now).
+constexpr uint32_t UMMA_HIGH = 1024u >> 4 | 1u << 14 | 2u << 29;
 __device__ __forceinline__ uint32_t umma_low(uint32_t addr, uint32_t lead) { return addr >> 4 | (lead >> 4) << 16; }
-__device__ __forceinline__ uint64_t umma_desc(uint32_t low) {
-    // 8-row groups 1,024 bytes apart, descriptor version 1, 128-byte swizzle
-    return (uint64_t)(1024u >> 4 | 1u << 14 | 2u << 29) << 32 | low;
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t me;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(me));
+    return me;
 }
 template <typename T>
 __device__ __forceinline__ uint32_t umma_idesc(int n, bool b_by_rows, bool negate) {
@@ -60,24 +67,30 @@ __device__ __forceinline__ uint32_t umma_idesc(int n, bool b_by_rows, bool negat
     return 1u << 4 | type << 7 | type << 10 | (negate ? 1u << 13 : 0u) | (b_by_rows ? 1u << 16 : 0u) |
            (uint32_t)(n >> 3) << 17 | (uint32_t)(CHUNK_ROWS >> 4) << 24;
 }
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add, uint32_t me) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+        "mov.b64 da, {%1, %6};\n\tmov.b64 db, {%2, %6};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "r"(me), "n"(UMMA_HIGH)
         : "memory");
 }
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+// A from tensor memory.
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add, uint32_t me) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\tsetp.ne.u32 p, %4, 0;\n\tsetp.ne.u32 q, %5, 0;\n\t"
+        "mov.b64 db, {%2, %6};\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "r"(me), "n"(UMMA_HIGH)
         : "memory");
 }
-// The barrier gets an arrival when all products that this thread issued so far are done.
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
+// The barrier gets an arrival when all products that this lane issued so far are done.
+__device__ __forceinline__ void umma_commit(uint64_t* bar, uint32_t me) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+        "r"(me)
+        : "memory");
 }
 __device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -266,7 +279,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     uint64_t* o_full = p_full + 4;
     int64_t* scratch = reinterpret_cast<int64_t*>(o_full + 2);  // THREADS / 32 + 2
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(scratch + CHUNK_THREADS / 32 + 2);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < RING; ++i) {
             mbar_init(kv_full + i, 1);
@@ -299,13 +312,13 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     });
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     tmem_fence_after();
-    const uint32_t tm = *tmem_at;
+    const uint32_t tm = __shfl_sync(FULL, *tmem_at, 0);
     KvWait wait{c.status};
     ChunkWalk walk{c, bt, shape, share, 0, 0, 0, false};
     ChunkSegment g;
-    // 384 threads start with 168 registers: 2 x 128 x 216 + 128 x 72 is the same sum
+    // 384 threads start with 168 registers: 2 x 128 x 200 + 128 x 104 is the same sum
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         // The ring's n-th fill; a segment's tiles come as keys, values, keys, values.
         int fill = 0;
         auto at = [&](int n) { return n % RING; };
@@ -355,44 +368,44 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                         atomicOr(c.status, ERR_DRAIN_TIMEOUT);
         } else if (warp == 8) {
             uint32_t q_phase = 0, p_phase = 0;  // p_phase: bit per tile
-            const int ks = (c.dim + 15) / 16;   // steps of 16 elements; the padding's products are left out
+            const uint32_t me = elect_lane();
+            const int ks = (c.dim + 15) / 16;  // steps of 16 elements; the padding's products are left out
             const uint32_t idesc_s = umma_idesc<T>(CHUNK_SLOTS, false, a.scale < 0.f);
             const uint32_t idesc_o = umma_idesc<T>(ks * 16, true, false);
             const uint32_t q_low = umma_low(smem_u32(smem_q), 16), k_low = umma_low(smem_u32(ring), 16);
             const uint32_t v_low = umma_low(smem_u32(ring), CHUNK_SLOTS * 128);
             while (walk.next(&g)) {
-                const int step = g.lone ? 4 : 2;
+                const bool lone = __shfl_sync(FULL, g.lone, 0);
+                const int count = __shfl_sync(FULL, g.count, 0), step = lone ? 4 : 2;
                 // keys of tile i's part of unit u of this segment, and its values the fill after it
-                auto key_fill = [&](int u, int i) { return fill + u * step + (g.lone ? 2 * i : 0); };
+                auto key_fill = [&](int u, int i) { return fill + u * step + (lone ? 2 * i : 0); };
                 auto scores = [&](int u, int i) {  // S_i = Q_i K^T
                     const int n = key_fill(u, i), slot = at(n);
+                    const uint32_t q = q_low + (lone ? 0 : i * HALVES * (CHUNK_ROWS * 8)), k = k_low + slot * (SLOT / 16);
                     wait(kv_full + slot, parity(n));
                     tmem_fence_after();
-                    if (lane == 0) {
-                        const uint32_t q = q_low + (g.lone ? 0 : i * HALVES * (CHUNK_ROWS * 8)), k = k_low + slot * (SLOT / 16);
 #pragma unroll
-                        for (int e = 0; e < KS; ++e) {
-                            const uint32_t off = (e >> 2) * (CHUNK_ROWS * 8) + (e & 3) * 2;
-                            if (e < ks) umma_ss(tm + TM_S + i * 128, umma_desc(q + off), umma_desc(k + off), idesc_s, e > 0);
-                        }
-                        umma_commit(s_full + i);
-                        if (g.lone || i == 1) umma_commit(kv_empty + slot);
+                    for (int e = 0; e < KS; ++e) {
+                        const uint32_t off = (e >> 2) * (CHUNK_ROWS * 8) + (e & 3) * 2;
+                        if (e < ks) umma_ss(tm + TM_S + i * 128, q + off, k + off, idesc_s, e > 0, me);
                     }
-                    __syncwarp();
+                    umma_commit(s_full + i, me);
+                    if (lone || i == 1) umma_commit(kv_empty + slot, me);
                 };
                 wait(q_full, q_phase);
                 q_phase ^= 1;
                 scores(0, 0);
                 scores(0, 1);
-                if (g.count == 1 && lane == 0) umma_commit(q_empty);
-                for (int u = 0; u < g.count; ++u) {
-#pragma unroll 1
+                if (count == 1) umma_commit(q_empty, me);
+                for (int u = 0; u < count; ++u) {
+#pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const int n = key_fill(u, i) + 1, slot = at(n);
                         // slots of the sequence in this tile
-                        const int held = g.s.len - (g.lone ? 2 * (g.t0 + u) + i : g.t0 + u) * CHUNK_SLOTS;
+                        const int held = __shfl_sync(FULL, g.s.len - (lone ? 2 * (g.t0 + u) + i : g.t0 + u) * CHUNK_SLOTS, 0);
+                        const uint32_t v = v_low + slot * (SLOT / 16), p = tm + TM_S + i * 128, o = tm + TM_O + i * 128;
                         wait(kv_full + slot, parity(n));
-                        if (held > 0 && held < CHUNK_SLOTS && (held & 15) && (g.lone || i == 0)) {
+                        if (held > 0 && held < CHUNK_SLOTS && (held & 15) && (lone || i == 0)) {
                             // The page's slots past the sequence hold anything: none may meet a weight of zero. The
                             // product stops at the 16 slots that hold the last one; their rest is cleared.
                             for (int r = held; r < (held + 15) / 16 * 16; ++r)
@@ -402,30 +415,26 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                             fence_proxy_async_smem();
                             __syncwarp();
                         }
-                        const uint32_t v = v_low + slot * (SLOT / 16), p = tm + TM_S + i * 128, o = tm + TM_O + i * 128;
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
                             wait(p_full + 2 * i + half, p_phase >> i & 1);
                             tmem_fence_after();
-                            if (lane == 0)
 #pragma unroll
-                                for (int e = 4 * half; e < 4 * half + 4; ++e)
-                                    if (16 * e < held) umma_ts(o, p + e * 8, umma_desc(v + e * 128), idesc_o, u > 0 || e > 0);
-                            __syncwarp();
+                            for (int e = 4 * half; e < 4 * half + 4; ++e)
+                                if (16 * e < held) umma_ts(o, p + e * 8, v + e * 128, idesc_o, u > 0 || e > 0, me);
                         }
                         p_phase ^= 1u << i;
-                        if (lane == 0 && (g.lone || i == 1)) umma_commit(kv_empty + slot);
-                        if (u + 1 < g.count) scores(u + 1, i);
-                        else if (lane == 0) umma_commit(o_full + i);
+                        if (lone || i == 1) umma_commit(kv_empty + slot, me);
+                        if (u + 1 < count) scores(u + 1, i);
+                        else umma_commit(o_full + i, me);
                     }
-                    if (u + 2 == g.count && lane == 0) umma_commit(q_empty);
-                    __syncwarp();
+                    if (u + 2 == count) umma_commit(q_empty, me);
                 }
-                fill += g.count * step;
+                fill += count * step;
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         const int i = warp >> 2, r = (warp & 3) * 32 + lane;  // tile and row
         const uint32_t lanes = tm + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t tm_s = lanes + TM_S + i * 128, tm_o = lanes + TM_O + i * 128;
@@ -454,55 +463,66 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 #pragma unroll
                     for (int e = 0; e < CHUNK_SLOTS; ++e) x[e] = e < see ? x[e] : -INFINITY;
                 }
-                float top4[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-                for (int e = 4; e < CHUNK_SLOTS; e += 4)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) top4[k] = fmaxf(top4[k], x[e + k]);
-                const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3]));
-                const bool grow = (top - m) * scale > 8.f;  // m = -inf: unless all is masked
-                if (t == g.t0) {
-                    m = top;
-                } else if (__any_sync(FULL, grow)) {
-                    const float f = grow ? part_factor(m * scale, top * scale) : 1.f;
-                    if (grow) m = top;
-                    l *= f;
-#pragma unroll 1
-                    for (int e = 0; e < c.dim; e += 32) {
-                        float o[32];
-                        __syncwarp();
-                        tmem_ld32(tm_o + e, o);
-                        tmem_wait_ld();
-                        uint32_t w[32];
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) w[k] = __float_as_uint(o[k] * f);
-                        tmem_st32(tm_o + e, w);
-                    }
-                }
-                const float ref = m == -INFINITY ? 0.f : m * scale;
-                const Pair scale2 = pair_of(scale, scale), ref2 = pair_of(-ref, -ref);
-                Pair sum0 = pair_of(0.f, 0.f), sum1 = sum0;
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t p[32];
+                // The first half's weights are taken against the reference so far, the maximum beside them; only where it
+                // has outgrown the reference they are taken again.
+                float ref = m == -INFINITY ? 0.f : m * scale;
+                const Pair scale2 = pair_of(scale, scale);
+                Pair sum0, sum1;
+                uint32_t p[32];
+                auto weights = [&](int from) {
+                    const Pair ref2 = pair_of(-ref, -ref);
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
-                        const int k = 64 * half + 2 * e;
-                        const Pair y = fma2(pair_of(x[k], x[k + 1]), scale2, ref2);
-                        float2 w = floats(y);
-                        // masked slots need the hardware's 2^-inf = 0
-                        if (e % 8 < CHUNK_POLY && !masked) w = exp2_poly(y);
-                        else w = make_float2(ex2(w.x), ex2(w.y));
+                        const Pair y = fma2(pair_of(x[from + 2 * e], x[from + 2 * e + 1]), scale2, ref2);
+                        const float2 z = floats(y), w = make_float2(ex2(z.x), ex2(z.y));
                         if (e & 1) sum1 = sum1 + pair_of(w.x, w.y);
                         else sum0 = sum0 + pair_of(w.x, w.y);
                         p[e] = pack2<T>(w.x, w.y);
                     }
+                };
+                auto hand_over = [&](int half) {
                     __syncwarp();
                     tmem_st32(tm_s + 32 * half, p);
                     tmem_wait_st();
                     tmem_fence_before();
                     mbar_arrive(p_full + 2 * i + half);
+                };
+                sum0 = sum1 = pair_of(0.f, 0.f);
+                weights(0);
+                float top = fmaxf(x[0], x[1]), top_b = fmaxf(x[2], x[3]);
+#pragma unroll
+                for (int e = 4; e < CHUNK_SLOTS; e += 4) {
+                    top = fmaxf(fmaxf(top, x[e]), x[e + 1]);
+                    top_b = fmaxf(fmaxf(top_b, x[e + 2]), x[e + 3]);
                 }
+                top = fmaxf(top, top_b);
+                const bool grow = (top - m) * scale > 8.f;  // m = -inf: unless all is masked
+                if (__any_sync(FULL, grow)) {
+                    const float f = grow ? part_factor(m * scale, top * scale) : 1.f;
+                    if (grow) {
+                        m = top;
+                        ref = m * scale;
+                    }
+                    l *= f;
+                    if (t > g.t0) {
+#pragma unroll 1
+                        for (int e = 0; e < c.dim; e += 32) {
+                            float o[32];
+                            __syncwarp();
+                            tmem_ld32(tm_o + e, o);
+                            tmem_wait_ld();
+                            uint32_t w[32];
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) w[k] = __float_as_uint(o[k] * f);
+                            tmem_st32(tm_o + e, w);
+                        }
+                    }
+                    sum0 = sum1 = pair_of(0.f, 0.f);
+                    weights(0);
+                }
+                hand_over(0);
+                weights(64);
+                hand_over(1);
                 const float2 sum = floats(sum0 + sum1);
                 l += sum.x + sum.y;
             }

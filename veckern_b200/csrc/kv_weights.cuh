@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     uint64_t* s_empty = s_full + 4;
     int64_t* scratch = reinterpret_cast<int64_t*>(s_empty + 4);
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(scratch + CHUNK_THREADS / 32 + 2);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < RING; ++i) {
             mbar_init(q_full + i, 1);
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     });
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     tmem_fence_after();
-    const uint32_t tm = *tmem_at;
+    const uint32_t tm = __shfl_sync(FULL, *tmem_at, 0);
     KvWait wait{c.status};
     WeightsWalk walk{c, bt, shape, share, 0, 0, 0, false};
     WeightsSegment g;
@@ -212,37 +212,37 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     } else if (warp == 8) {
         const uint32_t idesc = umma_idesc<T>(CHUNK_ROWS, false, a.scale < 0.f);
         const uint32_t k_low = umma_low(smem_u32(smem_k), 16), q_low = umma_low(smem_u32(ring), 16);
-        int slot = 0, buf = 0;
-        uint32_t phase = 0, k_phase = 0, buf_phase[2] = {0, 0};  // of the first or second warpgroup's buffers
-        int used[2] = {0, 0};
+        int slot = 0, used[2] = {0, 0};  // row tiles that went to each warpgroup's two buffers
+        uint32_t phase = 0, k_phase = 0;
+        const uint32_t me = elect_lane();
+        const int ks = (c.dim + 15) / 16;  // steps of 16 elements; the padding's products are left out
         while (walk.next(&g)) {
+            const bool both = __shfl_sync(FULL, g.both, 0);
+            const int count = __shfl_sync(FULL, g.count, 0);
             wait(k_full, k_phase);
             k_phase ^= 1;
-            for (int q = 0; q < g.count; ++q) {
+            for (int q = 0; q < count; ++q) {
                 wait(q_full + slot, phase);
-                for (int i = 0; i < (g.both ? 2 : 1); ++i) {
-                    buf = used[i] & 1;
-                    buf_phase[i] = (used[i] >> 1) & 1;
-                    ++used[i];
-                    wait(s_empty + 2 * i + buf, buf_phase[i] ^ 1);
-                    tmem_fence_after();
-                    if (lane == 0) {
-                        const uint32_t k = k_low + i * (SLOT / 16), rows = q_low + slot * (SLOT / 16);
+                const uint32_t rows = q_low + slot * (SLOT / 16);
 #pragma unroll
-                        for (int e = 0; e < KS; ++e) {
-                            const uint32_t off = (e >> 2) * (CHUNK_ROWS * 8) + (e & 3) * 2;
-                            umma_ss(tm + (2 * i + buf) * 128, umma_desc(k + off), umma_desc(rows + off), idesc, e > 0);
-                        }
-                        umma_commit(s_full + 2 * i + buf);
+                for (int i = 0; i < 2; ++i) {
+                    if (i == 1 && !both) continue;
+                    const int buf = used[i] & 1;
+                    const uint32_t at = tm + (2 * i + buf) * 128, k = k_low + i * (SLOT / 16);
+                    wait(s_empty + 2 * i + buf, (used[i] >> 1 & 1) ^ 1);
+                    tmem_fence_after();
+                    ++used[i];
+#pragma unroll
+                    for (int e = 0; e < KS; ++e) {
+                        const uint32_t off = (e >> 2) * (CHUNK_ROWS * 8) + (e & 3) * 2;
+                        if (e < ks) umma_ss(at, k + off, rows + off, idesc, e > 0, me);
                     }
-                    __syncwarp();
+                    umma_commit(s_full + 2 * i + buf, me);
                 }
-                if (lane == 0) umma_commit(q_empty + slot);
-                __syncwarp();
+                umma_commit(q_empty + slot, me);
                 if (++slot == RING) slot = 0, phase ^= 1;
             }
-            if (lane == 0) umma_commit(k_empty);
-            __syncwarp();
+            umma_commit(k_empty, me);
         }
     } else if (warp < 8) {
         const int i = warp >> 2, r = (warp & 3) * 32 + lane;
