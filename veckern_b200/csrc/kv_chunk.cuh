@@ -12,9 +12,13 @@
 // O stays in tensor memory; it is rescaled only when a row's maximum has grown by more than 2^8 since the reference that
 // its weights use, which the sums allow (weights up to 256 in 16 bits keep their relative precision).
 //
-// Bound: 4 x 128 x 128 x head size operations per tile and unit on the tensor cores (1,024 cycles at a head size of 128),
-// their operands from shared memory (8 KB per 64-cycle product of S: all of its 128 bytes a clock), and 128 x 128
-// exponentials: 1,024 cycles on the special function units, which is why a part of them is computed by a polynomial.
+// Bound: 4 x 128 x 128 x head size operations per tile and unit on the tensor cores (1,024 cycles at a head size of 128)
+// and 128 x 128 exponentials on the special function units (1,024 cycles as well). Tensor memory holds S and O of two
+// tiles and no more, so a tile's products wait for its weights and the other way round: a unit takes as long as one tile's
+// weights (1,400 cycles), its products (1,200) and the hand-overs between them (800), while the other tile fills the gaps.
+// Measured (4,096 tokens over 16,384 slots, 32 heads over 8, head size 128): 752 us, 1,280 TFLOP/s, in a short run at
+// 1.8 GHz. What did not pay: a part of the exponentials by a polynomial (1 in 8: 758 us, 2 in 8: 777), the weights handed
+// over in two halves (770), a warp of its own for each tile's products (920; taking turns 781).
 #pragma once
 #include "kv_step.cuh"
 
@@ -29,8 +33,6 @@ template <int DP>
 constexpr int CHUNK_SLOT = CHUNK_SLOTS * DP * 2;   // bytes of a tile of keys or values
 template <int DP>
 constexpr int CHUNK_RING = DP == 128 ? 5 : 10;     // tiles in flight, keys and values alternating
-// Pairs of exponentials of every 8 that the polynomial takes.
-constexpr int CHUNK_POLY = 2;
 template <int DP>
 constexpr int chunk_smem() {
     return CHUNK_Q<DP> + CHUNK_RING<DP> * CHUNK_SLOT<DP> + CHUNK_ROWS * 8 + 512;
@@ -109,6 +111,12 @@ __device__ __forceinline__ void tmem_ld32(uint32_t at, float* x) {
         : VK_R8(x, 0), VK_R8(x, 8), VK_R8(x, 16), VK_R8(x, 24)
         : "r"(at));
 }
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* x) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at),
+        VK_W8(x, 0), VK_W8(x, 8)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_st32(uint32_t at, const uint32_t* x) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
@@ -141,26 +149,6 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p.v) : "l"(a.v), "l"(b.v), "l"(c.v));
     return p;
 }
-// 2^x without the special function units, x at most 127: x = j + f with j whole and |f| <= 1/2 (adding and taking away
-// 1.5 x 2^23 rounds to whole), 2^f by the degree-5 polynomial of least largest relative error on [-1/2, 1/2] (Remez
-// exchange; 2.1e-7 in 32-bit arithmetic, as the hardware's approximation), j added to the exponent. Below -126: 2^-126.
-__device__ __forceinline__ float2 exp2_poly(Pair x) {
-    float2 y = floats(x);
-    const Pair t = pair_of(fmaxf(y.x, -126.f), fmaxf(y.y, -126.f));
-    const Pair big = pair_of(12582912.f, 12582912.f), minus = pair_of(-12582912.f, -12582912.f);
-    const Pair z = t + big, j = z + minus, f = fma2(j, pair_of(-1.f, -1.f), t);
-    Pair p = pair_of(1.32764725e-3f, 1.32764725e-3f);
-    p = fma2(p, f, pair_of(9.67554096e-3f, 9.67554096e-3f));
-    p = fma2(p, f, pair_of(5.55071309e-2f, 5.55071309e-2f));
-    p = fma2(p, f, pair_of(2.40221202e-1f, 2.40221202e-1f));
-    p = fma2(p, f, pair_of(6.93146944e-1f, 6.93146944e-1f));
-    p = fma2(p, f, pair_of(1.00000012f, 1.00000012f));
-    const float2 r = floats(p), w = floats(z);
-    // z's low bits hold j (in two's complement); shifting leaves them where the exponent is
-    return make_float2(__int_as_float(__float_as_int(r.x) + (__float_as_int(w.x) << 23)),
-                       __int_as_float(__float_as_int(r.y) + (__float_as_int(w.y) << 23)));
-}
-
 // ---- the order of units
 // sum of floor((a i + b) / m) over 0 <= i < n, by Euclid's steps on (m, a); a, b >= 0
 __device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
@@ -275,8 +263,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     uint64_t* q_full = kv_empty + RING;
     uint64_t* q_empty = q_full + 1;
     uint64_t* s_full = q_empty + 1;  // [tile]
-    uint64_t* p_full = s_full + 2;   // [tile][half of the slots]
-    uint64_t* o_full = p_full + 4;
+    uint64_t* p_full = s_full + 2;
+    uint64_t* o_full = p_full + 2;
     int64_t* scratch = reinterpret_cast<int64_t*>(o_full + 2);  // THREADS / 32 + 2
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(scratch + CHUNK_THREADS / 32 + 2);
     const int warp = __shfl_sync(FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -289,8 +277,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         mbar_init(q_empty, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(s_full + i, 1);
-            mbar_init(p_full + 2 * i, 128);
-            mbar_init(p_full + 2 * i + 1, 128);
+            mbar_init(p_full + i, 4);
             mbar_init(o_full + i, 1);
         }
         fence_mbar_init();
@@ -382,12 +369,20 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                 auto scores = [&](int u, int i) {  // S_i = Q_i K^T
                     const int n = key_fill(u, i), slot = at(n);
                     const uint32_t q = q_low + (lone ? 0 : i * HALVES * (CHUNK_ROWS * 8)), k = k_low + slot * (SLOT / 16);
-                    wait(kv_full + slot, parity(n));
+                    if (lone || i == 0) wait(kv_full + slot, parity(n));
                     tmem_fence_after();
+                    if (ks == KS) {
 #pragma unroll
-                    for (int e = 0; e < KS; ++e) {
-                        const uint32_t off = (e >> 2) * (CHUNK_ROWS * 8) + (e & 3) * 2;
-                        if (e < ks) umma_ss(tm + TM_S + i * 128, q + off, k + off, idesc_s, e > 0, me);
+                        for (int e = 0; e < KS; ++e) {
+                            const uint32_t off = (e >> 2) * (CHUNK_ROWS * 8) + (e & 3) * 2;
+                            umma_ss(tm + TM_S + i * 128, q + off, k + off, idesc_s, e > 0, me);
+                        }
+                    } else {
+#pragma unroll 1
+                        for (int e = 0; e < ks; ++e) {
+                            const uint32_t off = (e >> 2) * (CHUNK_ROWS * 8) + (e & 3) * 2;
+                            umma_ss(tm + TM_S + i * 128, q + off, k + off, idesc_s, e > 0, me);
+                        }
                     }
                     umma_commit(s_full + i, me);
                     if (lone || i == 1) umma_commit(kv_empty + slot, me);
@@ -404,7 +399,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                         // slots of the sequence in this tile
                         const int held = __shfl_sync(FULL, g.s.len - (lone ? 2 * (g.t0 + u) + i : g.t0 + u) * CHUNK_SLOTS, 0);
                         const uint32_t v = v_low + slot * (SLOT / 16), p = tm + TM_S + i * 128, o = tm + TM_O + i * 128;
-                        wait(kv_full + slot, parity(n));
+                        if (lone || i == 0) wait(kv_full + slot, parity(n));
                         if (held > 0 && held < CHUNK_SLOTS && (held & 15) && (lone || i == 0)) {
                             // The page's slots past the sequence hold anything: none may meet a weight of zero. The
                             // product stops at the 16 slots that hold the last one; their rest is cleared.
@@ -415,13 +410,16 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                             fence_proxy_async_smem();
                             __syncwarp();
                         }
+                        wait(p_full + i, p_phase >> i & 1);
+                        tmem_fence_after();
+                        if (held >= CHUNK_SLOTS) {
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            wait(p_full + 2 * i + half, p_phase >> i & 1);
-                            tmem_fence_after();
-#pragma unroll
-                            for (int e = 4 * half; e < 4 * half + 4; ++e)
-                                if (16 * e < held) umma_ts(o, p + e * 8, v + e * 128, idesc_o, u > 0 || e > 0, me);
+                            for (int e = 0; e < CHUNK_SLOTS / 16; ++e)
+                                umma_ts(o, p + e * 8, v + e * 128, idesc_o, u > 0 || e > 0, me);
+                        } else {
+#pragma unroll 1
+                            for (int e = 0; 16 * e < held; ++e)
+                                umma_ts(o, p + e * 8, v + e * 128, idesc_o, u > 0 || e > 0, me);
                         }
                         p_phase ^= 1u << i;
                         if (lone || i == 1) umma_commit(kv_empty + slot, me);
@@ -447,7 +445,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             const bool live = r < shape.tokens * a.group && token < g.s.count;
             const int lim = live ? max(0, row_limit(g.s, a.causal, token)) : 0;
             const int open = max(0, min(g.s.len, row_limit(g.s, a.causal, token1)));  // slots that every row sees
-            float m = -INFINITY, l = 0.f;
+            float ref = 0.f, l = 0.f;  // base 2
             for (int t = g.t0; t < g.t0 + g.count; ++t) {
                 const int slot0 = (g.lone ? 2 * t + i : t) * CHUNK_SLOTS;
                 float x[CHUNK_SLOTS];
@@ -463,48 +461,45 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 #pragma unroll
                     for (int e = 0; e < CHUNK_SLOTS; ++e) x[e] = e < see ? x[e] : -INFINITY;
                 }
-                // The first half's weights are taken against the reference so far, the maximum beside them; only where it
-                // has outgrown the reference they are taken again.
-                float ref = m == -INFINITY ? 0.f : m * scale;
+                // Weights are taken against the reference so far. Their sum says whether one may have outgrown 2^8; only
+                // then, and in a segment's first tile, is the maximum looked for and the reference moved. (A row that
+                // sees nothing of its first tile sees nothing of the later ones.)
                 const Pair scale2 = pair_of(scale, scale);
-                Pair sum0, sum1;
-                uint32_t p[32];
-                auto weights = [&](int from) {
+                float sum = 0.f;
+                auto weights = [&] {
                     const Pair ref2 = pair_of(-ref, -ref);
+                    Pair part[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const Pair y = fma2(pair_of(x[from + 2 * e], x[from + 2 * e + 1]), scale2, ref2);
-                        const float2 z = floats(y), w = make_float2(ex2(z.x), ex2(z.y));
-                        if (e & 1) sum1 = sum1 + pair_of(w.x, w.y);
-                        else sum0 = sum0 + pair_of(w.x, w.y);
-                        p[e] = pack2<T>(w.x, w.y);
-                    }
-                };
-                auto hand_over = [&](int half) {
-                    __syncwarp();
-                    tmem_st32(tm_s + 32 * half, p);
-                    tmem_wait_st();
-                    tmem_fence_before();
-                    mbar_arrive(p_full + 2 * i + half);
-                };
-                sum0 = sum1 = pair_of(0.f, 0.f);
-                weights(0);
-                float top = fmaxf(x[0], x[1]), top_b = fmaxf(x[2], x[3]);
+                    for (int h = 0; h < 4; ++h) {
+                        uint32_t p[16];
 #pragma unroll
-                for (int e = 4; e < CHUNK_SLOTS; e += 4) {
-                    top = fmaxf(fmaxf(top, x[e]), x[e + 1]);
-                    top_b = fmaxf(fmaxf(top_b, x[e + 2]), x[e + 3]);
-                }
-                top = fmaxf(top, top_b);
-                const bool grow = (top - m) * scale > 8.f;  // m = -inf: unless all is masked
-                if (__any_sync(FULL, grow)) {
-                    const float f = grow ? part_factor(m * scale, top * scale) : 1.f;
-                    if (grow) {
-                        m = top;
-                        ref = m * scale;
+                        for (int e = 0; e < 16; ++e) {
+                            const int k = 32 * h + 2 * e;
+                            const Pair y = fma2(pair_of(x[k], x[k + 1]), scale2, ref2);
+                            const float2 z = floats(y), w = make_float2(ex2(z.x), ex2(z.y));
+                            part[e & 1] = part[e & 1] + pair_of(w.x, w.y);
+                            p[e] = pack2<T>(w.x, w.y);
+                        }
+                        tmem_st16(tm_s + 16 * h, p);
                     }
-                    l *= f;
-                    if (t > g.t0) {
+                    const float2 w = floats(part[0] + part[1]);
+                    sum = w.x + w.y;
+                };
+                if (t > g.t0) weights();
+                if (t == g.t0 || __any_sync(FULL, sum > 256.f)) {
+                    float top = fmaxf(x[0], x[1]), top_b = fmaxf(x[2], x[3]);
+#pragma unroll
+                    for (int e = 4; e < CHUNK_SLOTS; e += 4) {
+                        top = fmaxf(fmaxf(top, x[e]), x[e + 1]);
+                        top_b = fmaxf(fmaxf(top_b, x[e + 2]), x[e + 3]);
+                    }
+                    top = fmaxf(top, top_b) * scale;
+                    if (t == g.t0) {
+                        ref = top == -INFINITY ? 0.f : top;
+                    } else {
+                        const float f = top > ref ? ex2(ref - top) : 1.f;
+                        ref = fmaxf(ref, top);
+                        l *= f;
 #pragma unroll 1
                         for (int e = 0; e < c.dim; e += 32) {
                             float o[32];
@@ -517,20 +512,19 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                             tmem_st32(tm_o + e, w);
                         }
                     }
-                    sum0 = sum1 = pair_of(0.f, 0.f);
-                    weights(0);
+                    weights();
                 }
-                hand_over(0);
-                weights(64);
-                hand_over(1);
-                const float2 sum = floats(sum0 + sum1);
-                l += sum.x + sum.y;
+                l += sum;
+                tmem_wait_st();
+                tmem_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full + i);
             }
             wait(o_full + i, o_phase);
             o_phase ^= 1;
             tmem_fence_after();
             // base 2 from here on. A tile past the sequence met no product: its O holds anything.
-            float top = m == -INFINITY ? -INFINITY : m * scale, total = l, f0 = 1.f, f1 = 0.f;
+            float top = l == 0.f ? -INFINITY : ref, total = l, f0 = 1.f, f1 = 0.f;
             const float top0 = top;
             if (g.lone) {  // the first warpgroup joins the two
                 if (i == 1) {

@@ -64,7 +64,7 @@ struct KvWait {
     int* status;
     bool dead = false;
     __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t parity) {
-        if (!dead && !mbar_wait_bounded(bar, parity, KV_WAIT_BUDGET)) {
+        if (!mbar_try_wait(bar, parity) && !dead && !mbar_wait_bounded(bar, parity, KV_WAIT_BUDGET)) {
             dead = true;
             atomicOr(status, ERR_WAIT_TIMEOUT);
         }
