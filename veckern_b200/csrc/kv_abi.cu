@@ -1,6 +1,9 @@
 // C ABI of the paged key/value cache (vk_kv_*): checks of arguments, the cache's handle, and the launches.
+#include <map>
+#include <mutex>
 #include <new>
 #include <type_traits>
+#include <utility>
 
 #include <cudaTypedefs.h>
 
@@ -100,6 +103,20 @@ AttendPlan plan_attend(const vk_kv* kv, const vk::KvBatch& bt, int group, int ma
     return p;
 }
 
+// Once per kernel and device: the dynamic shared memory that it may take, clusters of more than 8.
+template <class Fn>
+int prepare_kernel(Fn* fn, int device, size_t smem, bool large_clusters = false) {
+    static std::mutex lock;
+    static std::map<std::pair<const void*, int>, bool> seen;
+    std::lock_guard<std::mutex> hold(lock);
+    bool& is = seen[{reinterpret_cast<const void*>(fn), device}];
+    if (is) return VK_OK;
+    VK_TRY_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (large_clusters) VK_TRY_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    is = true;
+    return VK_OK;
+}
+
 // Launches fn so that it may start while the kernel before it on the stream ends; it waits for that one's results itself.
 template <class... Args>
 int launch_behind(void (*fn)(Args...), dim3 grid, int threads, size_t smem, cudaStream_t st, Args... args) {
@@ -122,7 +139,7 @@ int launch_step_as(const vk_kv* kv, const vk::KvPages& c, const vk::KvBatch& bt,
                    const vk::KvParts& parts, int ctas, cudaStream_t st) {
     const auto fn = &vk::kv_step_kernel<T, DP, R, SCORES>;
     constexpr int smem = vk::step_smem<DP>();
-    VK_TRY_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    VK_TRY(prepare_kernel(fn, kv->desc.device, smem));
     fn<<<ctas, vk::STEP_THREADS, smem, st>>>(kv->map_k, kv->map_v, c, bt, a, parts);
     VK_TRY_CUDA(cudaGetLastError());
     if constexpr (SCORES) {
@@ -197,13 +214,13 @@ int launch_chunk(const vk_kv* kv, const vk::KvPages& c, const vk::KvBatch& bt, c
     VK_TRY(encode_rows(a, c.dim, bt.tokens, &map_q));
     const auto fn = &vk::kv_chunk_kernel<T, DP>;
     constexpr int smem = vk::chunk_smem<DP>();
-    VK_TRY_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    VK_TRY(prepare_kernel(fn, kv->desc.device, smem));
     fn<<<p.chunk_ctas, vk::CHUNK_THREADS, smem, st>>>(map_q, kv->map_k, kv->map_v, c, bt, a, parts);
     VK_TRY_CUDA(cudaGetLastError());
     if (!a.scores || a.scores_width == 0) return VK_OK;
     const auto weights = &vk::kv_weights_kernel<T, DP>;
     constexpr int weights_smem = vk::weights_smem<DP>();
-    VK_TRY_CUDA(cudaFuncSetAttribute(weights, cudaFuncAttributeMaxDynamicSharedMemorySize, weights_smem));
+    VK_TRY(prepare_kernel(weights, kv->desc.device, weights_smem));
     return launch_behind(weights, dim3(p.chunk_ctas), vk::CHUNK_THREADS, weights_smem, st, map_q, kv->map_k, c, bt, a, parts);
 }
 
@@ -412,12 +429,36 @@ int vk_kv_evict(vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_evict_t* ar
     e.new_lens = args->new_lens;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const vk::KvPages c = pages_of(kv);
-    vk::kv_select_kernel<<<dim3(c.heads, bt.batch), vk::SELECT_THREADS, 0, st>>>(c, bt, e);
-    VK_TRY_CUDA(cudaGetLastError());
+    // CTAs per (sequence, kv head): slices of 2,048 slots or fewer while there are SMs for them; a power of two.
+    const int64_t slots = (int64_t)bt.width << c.page_shift, groups = (int64_t)bt.batch * c.heads;
+    const int64_t want = ceil_div(slots, 2048);
+    int ctas = 1;
+    while (ctas < vk::SELECT_CLUSTER && ctas < want && (ctas * groups <= kv->sm_count || slots / ctas > 16384)) ctas *= 2;
+    const size_t smem = 5 * vk::SELECT_BINS * sizeof(int) +
+                        (size_t)std::min<int64_t>(ceil_div(slots, ctas), vk::SELECT_HELD) * sizeof(uint32_t);
+    const auto select = ctas == 1   ? &vk::kv_select_kernel<1>
+                        : ctas == 2 ? &vk::kv_select_kernel<2>
+                        : ctas == 4 ? &vk::kv_select_kernel<4>
+                        : ctas == 8 ? &vk::kv_select_kernel<8>
+                                    : &vk::kv_select_kernel<vk::SELECT_CLUSTER>;
+    VK_TRY(prepare_kernel(select, kv->desc.device,
+                          5 * vk::SELECT_BINS * sizeof(int) + vk::SELECT_HELD * sizeof(uint32_t), true));
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = ctas;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas, c.heads, bt.batch);
+    cfg.blockDim = dim3(vk::SELECT_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    VK_TRY_CUDA(cudaLaunchKernelEx(&cfg, select, c, bt, e));
     if (e.keep > 0) {
-        const unsigned tiles = (unsigned)std::min<int64_t>(ceil_div((int64_t)e.keep * (c.dim / 8), 256), 4096);
-        vk::kv_compact_kernel<<<dim3(tiles, c.heads, bt.batch), 256, 0, st>>>(c, bt, e);
-        VK_TRY_CUDA(cudaGetLastError());
+        const int64_t most = std::min<int64_t>(e.keep, slots);  // slots that can be kept
+        const unsigned tiles = (unsigned)std::min<int64_t>(ceil_div(most * (c.dim / 8), 256), 4096);
+        if (tiles) VK_TRY(launch_behind(&vk::kv_compact_kernel, dim3(tiles, c.heads, bt.batch), 256, 0, st, c, bt, e));
     }
     return VK_OK;
 }

@@ -59,7 +59,7 @@ class PagedCache:
     def __init__(self, k_pages, v_pages):
         import torch
 
-        self._torch = torch
+        self._torch, self._i32, self._lib = torch, torch.int32, lib()
         self._h = C.c_void_p()
         for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
             if t.dim() != 4 or t.shape != k_pages.shape or t.dtype != k_pages.dtype or t.device != k_pages.device:
@@ -79,34 +79,42 @@ class PagedCache:
                      v_stride=(C.c_int64 * 3)(*v_pages.stride()[:3]))
         check(lib().vk_kv_create(C.byref(d), C.byref(self._h)), "vk_kv_create")
         self._sizes = {}  # bytes of attention's working memory by what they depend on
+        self._strides = (C.c_int64 * 2)(), (C.c_int64 * 2)()
         # argument structs, filled anew by every call
         self._batch, self._attend, self._evict = N.KvBatch(), N.KvAttend(), N.KvEvict()
         self._batch_ref, self._attend_ref, self._evict_ref = (C.byref(x) for x in
                                                               (self._batch, self._attend, self._evict))
 
     def _sequences(self, table, lens, offsets=None, tokens: int = 0) -> int:
-        i32, dev = self._torch.int32, self.device
-        _want(table, "table", i32, 2, dev)
-        _want(lens, "lens", i32, 1, dev)
+        i32, dev, b = self._i32, self.device, self._batch
+        if table.dtype != i32 or table.dim() != 2 or table.device != dev:
+            _want(table, "table", i32, 2, dev)
+        if lens.dtype != i32 or lens.dim() != 1 or lens.device != dev:
+            _want(lens, "lens", i32, 1, dev)
         n, width = table.shape
-        if lens.shape[0] != n or not lens.is_contiguous() or (width > 1 and table.stride(1) != 1):
+        stride, step = table.stride()
+        if lens.shape[0] != n or not lens.is_contiguous() or (step != 1 and width > 1):
             raise ValueError("lens must be contiguous, one per row of table, and table's rows contiguous")
-        b = self._batch
-        if offsets is not None:
-            _want(offsets, "offsets", i32, 1, dev)
+        if offsets is None:
+            b.offsets = None
+        else:
+            if offsets.dtype != i32 or offsets.dim() != 1 or offsets.device != dev:
+                _want(offsets, "offsets", i32, 1, dev)
             if offsets.shape[0] != n + 1 or not offsets.is_contiguous():
                 raise ValueError("offsets must be contiguous [batch + 1]")
             b.offsets = offsets.data_ptr()
-        else:
-            b.offsets = None
-        b.batch, b.table_width, b.table_stride, b.tokens = n, width, table.stride(0), tokens
+        b.batch, b.table_width, b.table_stride, b.tokens = n, width, stride, tokens
         b.table, b.lens = table.data_ptr(), lens.data_ptr()
         return n
 
-    def _rows(self, t, name: str, heads: int) -> None:
-        _want(t, name, self.dtype, 3, self.device)
-        if t.shape[1] != heads or t.shape[2] != self.head_dim or t.stride(2) != 1:
+    def _rows(self, t, name: str, heads: int):
+        """Checks rows of tokens; their strides."""
+        if t.dtype != self.dtype or t.dim() != 3 or t.device != self.device:
+            _want(t, name, self.dtype, 3, self.device)
+        strides = t.stride()
+        if t.shape[1] != heads or t.shape[2] != self.head_dim or strides[2] != 1:
             raise ValueError(f"{name} must be [tokens, {heads}, {self.head_dim}] with the last dimension contiguous")
+        return strides
 
     def _stream(self, stream):
         if stream is None:
@@ -116,14 +124,16 @@ class PagedCache:
     def append(self, k, v, offsets, table, lens, *, stream=None) -> None:
         """New token t of sequence b (of T) is written to slot lens[b] - T + t. k, v: [tokens, kv_heads, head_dim],
         strides multiples of 8 elements (slices of one projection's output are fine)."""
-        self._rows(k, "k", self.kv_heads)
-        self._rows(v, "v", self.kv_heads)
-        if v.shape[0] != k.shape[0]:
+        ks, vs = self._strides
+        ks[0], ks[1], _ = self._rows(k, "k", self.kv_heads)
+        vs[0], vs[1], _ = self._rows(v, "v", self.kv_heads)
+        tokens = k.shape[0]
+        if v.shape[0] != tokens:
             raise ValueError("k and v must have the same number of tokens")
-        self._sequences(table, lens, offsets, k.shape[0])
-        ks, vs = (C.c_int64 * 2)(*k.stride()[:2]), (C.c_int64 * 2)(*v.stride()[:2])
-        check(lib().vk_kv_append(self._h, self._batch_ref, k.data_ptr(), ks, v.data_ptr(), vs, self._stream(stream)),
-              "append")
+        self._sequences(table, lens, offsets, tokens)
+        code = self._lib.vk_kv_append(self._h, self._batch_ref, k.data_ptr(), ks, v.data_ptr(), vs, self._stream(stream))
+        if code:
+            check(code, "append")
 
     def attend(self, q, offsets, table, lens, *, causal: bool = True, scale: float | None = None, scores=None,
                max_q: int = 0, out=None, lse=None, stream=None):
@@ -136,13 +146,15 @@ class PagedCache:
         torch = self._torch
         if q.dim() != 3:
             raise ValueError("q must be [tokens, heads, head_dim]")
-        tokens, heads = q.shape[0], q.shape[1]
-        self._rows(q, "q", heads)
+        a = self._attend
+        tokens, heads, _ = q.shape
+        a.q_stride[0], a.q_stride[1], _ = self._rows(q, "q", heads)
         n = self._sequences(table, lens, offsets, tokens)
         if out is None:
-            out = torch.empty((tokens, heads, self.head_dim), dtype=self.dtype, device=self.device)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            a.out_stride[0], a.out_stride[1] = heads * self.head_dim, self.head_dim
         else:
-            self._rows(out, "out", heads)
+            a.out_stride[0], a.out_stride[1], _ = self._rows(out, "out", heads)
             if out.shape[0] != tokens:
                 raise ValueError("out must have q's shape")
         if lse is None:
@@ -151,12 +163,10 @@ class PagedCache:
             _want(lse, "lse", torch.float32, 2, self.device)
             if lse.shape != (tokens, heads) or not lse.is_contiguous():
                 raise ValueError("lse must be contiguous [tokens, heads]")
-        a = self._attend
         a.q, a.out, a.lse = q.data_ptr(), out.data_ptr(), lse.data_ptr()
-        a.q_stride[0], a.q_stride[1] = q.stride(0), q.stride(1)
-        a.out_stride[0], a.out_stride[1] = out.stride(0), out.stride(1)
-        a.scores = None
-        if scores is not None:
+        if scores is None:
+            a.scores = None
+        else:
             self._check_scores(scores, n)
             a.scores, a.scores_width = scores.data_ptr(), scores.shape[2]
             a.scores_stride[0], a.scores_stride[1] = scores.stride(0), scores.stride(1)
@@ -173,7 +183,9 @@ class PagedCache:
         s = self._stream(stream)
         work = _workspace(torch, self.device, s, need)
         a.workspace, a.workspace_bytes = work.data_ptr(), work.numel()
-        check(lib().vk_kv_attend(self._h, self._batch_ref, self._attend_ref, s), "attend")
+        code = self._lib.vk_kv_attend(self._h, self._batch_ref, self._attend_ref, s)
+        if code:
+            check(code, "attend")
         return out, lse
 
     def evict(self, table, lens, new_table, keep: int, recent: int, scores, *, stream=None):
@@ -190,15 +202,17 @@ class PagedCache:
         if not 0 <= recent <= keep:
             raise ValueError("keep and recent must satisfy 0 <= recent <= keep")
         kept = torch.empty((n, self.kv_heads, keep), dtype=torch.int32, device=self.device)
-        new_lens = torch.empty((n,), dtype=torch.int32, device=self.device)
-        new_scores = torch.empty(scores.shape, dtype=torch.float32, device=self.device)
+        new_lens = torch.empty_like(lens)
+        new_scores = torch.empty_like(scores, memory_format=torch.contiguous_format)
         e = self._evict
         e.new_table, e.new_table_stride, e.new_table_width = new_table.data_ptr(), new_table.stride(0), new_table.shape[1]
         e.keep, e.recent = keep, recent
         e.scores, e.scores_width = scores.data_ptr(), scores.shape[2]
         e.scores_stride[0], e.scores_stride[1] = scores.stride(0), scores.stride(1)
         e.new_scores, e.kept, e.new_lens = new_scores.data_ptr(), kept.data_ptr(), new_lens.data_ptr()
-        check(lib().vk_kv_evict(self._h, self._batch_ref, self._evict_ref, self._stream(stream)), "evict")
+        code = self._lib.vk_kv_evict(self._h, self._batch_ref, self._evict_ref, self._stream(stream))
+        if code:
+            check(code, "evict")
         return kept, new_lens, new_scores
 
     def _check_scores(self, scores, n: int) -> None:
