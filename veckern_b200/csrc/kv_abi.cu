@@ -140,8 +140,7 @@ int launch_step_as(const vk_kv* kv, const vk::KvPages& c, const vk::KvBatch& bt,
     const auto fn = &vk::kv_step_kernel<T, DP, R, SCORES>;
     constexpr int smem = vk::step_smem<DP>();
     VK_TRY(prepare_kernel(fn, kv->desc.device, smem));
-    fn<<<ctas, vk::STEP_THREADS, smem, st>>>(kv->map_k, kv->map_v, c, bt, a, parts);
-    VK_TRY_CUDA(cudaGetLastError());
+    VK_TRY(launch_behind(fn, dim3(ctas), vk::STEP_THREADS, smem, st, kv->map_k, kv->map_v, c, bt, a, parts));
     if constexpr (SCORES) {
         const int64_t width = std::min(parts.s_slots, a.scores_width);
         if (width > 0)
@@ -215,8 +214,7 @@ int launch_chunk(const vk_kv* kv, const vk::KvPages& c, const vk::KvBatch& bt, c
     const auto fn = &vk::kv_chunk_kernel<T, DP>;
     constexpr int smem = vk::chunk_smem<DP>();
     VK_TRY(prepare_kernel(fn, kv->desc.device, smem));
-    fn<<<p.chunk_ctas, vk::CHUNK_THREADS, smem, st>>>(map_q, kv->map_k, kv->map_v, c, bt, a, parts);
-    VK_TRY_CUDA(cudaGetLastError());
+    VK_TRY(launch_behind(fn, dim3(p.chunk_ctas), vk::CHUNK_THREADS, smem, st, map_q, kv->map_k, kv->map_v, c, bt, a, parts));
     if (!a.scores || a.scores_width == 0) return VK_OK;
     const auto weights = &vk::kv_weights_kernel<T, DP>;
     constexpr int weights_smem = vk::weights_smem<DP>();
@@ -338,11 +336,9 @@ int vk_kv_append(vk_kv_t* kv, const vk_kv_batch_t* batch, const void* k, const i
     if (guard.err != cudaSuccess) return fail(VK_ERR_CUDA, "cudaSetDevice: %s", cudaGetErrorString(guard.err));
     const int64_t threads = bt.tokens * kv->desc.kv_heads * (kv->desc.head_dim / 8);
     const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(threads, 256), (int64_t)kv->sm_count * 32);
-    vk::kv_append_kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(
-        pages_of(kv), bt, static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), k_stride[0], k_stride[1],
-        v_stride[0], v_stride[1]);
-    VK_TRY_CUDA(cudaGetLastError());
-    return VK_OK;
+    return launch_behind(&vk::kv_append_kernel, dim3(grid), 256, 0, static_cast<cudaStream_t>(stream), pages_of(kv), bt,
+                         static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), k_stride[0], k_stride[1],
+                         v_stride[0], v_stride[1]);
 }
 
 int vk_kv_attend(vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_attend_t* args, void* stream) {
@@ -376,6 +372,11 @@ int vk_kv_attend(vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_attend_t* 
     a.max_q = max_q_of(args, bt.tokens);
     a.causal = args->causal != 0;
     a.scale = args->scale;
+    // The kernels count their units of work (tiles and pairs of tiles, of every kv head) in 32 bits.
+    const int64_t tiles = ceil_div((int64_t)bt.width << kv->page_shift, vk::STEP_TILE) + 1;
+    if (tiles * g * ((double)bt.tokens * a.group / vk::CHUNK_ROWS + 2.0 * bt.batch) >= 2147483648.0)
+        return fail(VK_ERR_UNSUPPORTED, "too many tiles (tables of %d pages, %lld tokens); use fewer sequences per call",
+                    bt.width, (long long)bt.tokens);
     const AttendPlan plan = plan_attend(kv, bt, a.group, a.max_q, a.scores != nullptr);
     if (args->workspace_bytes < plan.bytes || !args->workspace || reinterpret_cast<uintptr_t>(args->workspace) % 256)
         return fail(VK_ERR_INVALID, "workspace must be 256-byte aligned and hold %zu bytes (vk_kv_attend_workspace)",
@@ -443,17 +444,19 @@ int vk_kv_evict(vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_evict_t* ar
                                     : &vk::kv_select_kernel<vk::SELECT_CLUSTER>;
     VK_TRY(prepare_kernel(select, kv->desc.device,
                           5 * vk::SELECT_BINS * sizeof(int) + vk::SELECT_HELD * sizeof(uint32_t), true));
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = ctas;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2]{};
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(ctas, c.heads, bt.batch);
     cfg.blockDim = dim3(vk::SELECT_THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
     VK_TRY_CUDA(cudaLaunchKernelEx(&cfg, select, c, bt, e));
     if (e.keep > 0) {
         const int64_t most = std::min<int64_t>(e.keep, slots);  // slots that can be kept

@@ -26,6 +26,7 @@ namespace vk {
 
 constexpr int CHUNK_ROWS = 128;                 // rows of a tile
 constexpr int CHUNK_SLOTS = 128;                // slots of a unit
+constexpr int CHUNK_LEAST = 1;                  // units of a CTA, at least
 constexpr int CHUNK_THREADS = 384;              // two softmax warpgroups; one with the MMA warp and the loading warp
 template <int DP>
 constexpr int CHUNK_Q = 2 * CHUNK_ROWS * DP * 2;   // bytes of the two query tiles
@@ -184,7 +185,7 @@ struct ChunkShape {
         return max(1, (limit(s, pair) + n - 1) / n);
     }
     // units of the pairs before `pair`
-    __device__ __forceinline__ int64_t before(const KvSeq& s, int pair) const {
+    __device__ __forceinline__ int before(const KvSeq& s, int pair) const {
         const int all = pairs(s), n = min(pair, all - 1), per = 2 * tokens;
         const int64_t a = (int64_t)s.len - s.count;
         int64_t sum;
@@ -194,7 +195,7 @@ struct ChunkShape {
             const int one = a > CHUNK_SLOTS ? 0 : (int)min((int64_t)n, (CHUNK_SLOTS - a) / per);  // pairs of one unit
             sum = one + floor_sum(n - one, CHUNK_SLOTS, per, a + (int64_t)(one + 1) * per + CHUNK_SLOTS - 1);
         }
-        return pair < all ? sum : sum + units(s, all - 1);
+        return (int)(pair < all ? sum : sum + units(s, all - 1));
     }
 };
 
@@ -221,9 +222,9 @@ struct ChunkWalk {
         }
         const int all = shape.pairs(s);
         if (!located) {  // the position of the share's first unit within its sequence
-            const int64_t per = shape.before(s, all);
-            head = (int)(share.off / per);
-            const int64_t off = share.off % per;
+            const int per = shape.before(s, all);
+            int off = share.off;
+            for (head = 0; off >= per; ++head) off -= per;
             int lo = 0, hi = all - 1;  // the last pair that begins at or before off
             while (lo < hi) {
                 const int mid = (lo + hi + 1) >> 1;
@@ -231,7 +232,7 @@ struct ChunkWalk {
                 else hi = mid - 1;
             }
             pair = lo;
-            t0 = (int)(off - shape.before(s, lo));
+            t0 = off - shape.before(s, lo);
             located = true;
         }
         g->s = s;
@@ -239,7 +240,7 @@ struct ChunkWalk {
         g->head = head;
         g->t0 = t0;
         g->units = shape.units(s, pair);
-        g->count = (int)min((int64_t)(g->units - t0), share.left);
+        g->count = min(g->units - t0, share.left);
         g->token0 = pair * 2 * shape.tokens;
         g->lone = shape.lone(s, pair);
         share.left -= g->count;
@@ -265,10 +266,13 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     uint64_t* s_full = q_empty + 1;  // [tile]
     uint64_t* p_full = s_full + 2;
     uint64_t* o_full = p_full + 2;
-    int64_t* scratch = reinterpret_cast<int64_t*>(o_full + 2);  // THREADS / 32 + 2
+    int* scratch = reinterpret_cast<int*>(o_full + 2);  // THREADS / 32 + 2
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(scratch + CHUNK_THREADS / 32 + 2);
     const int warp = __shfl_sync(FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
+        prefetch_map(&map_q);
+        prefetch_map(&map_k);
+        prefetch_map(&map_v);
         for (int i = 0; i < RING; ++i) {
             mbar_init(kv_full + i, 1);
             mbar_init(kv_empty + i, 1);
@@ -294,7 +298,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     tmem_fence_before();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const ChunkShape shape{a.group, a.causal, CHUNK_ROWS / a.group};
-    KvShare share = kv_share<CHUNK_THREADS>(c, bt, scratch, [&](const KvSeq& s) -> int64_t {
+    KvShare share = kv_share<CHUNK_THREADS>(c, bt, scratch, CHUNK_LEAST, [&](const KvSeq& s) {
         return shape.takes(s) ? shape.before(s, shape.pairs(s)) * c.heads : 0;
     });
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

@@ -10,6 +10,8 @@ namespace vk {
 // for a step's few tokens.
 __global__ void __launch_bounds__(256) kv_append_kernel(KvPages c, KvBatch bt, const uint16_t* k, const uint16_t* v,
                                                         int64_t k_tok, int64_t k_head, int64_t v_tok, int64_t v_head) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int parts = c.dim >> 3;
     const int64_t all = bt.tokens * c.heads * parts;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < all; i += (int64_t)gridDim.x * blockDim.x) {
@@ -79,6 +81,7 @@ __device__ __forceinline__ float kv_score(uint32_t u) {
 template <int C>
 __global__ void __launch_bounds__(SELECT_THREADS, 2) kv_select_kernel(KvPages c, KvBatch bt, KvEvict e) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     extern __shared__ __align__(1024) uint8_t ring[];
     int* hist = reinterpret_cast<int*>(ring);  // [digit][SELECT_BINS], sums of the cluster, one share of all CTAs' counts
     uint32_t* held = reinterpret_cast<uint32_t*>(hist + 5 * SELECT_BINS);  // [min(slice, SELECT_HELD)]

@@ -20,6 +20,7 @@
 namespace vk {
 
 constexpr int STEP_TILE = 64;  // slots of a tile
+constexpr int STEP_LEAST = 2;  // tiles of a CTA, at least
 constexpr int STEP_ROWS = 16;  // most rows of a sequence's kv head
 constexpr int STEP_WARPS = 4;  // consumers; one more warp loads
 constexpr int STEP_THREADS = 32 * (STEP_WARPS + 1);
@@ -43,6 +44,9 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 // A 2-d box of a page (box slots x 64 elements of one head) into shared memory.
 __device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int d, int slot, int head, int page,
                                          uint64_t* bar) {
@@ -74,7 +78,6 @@ struct KvWait {
 
 // Part `i` is written (by threads that a barrier has joined since): tell the CTA that adds it up.
 __device__ __forceinline__ void part_publish(const KvParts& parts, int i) {
-    __threadfence();
     asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(parts.ready + i), "r"(1u) : "memory");
 }
 // Waits, with a limit, for part i. Its CTA comes to it before anything else and waits for nobody to make it.
@@ -127,60 +130,73 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 
 // The share of one CTA: a walk over units laid end to end, sequence by sequence. Count(s) is the number of units of a
-// sequence; the caller splits a sequence's units into its heads and tiles.
+// sequence; the caller splits a sequence's units into its heads and tiles. The host has checked that all units together
+// are fewer than 2^31.
 struct KvShare {
-    int b;        // sequence of the next unit
-    int64_t off;  // unit within it
-    int64_t left;  // units of this CTA that are not taken yet
-    int64_t total;
-    int ctas;  // CTAs with a share; none of these is empty
+    int b;     // sequence of the next unit
+    int off;   // unit within it
+    int left;  // units of this CTA that are not taken yet
+    int each;  // units of a CTA; the first `more` of them have one more
+    int more;
+    int ctas;  // CTAs with a share
+    __device__ __forceinline__ int first(int cta) const { return each * cta + min(cta, more); }
     // CTAs that hold the next `rest` units after this CTA's share
-    __device__ __forceinline__ int followers(int64_t rest) const {
-        const int me = blockIdx.x + 1;
-        const int64_t end = total * me / ctas + rest;
+    __device__ __forceinline__ int followers(int rest) const {
+        const int me = blockIdx.x + 1, end = first(me) + rest;
         int n = 0;
-        while (me + n < ctas && total * (me + n) / ctas < end) ++n;
+        while (me + n < ctas && first(me + n) < end) ++n;
         return n;
     }
 };
 
 template <int THREADS, class Count>
-__device__ __forceinline__ KvShare kv_share(const KvPages& c, const KvBatch& bt, int64_t* scratch, Count&& count) {
-    // scratch: THREADS / 32 + 4 values of shared memory. Thread t sums a contiguous range of the sequences.
+__device__ __forceinline__ KvShare kv_share(const KvPages& c, const KvBatch& bt, int* scratch, int least, Count&& count) {
+    // scratch: THREADS / 32 + 2 values of shared memory. Thread t sums a contiguous range of the sequences. A CTA gets
+    // `least` units or more, except where there are fewer. No CTA without a share lies between others: the parts of a cut
+    // segment belong to consecutive CTAs.
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     constexpr int WARPS = THREADS / 32;
-    const int each = (bt.batch + THREADS - 1) / THREADS;
-    const int b0 = min(bt.batch, t * each), b1 = min(bt.batch, b0 + each);
-    int64_t sum = 0;
+    const int span = (bt.batch + THREADS - 1) / THREADS;
+    const int b0 = min(bt.batch, t * span), b1 = min(bt.batch, b0 + span);
+    int sum = 0;
     for (int b = b0; b < b1; ++b) sum += count(kv_seq(c, bt, b));
-    int64_t incl = sum;
+    int incl = sum;
+#pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int64_t x = __shfl_up_sync(FULL, incl, o);
+        const int x = __shfl_up_sync(FULL, incl, o);
         if (lane >= o) incl += x;
     }
     if (lane == 31) scratch[warp] = incl;
     __syncthreads();
-    int64_t before = 0, total = 0;
+    int before = 0, total = 0;
+#pragma unroll
     for (int w = 0; w < WARPS; ++w) {
         if (w < warp) before += scratch[w];
         total += scratch[w];
     }
-    const int64_t ctas = min((int64_t)gridDim.x, total), i = min((int64_t)blockIdx.x, ctas);
-    const int64_t first = ctas ? total * i / ctas : 0, last = ctas ? total * min(i + 1, ctas) / ctas : 0;
+    KvShare s;
+    s.ctas = min((int)gridDim.x, (total + least - 1) / least);
+    const uint32_t parts = max(s.ctas, 1);
+    s.each = (int)((uint32_t)total / parts);
+    s.more = total - s.each * (int)parts;
+    const int me = min((int)blockIdx.x, s.ctas), first = s.first(me);
+    s.left = me < s.ctas ? s.first(me + 1) - first : 0;
     before += incl - sum;
     if (first >= before && first < before + sum) {
-        int64_t off = first - before;
-        int b = b0;
-        for (;; ++b) {
-            const int64_t n = count(kv_seq(c, bt, b));
-            if (off < n) break;
-            off -= n;
-        }
+        int off = first - before, b = b0;
+        if (b1 - b0 > 1)
+            for (;; ++b) {
+                const int n = count(kv_seq(c, bt, b));
+                if (off < n) break;
+                off -= n;
+            }
         scratch[WARPS] = b;
         scratch[WARPS + 1] = off;
     }
     __syncthreads();
-    return {(int)scratch[WARPS], scratch[WARPS + 1], last - first, total, (int)ctas};
+    s.b = scratch[WARPS];
+    s.off = scratch[WARPS + 1];
+    return s;
 }
 
 // Lowest slot that some row does not see: n for every row, or the first row's limit under the causal mask.
@@ -211,9 +227,11 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
     float2* sum_ml = reinterpret_cast<float2*>(sum_o + STEP_WARPS * 8 * DP);                // [warp][16]
     uint64_t* full = reinterpret_cast<uint64_t*>(sum_ml + STEP_WARPS * STEP_ROWS);
     uint64_t* empty = full + STAGES;
-    int64_t* scratch = reinterpret_cast<int64_t*>(empty + STAGES);
+    int* scratch = reinterpret_cast<int*>(empty + STAGES);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
+        prefetch_map(&map_k);
+        prefetch_map(&map_v);
         for (int i = 0; i < STAGES; ++i) {
             mbar_init(full + i, 1);
             mbar_init(empty + i, STEP_WARPS);
@@ -222,10 +240,8 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     auto tiles_of = [&](const KvSeq& s) { return max(1, (s.len + STEP_TILE - 1) / STEP_TILE); };
-    auto units_of = [&](const KvSeq& s) -> int64_t {
-        return step_takes(s, a.group) ? (int64_t)tiles_of(s) * c.heads : 0;
-    };
-    KvShare share = kv_share<STEP_THREADS>(c, bt, scratch, units_of);
+    auto units_of = [&](const KvSeq& s) { return step_takes(s, a.group) ? tiles_of(s) * c.heads : 0; };
+    KvShare share = kv_share<STEP_THREADS>(c, bt, scratch, STEP_LEAST, units_of);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     KvWait wait{c.status};
     int stage = 0;
@@ -235,13 +251,13 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
     while (share.left > 0) {
         const KvSeq s = kv_seq(c, bt, share.b);
         const int tiles = tiles_of(s);
-        if (!step_takes(s, a.group) || share.off >= (int64_t)tiles * c.heads) {
+        if (!step_takes(s, a.group) || share.off >= tiles * c.heads) {
             ++share.b;
             share.off = 0;
             continue;
         }
-        const int head = (int)(share.off / tiles), t0 = (int)(share.off % tiles);
-        const int count = (int)min((int64_t)(tiles - t0), share.left);
+        const int head = (int)((uint32_t)share.off / (uint32_t)tiles), t0 = share.off - head * tiles;
+        const int count = min(tiles - t0, share.left);
         share.off += count;
         share.left -= count;
         const int32_t* table = bt.table + share.b * bt.table_stride;
@@ -385,58 +401,94 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
                 l[u] += __shfl_xor_sync(FULL, l[u], 2);
                 if ((lane & 3) == 0) sum_ml[warp * STEP_ROWS + 8 * u + g] = make_float2(m[u], l[u]);
             }
+            // Thread (row, eight elements), for a head size of 64 the first half of the threads.
+            constexpr int U = R / 8;
+            const int r8 = threadIdx.x / (DP / 8), d = threadIdx.x % (DP / 8) * 8;
+            const bool works = r8 < 8;
+            float top[U], total[U] = {}, v[U][8] = {};
 #pragma unroll
-            for (int u = 0; u < R / 8; ++u) {
+            for (int u = 0; u < U; ++u) {
 #pragma unroll
                 for (int i = 0; i < DP / 8; ++i)
                     *reinterpret_cast<float2*>(sum_o + (warp * 8 + g) * DP + 8 * i + q2) =
                         make_float2(o[i][2 * u], o[i][2 * u + 1]);
                 asm volatile("bar.sync 1, 128;" ::: "memory");
-                for (int i = threadIdx.x; i < 8 * (DP / 8); i += 32 * STEP_WARPS) {
-                    const int r8 = i / (DP / 8), r = 8 * u + r8, d = i % (DP / 8) * 8;
-                    if (r >= rows) continue;
-                    float top = -INFINITY, total = 0.f, v[8] = {};
+                top[u] = -INFINITY;
+                if (works) {
+                    const int r = 8 * u + r8;
 #pragma unroll
-                    for (int w = 0; w < STEP_WARPS; ++w) top = fmaxf(top, sum_ml[w * STEP_ROWS + r].x);
+                    for (int w = 0; w < STEP_WARPS; ++w) top[u] = fmaxf(top[u], sum_ml[w * STEP_ROWS + r].x);
 #pragma unroll
                     for (int w = 0; w < STEP_WARPS; ++w) {
                         const float2 ml = sum_ml[w * STEP_ROWS + r];
-                        const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
-                        total += f * ml.y;
+                        const float f = part_factor(ml.x, top[u]);
+                        total[u] += f * ml.y;
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] += f * sum_o[(w * 8 + r8) * DP + d + e];
+                        for (int e = 0; e < 8; ++e) v[u][e] += f * sum_o[(w * 8 + r8) * DP + d + e];
                     }
-                    if (leaves) {
-                        float4* po = reinterpret_cast<float4*>(parts.o + ((int64_t)blockIdx.x * STEP_ROWS + r) * DP + d);
-                        po[0] = make_float4(v[0], v[1], v[2], v[3]);
-                        po[1] = make_float4(v[4], v[5], v[6], v[7]);
-                        if (d == 0) parts.ml[(int64_t)blockIdx.x * STEP_ROWS + r] = make_float2(top, total);
-                        continue;
-                    }
-#pragma unroll 4
-                    for (int k = 0; k < follow; ++k) {
-                        const int64_t p = (int64_t)(blockIdx.x + 1 + k) * STEP_ROWS + r;
-                        const float2 ml = __ldcg(parts.ml + p);
-                        const float4* po = reinterpret_cast<const float4*>(parts.o + p * DP + d);
-                        const float4 x = __ldcg(po), y = __ldcg(po + 1);
-                        const float next = fmaxf(top, ml.x), f = part_factor(top, next), h = part_factor(ml.x, next);
-                        total = total * f + ml.y * h;
-                        v[0] = v[0] * f + x.x * h, v[1] = v[1] * f + x.y * h, v[2] = v[2] * f + x.z * h;
-                        v[3] = v[3] * f + x.w * h, v[4] = v[4] * f + y.x * h, v[5] = v[5] * f + y.y * h;
-                        v[6] = v[6] * f + y.z * h, v[7] = v[7] * f + y.w * h;
-                        top = next;
-                    }
-                    const int64_t tok = s.first + r / a.group;
-                    const int h = head * a.group + r % a.group;
-                    const float inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
-                    if (d < c.dim)
-                        *reinterpret_cast<uint4*>(a.out + tok * a.os[0] + h * a.os[1] + d) =
-                            make_uint4(pack2<T>(v[0] * inv, v[1] * inv), pack2<T>(v[2] * inv, v[3] * inv),
-                                       pack2<T>(v[4] * inv, v[5] * inv), pack2<T>(v[6] * inv, v[7] * inv));
-                    if (d == 0) a.lse[tok * a.heads + h] = (top + log2f(total)) * 0.6931471805599453f;
                 }
                 asm volatile("bar.sync 1, 128;" ::: "memory");
             }
+            if (works && leaves) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int64_t p = (int64_t)blockIdx.x * STEP_ROWS + 8 * u + r8;
+                    float4* po = reinterpret_cast<float4*>(parts.o + p * DP + d);
+                    po[0] = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
+                    po[1] = make_float4(v[u][4], v[u][5], v[u][6], v[u][7]);
+                    if (d == 0) parts.ml[p] = make_float2(top[u], total[u]);
+                }
+            } else if (works) {
+                constexpr int FLY = 8 / U;  // parts in flight; the last ones again, for nothing
+                for (int k0 = 0; k0 < follow; k0 += FLY) {
+                    float2 ml[FLY][U];
+                    float4 x[FLY][U], y[FLY][U];
+#pragma unroll
+                    for (int k = 0; k < FLY; ++k)
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {
+                            const int64_t p = (int64_t)(blockIdx.x + 1 + min(k0 + k, follow - 1)) * STEP_ROWS + 8 * u + r8;
+                            const float4* po = reinterpret_cast<const float4*>(parts.o + p * DP + d);
+                            ml[k][u] = __ldcg(parts.ml + p);
+                            x[k][u] = __ldcg(po);
+                            y[k][u] = __ldcg(po + 1);
+                        }
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        float next = top[u];
+#pragma unroll
+                        for (int k = 0; k < FLY; ++k) next = fmaxf(next, ml[k][u].x);
+                        const float f = part_factor(top[u], next);
+                        total[u] *= f;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[u][e] *= f;
+#pragma unroll
+                        for (int k = 0; k < FLY; ++k) {
+                            const float h = k0 + k < follow ? part_factor(ml[k][u].x, next) : 0.f;
+                            if (h == 0.f) continue;
+                            total[u] += ml[k][u].y * h;
+                            v[u][0] += x[k][u].x * h, v[u][1] += x[k][u].y * h, v[u][2] += x[k][u].z * h;
+                            v[u][3] += x[k][u].w * h, v[u][4] += y[k][u].x * h, v[u][5] += y[k][u].y * h;
+                            v[u][6] += y[k][u].z * h, v[u][7] += y[k][u].w * h;
+                        }
+                        top[u] = next;
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int r = 8 * u + r8;
+                    if (r >= rows) continue;
+                    const int64_t tok = s.first + r / a.group;
+                    const int h = head * a.group + r % a.group;
+                    const float inv = total[u] > 0.f ? 1.f / total[u] : total[u] == 0.f ? 0.f : total[u];
+                    if (d < c.dim)
+                        *reinterpret_cast<uint4*>(a.out + tok * a.os[0] + h * a.os[1] + d) =
+                            make_uint4(pack2<T>(v[u][0] * inv, v[u][1] * inv), pack2<T>(v[u][2] * inv, v[u][3] * inv),
+                                       pack2<T>(v[u][4] * inv, v[u][5] * inv), pack2<T>(v[u][6] * inv, v[u][7] * inv));
+                    if (d == 0) a.lse[tok * a.heads + h] = (top[u] + log2f(total[u])) * 0.6931471805599453f;
+                }
+            }
+            if (leaves || follow) asm volatile("bar.sync 1, 128;" ::: "memory");
             if (leaves && threadIdx.x == 0) part_publish(parts, blockIdx.x);
             for (int i = threadIdx.x; i < follow; i += 32 * STEP_WARPS) parts.ready[blockIdx.x + 1 + i] = 0;
         }

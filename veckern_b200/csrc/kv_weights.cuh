@@ -41,14 +41,14 @@ struct WeightsShape {
         return causal && x > 0 ? (int)(x / tokens) : 0;
     }
     // units of the pairs before `pair`
-    __device__ __forceinline__ int64_t before(const KvSeq& s, int pair) const {
+    __device__ __forceinline__ int before(const KvSeq& s, int pair) const {
         int64_t sum = (int64_t)pair * row_tiles(s);
         if (causal) {
             const int64_t a = (int64_t)s.len - s.count;
             const int64_t p0 = a < 0 ? 0 : min((int64_t)pair, (a + WEIGHTS_PAIR - 1) / WEIGHTS_PAIR);
             sum -= floor_sum(pair - p0, tokens, WEIGHTS_PAIR, p0 * WEIGHTS_PAIR - a);
         }
-        return sum;
+        return (int)sum;
     }
 };
 
@@ -76,9 +76,9 @@ struct WeightsWalk {
         }
         const int all = shape.pairs(s);
         if (!located) {
-            const int64_t per = shape.before(s, all);
-            head = (int)(share.off / per);
-            const int64_t off = share.off % per;
+            const int per = shape.before(s, all);
+            int off = share.off;
+            for (head = 0; off >= per; ++head) off -= per;
             int lo = 0, hi = all - 1;
             while (lo < hi) {
                 const int mid = (lo + hi + 1) >> 1;
@@ -86,7 +86,7 @@ struct WeightsWalk {
                 else hi = mid - 1;
             }
             pair = lo;
-            skip = (int)(off - shape.before(s, lo));
+            skip = off - shape.before(s, lo);
             located = true;
         }
         const int tiles = shape.row_tiles(s) - shape.first(s, pair);
@@ -95,7 +95,7 @@ struct WeightsWalk {
         g->head = head;
         g->pair = pair;
         g->q0 = shape.first(s, pair) + skip;
-        g->count = (int)min((int64_t)(tiles - skip), share.left);
+        g->count = min(tiles - skip, share.left);
         g->leaves = skip > 0;
         g->rest = tiles - skip - g->count;
         g->both = min((int64_t)s.len, shape.width) > (int64_t)pair * WEIGHTS_PAIR + CHUNK_SLOTS;
@@ -120,10 +120,12 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     uint64_t* k_empty = k_full + 1;
     uint64_t* s_full = k_empty + 1;  // [warpgroup][2]
     uint64_t* s_empty = s_full + 4;
-    int64_t* scratch = reinterpret_cast<int64_t*>(s_empty + 4);
+    int* scratch = reinterpret_cast<int*>(s_empty + 4);
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(scratch + CHUNK_THREADS / 32 + 2);
     const int warp = __shfl_sync(FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
+        prefetch_map(&map_q);
+        prefetch_map(&map_k);
         for (int i = 0; i < RING; ++i) {
             mbar_init(q_full + i, 1);
             mbar_init(q_empty + i, 1);
@@ -148,7 +150,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     tmem_fence_before();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const WeightsShape shape{a.group, a.causal, CHUNK_ROWS / a.group, a.scores_width};
-    KvShare share = kv_share<CHUNK_THREADS>(c, bt, scratch, [&](const KvSeq& s) -> int64_t {
+    KvShare share = kv_share<CHUNK_THREADS>(c, bt, scratch, CHUNK_LEAST, [&](const KvSeq& s) {
         return shape.takes(s) ? shape.before(s, shape.pairs(s)) * c.heads : 0;
     });
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
