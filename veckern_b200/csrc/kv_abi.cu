@@ -369,6 +369,10 @@ int vk_kv_attend(vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_attend_t* 
     a.scores_width = args->scores_width;
     a.heads = args->heads;
     a.group = args->heads / g;
+    a.tokens = vk::CHUNK_ROWS / a.group;
+    a.by_group = vk::Divisor::of(a.group);
+    a.by_tokens = vk::Divisor::of(a.tokens);
+    a.by_pair = vk::Divisor::of(2 * a.tokens);
     a.max_q = max_q_of(args, bt.tokens);
     a.causal = args->causal != 0;
     a.scale = args->scale;

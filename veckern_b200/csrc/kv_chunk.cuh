@@ -151,34 +151,50 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
     return p;
 }
 // ---- the order of units
-// sum of floor((a i + b) / m) over 0 <= i < n, by Euclid's steps on (m, a); a, b >= 0
-__device__ __forceinline__ int64_t floor_sum(int64_t n, int64_t m, int64_t a, int64_t b) {
-    int64_t sum = 0;
+// sum of floor((a i + b) / m) over 0 <= i < n, by Euclid's steps on (m, a). The sum is below 2^31 (the host has checked
+// the units), so that arithmetic modulo 2^32 gives it; a n + b after the first reduction is below m (n + 1).
+__device__ __forceinline__ uint32_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
+    uint32_t sum = 0;
     while (n > 0) {
-        sum += n * (n - 1) / 2 * (a / m) + n * (b / m);
-        a %= m;
-        b %= m;
-        const int64_t y = a * n + b;
+        const uint32_t qa = a / m, qb = b / m;
+        sum += ((n & 1) ? n * ((n - 1) / 2) : n / 2 * (n - 1)) * qa + n * qb;
+        a -= qa * m;
+        b -= qb * m;
+        const uint32_t y = a * n + b;
         if (y < m) break;
         n = y / m;
-        b = y % m;
-        const int64_t t = m;
+        b = y - n * m;
+        const uint32_t t = m;
         m = a;
         a = t;
     }
     return sum;
 }
 
+// The last of `all` pairs with before(pair) <= off, by a whole warp: 32 candidates at a time.
+template <class Before>
+__device__ __forceinline__ int locate_pair(int all, int off, Before&& before) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = all;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+        const unsigned fits = __ballot_sync(FULL, at < hi && before(min(at, hi - 1)) <= off);
+        lo += (31 - __clz(fits)) * step;  // lane 0's candidate always fits
+        hi = min(hi, lo + step);
+    }
+    return lo;
+}
+
 struct ChunkShape {
-    int group, causal;
+    const KvAttend& a;
     int tokens;  // of a row tile
-    __device__ __forceinline__ bool takes(const KvSeq& s) const { return s.count > 0 && !step_takes(s, group); }
-    __device__ __forceinline__ int pairs(const KvSeq& s) const { return (s.count + 2 * tokens - 1) / (2 * tokens); }
+    __device__ __forceinline__ bool takes(const KvSeq& s) const { return s.count > 0 && !step_takes(s, a.group); }
+    __device__ __forceinline__ int pairs(const KvSeq& s) const { return (int)a.by_pair(s.count + 2 * tokens - 1); }
     // a sequence's last pair may have one tile only
     __device__ __forceinline__ bool lone(const KvSeq& s, int pair) const { return s.count <= (2 * pair + 1) * tokens; }
     // slots that the pair's last row sees
     __device__ __forceinline__ int limit(const KvSeq& s, int pair) const {
-        return causal ? max(0, s.len - s.count + min(s.count, (pair + 1) * 2 * tokens)) : s.len;
+        return a.causal ? max(0, s.len - s.count + min(s.count, (pair + 1) * 2 * tokens)) : s.len;
     }
     __device__ __forceinline__ int units(const KvSeq& s, int pair) const {
         const int n = lone(s, pair) ? 2 * CHUNK_SLOTS : CHUNK_SLOTS;
@@ -187,15 +203,15 @@ struct ChunkShape {
     // units of the pairs before `pair`
     __device__ __forceinline__ int before(const KvSeq& s, int pair) const {
         const int all = pairs(s), n = min(pair, all - 1), per = 2 * tokens;
-        const int64_t a = (int64_t)s.len - s.count;
-        int64_t sum;
-        if (!causal) {
-            sum = (int64_t)n * max(1, (s.len + CHUNK_SLOTS - 1) / CHUNK_SLOTS);
+        const int ahead = s.len - s.count;  // more than -2^31: both are counts
+        int sum;
+        if (!a.causal) {
+            sum = n * max(1, (s.len + CHUNK_SLOTS - 1) / CHUNK_SLOTS);
         } else {
-            const int one = a > CHUNK_SLOTS ? 0 : (int)min((int64_t)n, (CHUNK_SLOTS - a) / per);  // pairs of one unit
-            sum = one + floor_sum(n - one, CHUNK_SLOTS, per, a + (int64_t)(one + 1) * per + CHUNK_SLOTS - 1);
+            const int one = ahead > CHUNK_SLOTS ? 0 : min(n, (int)a.by_pair(CHUNK_SLOTS - ahead));  // pairs of one unit
+            sum = one + (int)floor_sum(n - one, CHUNK_SLOTS, per, ahead + (one + 1) * per + CHUNK_SLOTS - 1);
         }
-        return (int)(pair < all ? sum : sum + units(s, all - 1));
+        return pair < all ? sum : sum + units(s, all - 1);
     }
 };
 
@@ -225,14 +241,8 @@ struct ChunkWalk {
             const int per = shape.before(s, all);
             int off = share.off;
             for (head = 0; off >= per; ++head) off -= per;
-            int lo = 0, hi = all - 1;  // the last pair that begins at or before off
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (shape.before(s, mid) <= off) lo = mid;
-                else hi = mid - 1;
-            }
-            pair = lo;
-            t0 = off - shape.before(s, lo);
+            pair = locate_pair(all, off, [&](int p) { return shape.before(s, p); });
+            t0 = off - shape.before(s, pair);
             located = true;
         }
         g->s = s;
@@ -291,13 +301,14 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // query rows past a tile's tokens are never loaded
-    for (int i = threadIdx.x; i < CHUNK_Q<DP> / 16; i += CHUNK_THREADS)
-        reinterpret_cast<uint4*>(smem_q)[i] = make_uint4(0u, 0u, 0u, 0u);
-    fence_proxy_async_smem();
+    if (a.tokens * a.group < CHUNK_ROWS) {  // the other rows are never loaded
+        for (int i = threadIdx.x; i < CHUNK_Q<DP> / 16; i += CHUNK_THREADS)
+            reinterpret_cast<uint4*>(smem_q)[i] = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async_smem();
+    }
     tmem_fence_before();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const ChunkShape shape{a.group, a.causal, CHUNK_ROWS / a.group};
+    const ChunkShape shape{a, a.tokens};
     KvShare share = kv_share<CHUNK_THREADS>(c, bt, scratch, CHUNK_LEAST, [&](const KvSeq& s) {
         return shape.takes(s) ? shape.before(s, shape.pairs(s)) * c.heads : 0;
     });
@@ -438,6 +449,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
         const int i = warp >> 2, r = (warp & 3) * 32 + lane;  // tile and row
+        const int r_token = (int)a.by_group(r);
         const uint32_t lanes = tm + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t tm_s = lanes + TM_S + i * 128, tm_o = lanes + TM_O + i * 128;
         // base 2; a scale of zero keeps -inf what it is
@@ -445,7 +457,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         uint32_t s_phase = 0, o_phase = 0;
         while (walk.next(&g)) {
             const int token1 = g.token0 + (g.lone ? 0 : i * shape.tokens);  // of the tile's first row
-            const int token = token1 + r / a.group;
+            const int token = token1 + r_token;
             const bool live = r < shape.tokens * a.group && token < g.s.count;
             const int lim = live ? max(0, row_limit(g.s, a.causal, token)) : 0;
             const int open = max(0, min(g.s.len, row_limit(g.s, a.causal, token1)));  // slots that every row sees
@@ -565,7 +577,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                     total += ml.y * part_factor(ml.x, top);
                 }
             }
-            const int h = g.head * a.group + r % a.group;
+            const int h = g.head * a.group + r - r_token * a.group;
             const int64_t tok = g.s.first + token;
             const float inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
 #pragma unroll 1
@@ -584,14 +596,26 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                     for (int k = 0; k < 32; ++k) o[k] += o1[k] * f1;
                 }
                 // parts: [four columns][row], so that a warp's accesses are contiguous
-                for (int k = 0; k < follow; ++k) {
-                    const int64_t part = part_of(1 + k);
-                    const float f = part_factor(__ldcg(parts.ml + part * CHUNK_ROWS + r).x, top);
-                    const float4* po = reinterpret_cast<const float4*>(parts.o) + (part * (DP / 4) + e / 4) * CHUNK_ROWS + r;
+                for (int k = 0; k < follow; k += 2) {  // two in flight; an odd last one again, for nothing
+                    float4 y[2][8];
+                    float f[2];
 #pragma unroll
-                    for (int w = 0; w < 8; ++w) {
-                        const float4 y = __ldcg(po + w * CHUNK_ROWS);
-                        o[4 * w] += y.x * f, o[4 * w + 1] += y.y * f, o[4 * w + 2] += y.z * f, o[4 * w + 3] += y.w * f;
+                    for (int u = 0; u < 2; ++u) {
+                        const int64_t part = part_of(1 + min(k + u, follow - 1));
+                        const float4* po = reinterpret_cast<const float4*>(parts.o) + (part * (DP / 4) + e / 4) * CHUNK_ROWS + r;
+                        f[u] = __ldcg(parts.ml + part * CHUNK_ROWS + r).x;
+#pragma unroll
+                        for (int w = 0; w < 8; ++w) y[u][w] = __ldcg(po + w * CHUNK_ROWS);
+                    }
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        f[u] = k + u < follow ? part_factor(f[u], top) : 0.f;
+                        if (f[u] == 0.f) continue;
+#pragma unroll
+                        for (int w = 0; w < 8; ++w) {
+                            o[4 * w] += y[u][w].x * f[u], o[4 * w + 1] += y[u][w].y * f[u];
+                            o[4 * w + 2] += y[u][w].z * f[u], o[4 * w + 3] += y[u][w].w * f[u];
+                        }
                     }
                 }
                 if (leaves) {

@@ -89,6 +89,28 @@ __device__ __forceinline__ int kv_find(const KvBatch& bt, int64_t row) {
     return lo;
 }
 
+// Division of 0 <= x < 2^31 by a number that a whole call shares: a multiplication by 2^(32 + shift) / by, rounded up
+// (Granlund and Montgomery, "Division by invariant integers using multiplication").
+struct Divisor {
+    uint32_t by, mul;
+    int shift;
+    __host__ static Divisor of(uint32_t by) {
+        int shift = 0;
+        while ((uint64_t(1) << shift) < by) ++shift;
+        // 2^shift >= by: the quotient fits 33 bits, its leading bit is left out and added back as x itself
+        const uint64_t m = ((uint64_t(1) << 32) * ((uint64_t(1) << shift) - by)) / by + 1;
+        return {by, (uint32_t)m, shift};
+    }
+    __host__ __device__ __forceinline__ uint32_t operator()(uint32_t x) const {
+#ifdef __CUDA_ARCH__
+        const uint32_t high = __umulhi(x, mul);
+#else
+        const uint32_t high = (uint32_t)((uint64_t)x * mul >> 32);
+#endif
+        return (uint32_t)(((uint64_t)high + x) >> shift);
+    }
+};
+
 struct KvAttend {
     const uint16_t* q;
     uint16_t* out;
@@ -97,6 +119,8 @@ struct KvAttend {
     int64_t qs[2], os[2], ss[2];
     int64_t scores_width;
     int heads, group;  // query heads; query heads per kv head
+    int tokens;        // of a chunk's row tile
+    Divisor by_group, by_tokens, by_pair;  // group, tokens, 2 tokens
     int max_q;
     int causal;
     float scale;

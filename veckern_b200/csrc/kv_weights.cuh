@@ -25,30 +25,29 @@ constexpr int weights_smem() {
 }
 
 struct WeightsShape {
-    int group, causal;
+    const KvAttend& a;
     int tokens;  // of a row tile
-    int64_t width;
     __device__ __forceinline__ bool takes(const KvSeq& s) const {
-        return s.count > 0 && s.len > 0 && !step_takes(s, group);
+        return s.count > 0 && s.len > 0 && !step_takes(s, a.group);
     }
     __device__ __forceinline__ int pairs(const KvSeq& s) const {
-        return (int)((min((int64_t)s.len, width) + WEIGHTS_PAIR - 1) / WEIGHTS_PAIR);
+        return (int)((min((int64_t)s.len, a.scores_width) + WEIGHTS_PAIR - 1) / WEIGHTS_PAIR);
     }
-    __device__ __forceinline__ int row_tiles(const KvSeq& s) const { return (s.count + tokens - 1) / tokens; }
+    __device__ __forceinline__ int row_tiles(const KvSeq& s) const { return (int)a.by_tokens(s.count + tokens - 1); }
     // the first row tile with a row that sees the pair's first slot
     __device__ __forceinline__ int first(const KvSeq& s, int pair) const {
-        const int64_t x = (int64_t)pair * WEIGHTS_PAIR - (s.len - s.count);
-        return causal && x > 0 ? (int)(x / tokens) : 0;
+        const int x = pair * WEIGHTS_PAIR - (s.len - s.count);
+        return a.causal && x > 0 ? (int)a.by_tokens(x) : 0;
     }
     // units of the pairs before `pair`
     __device__ __forceinline__ int before(const KvSeq& s, int pair) const {
-        int64_t sum = (int64_t)pair * row_tiles(s);
-        if (causal) {
-            const int64_t a = (int64_t)s.len - s.count;
-            const int64_t p0 = a < 0 ? 0 : min((int64_t)pair, (a + WEIGHTS_PAIR - 1) / WEIGHTS_PAIR);
-            sum -= floor_sum(pair - p0, tokens, WEIGHTS_PAIR, p0 * WEIGHTS_PAIR - a);
+        int sum = pair * row_tiles(s);
+        if (a.causal) {
+            const int ahead = s.len - s.count;
+            const int p0 = ahead < 0 ? 0 : min(pair, (ahead + WEIGHTS_PAIR - 1) / WEIGHTS_PAIR);
+            sum -= (int)floor_sum(pair - p0, tokens, WEIGHTS_PAIR, p0 * WEIGHTS_PAIR - ahead);
         }
-        return (int)sum;
+        return sum;
     }
 };
 
@@ -79,14 +78,8 @@ struct WeightsWalk {
             const int per = shape.before(s, all);
             int off = share.off;
             for (head = 0; off >= per; ++head) off -= per;
-            int lo = 0, hi = all - 1;
-            while (lo < hi) {
-                const int mid = (lo + hi + 1) >> 1;
-                if (shape.before(s, mid) <= off) lo = mid;
-                else hi = mid - 1;
-            }
-            pair = lo;
-            skip = off - shape.before(s, lo);
+            pair = locate_pair(all, off, [&](int p) { return shape.before(s, p); });
+            skip = off - shape.before(s, pair);
             located = true;
         }
         const int tiles = shape.row_tiles(s) - shape.first(s, pair);
@@ -98,7 +91,7 @@ struct WeightsWalk {
         g->count = min(tiles - skip, share.left);
         g->leaves = skip > 0;
         g->rest = tiles - skip - g->count;
-        g->both = min((int64_t)s.len, shape.width) > (int64_t)pair * WEIGHTS_PAIR + CHUNK_SLOTS;
+        g->both = min((int64_t)s.len, shape.a.scores_width) > (int64_t)pair * WEIGHTS_PAIR + CHUNK_SLOTS;
         share.left -= g->count;
         skip = 0;
         if (++pair == all) pair = 0, ++head;
@@ -143,13 +136,14 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // query rows past a tile's tokens are never loaded: their products must not be NaN
-    for (int i = threadIdx.x; i < RING * SLOT / 16; i += CHUNK_THREADS)
-        reinterpret_cast<uint4*>(ring)[i] = make_uint4(0u, 0u, 0u, 0u);
-    fence_proxy_async_smem();
+    if (a.tokens * a.group < CHUNK_ROWS) {  // the other rows are never loaded: their products must not be NaN
+        for (int i = threadIdx.x; i < RING * SLOT / 16; i += CHUNK_THREADS)
+            reinterpret_cast<uint4*>(ring)[i] = make_uint4(0u, 0u, 0u, 0u);
+        fence_proxy_async_smem();
+    }
     tmem_fence_before();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const WeightsShape shape{a.group, a.causal, CHUNK_ROWS / a.group, a.scores_width};
+    const WeightsShape shape{a, a.tokens};
     KvShare share = kv_share<CHUNK_THREADS>(c, bt, scratch, CHUNK_LEAST, [&](const KvSeq& s) {
         return shape.takes(s) ? shape.before(s, shape.pairs(s)) * c.heads : 0;
     });
@@ -247,7 +241,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             umma_commit(k_empty, me);
         }
     } else if (warp < 8) {
-        const int i = warp >> 2, r = (warp & 3) * 32 + lane;
+        const int i = warp >> 2, r = (warp & 3) * 32 + lane, r_token = (int)a.by_group(r);
         const uint32_t lanes = tm + ((uint32_t)((warp & 3) * 32) << 16) + i * 256;
         float* lse = s_lse + i * 256;
         const float scale = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-37f);
@@ -257,9 +251,9 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                 const int j = g.pair * WEIGHTS_PAIR + i * CHUNK_SLOTS + r;
                 // row r of tile q: its token and head, and its lse in base 2; no row, or one that saw nothing, has weight 0
                 auto lse_of = [&](int q) {
-                    const int token = q * shape.tokens + r / a.group;
+                    const int token = q * shape.tokens + r_token;
                     if (r >= shape.tokens * a.group || token >= g.s.count) return INFINITY;
-                    const float v = __ldg(a.lse + (g.s.first + token) * a.heads + g.head * a.group + r % a.group);
+                    const float v = __ldg(a.lse + (g.s.first + token) * a.heads + g.head * a.group + r - r_token * a.group);
                     return v == -INFINITY ? INFINITY : v * 1.4426950408889634f;
                 };
                 float sum = 0.f, next = lse_of(g.q0);
