@@ -219,7 +219,7 @@ int launch_chunk(const vk_kv* kv, const vk::KvPages& c, const vk::KvBatch& bt, c
     const auto weights = &vk::kv_weights_kernel<T, DP>;
     constexpr int weights_smem = vk::weights_smem<DP>();
     VK_TRY(prepare_kernel(weights, kv->desc.device, weights_smem));
-    return launch_behind(weights, dim3(p.chunk_ctas), vk::CHUNK_THREADS, weights_smem, st, map_q, kv->map_k, c, bt, a, parts);
+    return launch_behind(weights, dim3(p.chunk_ctas), vk::WEIGHTS_THREADS, weights_smem, st, map_q, kv->map_k, c, bt, a, parts);
 }
 
 template <typename T>

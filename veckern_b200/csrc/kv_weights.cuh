@@ -5,7 +5,8 @@
 // lanes: S^T = K Q^T puts a slot's products with 128 rows into one thread's columns, so that its weights are summed in
 // registers, without a shuffle or an atomic, and every row's lse is read by all threads alike from shared memory.
 //
-// A unit is a pair of slot tiles (2 x 128, one per warpgroup) against one row tile. Units run row tile by row tile within
+// A unit is a pair of slot tiles (2 x 128) against one row tile; two warpgroups share a slot tile, half of the rows each
+// (four warps per scheduler: with two, their latencies were not covered and the exponentials took twice as long). Units run row tile by row tile within
 // a pair, the pair's keys stay in shared memory and the rows stream; the units of all (sequence, kv head, pair)s are laid
 // end to end and shared out equally, and cut pairs are finished from parts, as in the step kernel.
 //
@@ -19,9 +20,10 @@ namespace vk {
 constexpr int WEIGHTS_PAIR = 2 * CHUNK_SLOTS;  // slots of a pair
 template <int DP>
 constexpr int WEIGHTS_RING = 4;  // row tiles in flight
+constexpr int WEIGHTS_THREADS = 576;  // four warpgroups that add up, the MMA warp, the loading warp
 template <int DP>
 constexpr int weights_smem() {
-    return (2 + WEIGHTS_RING<DP>) * CHUNK_SLOT<DP> + 2 * 2 * 128 * 4 + 512;
+    return (2 + WEIGHTS_RING<DP>) * CHUNK_SLOT<DP> + 4 * 2 * 64 * 4 + 2 * 2 * 128 * 4 + 512;
 }
 
 struct WeightsShape {
@@ -100,21 +102,22 @@ struct WeightsWalk {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(CHUNK_THREADS, 1)
+__global__ void __launch_bounds__(WEIGHTS_THREADS, 1)
     kv_weights_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, KvPages c,
                       KvBatch bt, KvAttend a, KvParts parts) {
     constexpr int HALVES = DP / 64, KS = DP / 16, RING = WEIGHTS_RING<DP>, SLOT = CHUNK_SLOT<DP>;
     extern __shared__ __align__(1024) uint8_t ring[];  // the swizzle goes by address bits: 1024-byte aligned
     uint8_t* smem_k = ring + RING * SLOT;              // the pair's two tiles
-    float* s_lse = reinterpret_cast<float*>(smem_k + 2 * SLOT);  // [warpgroup][2][128]
-    uint64_t* q_full = reinterpret_cast<uint64_t*>(s_lse + 2 * 2 * 128);
+    float* s_lse = reinterpret_cast<float*>(smem_k + 2 * SLOT);  // [warpgroup][2][64]: minus a row's lse, base 2
+    float* s_sum = s_lse + 4 * 2 * 64;                           // [2][slot tile][128]: of the second half of the rows
+    uint64_t* q_full = reinterpret_cast<uint64_t*>(s_sum + 2 * 2 * 128);
     uint64_t* q_empty = q_full + RING;
     uint64_t* k_full = q_empty + RING;
     uint64_t* k_empty = k_full + 1;
-    uint64_t* s_full = k_empty + 1;  // [warpgroup][2]
+    uint64_t* s_full = k_empty + 1;  // [slot tile][2]
     uint64_t* s_empty = s_full + 4;
     int* scratch = reinterpret_cast<int*>(s_empty + 4);
-    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(scratch + CHUNK_THREADS / 32 + 2);
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(scratch + WEIGHTS_THREADS / 32 + 2);
     const int warp = __shfl_sync(FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         prefetch_map(&map_q);
@@ -127,24 +130,24 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         mbar_init(k_empty, 1);
         for (int i = 0; i < 4; ++i) {
             mbar_init(s_full + i, 1);
-            mbar_init(s_empty + i, 128);
+            mbar_init(s_empty + i, 8);
         }
         fence_mbar_init();
     }
-    if (warp == 8) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(tmem_at))
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     if (a.tokens * a.group < CHUNK_ROWS) {  // the other rows are never loaded: their products must not be NaN
-        for (int i = threadIdx.x; i < RING * SLOT / 16; i += CHUNK_THREADS)
+        for (int i = threadIdx.x; i < RING * SLOT / 16; i += WEIGHTS_THREADS)
             reinterpret_cast<uint4*>(ring)[i] = make_uint4(0u, 0u, 0u, 0u);
         fence_proxy_async_smem();
     }
     tmem_fence_before();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const WeightsShape shape{a, a.tokens};
-    KvShare share = kv_share<CHUNK_THREADS>(c, bt, scratch, CHUNK_LEAST, [&](const KvSeq& s) {
+    KvShare share = kv_share<WEIGHTS_THREADS>(c, bt, scratch, CHUNK_LEAST, [&](const KvSeq& s) {
         return shape.takes(s) ? shape.before(s, shape.pairs(s)) * c.heads : 0;
     });
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -153,7 +156,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     KvWait wait{c.status};
     WeightsWalk walk{c, bt, shape, share, 0, 0, 0, false};
     WeightsSegment g;
-    if (warp == 9) {
+    if (warp == 17) {
         int slot = 0, loaded = 0;
         uint32_t phase = 0, k_phase = 0;
         const int box_shift = min(c.page_shift, 6), boxes = CHUNK_SLOTS >> box_shift;
@@ -205,7 +208,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             }
             if (loaded && !mbar_wait_bounded(k_full, k_phase ^ 1, 2 * KV_WAIT_BUDGET)) atomicOr(c.status, ERR_DRAIN_TIMEOUT);
         }
-    } else if (warp == 8) {
+    } else if (warp == 16) {
         const uint32_t idesc = umma_idesc<T>(CHUNK_ROWS, false, a.scale < 0.f);
         const uint32_t k_low = umma_low(smem_u32(smem_k), 16), q_low = umma_low(smem_u32(ring), 16);
         int slot = 0, used[2] = {0, 0};  // row tiles that went to each warpgroup's two buffers
@@ -240,77 +243,92 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             }
             umma_commit(k_empty, me);
         }
-    } else if (warp < 8) {
-        const int i = warp >> 2, r = (warp & 3) * 32 + lane, r_token = (int)a.by_group(r);
-        const uint32_t lanes = tm + ((uint32_t)((warp & 3) * 32) << 16) + i * 256;
-        float* lse = s_lse + i * 256;
+    } else {
+        const int wg = warp >> 2, i = wg & 1, half = wg >> 1, r = (warp & 3) * 32 + lane;
+        const int row = half * 64 + (r & 63), row_token = (int)a.by_group(row);  // whose lse this thread fetches
+        const uint32_t lanes = tm + ((uint32_t)((warp & 3) * 32) << 16) + i * 256 + half * 64;
+        float* lse = s_lse + wg * 128;
         const float scale = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-37f);
-        int used = 0;
+        const Pair scale2 = pair_of(scale, scale);
+        int used = 0, turn = 0;
         while (walk.next(&g)) {
-            if (i == 0 || g.both) {
-                const int j = g.pair * WEIGHTS_PAIR + i * CHUNK_SLOTS + r;
-                // row r of tile q: its token and head, and its lse in base 2; no row, or one that saw nothing, has weight 0
-                auto lse_of = [&](int q) {
-                    const int token = q * shape.tokens + r_token;
-                    if (r >= shape.tokens * a.group || token >= g.s.count) return INFINITY;
-                    const float v = __ldg(a.lse + (g.s.first + token) * a.heads + g.head * a.group + r - r_token * a.group);
-                    return v == -INFINITY ? INFINITY : v * 1.4426950408889634f;
-                };
-                float sum = 0.f, next = lse_of(g.q0);
-                for (int q = g.q0; q < g.q0 + g.count; ++q) {
-                    const int buf = used & 1;
-                    const uint32_t phase = (used >> 1) & 1;
-                    ++used;
-                    lse[buf * 128 + r] = next;
-                    if (q + 1 < g.q0 + g.count) next = lse_of(q + 1);
-                    asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
-                    wait(s_full + 2 * i + buf, phase);
-                    tmem_fence_after();
-                    float x[CHUNK_ROWS];
+            if (i == 1 && !g.both) continue;
+            const int j = g.pair * WEIGHTS_PAIR + i * CHUNK_SLOTS + r;
+            // no row, or one that saw nothing: weight 0
+            auto minus_lse = [&](int q) {
+                const int token = q * shape.tokens + row_token;
+                if (row >= shape.tokens * a.group || token >= g.s.count) return -INFINITY;
+                const float v = __ldg(a.lse + (g.s.first + token) * a.heads + g.head * a.group + row - row_token * a.group);
+                return v == -INFINITY ? -INFINITY : -v * 1.4426950408889634f;
+            };
+            Pair sum[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
+            float next = minus_lse(g.q0);
+            for (int q = g.q0; q < g.q0 + g.count; ++q) {
+                const int buf = used & 1;
+                if (r < 64) lse[buf * 64 + r] = next;
+                if (q + 1 < g.q0 + g.count) next = minus_lse(q + 1);
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");
+                wait(s_full + 2 * i + buf, used >> 1 & 1);
+                ++used;
+                tmem_fence_after();
+                // rows that see this slot: from `from` on; the tile's rows end at `to`; counted from this half's first
+                const int to = min(shape.tokens, g.s.count - q * shape.tokens) * a.group - half * 64;
+                const int from =
+                    (a.causal ? max(0, j - (g.s.len - g.s.count) - q * shape.tokens) * a.group : 0) - half * 64;
+                const bool masked = __any_sync(FULL, from > 0) || to < min(64, shape.tokens * a.group - half * 64);
+                const float4* l4 = reinterpret_cast<const float4*>(lse + buf * 64);
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) tmem_ld32(lanes + buf * 128 + 32 * e, x + 32 * e);
+                for (int h = 0; h < 64; h += 32) {
+                    float x[32];
+                    tmem_ld32(lanes + buf * 128 + h, x);
                     tmem_wait_ld();
-                    tmem_fence_before();
-                    mbar_arrive(s_empty + 2 * i + buf);
-                    // rows that see this slot: from `from` on; the tile's rows end at `to`
-                    const int to = min(shape.tokens, g.s.count - q * shape.tokens) * a.group;
-                    const int from = a.causal ? max(0, j - (g.s.len - g.s.count) - q * shape.tokens) * a.group : 0;
-                    if (__any_sync(FULL, from > 0) || to < shape.tokens * a.group) {
+                    if (h == 32) {
+                        tmem_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(s_empty + 2 * i + buf);
+                    }
+                    if (masked) {
 #pragma unroll
-                        for (int e = 0; e < CHUNK_ROWS; ++e) x[e] = e >= from && e < to ? x[e] : -INFINITY;
+                        for (int e = 0; e < 32; ++e) x[e] = h + e >= from && h + e < to ? x[e] : -INFINITY;
                     }
-                    float part[4] = {0.f, 0.f, 0.f, 0.f};
-                    const float4* l4 = reinterpret_cast<const float4*>(lse + buf * 128);
 #pragma unroll
-                    for (int e = 0; e < CHUNK_ROWS / 4; ++e) {
-                        const float4 y = l4[e];
-                        part[0] += ex2(fmaf(x[4 * e], scale, -y.x));
-                        part[1] += ex2(fmaf(x[4 * e + 1], scale, -y.y));
-                        part[2] += ex2(fmaf(x[4 * e + 2], scale, -y.z));
-                        part[3] += ex2(fmaf(x[4 * e + 3], scale, -y.w));
+                    for (int e = 0; e < 8; ++e) {
+                        const float4 y = l4[h / 4 + e];
+                        const float2 u = floats(fma2(pair_of(x[4 * e], x[4 * e + 1]), scale2, pair_of(y.x, y.y)));
+                        const float2 w = floats(fma2(pair_of(x[4 * e + 2], x[4 * e + 3]), scale2, pair_of(y.z, y.w)));
+                        sum[0] = sum[0] + pair_of(ex2(u.x), ex2(u.y));
+                        sum[1] = sum[1] + pair_of(ex2(w.x), ex2(w.y));
                     }
-                    sum += (part[0] + part[1]) + (part[2] + part[3]);
                 }
-                const int part = 2 * blockIdx.x + i;
-                if (g.leaves) {
-                    parts.o[(int64_t)part * CHUNK_SLOTS + r] = sum;
-                    asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
-                    if (r == 0) part_publish(parts, part);
-                } else {
-                    const int follow = walk.share.followers(g.rest);
-                    if (follow) {
-                        for (int k = r; k < follow; k += 128) part_await(parts, part + 2 + 2 * k, wait);
-                        asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
-                        for (int k = 0; k < follow; ++k) sum += __ldcg(parts.o + (int64_t)(part + 2 + 2 * k) * CHUNK_SLOTS + r);
-                        for (int k = r; k < follow; k += 128) parts.ready[part + 2 + 2 * k] = 0;
-                    }
-                    if (j < min((int64_t)g.s.len, a.scores_width)) a.scores[g.b * a.ss[0] + g.head * a.ss[1] + j] += sum;
+            }
+            const float2 both = floats(sum[0] + sum[1]);
+            float total = both.x + both.y;
+            // The second half's warpgroup hands its sum over, into the other buffer each time: it cannot be two ahead.
+            float* other = s_sum + (turn & 1) * 256 + i * 128 + r;
+            turn ^= 1;
+            if (half == 1) *other = total;
+            asm volatile("bar.sync %0, 256;" ::"r"(5 + i) : "memory");
+            if (half == 1) continue;
+            total += *other;
+            const int part = 2 * blockIdx.x + i;
+            if (g.leaves) {
+                parts.o[(int64_t)part * CHUNK_SLOTS + r] = total;
+                asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");
+                if (r == 0) part_publish(parts, part);
+            } else {
+                const int follow = walk.share.followers(g.rest);
+                if (follow) {
+                    for (int k = r; k < follow; k += 128) part_await(parts, part + 2 + 2 * k, wait);
+                    asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");
+                    for (int k = 0; k < follow; ++k) total += __ldcg(parts.o + (int64_t)(part + 2 + 2 * k) * CHUNK_SLOTS + r);
+                    for (int k = r; k < follow; k += 128) parts.ready[part + 2 + 2 * k] = 0;
                 }
+                if (j < min((int64_t)g.s.len, a.scores_width)) a.scores[g.b * a.ss[0] + g.head * a.ss[1] + j] += total;
             }
         }
     }
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 16) {
         __syncwarp();
         tmem_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tm) : "memory");
