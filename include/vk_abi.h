@@ -376,7 +376,8 @@ typedef struct {
     int64_t scores_stride[2];
     int64_t scores_width;
     int heads; /* a multiple of kv_heads, at most 128 times it */
-    int max_q; /* at least the largest number of new tokens of a sequence; 0 = unknown (`tokens` is assumed) */
+    int max_q; /* at least the largest number of new tokens of a sequence; 0 = unknown (`tokens` is assumed). A sequence
+                  that has more may be left out, which vk_kv_sync reports */
     int causal;
     float scale;
     void* workspace; /* DEVICE, 256-byte aligned, at least vk_kv_attend_workspace bytes, for one call at a time (the

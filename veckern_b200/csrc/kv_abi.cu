@@ -74,28 +74,30 @@ int check_rows(const char* what, const void* p, const int64_t* stride) {
 
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 
-// How a call's attention is laid out: which kernels may have work, their CTAs, and the workspace.
+// How a call's attention is laid out: which kernel, its CTAs, and the workspace.
+//
+// Where every sequence has at most 16 rows (tokens x query heads of a kv head) the step kernel reads the cache at the
+// memory's rate on mma.sync; with a longer sequence in the call the chunk kernel takes them all. Its tile of 128 rows is
+// mostly empty for a short sequence, but it reads 2 x 128 slots per 3,300 cycles and SM, which is the memory's rate too
+// (a step of 32 sequences of up to 8,192 slots: 132 us, the step kernel 119), so that a launch for the short ones of a
+// mixed call would cost more than it saves.
 struct AttendPlan {
-    bool step, chunk;
+    bool step;
     int rows;  // of the step path: 8 or 16
-    int step_ctas, chunk_ctas;
+    int ctas;
     size_t ready, o, ml, s, bytes;  // offsets
 };
 
 AttendPlan plan_attend(const vk_kv* kv, const vk::KvBatch& bt, int group, int max_q, bool scores) {
     AttendPlan p{};
     const int64_t rows = (int64_t)max_q * group;
-    p.chunk = rows > vk::STEP_ROWS;
-    p.step = group <= vk::STEP_ROWS && !(bt.batch == 1 && bt.tokens * group > vk::STEP_ROWS);
-    p.rows = std::min<int64_t>(rows, vk::STEP_ROWS) <= 8 ? 8 : 16;
-    p.step_ctas = 2 * kv->sm_count;
-    p.chunk_ctas = kv->sm_count;
+    p.step = rows <= vk::STEP_ROWS;
+    p.rows = rows <= 8 ? 8 : 16;
+    p.ctas = p.step ? 2 * kv->sm_count : kv->sm_count;
     const int dp = kv->desc.head_dim <= 64 ? 64 : 128;
     const int64_t slots = (int64_t)bt.width << kv->page_shift;
-    // The two paths run one after the other on the stream: they share the parts' room. What has to be zero before a call
-    // lies at the start, whatever the sizes.
-    const size_t rows_of_parts = std::max(p.step ? (size_t)p.step_ctas * vk::STEP_ROWS : 0,
-                                          p.chunk ? 2 * (size_t)p.chunk_ctas * vk::CHUNK_ROWS : 0);
+    // What has to be zero before a call lies at the start, whatever the sizes.
+    const size_t rows_of_parts = (size_t)p.ctas * (p.step ? vk::STEP_ROWS : 2 * vk::CHUNK_ROWS);
     p.o = VK_KV_WORKSPACE_ZEROED;
     p.ml = p.o + align256(rows_of_parts * dp * sizeof(float));
     p.s = p.ml + align256(rows_of_parts * sizeof(float2));
@@ -155,10 +157,10 @@ template <typename T, int DP>
 int launch_step(const vk_kv* kv, const vk::KvPages& c, const vk::KvBatch& bt, const vk::KvAttend& a,
                 const vk::KvParts& parts, const AttendPlan& p, cudaStream_t st) {
     if (p.rows == 8)
-        return a.scores ? launch_step_as<T, DP, 8, true>(kv, c, bt, a, parts, p.step_ctas, st)
-                        : launch_step_as<T, DP, 8, false>(kv, c, bt, a, parts, p.step_ctas, st);
-    return a.scores ? launch_step_as<T, DP, 16, true>(kv, c, bt, a, parts, p.step_ctas, st)
-                    : launch_step_as<T, DP, 16, false>(kv, c, bt, a, parts, p.step_ctas, st);
+        return a.scores ? launch_step_as<T, DP, 8, true>(kv, c, bt, a, parts, p.ctas, st)
+                        : launch_step_as<T, DP, 8, false>(kv, c, bt, a, parts, p.ctas, st);
+    return a.scores ? launch_step_as<T, DP, 16, true>(kv, c, bt, a, parts, p.ctas, st)
+                    : launch_step_as<T, DP, 16, false>(kv, c, bt, a, parts, p.ctas, st);
 }
 
 int encoder(PFN_cuTensorMapEncodeTiled_v12000* out) {
@@ -214,12 +216,12 @@ int launch_chunk(const vk_kv* kv, const vk::KvPages& c, const vk::KvBatch& bt, c
     const auto fn = &vk::kv_chunk_kernel<T, DP>;
     constexpr int smem = vk::chunk_smem<DP>();
     VK_TRY(prepare_kernel(fn, kv->desc.device, smem));
-    VK_TRY(launch_behind(fn, dim3(p.chunk_ctas), vk::CHUNK_THREADS, smem, st, map_q, kv->map_k, kv->map_v, c, bt, a, parts));
+    VK_TRY(launch_behind(fn, dim3(p.ctas), vk::CHUNK_THREADS, smem, st, map_q, kv->map_k, kv->map_v, c, bt, a, parts));
     if (!a.scores || a.scores_width == 0) return VK_OK;
     const auto weights = &vk::kv_weights_kernel<T, DP>;
     constexpr int weights_smem = vk::weights_smem<DP>();
     VK_TRY(prepare_kernel(weights, kv->desc.device, weights_smem));
-    return launch_behind(weights, dim3(p.chunk_ctas), vk::WEIGHTS_THREADS, weights_smem, st, map_q, kv->map_k, c, bt, a, parts);
+    return launch_behind(weights, dim3(p.ctas), vk::WEIGHTS_THREADS, weights_smem, st, map_q, kv->map_k, c, bt, a, parts);
 }
 
 template <typename T>
@@ -233,13 +235,9 @@ int launch_attend(const vk_kv* kv, const vk::KvBatch& bt, const vk::KvAttend& a,
     parts.ml = reinterpret_cast<float2*>(w + p.ml);
     parts.s = reinterpret_cast<float*>(w + p.s);
     parts.s_slots = (int64_t)bt.width << kv->page_shift;
-    if (p.step) VK_TRY((c.dim <= 64 ? launch_step<T, 64>(kv, c, bt, a, parts, p, st)
-                                    : launch_step<T, 128>(kv, c, bt, a, parts, p, st)));
-    if (p.chunk) {
-        VK_TRY((c.dim <= 64 ? launch_chunk<T, 64>(kv, c, bt, a, parts, p, st)
-                            : launch_chunk<T, 128>(kv, c, bt, a, parts, p, st)));
-    }
-    return VK_OK;
+    if (p.step)
+        return c.dim <= 64 ? launch_step<T, 64>(kv, c, bt, a, parts, p, st) : launch_step<T, 128>(kv, c, bt, a, parts, p, st);
+    return c.dim <= 64 ? launch_chunk<T, 64>(kv, c, bt, a, parts, p, st) : launch_chunk<T, 128>(kv, c, bt, a, parts, p, st);
 }
 
 // Checks what attention's launches and its workspace's size depend on.

@@ -188,7 +188,7 @@ __device__ __forceinline__ int locate_pair(int all, int off, Before&& before) {
 struct ChunkShape {
     const KvAttend& a;
     int tokens;  // of a row tile
-    __device__ __forceinline__ bool takes(const KvSeq& s) const { return s.count > 0 && !step_takes(s, a.group); }
+    __device__ __forceinline__ bool takes(const KvSeq& s) const { return s.count > 0; }
     __device__ __forceinline__ int pairs(const KvSeq& s) const { return (int)a.by_pair(s.count + 2 * tokens - 1); }
     // a sequence's last pair may have one tile only
     __device__ __forceinline__ bool lone(const KvSeq& s, int pair) const { return s.count <= (2 * pair + 1) * tokens; }

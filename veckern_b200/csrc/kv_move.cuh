@@ -113,6 +113,10 @@ __global__ void __launch_bounds__(SELECT_THREADS, 2) kv_select_kernel(KvPages c,
                 if (i0 + u * SELECT_THREADS < size) held[i0 + u * SELECT_THREADS] = kv_rank(x[u]);
         }
     __syncthreads();
+    auto cluster_sync = [&] {
+        if constexpr (C > 1) cluster.sync();
+        else __syncthreads();
+    };
     auto rank_of = [&](int i) { return fits ? held[i] : kv_rank(score(from + i)); };
     // sum over the threads before this one, and the block's total
     auto scan = [&](int x, int* total) {
@@ -150,7 +154,7 @@ __global__ void __launch_bounds__(SELECT_THREADS, 2) kv_select_kernel(KvPages c,
                 const uint32_t u = rank_of(i);
                 if ((u & mask) == cut) atomicAdd(h + (u >> shift & low), 1);
             }
-            cluster.sync();
+            cluster_sync();
             // thread t takes PER digits, from the largest down
             const int first = SELECT_BINS - PER * (tid + 1);
             int sum[PER] = {};
@@ -200,12 +204,14 @@ __global__ void __launch_bounds__(SELECT_THREADS, 2) kv_select_kernel(KvPages c,
     // each warp takes a contiguous range of the slice: count, then emit behind the ranges and CTAs before it
     const int span = ((size + WARPS - 1) / WARPS + 31) / 32 * 32, lo = min(size, warp * span), hi = min(size, lo + span);
     int gt = 0, eq = 0;
-    for (int i = lo; i < hi; i += 32) {
-        const bool in = i + lane < hi;
-        const uint32_t u = in ? rank_of(i + lane) : 0u;
-        gt += __popc(__ballot_sync(FULL, in && u > cut));
-        eq += __popc(__ballot_sync(FULL, in && u == cut));
+#pragma unroll 4
+    for (int i = lo + lane; i < hi; i += 32) {
+        const uint32_t u = rank_of(i);
+        gt += u > cut;
+        eq += u == cut;
     }
+    gt = __reduce_add_sync(FULL, gt);
+    eq = __reduce_add_sync(FULL, eq);
     __syncthreads();
     if (lane == 0) {
         warp_a[warp] = gt;
@@ -217,31 +223,42 @@ __global__ void __launch_bounds__(SELECT_THREADS, 2) kv_select_kernel(KvPages c,
         if (w < warp) before_gt += warp_a[w], before_eq += warp_b[w];
         all_gt += warp_a[w], all_eq += warp_b[w];
     }
-    if (tid == 0) mine_gt = all_gt, mine_eq = all_eq;
-    cluster.sync();
     int cta_gt = 0, cta_eq = 0;  // of the CTAs before this one: one lane each
-    if (lane < rank) {
-        cta_gt = *cluster.map_shared_rank(&mine_gt, lane);
-        cta_eq = *cluster.map_shared_rank(&mine_eq, lane);
-    }
-    cta_gt = __reduce_add_sync(FULL, cta_gt);
-    cta_eq = __reduce_add_sync(FULL, cta_eq);
-    cluster.sync();  // nobody reads this CTA's shared memory from here on
-    before_gt += cta_gt, before_eq += cta_eq;
-    for (int i = lo; i < hi; i += 32) {
-        const int slot = from + i + lane;
-        const bool in = i + lane < hi;
-        const uint32_t u = in ? rank_of(i + lane) : 0u;
-        const unsigned mg = __ballot_sync(FULL, in && u > cut), me = __ballot_sync(FULL, in && u == cut);
-        const unsigned below = (1u << lane) - 1u;
-        const int eq_before = before_eq + __popc(me & below);
-        if ((mg >> lane & 1u) || ((me >> lane & 1u) && eq_before < need)) {
-            const int at = before_gt + __popc(mg & below) + min(eq_before, need);
-            kept[at] = slot;
-            if (at < e.width) ns[at] = kv_score(u);
+    if constexpr (C > 1) {
+        if (tid == 0) mine_gt = all_gt, mine_eq = all_eq;
+        cluster.sync();
+        if (lane < rank) {
+            cta_gt = *cluster.map_shared_rank(&mine_gt, lane);
+            cta_eq = *cluster.map_shared_rank(&mine_eq, lane);
         }
-        before_gt += __popc(mg);
-        before_eq += __popc(me);
+        cta_gt = __reduce_add_sync(FULL, cta_gt);
+        cta_eq = __reduce_add_sync(FULL, cta_eq);
+        cluster.sync();  // nobody reads this CTA's shared memory from here on
+    }
+    before_gt += cta_gt, before_eq += cta_eq;
+    const unsigned below = (1u << lane) - 1u;
+    const int width = (int)min(e.width, (int64_t)INT32_MAX);
+    int at0 = before_gt + min(before_eq, need);
+    for (int i0 = lo; i0 < hi; i0 += 128) {  // four groups of 32 at a time, their ranks fetched together
+        uint32_t u[4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) u[w] = i0 + 32 * w + lane < hi ? rank_of(i0 + 32 * w + lane) : 0u;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const int i = i0 + 32 * w + lane;
+            unsigned keep = __ballot_sync(FULL, i < hi && u[w] > cut);
+            const unsigned me = __ballot_sync(FULL, i < hi && u[w] == cut);
+            if (me) {  // the first ones of those that tie
+                keep |= __ballot_sync(FULL, (me >> lane & 1u) && before_eq + __popc(me & below) < need);
+                before_eq += __popc(me);
+            }
+            if (keep >> lane & 1u) {
+                const int at = at0 + __popc(keep & below);
+                kept[at] = from + i;
+                if (at < width) ns[at] = kv_score(u[w]);
+            }
+            at0 += __popc(keep);
+        }
     }
     // a share of the latest slots, and what lies behind the kept ones
     for (int i = rank * SELECT_THREADS + tid; i < r; i += C * SELECT_THREADS) {

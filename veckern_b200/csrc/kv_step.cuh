@@ -204,8 +204,10 @@ __device__ __forceinline__ int row_limit(const KvSeq& s, int causal, int token) 
     return causal ? s.len - s.count + token + 1 : s.len;
 }
 
-__device__ __forceinline__ bool step_takes(const KvSeq& s, int group) {
-    return s.count > 0 && s.count * (int64_t)group <= STEP_ROWS;
+// The host launches this kernel where the caller's bound says that no sequence has more rows; one that has all the same
+// is left out and reported.
+__device__ __forceinline__ bool step_takes(const KvSeq& s, int group, int rows) {
+    return s.count > 0 && s.count * (int64_t)group <= rows;
 }
 
 template <int DP>
@@ -240,7 +242,10 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     auto tiles_of = [&](const KvSeq& s) { return max(1, (s.len + STEP_TILE - 1) / STEP_TILE); };
-    auto units_of = [&](const KvSeq& s) { return step_takes(s, a.group) ? tiles_of(s) * c.heads : 0; };
+    auto units_of = [&](const KvSeq& s) {
+        if (s.count > 0 && !step_takes(s, a.group, R)) atomicOr(c.status, ERR_LAYOUT);
+        return step_takes(s, a.group, R) ? tiles_of(s) * c.heads : 0;
+    };
     KvShare share = kv_share<STEP_THREADS>(c, bt, scratch, STEP_LEAST, units_of);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     KvWait wait{c.status};
@@ -251,7 +256,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
     while (share.left > 0) {
         const KvSeq s = kv_seq(c, bt, share.b);
         const int tiles = tiles_of(s);
-        if (!step_takes(s, a.group) || share.off >= tiles * c.heads) {
+        if (!step_takes(s, a.group, R) || share.off >= tiles * c.heads) {
             ++share.b;
             share.off = 0;
             continue;
@@ -509,7 +514,7 @@ __global__ void __launch_bounds__(256) kv_step_weights_kernel(KvPages c, KvBatch
     __shared__ float s_lse[R];
     const int b = blockIdx.z, head = blockIdx.y;
     const KvSeq s = kv_seq(c, bt, b);
-    if (!step_takes(s, a.group)) return;
+    if (!step_takes(s, a.group, R)) return;
     const int rows = s.count * a.group;
     if (threadIdx.x < R) {
         const int r = threadIdx.x;

@@ -30,7 +30,7 @@ struct WeightsShape {
     const KvAttend& a;
     int tokens;  // of a row tile
     __device__ __forceinline__ bool takes(const KvSeq& s) const {
-        return s.count > 0 && s.len > 0 && !step_takes(s, a.group);
+        return s.count > 0 && s.len > 0;
     }
     __device__ __forceinline__ int pairs(const KvSeq& s) const {
         return (int)((min((int64_t)s.len, a.scores_width) + WEIGHTS_PAIR - 1) / WEIGHTS_PAIR);

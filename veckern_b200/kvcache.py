@@ -59,7 +59,7 @@ class PagedCache:
     def __init__(self, k_pages, v_pages):
         import torch
 
-        self._torch, self._i32, self._lib = torch, torch.int32, lib()
+        self._torch, self._i32, self._f32, self._lib = torch, torch.int32, torch.float32, lib()
         self._h = C.c_void_p()
         for name, t in (("k_pages", k_pages), ("v_pages", v_pages)):
             if t.dim() != 4 or t.shape != k_pages.shape or t.dtype != k_pages.dtype or t.device != k_pages.device:
@@ -196,12 +196,13 @@ class PagedCache:
         torch = self._torch
         n = self._sequences(table, lens)
         self._check_scores(scores, n)
-        _want(new_table, "new_table", torch.int32, 2, self.device)
+        if new_table.dtype != self._i32 or new_table.dim() != 2 or new_table.device != self.device:
+            _want(new_table, "new_table", self._i32, 2, self.device)
         if new_table.shape[0] != n or (new_table.shape[1] > 1 and new_table.stride(1) != 1):
             raise ValueError("new_table must have one row per sequence, rows contiguous")
         if not 0 <= recent <= keep:
             raise ValueError("keep and recent must satisfy 0 <= recent <= keep")
-        kept = torch.empty((n, self.kv_heads, keep), dtype=torch.int32, device=self.device)
+        kept = torch.empty((n, self.kv_heads, keep), dtype=self._i32, device=self.device)
         new_lens = torch.empty_like(lens)
         new_scores = torch.empty_like(scores, memory_format=torch.contiguous_format)
         e = self._evict
@@ -216,7 +217,8 @@ class PagedCache:
         return kept, new_lens, new_scores
 
     def _check_scores(self, scores, n: int) -> None:
-        _want(scores, "scores", self._torch.float32, 3, self.device)
+        if scores.dtype != self._f32 or scores.dim() != 3 or scores.device != self.device:
+            _want(scores, "scores", self._f32, 3, self.device)
         if scores.shape[0] != n or scores.shape[1] != self.kv_heads or (scores.shape[2] > 1 and scores.stride(2) != 1):
             raise ValueError(f"scores must be [batch, {self.kv_heads}, width] with the last dimension contiguous")
 
