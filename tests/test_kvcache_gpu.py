@@ -287,6 +287,34 @@ def test_offsets_beyond_32_bits(counts):
                 assert torch.equal(big[new[b, 0].long(), :50, h], big[table[b].long()[j // 64], j % 64, h])
 
 
+@pytest.mark.parametrize("most", [1, 40])
+def test_attend_many_short_sequences(most):
+    """More sequences than a block has threads, of all small lengths, some without new tokens."""
+    rng = np.random.default_rng(most)
+    lens = [int(x) for x in rng.integers(0, 70, 1500)]
+    counts = [int(x) for x in rng.integers(0, most + 1, 1500)]
+    c = Cache(lens, 8, 1, 32, "float16", seed=most)
+    heads = 2
+    q = c.random(sum(counts), heads, 32, scale=2.0)
+    s = c.t.zeros((1500, 1, 70), device="cuda")
+    before = s.clone()
+    out, lse = c.cache.attend(q, c.offsets(counts), c.table, c.lens, scores=s, max_q=most)
+    c.cache.sync()
+    check_attend(c, q, counts, out, lse, True, None, s, before)
+
+
+def test_attend_reports_a_bound_that_does_not_hold():
+    """A sequence with more new tokens than max_q says is left out, and reported."""
+    torch = __import__("torch")
+    c = Cache([100, 60], 16, 1, 64, seed=6)
+    counts = [1, 5]
+    q = c.random(6, 4, 64)
+    for s in (None, torch.zeros((2, 1, 100), device="cuda")):
+        c.cache.attend(q, c.offsets(counts), c.table, c.lens, max_q=1, scores=s)
+        with pytest.raises(N.VkError, match="out of range"):
+            c.cache.sync()
+
+
 def test_attend_no_tokens_and_no_sequences():
     torch = __import__("torch")
     c = Cache([30], 8, 1, 64)

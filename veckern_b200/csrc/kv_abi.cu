@@ -83,7 +83,7 @@ size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 // mixed call would cost more than it saves.
 struct AttendPlan {
     bool step;
-    int rows;  // of the step path: 8 or 16
+    int rows, s_rows;  // of the step path, rounded up to 8 or 16; to 4, 8 or 16
     int ctas;
     size_t ready, o, ml, s, bytes;  // offsets
 };
@@ -93,6 +93,7 @@ AttendPlan plan_attend(const vk_kv* kv, const vk::KvBatch& bt, int group, int ma
     const int64_t rows = (int64_t)max_q * group;
     p.step = rows <= vk::STEP_ROWS;
     p.rows = rows <= 8 ? 8 : 16;
+    p.s_rows = rows <= 4 ? 4 : p.rows;
     p.ctas = p.step ? 2 * kv->sm_count : kv->sm_count;
     const int dp = kv->desc.head_dim <= 64 ? 64 : 128;
     const int64_t slots = (int64_t)bt.width << kv->page_shift;
@@ -101,7 +102,7 @@ AttendPlan plan_attend(const vk_kv* kv, const vk::KvBatch& bt, int group, int ma
     p.o = VK_KV_WORKSPACE_ZEROED;
     p.ml = p.o + align256(rows_of_parts * dp * sizeof(float));
     p.s = p.ml + align256(rows_of_parts * sizeof(float2));
-    p.bytes = p.s + (scores && p.step ? align256((size_t)bt.batch * kv->desc.kv_heads * slots * p.rows * sizeof(float)) : 0);
+    p.bytes = p.s + (scores && p.step ? align256((size_t)bt.batch * kv->desc.kv_heads * slots * p.s_rows * sizeof(float)) : 0);
     return p;
 }
 
@@ -145,10 +146,13 @@ int launch_step_as(const vk_kv* kv, const vk::KvPages& c, const vk::KvBatch& bt,
     VK_TRY(launch_behind(fn, dim3(ctas), vk::STEP_THREADS, smem, st, kv->map_k, kv->map_v, c, bt, a, parts));
     if constexpr (SCORES) {
         const int64_t width = std::min(parts.s_slots, a.scores_width);
-        if (width > 0)
-            VK_TRY(launch_behind(&vk::kv_step_weights_kernel<R>,
-                                 dim3((unsigned)std::min<int64_t>(ceil_div(width, 256), 4096), c.heads, bt.batch), 256, 0, st,
-                                 c, bt, a, parts));
+        if (width > 0) {
+            const auto weights = parts.s_rows == 4   ? &vk::kv_step_weights_kernel<4>
+                                 : parts.s_rows == 8 ? &vk::kv_step_weights_kernel<8>
+                                                     : &vk::kv_step_weights_kernel<16>;
+            const int64_t blocks = std::min<int64_t>(ceil_div(width, vk::STEP_WEIGHTS_SLOTS), 4096);
+            VK_TRY(launch_behind(weights, dim3((unsigned)blocks, c.heads, bt.batch), 256, 0, st, c, bt, a, parts));
+        }
     }
     return VK_OK;
 }
@@ -235,6 +239,7 @@ int launch_attend(const vk_kv* kv, const vk::KvBatch& bt, const vk::KvAttend& a,
     parts.ml = reinterpret_cast<float2*>(w + p.ml);
     parts.s = reinterpret_cast<float*>(w + p.s);
     parts.s_slots = (int64_t)bt.width << kv->page_shift;
+    parts.s_rows = p.s_rows;
     if (p.step)
         return c.dim <= 64 ? launch_step<T, 64>(kv, c, bt, a, parts, p, st) : launch_step<T, 128>(kv, c, bt, a, parts, p, st);
     return c.dim <= 64 ? launch_chunk<T, 64>(kv, c, bt, a, parts, p, st) : launch_chunk<T, 128>(kv, c, bt, a, parts, p, st);

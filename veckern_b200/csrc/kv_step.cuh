@@ -34,8 +34,9 @@ struct KvParts {
     uint32_t* ready;
     float* o;    // [part]: unnormalised sums
     float2* ml;  // [part][row]: maximum (base 2) and sum
-    float* s;    // [sequence][kv head][slot][R]: scaled scores (base 2) of the step path, for the weights
+    float* s;    // [sequence][kv head][slot][s_rows]: scaled scores (base 2) of the step path, for the weights
     int64_t s_slots;
+    int s_rows;  // rows rounded up to 4, 8 or 16
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -242,9 +243,10 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     auto tiles_of = [&](const KvSeq& s) { return max(1, (s.len + STEP_TILE - 1) / STEP_TILE); };
+    const int most = SCORES ? parts.s_rows : R;  // rows
     auto units_of = [&](const KvSeq& s) {
-        if (s.count > 0 && !step_takes(s, a.group, R)) atomicOr(c.status, ERR_LAYOUT);
-        return step_takes(s, a.group, R) ? tiles_of(s) * c.heads : 0;
+        if (s.count > 0 && !step_takes(s, a.group, most)) atomicOr(c.status, ERR_LAYOUT);
+        return step_takes(s, a.group, most) ? tiles_of(s) * c.heads : 0;
     };
     KvShare share = kv_share<STEP_THREADS>(c, bt, scratch, STEP_LEAST, units_of);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -256,7 +258,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
     while (share.left > 0) {
         const KvSeq s = kv_seq(c, bt, share.b);
         const int tiles = tiles_of(s);
-        if (!step_takes(s, a.group, R) || share.off >= tiles * c.heads) {
+        if (!step_takes(s, a.group, most) || share.off >= tiles * c.heads) {
             ++share.b;
             share.off = 0;
             continue;
@@ -349,13 +351,14 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
                             top = fmaxf(top, y);
                         }
                         if constexpr (SCORES) {
-                            float* sp = parts.s + (((int64_t)share.b * c.heads + head) * parts.s_slots + slot0 + q2) * R +
-                                        g + 8 * u;
+                            const int64_t first = ((int64_t)share.b * c.heads + head) * parts.s_slots + slot0 + q2;
+                            float* sp = parts.s + first * parts.s_rows + g + 8 * u;
                             // a slot past the sequence may lie past the workspace's last slot: only its own are written
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 const int j = (e >> 1) * 8 + (e & 1);
-                                if (slot0 + q2 + j < s.len) sp[(int64_t)j * R] = x[e >> 1][2 * u + (e & 1)];
+                                if (slot0 + q2 + j < s.len && g + 8 * u < parts.s_rows)
+                                    sp[j * parts.s_rows] = x[e >> 1][2 * u + (e & 1)];
                             }
                         }
                         top = fmaxf(top, __shfl_xor_sync(FULL, top, 1));
@@ -507,14 +510,18 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
         }
 }
 
-// Weights that the rows of the step path gave each slot, from the scores that the step kernel left; one thread per slot.
+// Weights that the rows of the step path gave each slot, from the scores that the step kernel left: R of them per slot,
+// four slots per thread. Bound by memory, which the step kernel's 4 R bytes per slot and kv head make a twelfth more for
+// four rows of 128 elements; keeping them is cheaper than reading the keys again (half of the cache's bytes).
+constexpr int STEP_WEIGHTS_SLOTS = 1024;  // of a block
 template <int R>
 __global__ void __launch_bounds__(256) kv_step_weights_kernel(KvPages c, KvBatch bt, KvAttend a, KvParts parts) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     __shared__ float s_lse[R];
     const int b = blockIdx.z, head = blockIdx.y;
     const KvSeq s = kv_seq(c, bt, b);
-    if (!step_takes(s, a.group, R)) return;
+    const int64_t end = min((int64_t)s.len, a.scores_width);
+    if (!step_takes(s, a.group, R) || (int64_t)blockIdx.x * STEP_WEIGHTS_SLOTS >= end) return;
     const int rows = s.count * a.group;
     if (threadIdx.x < R) {
         const int r = threadIdx.x;
@@ -526,19 +533,32 @@ __global__ void __launch_bounds__(256) kv_step_weights_kernel(KvPages c, KvBatch
         s_lse[r] = x;
     }
     __syncthreads();
-    const int64_t end = min((int64_t)s.len, a.scores_width);
-    for (int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x; j < end; j += (int64_t)gridDim.x * 256) {
-        const float4* sp = reinterpret_cast<const float4*>(parts.s + (((int64_t)b * c.heads + head) * parts.s_slots + j) * R);
-        float sum = 0.f;
+    const float4* sp = reinterpret_cast<const float4*>(parts.s + ((int64_t)b * c.heads + head) * parts.s_slots * R);
+    float* out = a.scores + b * a.ss[0] + head * a.ss[1];
+    for (int64_t j0 = (int64_t)blockIdx.x * STEP_WEIGHTS_SLOTS + threadIdx.x; j0 < end;
+         j0 += (int64_t)gridDim.x * STEP_WEIGHTS_SLOTS) {
+        float4 x[4][R / 4];
+        float before[4];
 #pragma unroll
-        for (int i = 0; i < R / 4; ++i) {
-            const float4 x = __ldg(sp + i);
-            if (4 * i < rows) sum += ex2(x.x - s_lse[4 * i]);
-            if (4 * i + 1 < rows) sum += ex2(x.y - s_lse[4 * i + 1]);
-            if (4 * i + 2 < rows) sum += ex2(x.z - s_lse[4 * i + 2]);
-            if (4 * i + 3 < rows) sum += ex2(x.w - s_lse[4 * i + 3]);
+        for (int u = 0; u < 4; ++u) {
+            const int64_t j = min(j0 + u * 256, end - 1);
+            before[u] = out[j];
+#pragma unroll
+            for (int i = 0; i < R / 4; ++i) x[u][i] = __ldg(sp + j * (R / 4) + i);
         }
-        a.scores[b * a.ss[0] + head * a.ss[1] + j] += sum;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < R / 4; ++i) {
+                // rows that are not there left anything
+                if (4 * i < rows) sum += ex2(x[u][i].x - s_lse[4 * i]);
+                if (4 * i + 1 < rows) sum += ex2(x[u][i].y - s_lse[4 * i + 1]);
+                if (4 * i + 2 < rows) sum += ex2(x[u][i].z - s_lse[4 * i + 2]);
+                if (4 * i + 3 < rows) sum += ex2(x[u][i].w - s_lse[4 * i + 3]);
+            }
+            if (j0 + u * 256 < end) out[j0 + u * 256] = before[u] + sum;
+        }
     }
 }
 
