@@ -520,3 +520,24 @@ def test_what_python_refuses():
               torch.zeros((4, 16, 2, 65), dtype=torch.float16, device="cuda")[..., :64]):
         with pytest.raises(N.VkError):
             PagedCache(k, k)
+
+
+def test_example_reads_what_it_found():
+    """The example's path: search, read, forget, go on. The passage that a question is made of is found, gathers the
+    largest weight, and its slots are what is kept of the passages; the last step agrees with the definition."""
+    torch = __import__("torch")
+    from veckern_b200.examples import retrieval_memory as ex
+
+    r = ex.run(passages=1500, questions=9, steps=3, seed=3)
+    hit = r["ids"] == r["about"][:, None]
+    assert hit.any(1).all(), "the index missed a question's passage"
+    assert torch.equal(r["read"].argmax(1), hit.int().argmax(1))
+    assert r["lens"].tolist() == [r["keep"] + 3] * 9
+    kept = r["kept"]
+    assert (kept[:, :, -r["asked"]:] == torch.arange(8 * 64, 8 * 64 + r["asked"], device="cuda")).all()
+    c = Cache.__new__(Cache)
+    c.t, c.dtype, c.u = torch, r["k"].dtype, 2.0 ** -8
+    c.k, c.v, c.table, c.page, c.kv_heads, c.dim = r["k"], r["v"], r["table"], ex.PAGE, ex.KV_HEADS, ex.DIM
+    c.lens_list = r["lens"].tolist()
+    check_attend(c, r["q"], [1] * 9, r["out"], r["lse"], True)
+    r["cache"].close()

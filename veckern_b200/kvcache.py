@@ -10,8 +10,9 @@ sequence, made e.g. from a search's ids, says which pages it reads.
 All tensors are torch tensors on the cache's device. Sequence b of a call has the new tokens offsets[b]:offsets[b + 1]
 (int32, [batch + 1]), lens[b] slots with the new tokens included (int32, [batch]) and the pages table[b] (int32,
 [batch, width]; entries past its last slot are not read). Calls are asynchronous on `stream` (a torch.cuda.Stream or raw
-handle; default: the current stream); sync() waits and raises what the kernels found wrong. The calls
-of one stream share their working memory. No derivatives: a cache is for inference.
+handle; default: the current stream); sync() waits and raises what the kernels found wrong. The calls of one stream share
+their working memory, those captured into CUDA graphs on one stream too: such graphs are replayed one after the other. No
+derivatives: a cache is for inference.
 """
 from __future__ import annotations
 
