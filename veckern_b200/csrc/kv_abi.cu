@@ -441,7 +441,7 @@ int vk_kv_evict(vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_evict_t* ar
     const int64_t slots = (int64_t)bt.width << c.page_shift, groups = (int64_t)bt.batch * c.heads;
     const int64_t want = ceil_div(slots, 2048);
     int ctas = 1;
-    while (ctas < vk::SELECT_CLUSTER && ctas < want && (ctas * groups <= kv->sm_count || slots / ctas > 16384)) ctas *= 2;
+    while (ctas < vk::SELECT_CLUSTER && ctas < want && (2 * ctas * groups <= kv->sm_count || slots / ctas > 16384)) ctas *= 2;
     const size_t smem = 5 * vk::SELECT_BINS * sizeof(int) +
                         (size_t)std::min<int64_t>(ceil_div(slots, ctas), vk::SELECT_HELD) * sizeof(uint32_t);
     const auto select = ctas == 1   ? &vk::kv_select_kernel<1>
