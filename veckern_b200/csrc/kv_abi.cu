@@ -1,9 +1,7 @@
 // C ABI of the paged key/value cache (vk_kv_*): checks of arguments, the cache's handle, and the launches.
-#include <map>
-#include <mutex>
+#include <atomic>
 #include <new>
 #include <type_traits>
-#include <utility>
 
 #include <cudaTypedefs.h>
 
@@ -107,16 +105,14 @@ AttendPlan plan_attend(const vk_kv* kv, const vk::KvBatch& bt, int group, int ma
 }
 
 // Once per kernel and device: the dynamic shared memory that it may take, clusters of more than 8.
-template <class Fn>
-int prepare_kernel(Fn* fn, int device, size_t smem, bool large_clusters = false) {
-    static std::mutex lock;
-    static std::map<std::pair<const void*, int>, bool> seen;
-    std::lock_guard<std::mutex> hold(lock);
-    bool& is = seen[{reinterpret_cast<const void*>(fn), device}];
-    if (is) return VK_OK;
-    VK_TRY_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    if (large_clusters) VK_TRY_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    is = true;
+template <auto* Fn>
+int prepare_kernel(int device, size_t smem, bool large_clusters = false) {
+    static std::atomic<uint64_t> done{0};  // a bit per device; from the 65th on the calls are made again
+    const uint64_t bit = device < 64 ? uint64_t(1) << device : 0;
+    if (done.load(std::memory_order_acquire) & bit) return VK_OK;
+    VK_TRY_CUDA(cudaFuncSetAttribute(Fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (large_clusters) VK_TRY_CUDA(cudaFuncSetAttribute(Fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    done.fetch_or(bit, std::memory_order_release);
     return VK_OK;
 }
 
@@ -140,9 +136,9 @@ int launch_behind(void (*fn)(Args...), dim3 grid, int threads, size_t smem, cuda
 template <typename T, int DP, int R, bool SCORES>
 int launch_step_as(const vk_kv* kv, const vk::KvPages& c, const vk::KvBatch& bt, const vk::KvAttend& a,
                    const vk::KvParts& parts, int ctas, cudaStream_t st) {
-    const auto fn = &vk::kv_step_kernel<T, DP, R, SCORES>;
+    constexpr auto fn = &vk::kv_step_kernel<T, DP, R, SCORES>;
     constexpr int smem = vk::step_smem<DP>();
-    VK_TRY(prepare_kernel(fn, kv->desc.device, smem));
+    VK_TRY(prepare_kernel<fn>(kv->desc.device, smem));
     VK_TRY(launch_behind(fn, dim3(ctas), vk::STEP_THREADS, smem, st, kv->map_k, kv->map_v, c, bt, a, parts));
     if constexpr (SCORES) {
         const int64_t width = std::min(parts.s_slots, a.scores_width);
@@ -168,7 +164,8 @@ int launch_step(const vk_kv* kv, const vk::KvPages& c, const vk::KvBatch& bt, co
 }
 
 int encoder(PFN_cuTensorMapEncodeTiled_v12000* out) {
-    static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+    static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> known{nullptr};
+    PFN_cuTensorMapEncodeTiled_v12000 encode = known.load();
     if (!encode) {
         void* fn = nullptr;
         cudaDriverEntryPointQueryResult found;
@@ -176,8 +173,31 @@ int encoder(PFN_cuTensorMapEncodeTiled_v12000* out) {
         if (!fn || found != cudaDriverEntryPointSuccess)
             return fail(VK_ERR_UNSUPPORTED, "the driver has no cuTensorMapEncodeTiled");
         encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+        known.store(encode);
     }
     *out = encode;
+    return VK_OK;
+}
+
+template <int C>
+int launch_select(int device, size_t smem, const vk::KvPages& c, const vk::KvBatch& bt, const vk::KvEvict& e,
+                  cudaStream_t st) {
+    constexpr auto fn = &vk::kv_select_kernel<C>;
+    VK_TRY(prepare_kernel<fn>(device, 5 * vk::SELECT_BINS * sizeof(int) + vk::SELECT_HELD * sizeof(uint32_t), true));
+    cudaLaunchAttribute attr[2]{};
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = C;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(C, c.heads, bt.batch);
+    cfg.blockDim = dim3(vk::SELECT_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    VK_TRY_CUDA(cudaLaunchKernelEx(&cfg, fn, c, bt, e));
     return VK_OK;
 }
 
@@ -217,14 +237,14 @@ int launch_chunk(const vk_kv* kv, const vk::KvPages& c, const vk::KvBatch& bt, c
                  const vk::KvParts& parts, const AttendPlan& p, cudaStream_t st) {
     CUtensorMap map_q;
     VK_TRY(encode_rows(a, c.dim, bt.tokens, &map_q));
-    const auto fn = &vk::kv_chunk_kernel<T, DP>;
+    constexpr auto fn = &vk::kv_chunk_kernel<T, DP>;
     constexpr int smem = vk::chunk_smem<DP>();
-    VK_TRY(prepare_kernel(fn, kv->desc.device, smem));
+    VK_TRY(prepare_kernel<fn>(kv->desc.device, smem));
     VK_TRY(launch_behind(fn, dim3(p.ctas), vk::CHUNK_THREADS, smem, st, map_q, kv->map_k, kv->map_v, c, bt, a, parts));
     if (!a.scores || a.scores_width == 0) return VK_OK;
-    const auto weights = &vk::kv_weights_kernel<T, DP>;
+    constexpr auto weights = &vk::kv_weights_kernel<T, DP>;
     constexpr int weights_smem = vk::weights_smem<DP>();
-    VK_TRY(prepare_kernel(weights, kv->desc.device, weights_smem));
+    VK_TRY(prepare_kernel<weights>(kv->desc.device, weights_smem));
     return launch_behind(weights, dim3(p.ctas), vk::WEIGHTS_THREADS, weights_smem, st, map_q, kv->map_k, c, bt, a, parts);
 }
 
@@ -444,27 +464,11 @@ int vk_kv_evict(vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_evict_t* ar
     while (ctas < vk::SELECT_CLUSTER && ctas < want && (2 * ctas * groups <= kv->sm_count || slots / ctas > 16384)) ctas *= 2;
     const size_t smem = 5 * vk::SELECT_BINS * sizeof(int) +
                         (size_t)std::min<int64_t>(ceil_div(slots, ctas), vk::SELECT_HELD) * sizeof(uint32_t);
-    const auto select = ctas == 1   ? &vk::kv_select_kernel<1>
-                        : ctas == 2 ? &vk::kv_select_kernel<2>
-                        : ctas == 4 ? &vk::kv_select_kernel<4>
-                        : ctas == 8 ? &vk::kv_select_kernel<8>
-                                    : &vk::kv_select_kernel<vk::SELECT_CLUSTER>;
-    VK_TRY(prepare_kernel(select, kv->desc.device,
-                          5 * vk::SELECT_BINS * sizeof(int) + vk::SELECT_HELD * sizeof(uint32_t), true));
-    cudaLaunchAttribute attr[2]{};
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = ctas;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ctas, c.heads, bt.batch);
-    cfg.blockDim = dim3(vk::SELECT_THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cfg.attrs = attr;
-    cfg.numAttrs = 2;
-    VK_TRY_CUDA(cudaLaunchKernelEx(&cfg, select, c, bt, e));
+    VK_TRY((ctas == 1   ? launch_select<1>(kv->desc.device, smem, c, bt, e, st)
+            : ctas == 2 ? launch_select<2>(kv->desc.device, smem, c, bt, e, st)
+            : ctas == 4 ? launch_select<4>(kv->desc.device, smem, c, bt, e, st)
+            : ctas == 8 ? launch_select<8>(kv->desc.device, smem, c, bt, e, st)
+                        : launch_select<vk::SELECT_CLUSTER>(kv->desc.device, smem, c, bt, e, st)));
     if (e.keep > 0) {
         const int64_t most = std::min<int64_t>(e.keep, slots);  // slots that can be kept
         const unsigned tiles = (unsigned)std::min<int64_t>(ceil_div(most * (c.dim / 8), 256), 4096);
