@@ -48,6 +48,8 @@ __device__ __forceinline__ void tma_rows(void* dst, const CUtensorMap* map, int 
         : "memory");
 }
 
+static_assert(2 * chunk_smem<64>() > 233472 && 2 * chunk_smem<128>() > 233472, "one CTA per SM: each takes all tensor memory");
+
 // ---- tcgen05
 // A descriptor's low word holds the operand's address and leading offset in units of 16 bytes, so that the next step's
 // operand is one 32-bit addition away; the high word is constant: 8-row groups 1,024 bytes apart, descriptor version 1,
@@ -602,7 +604,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
                         const int64_t part = part_of(1 + min(k + u, follow - 1));
-                        const float4* po = reinterpret_cast<const float4*>(parts.o) + (part * (DP / 4) + e / 4) * CHUNK_ROWS + r;
+                        const float4* po =
+                            reinterpret_cast<const float4*>(parts.o) + (part * (DP / 4) + e / 4) * CHUNK_ROWS + r;
                         f[u] = __ldcg(parts.ml + part * CHUNK_ROWS + r).x;
 #pragma unroll
                         for (int w = 0; w < 8; ++w) y[u][w] = __ldcg(po + w * CHUNK_ROWS);

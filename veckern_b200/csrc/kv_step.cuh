@@ -12,6 +12,10 @@
 // swizzle that ldmatrix reads without conflicts); four warps take 16 slots of each tile, with their own running maximum
 // and sum, on mma.sync m16n8k16: at 16 rows the tensor work is under a fifth of its rate while memory is saturated, and
 // the operands stay in registers from the scores to the values, which tcgen05's 128-row tiles would not allow.
+//
+// Measured: 32 sequences of up to 8,192 slots, 32 heads over 8 of 128: 118 us, 6.15 TB/s; one token over 1,000 slots: 9.4 us
+// in a graph, of which reading is one. A CTA takes two tiles or more (a part costs about as much as a tile), two CTAs share
+// an SM (three at a head size of 64: no difference, four: half as fast).
 #pragma once
 #include <cuda.h>
 
