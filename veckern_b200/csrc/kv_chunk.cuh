@@ -26,7 +26,7 @@ namespace vk {
 
 constexpr int CHUNK_ROWS = 128;                 // rows of a tile
 constexpr int CHUNK_SLOTS = 128;                // slots of a unit
-constexpr int CHUNK_LEAST = 1;                  // units of a CTA, at least
+constexpr float CHUNK_PART_COST = 0.8f;         // of a unit
 constexpr int CHUNK_THREADS = 384;              // two softmax warpgroups; one with the MMA warp and the loading warp
 template <int DP>
 constexpr int CHUNK_Q = 2 * CHUNK_ROWS * DP * 2;   // bytes of the two query tiles
@@ -278,8 +278,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     uint64_t* s_full = q_empty + 1;  // [tile]
     uint64_t* p_full = s_full + 2;
     uint64_t* o_full = p_full + 2;
-    int* scratch = reinterpret_cast<int*>(o_full + 2);  // THREADS / 32 + 2
-    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(scratch + CHUNK_THREADS / 32 + 2);
+    int* scratch = reinterpret_cast<int*>(o_full + 2);
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(scratch + KV_SHARE_SCRATCH);
     const int warp = __shfl_sync(FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         prefetch_map(&map_q);
@@ -311,8 +311,11 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     tmem_fence_before();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const ChunkShape shape{a, a.tokens};
-    KvShare share = kv_share<CHUNK_THREADS>(c, bt, scratch, CHUNK_LEAST, [&](const KvSeq& s) {
-        return shape.takes(s) ? shape.before(s, shape.pairs(s)) * c.heads : 0;
+    KvShare share = kv_share<CHUNK_THREADS>(c, bt, scratch, CHUNK_PART_COST, [&](const KvSeq& s, int* longest) {
+        if (!shape.takes(s)) return 0;
+        const int pairs = shape.pairs(s);
+        *longest = max(*longest, max(shape.units(s, pairs - 1), shape.units(s, max(0, pairs - 2))));
+        return shape.before(s, pairs) * c.heads;
     });
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     tmem_fence_after();

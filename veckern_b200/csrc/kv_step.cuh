@@ -14,8 +14,8 @@
 // the operands stay in registers from the scores to the values, which tcgen05's 128-row tiles would not allow.
 //
 // Measured: 32 sequences of up to 8,192 slots, 32 heads over 8 of 128: 118 us, 6.15 TB/s; one token over 1,000 slots: 9.4 us
-// in a graph, of which reading is one. A CTA takes two tiles or more (a part costs about as much as a tile), two CTAs share
-// an SM (three at a head size of 64: no difference, four: half as fast).
+// in a graph, of which reading is one. Two CTAs share an SM (three at a head size of 64: no
+// difference, four: half as fast).
 #pragma once
 #include <cuda.h>
 
@@ -24,7 +24,7 @@
 namespace vk {
 
 constexpr int STEP_TILE = 64;  // slots of a tile
-constexpr int STEP_LEAST = 2;  // tiles of a CTA, at least
+constexpr float STEP_PART_COST = 0.15f;  // of a tile
 constexpr int STEP_ROWS = 16;  // most rows of a sequence's kv head
 constexpr int STEP_WARPS = 4;  // consumers; one more warp loads
 constexpr int STEP_THREADS = 32 * (STEP_WARPS + 1);
@@ -154,31 +154,41 @@ struct KvShare {
     }
 };
 
+constexpr int KV_SHARE_SCRATCH = 40;
+// Count(s, &longest) also raises `longest` to the units of the sequence's longest segment. A segment of L units that is cut
+// every m units takes m of a unit's time and L / m of a part's: least with m = sqrt(L part / unit), which is the least that
+// a CTA gets (part_cost: part / unit), except where all units together are fewer.
 template <int THREADS, class Count>
-__device__ __forceinline__ KvShare kv_share(const KvPages& c, const KvBatch& bt, int* scratch, int least, Count&& count) {
-    // scratch: THREADS / 32 + 2 values of shared memory. Thread t sums a contiguous range of the sequences. A CTA gets
-    // `least` units or more, except where there are fewer. No CTA without a share lies between others: the parts of a cut
-    // segment belong to consecutive CTAs.
+__device__ __forceinline__ KvShare kv_share(const KvPages& c, const KvBatch& bt, int* scratch, float part_cost,
+                                            Count&& count) {
+    // scratch: KV_SHARE_SCRATCH values of shared memory. Thread t sums a contiguous range of the sequences. No CTA without a
+    // share lies between others: the parts of a cut segment belong to consecutive CTAs.
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     constexpr int WARPS = THREADS / 32;
     const int span = (bt.batch + THREADS - 1) / THREADS;
     const int b0 = min(bt.batch, t * span), b1 = min(bt.batch, b0 + span);
-    int sum = 0;
-    for (int b = b0; b < b1; ++b) sum += count(kv_seq(c, bt, b));
+    int sum = 0, longest = 0;
+    for (int b = b0; b < b1; ++b) sum += count(kv_seq(c, bt, b), &longest);
+    longest = __reduce_max_sync(FULL, longest);
     int incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int x = __shfl_up_sync(FULL, incl, o);
         if (lane >= o) incl += x;
     }
-    if (lane == 31) scratch[warp] = incl;
+    if (lane == 31) {
+        scratch[warp] = incl;
+        scratch[WARPS + warp] = longest;
+    }
     __syncthreads();
     int before = 0, total = 0;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
         if (w < warp) before += scratch[w];
         total += scratch[w];
+        longest = max(longest, scratch[WARPS + w]);
     }
+    const int least = max(1, (int)(sqrtf(longest * part_cost) + 0.5f));
     KvShare s;
     s.ctas = min((int)gridDim.x, (total + least - 1) / least);
     const uint32_t parts = max(s.ctas, 1);
@@ -191,16 +201,16 @@ __device__ __forceinline__ KvShare kv_share(const KvPages& c, const KvBatch& bt,
         int off = first - before, b = b0;
         if (b1 - b0 > 1)
             for (;; ++b) {
-                const int n = count(kv_seq(c, bt, b));
+                const int n = count(kv_seq(c, bt, b), &longest);
                 if (off < n) break;
                 off -= n;
             }
-        scratch[WARPS] = b;
-        scratch[WARPS + 1] = off;
+        scratch[2 * WARPS] = b;
+        scratch[2 * WARPS + 1] = off;
     }
     __syncthreads();
-    s.b = scratch[WARPS];
-    s.off = scratch[WARPS + 1];
+    s.b = scratch[2 * WARPS];
+    s.off = scratch[2 * WARPS + 1];
     return s;
 }
 
@@ -248,11 +258,13 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     auto tiles_of = [&](const KvSeq& s) { return max(1, (s.len + STEP_TILE - 1) / STEP_TILE); };
     const int most = SCORES ? parts.s_rows : R;  // rows
-    auto units_of = [&](const KvSeq& s) {
+    auto units_of = [&](const KvSeq& s, int* longest) {
         if (s.count > 0 && !step_takes(s, a.group, most)) atomicOr(c.status, ERR_LAYOUT);
-        return step_takes(s, a.group, most) ? tiles_of(s) * c.heads : 0;
+        if (!step_takes(s, a.group, most)) return 0;
+        *longest = max(*longest, tiles_of(s));
+        return tiles_of(s) * c.heads;
     };
-    KvShare share = kv_share<STEP_THREADS>(c, bt, scratch, STEP_LEAST, units_of);
+    KvShare share = kv_share<STEP_THREADS>(c, bt, scratch, STEP_PART_COST, units_of);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     KvWait wait{c.status};
     int stage = 0;

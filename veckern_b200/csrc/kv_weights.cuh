@@ -19,6 +19,7 @@
 namespace vk {
 
 constexpr int WEIGHTS_PAIR = 2 * CHUNK_SLOTS;  // slots of a pair
+constexpr float WEIGHTS_PART_COST = 0.15f;       // of a unit
 // Row tiles in flight. At a head size of 64 more than are needed: with over half of an SM's shared memory no two of these
 // CTAs meet on an SM, where one would wait for the other's tensor memory while both wait for parts of CTAs elsewhere.
 template <int DP>
@@ -121,7 +122,7 @@ __global__ void __launch_bounds__(WEIGHTS_THREADS, 1)
     uint64_t* s_full = k_empty + 1;  // [slot tile][2]
     uint64_t* s_empty = s_full + 4;
     int* scratch = reinterpret_cast<int*>(s_empty + 4);
-    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(scratch + WEIGHTS_THREADS / 32 + 2);
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(scratch + KV_SHARE_SCRATCH);
     const int warp = __shfl_sync(FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         prefetch_map(&map_q);
@@ -151,8 +152,10 @@ __global__ void __launch_bounds__(WEIGHTS_THREADS, 1)
     tmem_fence_before();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const WeightsShape shape{a, a.tokens};
-    KvShare share = kv_share<WEIGHTS_THREADS>(c, bt, scratch, CHUNK_LEAST, [&](const KvSeq& s) {
-        return shape.takes(s) ? shape.before(s, shape.pairs(s)) * c.heads : 0;
+    KvShare share = kv_share<WEIGHTS_THREADS>(c, bt, scratch, WEIGHTS_PART_COST, [&](const KvSeq& s, int* longest) {
+        if (!shape.takes(s)) return 0;
+        *longest = max(*longest, shape.row_tiles(s));
+        return shape.before(s, shape.pairs(s)) * c.heads;
     });
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     tmem_fence_after();
