@@ -36,7 +36,7 @@ template <int DP>
 constexpr int CHUNK_RING = DP == 128 ? 5 : 10;     // tiles in flight, keys and values alternating
 template <int DP>
 constexpr int chunk_smem() {
-    return CHUNK_Q<DP> + CHUNK_RING<DP> * CHUNK_SLOT<DP> + CHUNK_ROWS * 8 + 512;
+    return CHUNK_Q<DP> + CHUNK_RING<DP> * CHUNK_SLOT<DP> + 2 * CHUNK_ROWS * 8 + 512;
 }
 
 // A row tile's box of the queries (64 elements of a kv head's query heads, for a tile's tokens) into shared memory.
@@ -270,8 +270,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     constexpr uint32_t TM_S = 0, TM_O = 256;  // columns: S (and P) of the two tiles, O of the two
     extern __shared__ __align__(1024) uint8_t ring[];  // the swizzle goes by address bits: 1024-byte aligned
     uint8_t* smem_q = ring + RING * SLOT;
-    float2* lone_ml = reinterpret_cast<float2*>(smem_q + CHUNK_Q<DP>);  // of a lone tile's second warpgroup
-    uint64_t* kv_full = reinterpret_cast<uint64_t*>(lone_ml + CHUNK_ROWS);
+    float2* lone_ml = reinterpret_cast<float2*>(smem_q + CHUNK_Q<DP>);  // [warpgroup][row] of a lone tile
+    uint64_t* kv_full = reinterpret_cast<uint64_t*>(lone_ml + 2 * CHUNK_ROWS);
     uint64_t* kv_empty = kv_full + RING;
     uint64_t* q_full = kv_empty + RING;
     uint64_t* q_empty = q_full + 1;
@@ -545,67 +545,73 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             o_phase ^= 1;
             tmem_fence_after();
             // base 2 from here on. A tile past the sequence met no product: its O holds anything.
-            float top = l == 0.f ? -INFINITY : ref, total = l, f0 = 1.f, f1 = 0.f;
-            const float top0 = top;
-            if (g.lone) {  // the first warpgroup joins the two
-                if (i == 1) {
-                    lone_ml[r] = make_float2(top, total);
-                    tmem_fence_before();
-                    asm volatile("bar.sync 3, 256;" ::: "memory");
-                    asm volatile("bar.sync 3, 256;" ::: "memory");  // read
-                    continue;
-                }
+            float top = l == 0.f ? -INFINITY : ref, total = l, f_mine = 1.f, f_other = 0.f;
+            if (g.lone) {  // each warpgroup joins the two for half of the elements
+                const float mine = top;
+                lone_ml[i * CHUNK_ROWS + r] = make_float2(top, total);
+                tmem_fence_before();
                 asm volatile("bar.sync 3, 256;" ::: "memory");
                 tmem_fence_after();
-                const float2 ml = lone_ml[r];
+                const float2 ml = lone_ml[(i ^ 1) * CHUNK_ROWS + r];
                 top = fmaxf(top, ml.x);
-                f0 = part_factor(top0, top);
-                f1 = part_factor(ml.x, top);
-                total = total * f0 + ml.y * f1;
+                f_mine = part_factor(mine, top);
+                f_other = part_factor(ml.x, top);
+                total = total * f_mine + ml.y * f_other;
             }
-            const bool none0 = (int64_t)g.t0 * (g.lone ? 2 : 1) * CHUNK_SLOTS >= g.s.len;
-            const bool none1 = !g.lone || (2 * (int64_t)g.t0 + 1) * CHUNK_SLOTS >= g.s.len;
+            const int64_t slot_a = (int64_t)g.t0 * (g.lone ? 2 : 1) * CHUNK_SLOTS;  // of the first unit's tiles
+            const bool none_mine = slot_a + (g.lone ? i * CHUNK_SLOTS : 0) >= g.s.len;
+            const bool none_other = !g.lone || slot_a + (i ^ 1) * CHUNK_SLOTS >= g.s.len;
+            const int e_from = g.lone ? i * (DP / 2) : 0, e_to = g.lone && i == 0 ? min(c.dim, DP / 2) : c.dim;
             const bool leaves = g.t0 > 0;                                                       // a part for an earlier CTA
             const int follow = leaves ? 0 : walk.share.followers(g.units - g.count);  // CTAs with the rest of this one
             auto part_of = [&](int k) -> int64_t { return 2 * (int64_t)(blockIdx.x + k) + i; };
             if (follow) {
                 for (int k = r; k < follow; k += 128) part_await(parts, (int)part_of(1 + k), wait);
                 asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
-                const float mine = top;
-                for (int k = 0; k < follow; ++k) top = fmaxf(top, __ldcg(parts.ml + part_of(1 + k) * CHUNK_ROWS + r).x);
-                const float f = part_factor(mine, top);
-                f0 *= f;
-                f1 *= f;
-                total *= f;
-                for (int k = 0; k < follow; ++k) {
-                    const float2 ml = __ldcg(parts.ml + part_of(1 + k) * CHUNK_ROWS + r);
-                    total += ml.y * part_factor(ml.x, top);
+                float f = 1.f;
+                for (int k0 = 0; k0 < follow; k0 += 8) {  // eight in flight; the last ones again, for nothing
+                    float2 ml[8];
+                    float next = top;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        ml[k] = __ldcg(parts.ml + part_of(1 + min(k0 + k, follow - 1)) * CHUNK_ROWS + r);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) next = fmaxf(next, ml[k].x);
+                    const float g0 = part_factor(top, next);
+                    f *= g0;
+                    total *= g0;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (k0 + k < follow) total += ml[k].y * part_factor(ml[k].x, next);
+                    top = next;
                 }
+                f_mine *= f;
+                f_other *= f;
             }
             const int h = g.head * a.group + r - r_token * a.group;
             const int64_t tok = g.s.first + token;
             const float inv = total > 0.f ? 1.f / total : total == 0.f ? 0.f : total;
 #pragma unroll 1
-            for (int e = 0; e < c.dim; e += 32) {
+            for (int e = e_from; e < e_to; e += 32) {
                 float o[32];
                 __syncwarp();  // lanes without a row come from another path
                 tmem_ld32(tm_o + e, o);
                 tmem_wait_ld();
 #pragma unroll
-                for (int k = 0; k < 32; ++k) o[k] = none0 ? 0.f : o[k] * f0;
-                if (!none1) {
-                    float o1[32];
-                    tmem_ld32(tm_o + 128 + e, o1);
+                for (int k = 0; k < 32; ++k) o[k] = none_mine ? 0.f : o[k] * f_mine;
+                if (!none_other) {
+                    float x[32];
+                    tmem_ld32(lanes + TM_O + (i ^ 1) * 128 + e, x);
                     tmem_wait_ld();
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) o[k] += o1[k] * f1;
+                    for (int k = 0; k < 32; ++k) o[k] += x[k] * f_other;
                 }
                 // parts: [four columns][row], so that a warp's accesses are contiguous
-                for (int k = 0; k < follow; k += 2) {  // two in flight; an odd last one again, for nothing
-                    float4 y[2][8];
-                    float f[2];
+                for (int k = 0; k < follow; k += 3) {  // three in flight; the last ones again, for nothing
+                    float4 y[3][8];
+                    float f[3];
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
+                    for (int u = 0; u < 3; ++u) {
                         const int64_t part = part_of(1 + min(k + u, follow - 1));
                         const float4* po =
                             reinterpret_cast<const float4*>(parts.o) + (part * (DP / 4) + e / 4) * CHUNK_ROWS + r;
@@ -614,7 +620,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                         for (int w = 0; w < 8; ++w) y[u][w] = __ldcg(po + w * CHUNK_ROWS);
                     }
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
+                    for (int u = 0; u < 3; ++u) {
                         f[u] = k + u < follow ? part_factor(f[u], top) : 0.f;
                         if (f[u] == 0.f) continue;
 #pragma unroll
@@ -641,13 +647,13 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                 }
             }
             tmem_fence_before();
-            if (g.lone) asm volatile("bar.sync 3, 256;" ::: "memory");
+            if (g.lone) asm volatile("bar.sync 3, 256;" ::: "memory");  // both have read the two sums
             if (leaves) {
                 parts.ml[part_of(0) * CHUNK_ROWS + r] = make_float2(top, total);
                 asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
                 if (r == 0) part_publish(parts, (int)part_of(0));
             } else {
-                if (live) a.lse[tok * a.heads + h] = (top + log2f(total)) * 0.6931471805599453f;
+                if (live && !(g.lone && i == 1)) a.lse[tok * a.heads + h] = (top + log2f(total)) * 0.6931471805599453f;
                 if (follow) {
                     asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
                     for (int k = r; k < follow; k += 128) parts.ready[part_of(1 + k)] = 0;

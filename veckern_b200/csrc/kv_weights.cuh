@@ -327,7 +327,14 @@ __global__ void __launch_bounds__(WEIGHTS_THREADS, 1)
                 if (follow) {
                     for (int k = r; k < follow; k += 128) part_await(parts, part + 2 + 2 * k, wait);
                     asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");
-                    for (int k = 0; k < follow; ++k) total += __ldcg(parts.o + (int64_t)(part + 2 + 2 * k) * CHUNK_SLOTS + r);
+                    for (int k0 = 0; k0 < follow; k0 += 8) {  // eight in flight; the last ones again, for nothing
+                        float x[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            x[k] = __ldcg(parts.o + (int64_t)(part + 2 + 2 * min(k0 + k, follow - 1)) * CHUNK_SLOTS + r);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) total += k0 + k < follow ? x[k] : 0.f;
+                    }
                     for (int k = r; k < follow; k += 128) parts.ready[part + 2 + 2 * k] = 0;
                 }
                 if (j < min((int64_t)g.s.len, a.scores_width)) a.scores[g.b * a.ss[0] + g.head * a.ss[1] + j] += total;
