@@ -24,7 +24,7 @@
 namespace vk {
 
 constexpr int STEP_TILE = 64;  // slots of a tile
-constexpr float STEP_PART_COST = 0.15f;  // of a tile
+constexpr float STEP_PART_COST = 0.5f;  // of a tile
 constexpr int STEP_ROWS = 16;  // most rows of a sequence's kv head
 constexpr int STEP_WARPS = 4;  // consumers; one more warp loads
 constexpr int STEP_THREADS = 32 * (STEP_WARPS + 1);
