@@ -61,11 +61,6 @@ static_assert(2 * chunk_smem<64>() > 233472 && 2 * chunk_smem<128>() > 233472, "
 // 1,105 us then, 770 now).
 constexpr uint32_t UMMA_HIGH = 1024u >> 4 | 1u << 14 | 2u << 29;
 __device__ __forceinline__ uint32_t umma_low(uint32_t addr, uint32_t lead) { return addr >> 4 | (lead >> 4) << 16; }
-__device__ __forceinline__ uint32_t elect_lane() {
-    uint32_t me;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(me));
-    return me;
-}
 template <typename T>
 __device__ __forceinline__ uint32_t umma_idesc(int n, bool b_by_rows, bool negate) {
     const uint32_t type = std::is_same_v<T, __half> ? 0u : 1u;
@@ -333,7 +328,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         if (warp == 9) {
             uint32_t q_phase = 0;
             const int box_shift = min(c.page_shift, 6);
-            const int boxes = CHUNK_SLOTS >> box_shift, i = lane % boxes, half = lane / boxes;
+            const int boxes = CHUNK_SLOTS >> box_shift;
+            const uint32_t me = elect_lane();
             while (walk.next(&g)) {
                 wait(q_empty, q_phase ^ 1);
                 q_phase ^= 1;
@@ -348,23 +344,24 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                 const int32_t* table = bt.table + g.b * bt.table_stride;
                 const int per = g.lone ? 2 : 1;
                 for (int t = g.t0 * per; t < (g.t0 + g.count) * per; ++t) {
-                    const int first = t * CHUNK_SLOTS + (i << box_shift);
-                    const bool live = half < HALVES && first < g.s.len;
-                    int page = 0;
-                    if (live) {
-                        page = (int)kv_page(c, table, first);
-                        if (page < 0) page = (int)c.pages;  // past the map: reads as zero
-                    }
-                    const int n = __popc(__ballot_sync(FULL, live));
+                    const TilePages tp = tile_pages(c, table, t * CHUNK_SLOTS, boxes, box_shift, g.s.len);
+                    // rolled: this warp's registers are few, and what it spills the other one waits for
+#pragma unroll 1
                     for (int side = 0; side < 2; ++side, ++fill) {
                         const int slot = at(fill);
                         wait(kv_empty + slot, parity(fill) ^ 1);
-                        if (lane == 0) mbar_arrive_expect_tx(kv_full + slot, n * (128 << box_shift));
+                        if (lane == 0) mbar_arrive_expect_tx(kv_full + slot, tp.count * HALVES * (128 << box_shift));
                         __syncwarp();
-                        if (live)
-                            tma_page(ring + slot * SLOT + half * (CHUNK_SLOTS * 128) + (i << box_shift) * 128,
-                                     side ? &map_v : &map_k, half * 64, first & ((1 << c.page_shift) - 1), g.head, page,
-                                     kv_full + slot);
+                        uint8_t* dst = ring + slot * SLOT;
+#pragma unroll 2
+                        for (int i = 0; i < tp.count; ++i) {
+                            const int page = __shfl_sync(FULL, tp.page, i), from = i << box_shift;
+                            const int in = (t * CHUNK_SLOTS + from) & ((1 << c.page_shift) - 1);
+#pragma unroll
+                            for (int half = 0; half < HALVES; ++half)
+                                tma_page(dst + half * (CHUNK_SLOTS * 128) + from * 128, side ? &map_v : &map_k, half * 64, in,
+                                         g.head, page, kv_full + slot, me);
+                        }
                     }
                 }
             }

@@ -52,14 +52,38 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
 }
-// A 2-d box of a page (box slots x 64 elements of one head) into shared memory.
+__device__ __forceinline__ uint32_t elect_lane() {
+    uint32_t me;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(me));
+    return me;
+}
+// A 2-d box of a page (box slots x 64 elements of one head) into shared memory. Reached by a whole warp with equal
+// arguments, copied once, by the lane whose `me` is nonzero: from lanes with arguments of their own a copy takes over 100
+// cycles each (2,048 tokens over 8,192 slots, 32 heads over 8 of 128, pages of 8 slots: 271 us then, 197 now).
 __device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int d, int slot, int head, int page,
-                                         uint64_t* bar) {
+                                         uint64_t* bar, uint32_t me) {
     asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
-            smem_u32(dst)),
-        "l"(map), "r"(d), "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar))
+        "{\n\t.reg .pred q;\n\tsetp.ne.u32 q, %7, 0;\n\t"
+        "@q cp.async.bulk.tensor.4d.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n\t"
+        "}" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(d), "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar)), "r"(me)
         : "memory");
+}
+// The pages of a tile's boxes, lane i the i-th box's (a page that does not exist lies past the map: it reads as zero), and
+// the number of boxes that the sequence reaches.
+struct TilePages {
+    int page, count;
+};
+__device__ __forceinline__ TilePages tile_pages(const KvPages& c, const int32_t* table, int first, int boxes, int box_shift,
+                                                int len) {
+    const int lane = threadIdx.x & 31, slot = first + (lane << box_shift);
+    const bool live = lane < boxes && slot < len;
+    int page = 0;
+    if (live) {
+        page = (int)kv_page(c, table, slot);
+        if (page < 0) page = (int)c.pages;
+    }
+    return {page, __popc(__ballot_sync(FULL, live))};
 }
 
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
@@ -285,24 +309,21 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
         share.left -= count;
         const int32_t* table = bt.table + share.b * bt.table_stride;
         if (warp == STEP_WARPS) {
-            // Loads: lane = (key or value, half of the head, page of the tile).
-            const int per = boxes * HALVES, i = lane % boxes, half = lane / boxes % HALVES, side = lane / per;
+            const uint32_t me = elect_lane();
             for (int t = t0; t < t0 + count; ++t) {
-                const int slot = t * STEP_TILE + (i << box_shift);
-                const bool live = lane < 2 * per && slot < s.len;
-                int page = 0;
-                if (live) {
-                    page = (int)kv_page(c, table, slot);
-                    if (page < 0) page = (int)c.pages;  // past the map: reads as zero
-                }
-                const int n = __popc(__ballot_sync(FULL, live));
+                const TilePages tp = tile_pages(c, table, t * STEP_TILE, boxes, box_shift, s.len);
                 wait(empty + stage, phase ^ 1);
-                if (lane == 0) mbar_arrive_expect_tx(full + stage, n * (128 << box_shift));
+                if (lane == 0) mbar_arrive_expect_tx(full + stage, tp.count * 2 * HALVES * (128 << box_shift));
                 __syncwarp();
-                if (live)
-                    tma_page(ring + stage * STAGE + (side * HALVES + half) * (STEP_TILE * 128) + (i << box_shift) * 128,
-                             side ? &map_v : &map_k, half * 64, slot & ((1 << c.page_shift) - 1), head, page,
-                             full + stage);
+                uint8_t* dst = ring + stage * STAGE;
+                for (int i = 0; i < tp.count; ++i) {
+                    const int page = __shfl_sync(FULL, tp.page, i), at = i << box_shift;
+                    const int slot = (t * STEP_TILE + at) & ((1 << c.page_shift) - 1);
+#pragma unroll
+                    for (int part = 0; part < 2 * HALVES; ++part)
+                        tma_page(dst + part * (STEP_TILE * 128) + at * 128, part < HALVES ? &map_k : &map_v,
+                                 part % HALVES * 64, slot, head, page, full + stage, me);
+                }
                 ++loaded;
                 if (++stage == STAGES) stage = 0, phase ^= 1;
             }

@@ -167,31 +167,27 @@ __global__ void __launch_bounds__(WEIGHTS_THREADS, 1)
         int slot = 0, loaded = 0;
         uint32_t phase = 0, k_phase = 0;
         const int box_shift = min(c.page_shift, 6), boxes = CHUNK_SLOTS >> box_shift;
+        const uint32_t me = elect_lane();
         while (walk.next(&g)) {
             const int32_t* table = bt.table + g.b * bt.table_stride;
-            const int i = lane % boxes, half = lane / boxes;
             wait(k_empty, k_phase ^ 1);
-            int pages[2];
-            int n = 0;
+            TilePages tp[2];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int at = g.pair * WEIGHTS_PAIR + u * CHUNK_SLOTS + (i << box_shift);
-                const bool live = half < HALVES && at < g.s.len && (u == 0 || g.both);
-                pages[u] = -1;
-                if (live) {
-                    pages[u] = (int)kv_page(c, table, at);
-                    if (pages[u] < 0) pages[u] = (int)c.pages;  // past the map: reads as zero
-                }
-                n += __popc(__ballot_sync(FULL, live));
-            }
-            if (lane == 0) mbar_arrive_expect_tx(k_full, n * (128 << box_shift));
+            for (int u = 0; u < 2; ++u)
+                tp[u] = tile_pages(c, table, g.pair * WEIGHTS_PAIR + u * CHUNK_SLOTS, u == 0 || g.both ? boxes : 0, box_shift,
+                                   g.s.len);
+            if (lane == 0) mbar_arrive_expect_tx(k_full, (tp[0].count + tp[1].count) * HALVES * (128 << box_shift));
             __syncwarp();
 #pragma unroll
             for (int u = 0; u < 2; ++u)
-                if (pages[u] >= 0)
-                    tma_page(smem_k + u * SLOT + half * (CHUNK_SLOTS * 128) + (i << box_shift) * 128, &map_k, half * 64,
-                             (u * CHUNK_SLOTS + (i << box_shift) + g.pair * WEIGHTS_PAIR) & ((1 << c.page_shift) - 1), g.head,
-                             pages[u], k_full);
+                for (int i = 0; i < tp[u].count; ++i) {
+                    const int page = __shfl_sync(FULL, tp[u].page, i), from = i << box_shift;
+                    const int in = (g.pair * WEIGHTS_PAIR + u * CHUNK_SLOTS + from) & ((1 << c.page_shift) - 1);
+#pragma unroll
+                    for (int half = 0; half < HALVES; ++half)
+                        tma_page(smem_k + u * SLOT + half * (CHUNK_SLOTS * 128) + from * 128, &map_k, half * 64, in, g.head,
+                                 page, k_full, me);
+                }
             k_phase ^= 1;
             for (int q = g.q0; q < g.q0 + g.count; ++q) {
                 wait(q_empty + slot, phase ^ 1);
