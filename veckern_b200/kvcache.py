@@ -17,9 +17,15 @@ derivatives: a cache is for inference.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 from . import _native as N
 from ._native import VkError, check, lib
+
+# The argument structs (N.KvBatch, N.KvAttend, N.KvEvict), packed in one step: a call's fields set one by one take longer
+# than its launch.
+_BATCH, _ATTEND, _EVICT = struct.Struct("@iiqqPPP"), struct.Struct("@PqqPqqPPqqqiiifPN"), struct.Struct("@PqiiiPqqqPPP")
+assert [x.size for x in (_BATCH, _ATTEND, _EVICT)] == [C.sizeof(x) for x in (N.KvBatch, N.KvAttend, N.KvEvict)]
 
 # Attention's working memory by (device, stream): the calls of a stream share one tensor, which grows and whose start is
 # zero between calls. Tensors that were outgrown are kept: a captured graph may hold their addresses.
@@ -29,16 +35,16 @@ _ZEROED = 8192  # VK_KV_WORKSPACE_ZEROED
 
 
 def _workspace(torch, device, stream: int, need: int):
+    """A larger working memory for a stream."""
     key = (device.index, stream)
     work = _WORK.get(key)
-    if work is None or work.numel() < need:
-        if work is not None:
-            _OUTGROWN.append(work)
-            need = max(need, work.numel() * 3 // 2)
-        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
-            work = torch.empty((need,), dtype=torch.uint8, device=device)
-            work[:_ZEROED].zero_()
-        _WORK[key] = work
+    if work is not None:
+        _OUTGROWN.append(work)
+        need = max(need, work.numel() * 3 // 2)
+    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+        work = torch.empty((need,), dtype=torch.uint8, device=device)
+        work[:_ZEROED].zero_()
+    _WORK[key] = work
     return work
 
 
@@ -74,6 +80,7 @@ class PagedCache:
         self.k_pages, self.v_pages = k_pages, v_pages
         self.pages, self.page_size, self.kv_heads, self.head_dim = k_pages.shape
         self.dtype, self.device = k_pages.dtype, k_pages.device
+        self._scale = self.head_dim ** -0.5
         d = N.KvDesc(device=self.device.index, dtype=_DTYPES[str(self.dtype)], page_size=self.page_size,
                      kv_heads=self.kv_heads, head_dim=self.head_dim, pages=self.pages, k=k_pages.data_ptr(),
                      k_stride=(C.c_int64 * 3)(*k_pages.stride()[:3]), v=v_pages.data_ptr(),
@@ -81,13 +88,14 @@ class PagedCache:
         check(lib().vk_kv_create(C.byref(d), C.byref(self._h)), "vk_kv_create")
         self._sizes = {}  # bytes of attention's working memory by what they depend on
         self._strides = (C.c_int64 * 2)(), (C.c_int64 * 2)()
-        # argument structs, filled anew by every call
-        self._batch, self._attend, self._evict = N.KvBatch(), N.KvAttend(), N.KvEvict()
-        self._batch_ref, self._attend_ref, self._evict_ref = (C.byref(x) for x in
-                                                              (self._batch, self._attend, self._evict))
+        # argument structs, filled anew by every call, and their addresses
+        self._args = C.create_string_buffer(_BATCH.size + max(_ATTEND.size, _EVICT.size))
+        self._batch_at = C.addressof(self._args)
+        self._call_at = self._batch_at + _BATCH.size
 
-    def _sequences(self, table, lens, offsets=None, tokens: int = 0) -> int:
-        i32, dev, b = self._i32, self.device, self._batch
+    def _sequences(self, table, lens, offsets=None, tokens: int = 0):
+        """Checks a call's sequences and packs them; (sequences, table width)."""
+        i32, dev = self._i32, self.device
         if table.dtype != i32 or table.dim() != 2 or table.device != dev:
             _want(table, "table", i32, 2, dev)
         if lens.dtype != i32 or lens.dim() != 1 or lens.device != dev:
@@ -96,17 +104,15 @@ class PagedCache:
         stride, step = table.stride()
         if lens.shape[0] != n or not lens.is_contiguous() or (step != 1 and width > 1):
             raise ValueError("lens must be contiguous, one per row of table, and table's rows contiguous")
-        if offsets is None:
-            b.offsets = None
-        else:
+        at = 0
+        if offsets is not None:
             if offsets.dtype != i32 or offsets.dim() != 1 or offsets.device != dev:
                 _want(offsets, "offsets", i32, 1, dev)
             if offsets.shape[0] != n + 1 or not offsets.is_contiguous():
                 raise ValueError("offsets must be contiguous [batch + 1]")
-            b.offsets = offsets.data_ptr()
-        b.batch, b.table_width, b.table_stride, b.tokens = n, width, stride, tokens
-        b.table, b.lens = table.data_ptr(), lens.data_ptr()
-        return n
+            at = offsets.data_ptr()
+        _BATCH.pack_into(self._args, 0, n, width, stride, tokens, at, table.data_ptr(), lens.data_ptr())
+        return n, width
 
     def _rows(self, t, name: str, heads: int):
         """Checks rows of tokens; their strides."""
@@ -132,7 +138,7 @@ class PagedCache:
         if v.shape[0] != tokens:
             raise ValueError("k and v must have the same number of tokens")
         self._sequences(table, lens, offsets, tokens)
-        code = self._lib.vk_kv_append(self._h, self._batch_ref, k.data_ptr(), ks, v.data_ptr(), vs, self._stream(stream))
+        code = self._lib.vk_kv_append(self._h, self._batch_at, k.data_ptr(), ks, v.data_ptr(), vs, self._stream(stream))
         if code:
             check(code, "append")
 
@@ -147,44 +153,48 @@ class PagedCache:
         torch = self._torch
         if q.dim() != 3:
             raise ValueError("q must be [tokens, heads, head_dim]")
-        a = self._attend
-        tokens, heads, _ = q.shape
-        a.q_stride[0], a.q_stride[1], _ = self._rows(q, "q", heads)
-        n = self._sequences(table, lens, offsets, tokens)
+        tokens, heads, dim = q.shape
+        q_token, q_head, _ = self._rows(q, "q", heads)
+        n, width = self._sequences(table, lens, offsets, tokens)
         if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
-            a.out_stride[0], a.out_stride[1] = heads * self.head_dim, self.head_dim
+            o_token, o_head = heads * dim, dim
+            out = torch.empty_strided((tokens, heads, dim), (o_token, o_head, 1), dtype=self.dtype, device=self.device)
         else:
-            a.out_stride[0], a.out_stride[1], _ = self._rows(out, "out", heads)
+            o_token, o_head, _ = self._rows(out, "out", heads)
             if out.shape[0] != tokens:
                 raise ValueError("out must have q's shape")
         if lse is None:
-            lse = torch.empty((tokens, heads), dtype=torch.float32, device=self.device)
+            lse = torch.empty_strided((tokens, heads), (heads, 1), dtype=self._f32, device=self.device)
         else:
-            _want(lse, "lse", torch.float32, 2, self.device)
+            _want(lse, "lse", self._f32, 2, self.device)
             if lse.shape != (tokens, heads) or not lse.is_contiguous():
                 raise ValueError("lse must be contiguous [tokens, heads]")
-        a.q, a.out, a.lse = q.data_ptr(), out.data_ptr(), lse.data_ptr()
-        if scores is None:
-            a.scores = None
-        else:
-            self._check_scores(scores, n)
-            a.scores, a.scores_width = scores.data_ptr(), scores.shape[2]
-            a.scores_stride[0], a.scores_stride[1] = scores.stride(0), scores.stride(1)
-        a.heads, a.max_q, a.causal = heads, max_q, causal
-        a.scale = self.head_dim ** -0.5 if scale is None else scale
-        sizes = (n, self._batch.table_width, tokens, heads, max_q, scores is not None)
+        s_at = s_seq = s_head = s_width = 0
+        if scores is not None:
+            s_seq, s_head = self._check_scores(scores, n)
+            s_at, s_width = scores.data_ptr(), scores.shape[2]
+        if scale is None:
+            scale = self._scale
+        stream = self._stream(stream)
+
+        def pack(work: int, size: int) -> None:
+            _ATTEND.pack_into(self._args, _BATCH.size, q.data_ptr(), q_token, q_head, out.data_ptr(), o_token, o_head,
+                              lse.data_ptr(), s_at, s_seq, s_head, s_width, heads, max_q, bool(causal), scale, work, size)
+
+        sizes = (n, width, tokens, heads, max_q, s_at != 0)
         need = self._sizes.get(sizes)
         if need is None:
+            pack(0, 0)
             size = C.c_size_t()
-            check(lib().vk_kv_attend_workspace(self._h, self._batch_ref, self._attend_ref, C.byref(size)), "attend")
+            check(lib().vk_kv_attend_workspace(self._h, self._batch_at, self._call_at, C.byref(size)), "attend")
             if len(self._sizes) >= 4096:
                 self._sizes.clear()
             need = self._sizes[sizes] = size.value
-        s = self._stream(stream)
-        work = _workspace(torch, self.device, s, need)
-        a.workspace, a.workspace_bytes = work.data_ptr(), work.numel()
-        code = self._lib.vk_kv_attend(self._h, self._batch_ref, self._attend_ref, s)
+        work = _WORK.get((self.device.index, stream))
+        if work is None or work.numel() < need:
+            work = _workspace(torch, self.device, stream, need)
+        pack(work.data_ptr(), work.numel())
+        code = self._lib.vk_kv_attend(self._h, self._batch_at, self._call_at, stream)
         if code:
             check(code, "attend")
         return out, lse
@@ -195,33 +205,35 @@ class PagedCache:
         no sequence of the call reads). Returns (kept [batch, kv_heads, keep] int32: the old slots, -1 behind the last;
         new lens [batch] int32; new scores like scores, contiguous, 0 behind the last)."""
         torch = self._torch
-        n = self._sequences(table, lens)
-        self._check_scores(scores, n)
+        n, _ = self._sequences(table, lens)
+        s_seq, s_head = self._check_scores(scores, n)
         if new_table.dtype != self._i32 or new_table.dim() != 2 or new_table.device != self.device:
             _want(new_table, "new_table", self._i32, 2, self.device)
-        if new_table.shape[0] != n or (new_table.shape[1] > 1 and new_table.stride(1) != 1):
+        new_stride, new_step = new_table.stride()
+        if new_table.shape[0] != n or (new_step != 1 and new_table.shape[1] > 1):
             raise ValueError("new_table must have one row per sequence, rows contiguous")
         if not 0 <= recent <= keep:
             raise ValueError("keep and recent must satisfy 0 <= recent <= keep")
-        kept = torch.empty((n, self.kv_heads, keep), dtype=self._i32, device=self.device)
+        heads, width = self.kv_heads, scores.shape[2]
+        kept = torch.empty_strided((n, heads, keep), (heads * keep, keep, 1), dtype=self._i32, device=self.device)
         new_lens = torch.empty_like(lens)
-        new_scores = torch.empty_like(scores, memory_format=torch.contiguous_format)
-        e = self._evict
-        e.new_table, e.new_table_stride, e.new_table_width = new_table.data_ptr(), new_table.stride(0), new_table.shape[1]
-        e.keep, e.recent = keep, recent
-        e.scores, e.scores_width = scores.data_ptr(), scores.shape[2]
-        e.scores_stride[0], e.scores_stride[1] = scores.stride(0), scores.stride(1)
-        e.new_scores, e.kept, e.new_lens = new_scores.data_ptr(), kept.data_ptr(), new_lens.data_ptr()
-        code = self._lib.vk_kv_evict(self._h, self._batch_ref, self._evict_ref, self._stream(stream))
+        new_scores = torch.empty_strided((n, heads, width), (heads * width, width, 1), dtype=self._f32, device=self.device)
+        _EVICT.pack_into(self._args, _BATCH.size, new_table.data_ptr(), new_stride, new_table.shape[1], keep, recent,
+                         scores.data_ptr(), s_seq, s_head, width, new_scores.data_ptr(), kept.data_ptr(),
+                         new_lens.data_ptr())
+        code = self._lib.vk_kv_evict(self._h, self._batch_at, self._call_at, self._stream(stream))
         if code:
             check(code, "evict")
         return kept, new_lens, new_scores
 
-    def _check_scores(self, scores, n: int) -> None:
+    def _check_scores(self, scores, n: int):
+        """Checks scores; their first two strides."""
         if scores.dtype != self._f32 or scores.dim() != 3 or scores.device != self.device:
             _want(scores, "scores", self._f32, 3, self.device)
-        if scores.shape[0] != n or scores.shape[1] != self.kv_heads or (scores.shape[2] > 1 and scores.stride(2) != 1):
+        seq, head, step = scores.stride()
+        if scores.shape[0] != n or scores.shape[1] != self.kv_heads or (step != 1 and scores.shape[2] > 1):
             raise ValueError(f"scores must be [batch, {self.kv_heads}, width] with the last dimension contiguous")
+        return seq, head
 
     def sync(self, stream=None) -> None:
         """Waits for the cache's work on the stream and raises VkError for anything its kernels found wrong."""
