@@ -133,7 +133,7 @@ ABI = {
     "vk_kv_create": (C.c_int, [C.POINTER(KvDesc), C.POINTER(_vp)]),
     "vk_kv_destroy": (C.c_int, [_vp]),
     "vk_kv_sync": (C.c_int, [_vp, _vp]),
-    "vk_kv_append": (C.c_int, [_vp, _vp, _vp, C.POINTER(_i64), _vp, C.POINTER(_i64), _vp]),
+    "vk_kv_append": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "vk_kv_attend": (C.c_int, [_vp, _vp, _vp, _vp]),
     "vk_kv_attend_workspace": (C.c_int, [_vp, _vp, _vp, C.POINTER(C.c_size_t)]),
     "vk_kv_evict": (C.c_int, [_vp, _vp, _vp, _vp]),

@@ -25,6 +25,7 @@ from ._native import VkError, check, lib
 # The argument structs (N.KvBatch, N.KvAttend, N.KvEvict), packed in one step: a call's fields set one by one take longer
 # than its launch.
 _BATCH, _ATTEND, _EVICT = struct.Struct("@iiqqPPP"), struct.Struct("@PqqPqqPPqqqiiifPN"), struct.Struct("@PqiiiPqqqPPP")
+_STRIDES = struct.Struct("@qqqq")  # of append's keys and values
 assert [x.size for x in (_BATCH, _ATTEND, _EVICT)] == [C.sizeof(x) for x in (N.KvBatch, N.KvAttend, N.KvEvict)]
 
 # Attention's working memory by (device, stream): the calls of a stream share one tensor, which grows and whose start is
@@ -87,7 +88,6 @@ class PagedCache:
                      v_stride=(C.c_int64 * 3)(*v_pages.stride()[:3]))
         check(lib().vk_kv_create(C.byref(d), C.byref(self._h)), "vk_kv_create")
         self._sizes = {}  # bytes of attention's working memory by what they depend on
-        self._strides = (C.c_int64 * 2)(), (C.c_int64 * 2)()
         # argument structs, filled anew by every call, and their addresses
         self._args = C.create_string_buffer(_BATCH.size + max(_ATTEND.size, _EVICT.size))
         self._batch_at = C.addressof(self._args)
@@ -131,14 +131,15 @@ class PagedCache:
     def append(self, k, v, offsets, table, lens, *, stream=None) -> None:
         """New token t of sequence b (of T) is written to slot lens[b] - T + t. k, v: [tokens, kv_heads, head_dim],
         strides multiples of 8 elements (slices of one projection's output are fine)."""
-        ks, vs = self._strides
-        ks[0], ks[1], _ = self._rows(k, "k", self.kv_heads)
-        vs[0], vs[1], _ = self._rows(v, "v", self.kv_heads)
+        k_token, k_head, _ = self._rows(k, "k", self.kv_heads)
+        v_token, v_head, _ = self._rows(v, "v", self.kv_heads)
         tokens = k.shape[0]
         if v.shape[0] != tokens:
             raise ValueError("k and v must have the same number of tokens")
         self._sequences(table, lens, offsets, tokens)
-        code = self._lib.vk_kv_append(self._h, self._batch_at, k.data_ptr(), ks, v.data_ptr(), vs, self._stream(stream))
+        _STRIDES.pack_into(self._args, _BATCH.size, k_token, k_head, v_token, v_head)
+        at = self._call_at
+        code = self._lib.vk_kv_append(self._h, self._batch_at, k.data_ptr(), at, v.data_ptr(), at + 16, self._stream(stream))
         if code:
             check(code, "append")
 
