@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(SELECT_THREADS, 2) kv_select_kernel(KvPages c,
 // Copies the kept slots' keys and values, 16 bytes of each per thread and step. A grid of its own: the selection's few
 // CTAs have too few loads in flight for it (131,072 slots cut to 16,384, 8 kv heads: 128 us in one kernel, 93
 // in two when that was tried, 52 since the selection got faster). Measured: 16 sequences of up to 8,192 slots cut to half,
-// 8 kv heads of 128, 529 MB: 87 us, 6.1 TB/s..
+// 8 kv heads of 128, 529 MB: 87 us, 6.1 TB/s.
 __global__ void __launch_bounds__(256) kv_compact_kernel(KvPages c, KvBatch bt, KvEvict e) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int parts = c.dim >> 3, b = blockIdx.z, head = blockIdx.y;

@@ -13,9 +13,9 @@
 // and sum, on mma.sync m16n8k16: at 16 rows the tensor work is under a fifth of its rate while memory is saturated, and
 // the operands stay in registers from the scores to the values, which tcgen05's 128-row tiles would not allow.
 //
-// Measured: 32 sequences of up to 8,192 slots, 32 heads over 8 of 128: 118 us, 6.15 TB/s; one token over 1,000 slots: 9.4 us
-// in a graph, of which reading is one. Two CTAs share an SM (three at a head size of 64: no
-// difference, four: half as fast).
+// Measured: 32 sequences of up to 8,192 slots, 32 heads over 8 of 128: 117-121 us, 6.0-6.2 TB/s; one token over 1,000
+// slots: 9.4 us in a graph, of which reading is one. Two CTAs share an SM (at a head size of 64, 8 x 5 tokens over 4,001
+// slots: three make no difference, four take 25.8 us where two take 17.5).
 #pragma once
 #include <cuda.h>
 
