@@ -1,0 +1,163 @@
+"""CPU: what PagedCache does on the host around the C entries (streams, working memory, threads), with torch and the native
+library replaced by stand-ins that write down what they are asked for."""
+import ctypes as C
+import sys
+import types
+
+import pytest
+import torch
+
+from veckern_b200 import _native as N
+from veckern_b200 import kvcache
+
+
+class Device:
+    index = 0
+
+
+class Tensor:
+    """Sizes, strides and an address; `made_on` is the stream that was current when it was made."""
+
+    def __init__(self, fake, shape, strides=None, dtype=torch.float32):
+        self.shape, self.dtype, self.device, self.is_cuda = tuple(shape), dtype, fake.device, True
+        if strides is None:
+            strides, step = [], 1
+            for n in reversed(self.shape):
+                strides.insert(0, step)
+                step *= n
+        self.strides, self.made_on, self.at = tuple(strides), fake.current, fake.address()
+        fake.made.append(self)
+
+    def dim(self):
+        return len(self.shape)
+
+    def stride(self, i=None):
+        return self.strides if i is None else self.strides[i]
+
+    def numel(self):
+        n = 1
+        for x in self.shape:
+            n *= x
+        return n
+
+    def is_contiguous(self):
+        return True
+
+    def data_ptr(self):
+        return self.at
+
+
+class Fake(types.ModuleType):
+    """The torch functions that PagedCache calls, and the C entries; streams are numbers."""
+
+    def __init__(self):
+        super().__init__("torch")
+        self.device, self.current, self.made, self.calls, self.next = Device(), 3, [], [], 1 << 20
+        self.capturing, self.cleared, self.need, self.sync_code = set(), [], 1000, N.VK_OK
+        self.int32, self.float32, self.uint8 = torch.int32, torch.float32, torch.uint8
+        self.float16, self.bfloat16 = torch.float16, torch.bfloat16
+        outer = self
+
+        class Cuda:
+            @staticmethod
+            def ExternalStream(raw, device=None):
+                return types.SimpleNamespace(cuda_stream=raw)
+
+            class stream:
+                def __init__(self, s):
+                    self.raw = s.cuda_stream
+
+                def __enter__(self):
+                    self.before, outer.current = outer.current, self.raw
+
+                def __exit__(self, *exc):
+                    outer.current = self.before
+
+            @staticmethod
+            def is_current_stream_capturing():
+                return outer.current in outer.capturing
+
+            @staticmethod
+            def synchronize(device=None):
+                outer.calls.append(("synchronize",))
+
+        self.cuda = Cuda
+        self._C = types.SimpleNamespace(_cuda_getCurrentRawStream=lambda index: outer.current)
+
+    def address(self):
+        self.next += 1 << 16
+        return self.next
+
+    def empty_strided(self, shape, strides, dtype, device):
+        return Tensor(self, shape, strides, dtype)
+
+    def empty_like(self, x):
+        return Tensor(self, x.shape, x.strides, x.dtype)
+
+    def empty(self, shape, dtype, device):
+        t = Tensor(self, shape, None, dtype)
+        t.zeroed_on = []
+
+        class Start:
+            def zero_(_):
+                t.zeroed_on.append("graph" if self.current in self.capturing else self.current)
+
+        t.__class__ = type("Work", (Tensor,), {"__getitem__": lambda _, i: Start()})
+        return t
+
+    # ---- the C entries
+    def vk_kv_create(self, desc, out):
+        return N.VK_OK
+
+    def vk_kv_destroy(self, h):
+        return N.VK_OK
+
+    def vk_kv_attend_workspace(self, h, batch, args, size):
+        C.cast(size, C.POINTER(C.c_size_t))[0] = self.need
+        return N.VK_OK
+
+    def vk_kv_attend(self, h, batch, args, stream):
+        self.calls.append(("attend", read(N.KvBatch, batch), read(N.KvAttend, args), stream))
+        return N.VK_OK
+
+    def vk_kv_evict(self, h, batch, args, stream):
+        self.calls.append(("evict", read(N.KvBatch, batch), read(N.KvEvict, args), stream))
+        return N.VK_OK
+
+    def vk_kv_sync(self, h, stream):
+        return self.sync_code
+
+
+def read(kind, x):
+    """A C struct behind what a call passes: an address or packed bytes."""
+    return kind.from_buffer_copy(x if isinstance(x, bytes) else C.string_at(x, C.sizeof(kind)))
+
+
+@pytest.fixture
+def fake(monkeypatch):
+    f = Fake()
+    monkeypatch.setitem(sys.modules, "torch", f)
+    monkeypatch.setattr(kvcache, "lib", lambda: f)
+    monkeypatch.setattr(kvcache, "_WORK", {})
+    return f
+
+
+def make(fake, batch=2, heads=4):
+    """A cache, and a call's tensors: (cache, q, offsets, table, lens, scores)."""
+    pages = Tensor(fake, (8, 16, 2, 64), dtype=torch.bfloat16)
+    i32 = dict(dtype=torch.int32)
+    return (kvcache.PagedCache(pages, pages), Tensor(fake, (batch, heads, 64), dtype=torch.bfloat16),
+            Tensor(fake, (batch + 1,), **i32), Tensor(fake, (batch, 4), **i32), Tensor(fake, (batch,), **i32),
+            Tensor(fake, (batch, 2, 64)))
+
+
+@pytest.mark.parametrize("stream", [None, 3, 7])
+def test_results_are_made_on_the_stream_that_writes_them(fake, stream):
+    """Memory that another stream still uses, or will use as soon as a result is dropped, must not become a result."""
+    cache, q, offsets, table, lens, scores = make(fake)
+    want = 3 if stream is None else stream
+    out, lse = cache.attend(q, offsets, table, lens, stream=stream)
+    kept, new_lens, new_scores = cache.evict(table, lens, table, 8, 2, scores, stream=stream)
+    assert [x.made_on for x in (out, lse, kept, new_lens, new_scores)] == [want] * 5
+    assert [c[3] for c in fake.calls] == [want] * 2 and fake.current == 3
+    assert kept.shape == (2, 2, 8) and new_lens.shape == (2,) and new_scores.shape == (2, 2, 64)

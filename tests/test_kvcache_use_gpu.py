@@ -1,0 +1,70 @@
+"""GPU: the paged key/value cache as a serving program uses it: several streams, graphs, threads and caches at once."""
+import pytest
+
+from test_kvcache_gpu import Cache, check_attend
+
+pytestmark = pytest.mark.gpu
+
+STEP, CHUNK = [1, 1, 1], [70, 33, 128]  # new tokens: the step kernel and the chunk kernel
+
+
+def wait_on_current(ms=20):
+    """Keeps the current stream busy."""
+    import torch
+
+    torch.cuda._sleep(int(ms * 1.5e6))
+
+
+def call(c, counts, heads=8, seed=1):
+    """(q, offsets, zero scores) of a call."""
+    torch = c.t
+    return c.random(sum(counts), heads, c.dim, scale=2.0), c.offsets(counts), \
+        torch.zeros((len(counts), c.kv_heads, max(c.lens_list)), device="cuda")
+
+
+@pytest.mark.parametrize("counts", [STEP, CHUNK])
+def test_results_on_another_stream(counts):
+    """A block that the current stream has still to write when it is given back must not become a result of a call on
+    another stream, nor a dropped result of that call become a tensor of the current one."""
+    import torch
+
+    c = Cache([900, 700, 300], 32, 2, 128, seed=3, extra=3)
+    q, off, s0 = call(c, counts)
+    want, want_lse = c.cache.attend(q, off, c.table, c.lens)
+    c.cache.sync()
+    check_attend(c, q, counts, want, want_lse, True)
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    c.cache.attend(q, off, c.table, c.lens, stream=st)  # the stream's working memory
+    torch.cuda.synchronize()
+    junk = [torch.empty_like(want) for _ in range(4)] + [torch.empty_like(want_lse) for _ in range(4)]
+    wait_on_current()
+    for x in junk:
+        x.fill_(7.0)  # after the wait
+    del junk, x
+    out, lse = c.cache.attend(q, off, c.table, c.lens, stream=st)
+    st.synchronize()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    # the other way round: the call waits, its results are dropped, the current stream makes tensors of their sizes
+    with torch.cuda.stream(st):
+        wait_on_current()
+    c.cache.attend(q, off, c.table, c.lens, stream=st)
+    mine = [torch.full_like(want, 5.0) for _ in range(4)] + [torch.full_like(want_lse, 5.0) for _ in range(4)]
+    torch.cuda.synchronize()
+    assert all((x == 5).all() for x in mine)
+    # eviction's results
+    new = c.spare[:3, None].contiguous()
+    scores = torch.rand((3, 2, 900), generator=c.g, device="cuda")
+    kept0, lens0, scores0 = c.cache.evict(c.table, c.lens, new, 32, 4, scores)
+    torch.cuda.synchronize()
+    junk = [torch.empty_like(x) for x in (scores0, lens0, kept0) for _ in range(4)]
+    wait_on_current()
+    for x in junk:
+        x.fill_(7)
+    del junk, x
+    kept, new_lens, new_scores = c.cache.evict(c.table, c.lens, new, 32, 4, scores, stream=st)
+    st.synchronize()
+    torch.cuda.synchronize()
+    assert torch.equal(kept, kept0) and torch.equal(new_lens, lens0) and torch.equal(new_scores, scores0)
+    c.cache.sync(st)

@@ -10,7 +10,8 @@ sequence, made e.g. from a search's ids, says which pages it reads.
 All tensors are torch tensors on the cache's device. Sequence b of a call has the new tokens offsets[b]:offsets[b + 1]
 (int32, [batch + 1]), lens[b] slots with the new tokens included (int32, [batch]) and the pages table[b] (int32,
 [batch, width]; entries past its last slot are not read). Calls are asynchronous on `stream` (a torch.cuda.Stream or raw
-handle; default: the current stream); sync() waits and raises what the kernels found wrong. The calls of one stream share
+handle; default: the current stream), which the results they make belong to as well: another stream waits before it reads
+them. sync() waits and raises what the kernels found wrong. The calls of one stream share
 their working memory, those captured into CUDA graphs on one stream too: such graphs are replayed one after the other. No
 derivatives: a cache is for inference.
 """
@@ -128,6 +129,17 @@ class PagedCache:
             return self._torch._C._cuda_getCurrentRawStream(self.device.index)
         return getattr(stream, "cuda_stream", stream)
 
+    def _empty(self, shape, strides, dtype, stream):
+        """A tensor for results whose memory is that of the call's stream (as the caller gave it): memory of the current
+        one may have kernels of that stream still to write it."""
+        torch = self._torch
+        if stream is not None:
+            raw = getattr(stream, "cuda_stream", stream)
+            if raw != torch._C._cuda_getCurrentRawStream(self.device.index):
+                with torch.cuda.stream(torch.cuda.ExternalStream(raw, device=self.device)):
+                    return torch.empty_strided(shape, strides, dtype=dtype, device=self.device)
+        return torch.empty_strided(shape, strides, dtype=dtype, device=self.device)
+
     def append(self, k, v, offsets, table, lens, *, stream=None) -> None:
         """New token t of sequence b (of T) is written to slot lens[b] - T + t. k, v: [tokens, kv_heads, head_dim],
         strides multiples of 8 elements (slices of one projection's output are fine)."""
@@ -159,13 +171,13 @@ class PagedCache:
         n, width = self._sequences(table, lens, offsets, tokens)
         if out is None:
             o_token, o_head = heads * dim, dim
-            out = torch.empty_strided((tokens, heads, dim), (o_token, o_head, 1), dtype=self.dtype, device=self.device)
+            out = self._empty((tokens, heads, dim), (o_token, o_head, 1), self.dtype, stream)
         else:
             o_token, o_head, _ = self._rows(out, "out", heads)
             if out.shape[0] != tokens:
                 raise ValueError("out must have q's shape")
         if lse is None:
-            lse = torch.empty_strided((tokens, heads), (heads, 1), dtype=self._f32, device=self.device)
+            lse = self._empty((tokens, heads), (heads, 1), self._f32, stream)
         else:
             _want(lse, "lse", self._f32, 2, self.device)
             if lse.shape != (tokens, heads) or not lse.is_contiguous():
@@ -205,7 +217,6 @@ class PagedCache:
         those with the largest scores (ties to the lower slot), in slot order, copied to the pages of new_table (which
         no sequence of the call reads). Returns (kept [batch, kv_heads, keep] int32: the old slots, -1 behind the last;
         new lens [batch] int32; new scores like scores, contiguous, 0 behind the last)."""
-        torch = self._torch
         n, _ = self._sequences(table, lens)
         s_seq, s_head = self._check_scores(scores, n)
         if new_table.dtype != self._i32 or new_table.dim() != 2 or new_table.device != self.device:
@@ -216,9 +227,9 @@ class PagedCache:
         if not 0 <= recent <= keep:
             raise ValueError("keep and recent must satisfy 0 <= recent <= keep")
         heads, width = self.kv_heads, scores.shape[2]
-        kept = torch.empty_strided((n, heads, keep), (heads * keep, keep, 1), dtype=self._i32, device=self.device)
-        new_lens = torch.empty_like(lens)
-        new_scores = torch.empty_strided((n, heads, width), (heads * width, width, 1), dtype=self._f32, device=self.device)
+        kept = self._empty((n, heads, keep), (heads * keep, keep, 1), self._i32, stream)
+        new_lens = self._empty((n,), (1,), self._i32, stream)
+        new_scores = self._empty((n, heads, width), (heads * width, width, 1), self._f32, stream)
         _EVICT.pack_into(self._args, _BATCH.size, new_table.data_ptr(), new_stride, new_table.shape[1], keep, recent,
                          scores.data_ptr(), s_seq, s_head, width, new_scores.data_ptr(), kept.data_ptr(),
                          new_lens.data_ptr())
