@@ -389,6 +389,11 @@ typedef struct {
 /* Bytes of working memory that vk_kv_attend needs for these sizes (pointers in batch and args are not read, except
  * whether args->scores is NULL). */
 int vk_kv_attend_workspace(const vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_attend_t* args, size_t* bytes);
+/* Working memory of `bytes` bytes whose start is zero when the call returns. Also while streams are being captured: nothing
+ * of it is recorded, so that every graph, and calls outside of graphs, may use it in any order, one at a time. It has to
+ * outlive the graphs that hold its address. */
+int vk_kv_workspace_create(int device, size_t bytes, void** out);
+int vk_kv_workspace_destroy(int device, void* workspace);
 int vk_kv_attend(vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_attend_t* args, void* stream);
 
 /* For every sequence of n slots and every kv head: k = min(n, keep) slots are kept, the last r = min(recent, k) and, of

@@ -112,6 +112,12 @@ class Fake(types.ModuleType):
     def vk_kv_destroy(self, h):
         return N.VK_OK
 
+    def vk_kv_workspace_create(self, device, size, out):
+        out = C.cast(out, C.POINTER(C.c_void_p))
+        out[0] = self.address()
+        self.cleared.append(out[0])
+        return N.VK_OK
+
     def vk_kv_attend_workspace(self, h, batch, args, size):
         C.cast(size, C.POINTER(C.c_size_t))[0] = self.need
         return N.VK_OK
@@ -161,3 +167,34 @@ def test_results_are_made_on_the_stream_that_writes_them(fake, stream):
     assert [x.made_on for x in (out, lse, kept, new_lens, new_scores)] == [want] * 5
     assert [c[3] for c in fake.calls] == [want] * 2 and fake.current == 3
     assert kept.shape == (2, 2, 8) and new_lens.shape == (2,) and new_scores.shape == (2, 2, 64)
+
+
+def test_working_memory_made_under_capture_is_clear_at_once(fake):
+    """A graph that was never replayed has cleared nothing: neither a second graph nor an eager call may depend on it."""
+    cache, q, offsets, table, lens, _ = make(fake)
+    fake.capturing.add(9)
+    cache.attend(q, offsets, table, lens, stream=9)
+    fake.need = 5000  # grows within the capture
+    cache.attend(Tensor(fake, (3, 4, 64), dtype=torch.bfloat16), offsets, table, lens, stream=9)
+    fake.capturing.clear()
+    cache.attend(q, offsets, table, lens, stream=9)
+    used = [c[2].workspace for c in fake.calls]
+    assert used[0] != used[1] == used[2]
+    assert set(used) <= set(fake.cleared), "cleared by a node of the graph alone"
+    assert not any("graph" in x.zeroed_on for x in fake.made if hasattr(x, "zeroed_on"))
+
+
+def test_working_memory_of_a_stream(fake):
+    """Outside a capture it is torch's, cleared in the stream's order, and shared by the stream's calls while it suffices."""
+    cache, q, offsets, table, lens, _ = make(fake)
+    for stream in (None, 3, 8, 8):
+        cache.attend(q, offsets, table, lens, stream=stream)
+    used = [c[2].workspace for c in fake.calls]
+    assert used[0] == used[1] != used[2] == used[3] and not fake.cleared
+    work = {x.at: x for x in fake.made if hasattr(x, "zeroed_on")}
+    assert work[used[0]].zeroed_on == [3] and work[used[0]].made_on == 3 and work[used[2]].zeroed_on == [8]
+
+
+def test_workspace_entries_refuse_null():
+    assert N.lib().vk_kv_workspace_create(0, 1 << 20, None) == N.VK_ERR_INVALID and "out" in N.last_error()
+    assert N.lib().vk_kv_workspace_destroy(0, None) == N.VK_OK

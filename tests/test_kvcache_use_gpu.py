@@ -68,3 +68,44 @@ def test_results_on_another_stream(counts):
     torch.cuda.synchronize()
     assert torch.equal(kept, kept0) and torch.equal(new_lens, lens0) and torch.equal(new_scores, scores0)
     c.cache.sync(st)
+
+
+@pytest.mark.parametrize("counts", [STEP, CHUNK])
+@pytest.mark.parametrize("first", [0, 1, None])
+def test_graphs_in_any_order(monkeypatch, counts, first):
+    """Two graphs captured on one stream that never ran a call before: either may be replayed first, or neither before an
+    eager call on that stream."""
+    import torch
+
+    from veckern_b200 import kvcache
+
+    c = Cache([4000, 2500, 700], 64, 2, 128, seed=2)
+    q, off, s0 = call(c, counts)
+    want, want_lse = c.cache.attend(q, off, c.table, c.lens, scores=s0)
+    c.cache.sync()
+    dirt = torch.full((64 << 20,), 0x01010101, dtype=torch.int32, device="cuda")  # what is allocated next is not zero
+    del dirt
+    torch.cuda.empty_cache()
+    monkeypatch.setattr(kvcache, "_WORK", {})
+    st = torch.cuda.Stream()
+    graphs, got = [], []
+    for _ in range(2):
+        s = torch.zeros_like(s0)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            out, lse = c.cache.attend(q, off, c.table, c.lens, scores=s)
+        graphs.append(g)
+        got.append((out, lse, s))
+    order = [] if first is None else [first, 1 - first]
+    if first is None:
+        s = torch.zeros_like(s0)
+        torch.cuda.synchronize()
+        out, lse = c.cache.attend(q, off, c.table, c.lens, scores=s, stream=st)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(lse, want_lse) and torch.equal(s, s0)
+    for i in order + order:
+        got[i][2].zero_()
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[i][0], want) and torch.equal(got[i][1], want_lse) and torch.equal(got[i][2], s0)
+    c.cache.sync(st)

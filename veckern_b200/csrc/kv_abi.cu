@@ -278,6 +278,23 @@ int max_q_of(const vk_kv_attend_t* args, int64_t tokens) {
     return args->max_q > 0 ? (int)std::min<int64_t>(args->max_q, tokens) : (int)tokens;
 }
 
+// While it lives, this thread's calls neither join a capture of a stream nor end one, whatever its mode.
+struct BesideCapture {
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    BesideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    ~BesideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+};
+
+// Clears a workspace's start, on a stream that nothing else uses, and waits for it.
+int clear_workspace(void* workspace) {
+    cudaStream_t st;
+    VK_TRY_CUDA(cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking));
+    cudaError_t e = cudaMemsetAsync(workspace, 0, VK_KV_WORKSPACE_ZEROED, st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+    cudaStreamDestroy(st);
+    return e == cudaSuccess ? VK_OK : fail(VK_ERR_CUDA, "clearing a workspace: %s", cudaGetErrorString(e));
+}
+
 }  // namespace
 
 extern "C" {
@@ -422,6 +439,31 @@ int vk_kv_attend_workspace(const vk_kv_t* kv, const vk_kv_batch_t* batch, const 
     VK_TRY(check_batch(kv, &sizes, true, &bt));
     VK_TRY(check_attend(kv, args));
     *bytes = plan_attend(kv, bt, args->heads / kv->desc.kv_heads, max_q_of(args, bt.tokens), args->scores != nullptr).bytes;
+    return VK_OK;
+}
+
+int vk_kv_workspace_create(int device, size_t bytes, void** out) {
+    if (!out) return fail(VK_ERR_INVALID, "out must not be NULL");
+    *out = nullptr;
+    DeviceGuard guard(device);
+    if (guard.err != cudaSuccess) return fail(VK_ERR_CUDA, "cudaSetDevice: %s", cudaGetErrorString(guard.err));
+    BesideCapture beside;
+    void* p = nullptr;
+    VK_TRY_CUDA(cudaMalloc(&p, std::max<size_t>(bytes, VK_KV_WORKSPACE_ZEROED)));
+    const int r = clear_workspace(p);
+    if (r != VK_OK) {
+        cudaFree(p);
+        return r;
+    }
+    *out = p;
+    return VK_OK;
+}
+
+int vk_kv_workspace_destroy(int device, void* workspace) {
+    if (!workspace) return VK_OK;
+    DeviceGuard guard(device);
+    if (guard.err != cudaSuccess) return fail(VK_ERR_CUDA, "cudaSetDevice: %s", cudaGetErrorString(guard.err));
+    VK_TRY_CUDA(cudaFree(workspace));
     return VK_OK;
 }
 

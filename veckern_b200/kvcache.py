@@ -12,8 +12,8 @@ All tensors are torch tensors on the cache's device. Sequence b of a call has th
 [batch, width]; entries past its last slot are not read). Calls are asynchronous on `stream` (a torch.cuda.Stream or raw
 handle; default: the current stream), which the results they make belong to as well: another stream waits before it reads
 them. sync() waits and raises what the kernels found wrong. The calls of one stream share
-their working memory, those captured into CUDA graphs on one stream too: such graphs are replayed one after the other. No
-derivatives: a cache is for inference.
+their working memory, those captured into CUDA graphs on it too: such graphs are replayed in any order, one after the
+other, and not while eager calls of that stream run. No derivatives: a cache is for inference.
 """
 from __future__ import annotations
 
@@ -30,10 +30,27 @@ _STRIDES = struct.Struct("@qqqq")  # of append's keys and values
 assert [x.size for x in (_BATCH, _ATTEND, _EVICT)] == [C.sizeof(x) for x in (N.KvBatch, N.KvAttend, N.KvEvict)]
 
 # Attention's working memory by (device, stream): the calls of a stream share one tensor, which grows and whose start is
-# zero between calls. Tensors that were outgrown are kept: a captured graph may hold their addresses.
+# zero between calls. What was outgrown is kept: a captured graph may hold its address.
 _WORK: dict = {}
 _OUTGROWN: list = []
 _ZEROED = 8192  # VK_KV_WORKSPACE_ZEROED
+
+
+class _Captured:
+    """Working memory that is made while its stream is being captured. The graph's own pool will not do: what a graph
+    records there (clearing it, or another node's use of the same memory) happens when that graph is replayed, while other
+    graphs and eager calls of the stream use the memory too. It is made outside the capture, cleared, and kept for good."""
+
+    def __init__(self, device, size: int):
+        at = C.c_void_p()
+        check(lib().vk_kv_workspace_create(device.index, size, C.byref(at)), "attend (working memory, while capturing)")
+        self._at, self._size = at.value, size
+
+    def data_ptr(self) -> int:
+        return self._at
+
+    def numel(self) -> int:
+        return self._size
 
 
 def _workspace(torch, device, stream: int, need: int):
@@ -44,8 +61,11 @@ def _workspace(torch, device, stream: int, need: int):
         _OUTGROWN.append(work)
         need = max(need, work.numel() * 3 // 2)
     with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
-        work = torch.empty((need,), dtype=torch.uint8, device=device)
-        work[:_ZEROED].zero_()
+        if torch.cuda.is_current_stream_capturing():
+            work = _Captured(device, need)
+        else:
+            work = torch.empty((need,), dtype=torch.uint8, device=device)
+            work[:_ZEROED].zero_()
     _WORK[key] = work
     return work
 
