@@ -2,6 +2,7 @@
 library replaced by stand-ins that write down what they are asked for."""
 import ctypes as C
 import sys
+import threading
 import types
 
 import pytest
@@ -53,6 +54,7 @@ class Fake(types.ModuleType):
     def __init__(self):
         super().__init__("torch")
         self.device, self.current, self.made, self.calls, self.next = Device(), 3, [], [], 1 << 20
+        self.inside = None  # called by an entry before it reads its arguments: the interpreter's lock is free then
         self.capturing, self.cleared, self.need, self.sync_code = set(), [], 1000, N.VK_OK
         self.int32, self.float32, self.uint8 = torch.int32, torch.float32, torch.uint8
         self.float16, self.bfloat16 = torch.float16, torch.bfloat16
@@ -122,11 +124,24 @@ class Fake(types.ModuleType):
         C.cast(size, C.POINTER(C.c_size_t))[0] = self.need
         return N.VK_OK
 
+    def vk_kv_append(self, h, batch, k, k_stride, v, v_stride, stream):
+        self.enter()
+        pair = C.c_int64 * 2
+        self.calls.append(("append", read(N.KvBatch, batch), (k, *read(pair, k_stride), v, *read(pair, v_stride)), stream))
+        return N.VK_OK
+
+    def enter(self):
+        if self.inside:
+            then, self.inside = self.inside, None
+            then()
+
     def vk_kv_attend(self, h, batch, args, stream):
+        self.enter()
         self.calls.append(("attend", read(N.KvBatch, batch), read(N.KvAttend, args), stream))
         return N.VK_OK
 
     def vk_kv_evict(self, h, batch, args, stream):
+        self.enter()
         self.calls.append(("evict", read(N.KvBatch, batch), read(N.KvEvict, args), stream))
         return N.VK_OK
 
@@ -193,6 +208,40 @@ def test_working_memory_of_a_stream(fake):
     assert used[0] == used[1] != used[2] == used[3] and not fake.cleared
     work = {x.at: x for x in fake.made if hasattr(x, "zeroed_on")}
     assert work[used[0]].zeroed_on == [3] and work[used[0]].made_on == 3 and work[used[2]].zeroed_on == [8]
+
+
+@pytest.mark.parametrize("op", ["append", "attend", "evict"])
+def test_threads_do_not_share_arguments(fake, op):
+    """A C entry reads its arguments without the interpreter's lock: another thread may call the same cache meanwhile."""
+    cache, q, offsets, table, lens, scores = make(fake)
+    more = make(fake, batch=5)[1:]
+
+    def run(q, offsets, table, lens, scores, stream):
+        if op == "append":
+            cache.append(Tensor(fake, (q.shape[0], 2, 64), dtype=torch.bfloat16),
+                         Tensor(fake, (q.shape[0], 2, 64), (256, 64, 1), torch.bfloat16), offsets, table, lens, stream=stream)
+        elif op == "attend":
+            cache.attend(q, offsets, table, lens, stream=stream)
+        else:
+            cache.evict(table, lens, table, q.shape[0], 1, scores, stream=stream)
+
+    def beside():
+        t = threading.Thread(target=run, args=(*more, 9))
+        t.start()
+        t.join()
+
+    fake.inside = beside
+    run(q, offsets, table, lens, scores, 3)
+    (_, batch9, args9, s9), (_, batch3, args3, s3) = fake.calls
+    assert (s9, s3) == (9, 3)
+    for (x, tensors, n), args in (((batch3, (table, lens), 2), args3), ((batch9, (more[2], more[3]), 5), args9)):
+        assert (x.batch, x.table, x.lens) == (n, tensors[0].at, tensors[1].at)
+        if op == "append":
+            assert args[1:3] == (128, 64) and args[4:] == (256, 64) and x.tokens == n
+        elif op == "attend":
+            assert args.q == (q if n == 2 else more[0]).at
+        else:
+            assert args.keep == n and args.scores == (scores if n == 2 else more[4]).at
 
 
 def test_workspace_entries_refuse_null():

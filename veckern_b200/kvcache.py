@@ -24,9 +24,9 @@ from . import _native as N
 from ._native import VkError, check, lib
 
 # The argument structs (N.KvBatch, N.KvAttend, N.KvEvict), packed in one step: a call's fields set one by one take longer
-# than its launch.
+# than its launch. Every call packs its own: the C entries run without the interpreter's lock, beside other threads' calls.
 _BATCH, _ATTEND, _EVICT = struct.Struct("@iiqqPPP"), struct.Struct("@PqqPqqPPqqqiiifPN"), struct.Struct("@PqiiiPqqqPPP")
-_STRIDES = struct.Struct("@qqqq")  # of append's keys and values
+_STRIDES = struct.Struct("@qq")  # of append's keys or values
 assert [x.size for x in (_BATCH, _ATTEND, _EVICT)] == [C.sizeof(x) for x in (N.KvBatch, N.KvAttend, N.KvEvict)]
 
 # Attention's working memory by (device, stream): the calls of a stream share one tensor, which grows and whose start is
@@ -82,8 +82,8 @@ def _want(t, name: str, dtype, ndim: int, device) -> None:
 class PagedCache:
     """k_pages and v_pages: [pages, page_size, kv_heads, head_dim], any strides that are multiples of 8 elements with
     the last dimension contiguous (a [pages, kv_heads, page_size, head_dim] tensor is passed transposed). The cache
-    refers to the tensors, it does not copy them. page_size: a power of two in [8, 1024]; head_dim: a multiple of 8 up
-    to 128."""
+    refers to the tensors, it does not copy them. page_size: a power of two in [8, 1024]; head_dim: a multiple of 8 up to
+    128. Threads may call a cache at the same time."""
 
     def __init__(self, k_pages, v_pages):
         import torch
@@ -109,13 +109,9 @@ class PagedCache:
                      v_stride=(C.c_int64 * 3)(*v_pages.stride()[:3]))
         check(lib().vk_kv_create(C.byref(d), C.byref(self._h)), "vk_kv_create")
         self._sizes = {}  # bytes of attention's working memory by what they depend on
-        # argument structs, filled anew by every call, and their addresses
-        self._args = C.create_string_buffer(_BATCH.size + max(_ATTEND.size, _EVICT.size))
-        self._batch_at = C.addressof(self._args)
-        self._call_at = self._batch_at + _BATCH.size
 
     def _sequences(self, table, lens, offsets=None, tokens: int = 0):
-        """Checks a call's sequences and packs them; (sequences, table width)."""
+        """Checks a call's sequences; (N.KvBatch packed, sequences, table width)."""
         i32, dev = self._i32, self.device
         if table.dtype != i32 or table.dim() != 2 or table.device != dev:
             _want(table, "table", i32, 2, dev)
@@ -132,8 +128,7 @@ class PagedCache:
             if offsets.shape[0] != n + 1 or not offsets.is_contiguous():
                 raise ValueError("offsets must be contiguous [batch + 1]")
             at = offsets.data_ptr()
-        _BATCH.pack_into(self._args, 0, n, width, stride, tokens, at, table.data_ptr(), lens.data_ptr())
-        return n, width
+        return _BATCH.pack(n, width, stride, tokens, at, table.data_ptr(), lens.data_ptr()), n, width
 
     def _rows(self, t, name: str, heads: int):
         """Checks rows of tokens; their strides."""
@@ -168,10 +163,9 @@ class PagedCache:
         tokens = k.shape[0]
         if v.shape[0] != tokens:
             raise ValueError("k and v must have the same number of tokens")
-        self._sequences(table, lens, offsets, tokens)
-        _STRIDES.pack_into(self._args, _BATCH.size, k_token, k_head, v_token, v_head)
-        at = self._call_at
-        code = self._lib.vk_kv_append(self._h, self._batch_at, k.data_ptr(), at, v.data_ptr(), at + 16, self._stream(stream))
+        batch, _, _ = self._sequences(table, lens, offsets, tokens)
+        code = self._lib.vk_kv_append(self._h, batch, k.data_ptr(), _STRIDES.pack(k_token, k_head), v.data_ptr(),
+                                      _STRIDES.pack(v_token, v_head), self._stream(stream))
         if code:
             check(code, "append")
 
@@ -188,7 +182,7 @@ class PagedCache:
             raise ValueError("q must be [tokens, heads, head_dim]")
         tokens, heads, dim = q.shape
         q_token, q_head, _ = self._rows(q, "q", heads)
-        n, width = self._sequences(table, lens, offsets, tokens)
+        batch, n, width = self._sequences(table, lens, offsets, tokens)
         if out is None:
             o_token, o_head = heads * dim, dim
             out = self._empty((tokens, heads, dim), (o_token, o_head, 1), self.dtype, stream)
@@ -210,24 +204,22 @@ class PagedCache:
             scale = self._scale
         stream = self._stream(stream)
 
-        def pack(work: int, size: int) -> None:
-            _ATTEND.pack_into(self._args, _BATCH.size, q.data_ptr(), q_token, q_head, out.data_ptr(), o_token, o_head,
-                              lse.data_ptr(), s_at, s_seq, s_head, s_width, heads, max_q, bool(causal), scale, work, size)
+        def pack(work: int, size: int) -> bytes:
+            return _ATTEND.pack(q.data_ptr(), q_token, q_head, out.data_ptr(), o_token, o_head, lse.data_ptr(), s_at, s_seq,
+                                s_head, s_width, heads, max_q, bool(causal), scale, work, size)
 
         sizes = (n, width, tokens, heads, max_q, s_at != 0)
         need = self._sizes.get(sizes)
         if need is None:
-            pack(0, 0)
             size = C.c_size_t()
-            check(lib().vk_kv_attend_workspace(self._h, self._batch_at, self._call_at, C.byref(size)), "attend")
+            check(lib().vk_kv_attend_workspace(self._h, batch, pack(0, 0), C.byref(size)), "attend")
             if len(self._sizes) >= 4096:
                 self._sizes.clear()
             need = self._sizes[sizes] = size.value
         work = _WORK.get((self.device.index, stream))
         if work is None or work.numel() < need:
             work = _workspace(torch, self.device, stream, need)
-        pack(work.data_ptr(), work.numel())
-        code = self._lib.vk_kv_attend(self._h, self._batch_at, self._call_at, stream)
+        code = self._lib.vk_kv_attend(self._h, batch, pack(work.data_ptr(), work.numel()), stream)
         if code:
             check(code, "attend")
         return out, lse
@@ -237,7 +229,7 @@ class PagedCache:
         those with the largest scores (ties to the lower slot), in slot order, copied to the pages of new_table (which
         no sequence of the call reads). Returns (kept [batch, kv_heads, keep] int32: the old slots, -1 behind the last;
         new lens [batch] int32; new scores like scores, contiguous, 0 behind the last)."""
-        n, _ = self._sequences(table, lens)
+        batch, n, _ = self._sequences(table, lens)
         s_seq, s_head = self._check_scores(scores, n)
         if new_table.dtype != self._i32 or new_table.dim() != 2 or new_table.device != self.device:
             _want(new_table, "new_table", self._i32, 2, self.device)
@@ -250,10 +242,9 @@ class PagedCache:
         kept = self._empty((n, heads, keep), (heads * keep, keep, 1), self._i32, stream)
         new_lens = self._empty((n,), (1,), self._i32, stream)
         new_scores = self._empty((n, heads, width), (heads * width, width, 1), self._f32, stream)
-        _EVICT.pack_into(self._args, _BATCH.size, new_table.data_ptr(), new_stride, new_table.shape[1], keep, recent,
-                         scores.data_ptr(), s_seq, s_head, width, new_scores.data_ptr(), kept.data_ptr(),
-                         new_lens.data_ptr())
-        code = self._lib.vk_kv_evict(self._h, self._batch_at, self._call_at, self._stream(stream))
+        args = _EVICT.pack(new_table.data_ptr(), new_stride, new_table.shape[1], keep, recent, scores.data_ptr(), s_seq,
+                           s_head, width, new_scores.data_ptr(), kept.data_ptr(), new_lens.data_ptr())
+        code = self._lib.vk_kv_evict(self._h, batch, args, self._stream(stream))
         if code:
             check(code, "evict")
         return kept, new_lens, new_scores
