@@ -12,7 +12,8 @@
  * (dist, id) pairs with ties broken by the lower id, ascending, padded with {+inf, -1}.
  * Inputs must be finite: NaN distances are never returned (the reference's heap keeps them in arbitrary order).
  *
- * Thread safety: one index may be used by one host thread at a time (as the reference's PQSearcher).
+ * Thread safety: one index may be used by one host thread at a time (as the reference's PQSearcher); a paged
+ * cache (vk_kv_*) by several.
  */
 #ifndef VK_ABI_H
 #define VK_ABI_H
@@ -312,7 +313,8 @@ int vk_ivf_assign_device(int device, const float* d_x, int64_t n, int d, const f
  * allocates, attention's working memory is the caller's (vk_kv_attend_workspace). All calls are asynchronous on `stream`
  * (cudaStream_t as void*; NULL = the default stream) and may be captured into a CUDA graph. A page number outside
  * [0, pages) or a length or offset outside its table is never followed: such a page reads as zeros and writes to it are
- * skipped; vk_kv_sync waits and then reports it as VK_ERR_INVALID. */
+ * skipped; vk_kv_sync waits and then reports it as VK_ERR_INVALID. The calls keep nothing on the host: several threads may
+ * use a cache at the same time (for working memory see vk_kv_attend_t). */
 enum {
     VK_KV_F16 = 0,
     VK_KV_BF16 = 1
@@ -381,7 +383,8 @@ typedef struct {
     int causal;
     float scale;
     void* workspace; /* DEVICE, 256-byte aligned, at least vk_kv_attend_workspace bytes, for one call at a time (the
-                        calls of one stream may share it, of several caches too). Its first VK_KV_WORKSPACE_ZEROED
+                        calls of one stream may share it, of several caches too, if one host thread issues them at a
+                        time: a call may be two launches). Its first VK_KV_WORKSPACE_ZEROED
                         bytes have to be zero; a call leaves them zero, unless vk_kv_sync reports VK_ERR_DEVICE */
     size_t workspace_bytes;
 } vk_kv_attend_t;

@@ -244,6 +244,34 @@ def test_threads_do_not_share_arguments(fake, op):
             assert args.keep == n and args.scores == (scores if n == 2 else more[4]).at
 
 
+def test_calls_that_share_working_memory_are_issued_one_at_a_time(fake):
+    """A call may be two launches: no other call of the stream comes between them."""
+    cache, q, offsets, table, lens, _ = make(fake)
+    other = make(fake)[0]
+    threads, order = [], []
+
+    def start(c, name, stream):
+        def run():
+            c.attend(q, offsets, table, lens, stream=stream)
+            order.append(name)
+
+        threads.append(threading.Thread(target=run))
+        threads[-1].start()
+
+    def beside():
+        start(other, "same stream", 3)
+        start(cache, "another stream", 9)
+        threads[1].join()
+        threads[0].join(0.2)
+        order.append("first")
+
+    cache.attend(q, offsets, table, lens)
+    fake.inside = beside
+    cache.attend(q, offsets, table, lens)
+    threads[0].join()
+    assert order == ["another stream", "first", "same stream"]
+
+
 def test_workspace_entries_refuse_null():
     assert N.lib().vk_kv_workspace_create(0, 1 << 20, None) == N.VK_ERR_INVALID and "out" in N.last_error()
     assert N.lib().vk_kv_workspace_destroy(0, None) == N.VK_OK

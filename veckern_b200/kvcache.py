@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import ctypes as C
 import struct
+import threading
 
 from . import _native as N
 from ._native import VkError, check, lib
@@ -29,44 +30,45 @@ _BATCH, _ATTEND, _EVICT = struct.Struct("@iiqqPPP"), struct.Struct("@PqqPqqPPqqq
 _STRIDES = struct.Struct("@qq")  # of append's keys or values
 assert [x.size for x in (_BATCH, _ATTEND, _EVICT)] == [C.sizeof(x) for x in (N.KvBatch, N.KvAttend, N.KvEvict)]
 
-# Attention's working memory by (device, stream): the calls of a stream share one tensor, which grows and whose start is
+# Attention's working memory by (device, stream): the calls of a stream share it, one at a time; it grows, and its start is
 # zero between calls. What was outgrown is kept: a captured graph may hold its address.
 _WORK: dict = {}
 _OUTGROWN: list = []
+_GROWING = threading.Lock()
 _ZEROED = 8192  # VK_KV_WORKSPACE_ZEROED
 
 
-class _Captured:
-    """Working memory that is made while its stream is being captured. The graph's own pool will not do: what a graph
-    records there (clearing it, or another node's use of the same memory) happens when that graph is replayed, while other
-    graphs and eager calls of the stream use the memory too. It is made outside the capture, cleared, and kept for good."""
+class _Work:
+    """Working memory of a stream. `lock` is held while a call is issued: a call may be two launches, and another thread's
+    call on the stream must not come between them."""
 
-    def __init__(self, device, size: int):
-        at = C.c_void_p()
-        check(lib().vk_kv_workspace_create(device.index, size, C.byref(at)), "attend (working memory, while capturing)")
-        self._at, self._size = at.value, size
+    def __init__(self, torch, device, stream: int, size: int):
+        self.size, self.lock = size, threading.Lock()
+        with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+            if torch.cuda.is_current_stream_capturing():
+                # The graph's own pool will not do: what a graph records there (clearing it, or another node's use of the
+                # same memory) happens when that graph is replayed, while other graphs and eager calls of the stream use
+                # the memory too. It is made outside the capture, cleared, and kept for good.
+                at = C.c_void_p()
+                check(lib().vk_kv_workspace_create(device.index, size, C.byref(at)), "attend (working memory, while capturing)")
+                self.at = at.value
+            else:
+                self._memory = torch.empty((size,), dtype=torch.uint8, device=device)
+                self._memory[:_ZEROED].zero_()
+                self.at = self._memory.data_ptr()
 
-    def data_ptr(self) -> int:
-        return self._at
 
-    def numel(self) -> int:
-        return self._size
-
-
-def _workspace(torch, device, stream: int, need: int):
-    """A larger working memory for a stream."""
+def _workspace(torch, device, stream: int, need: int) -> _Work:
+    """Larger working memory for a stream."""
     key = (device.index, stream)
-    work = _WORK.get(key)
-    if work is not None:
-        _OUTGROWN.append(work)
-        need = max(need, work.numel() * 3 // 2)
-    with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
-        if torch.cuda.is_current_stream_capturing():
-            work = _Captured(device, need)
-        else:
-            work = torch.empty((need,), dtype=torch.uint8, device=device)
-            work[:_ZEROED].zero_()
-    _WORK[key] = work
+    with _GROWING:
+        work = _WORK.get(key)
+        if work is not None:
+            if work.size >= need:  # another thread was here first
+                return work
+            _OUTGROWN.append(work)
+            need = max(need, work.size * 3 // 2)
+        work = _WORK[key] = _Work(torch, device, stream, need)
     return work
 
 
@@ -83,7 +85,7 @@ class PagedCache:
     """k_pages and v_pages: [pages, page_size, kv_heads, head_dim], any strides that are multiples of 8 elements with
     the last dimension contiguous (a [pages, kv_heads, page_size, head_dim] tensor is passed transposed). The cache
     refers to the tensors, it does not copy them. page_size: a power of two in [8, 1024]; head_dim: a multiple of 8 up to
-    128. Threads may call a cache at the same time."""
+    128. Threads may call a cache at the same time, on one stream or on several."""
 
     def __init__(self, k_pages, v_pages):
         import torch
@@ -217,9 +219,11 @@ class PagedCache:
                 self._sizes.clear()
             need = self._sizes[sizes] = size.value
         work = _WORK.get((self.device.index, stream))
-        if work is None or work.numel() < need:
+        if work is None or work.size < need:
             work = _workspace(torch, self.device, stream, need)
-        code = self._lib.vk_kv_attend(self._h, batch, pack(work.data_ptr(), work.numel()), stream)
+        args = pack(work.at, work.size)
+        with work.lock:
+            code = self._lib.vk_kv_attend(self._h, batch, args, stream)
         if code:
             check(code, "attend")
         return out, lse
