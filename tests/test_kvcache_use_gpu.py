@@ -109,3 +109,70 @@ def test_graphs_in_any_order(monkeypatch, counts, first):
         torch.cuda.synchronize()
         assert torch.equal(got[i][0], want) and torch.equal(got[i][1], want_lse) and torch.equal(got[i][2], s0)
     c.cache.sync(st)
+
+
+@pytest.mark.parametrize("kinds", [(STEP, STEP), (CHUNK, CHUNK), (STEP, CHUNK)])
+def test_calls_on_two_streams_at_once(kinds):
+    """Calls whose segments are cut between many CTAs, on two streams beside kernels that keep the SMs busy: whoever waits
+    for a part waits for a CTA that has started, so that neither call can keep the other from ending."""
+    import torch
+
+    caches = [Cache([9000, 5000, 700], 32, 2, 128, seed=11 + i) for i in range(2)]
+    sides = []
+    for c, counts in zip(caches, kinds):
+        q, off, s0 = call(c, counts)
+        out, lse = c.cache.attend(q, off, c.table, c.lens, scores=s0, max_q=max(counts))
+        c.cache.sync()
+        sides.append((c, q, off, s0, out, lse, max(counts)))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    x = torch.randn((4096, 4096), device="cuda", dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(40):
+        with torch.cuda.stream(streams[2]):
+            x @ x
+        for (c, q, off, s0, _, _, most), st in zip(sides, streams):
+            with torch.cuda.stream(st):
+                s = torch.zeros_like(s0)
+                got.append((*c.cache.attend(q, off, c.table, c.lens, scores=s, max_q=most), s))
+    torch.cuda.synchronize()
+    for st, (c, *_) in zip(streams, sides):
+        c.cache.sync(st)
+    for i, (out, lse, s) in enumerate(got):
+        _, _, _, s0, want, want_lse, _ = sides[i % 2]
+        assert torch.equal(out, want) and torch.equal(lse, want_lse) and torch.equal(s, s0)
+
+
+def test_threads_with_a_stream_each():
+    """Two threads call one cache with other sizes, other tensors and streams of their own."""
+    import threading
+
+    import torch
+
+    c = Cache([2000, 1500, 700], 32, 2, 128, seed=7)
+    work = []
+    for counts in (STEP, CHUNK):
+        q, off, s = call(c, counts)
+        out, lse = c.cache.attend(q, off, c.table, c.lens, scores=s, max_q=max(counts))
+        work.append((counts, q, off, s, out, lse))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def run(counts, q, off, s0, want, want_lse):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            for _ in range(150):
+                s = torch.zeros_like(s0)
+                out, lse = c.cache.attend(q, off, c.table, c.lens, scores=s, max_q=max(counts))
+                kept, _, _ = c.cache.evict(c.table, c.lens, c.table[:, :0], 0, 0, s0)
+                if not (torch.equal(out, want) and torch.equal(lse, want_lse) and torch.equal(s, s0) and kept.numel() == 0):
+                    wrong.append(counts)
+        st.synchronize()
+
+    threads = [threading.Thread(target=run, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    c.cache.sync()
+    assert not wrong

@@ -83,7 +83,7 @@ struct AttendPlan {
     bool step;
     int rows, s_rows;  // of the step path, rounded up to 8 or 16; to 4, 8 or 16
     int ctas;
-    size_t ready, o, ml, s, bytes;  // offsets
+    size_t ready, started, o, ml, s, bytes;  // offsets
 };
 
 AttendPlan plan_attend(const vk_kv* kv, const vk::KvBatch& bt, int group, int max_q, bool scores) {
@@ -97,6 +97,7 @@ AttendPlan plan_attend(const vk_kv* kv, const vk::KvBatch& bt, int group, int ma
     const int64_t slots = (int64_t)bt.width << kv->page_shift;
     // What has to be zero before a call lies at the start, whatever the sizes.
     const size_t rows_of_parts = (size_t)p.ctas * (p.step ? vk::STEP_ROWS : 2 * vk::CHUNK_ROWS);
+    p.started = VK_KV_WORKSPACE_ZEROED - sizeof(uint32_t);
     p.o = VK_KV_WORKSPACE_ZEROED;
     p.ml = p.o + align256(rows_of_parts * dp * sizeof(float));
     p.s = p.ml + align256(rows_of_parts * sizeof(float2));
@@ -255,6 +256,7 @@ int launch_attend(const vk_kv* kv, const vk::KvBatch& bt, const vk::KvAttend& a,
     uint8_t* w = static_cast<uint8_t*>(workspace);
     vk::KvParts parts{};
     parts.ready = reinterpret_cast<uint32_t*>(w + p.ready);
+    parts.started = reinterpret_cast<uint32_t*>(w + p.started);
     parts.o = reinterpret_cast<float*>(w + p.o);
     parts.ml = reinterpret_cast<float2*>(w + p.ml);
     parts.s = reinterpret_cast<float*>(w + p.s);

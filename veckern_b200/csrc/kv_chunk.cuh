@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     tmem_fence_before();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const ChunkShape shape{a, a.tokens};
-    KvShare share = kv_share<CHUNK_THREADS>(c, bt, scratch, CHUNK_PART_COST, [&](const KvSeq& s, int* longest) {
+    KvShare share = kv_share<CHUNK_THREADS>(c, bt, parts, scratch, CHUNK_PART_COST, [&](const KvSeq& s, int* longest) {
         if (!shape.takes(s)) return 0;
         const int pairs = shape.pairs(s);
         *longest = max(*longest, max(shape.units(s, pairs - 1), shape.units(s, max(0, pairs - 2))));
@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             const int e_from = g.lone ? i * (DP / 2) : 0, e_to = g.lone && i == 0 ? min(c.dim, DP / 2) : c.dim;
             const bool leaves = g.t0 > 0;                                                       // a part for an earlier CTA
             const int follow = leaves ? 0 : walk.share.followers(g.units - g.count);  // CTAs with the rest of this one
-            auto part_of = [&](int k) -> int64_t { return 2 * (int64_t)(blockIdx.x + k) + i; };
+            auto part_of = [&](int k) -> int64_t { return 2 * (int64_t)(walk.share.me + k) + i; };
             if (follow) {
                 for (int k = r; k < follow; k += 128) part_await(parts, (int)part_of(1 + k), wait);
                 asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");

@@ -7,6 +7,8 @@
 // sequence's head that a CTA holds whole is finished in place. One that is cut is finished by the CTA that holds its
 // beginning, which comes to it last and finds the parts of the CTAs that follow (unnormalised sums with their maximum
 // and total; they come to theirs first) in the workspace. It adds them up in order: results do not depend on timing.
+// Shares are handed out from the last to the first, in the order in which CTAs start: who waits for a part waits for a CTA
+// that runs already and that waits for nobody before it has made the part, whatever else has the rest of the SMs.
 //
 // Inside a CTA one warp keeps a ring of tiles filled by TMA (one box per page and 64 head elements, in the 128-byte
 // swizzle that ldmatrix reads without conflicts); four warps take 16 slots of each tile, with their own running maximum
@@ -36,6 +38,7 @@ constexpr long long KV_WAIT_BUDGET = 4000000000LL;  // cycles: about two seconds
 // the call is done.
 struct KvParts {
     uint32_t* ready;
+    uint32_t* started;  // CTAs of the running kernel that have begun; the last one makes it zero again
     float* o;    // [part]: unnormalised sums
     float2* ml;  // [part][row]: maximum (base 2) and sum
     float* s;    // [sequence][kv head][slot][s_rows]: scaled scores (base 2) of the step path, for the weights
@@ -109,7 +112,7 @@ struct KvWait {
 __device__ __forceinline__ void part_publish(const KvParts& parts, int i) {
     asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(parts.ready + i), "r"(1u) : "memory");
 }
-// Waits, with a limit, for part i. Its CTA comes to it before anything else and waits for nobody to make it.
+// Waits, with a limit, for part i. Its CTA has started, comes to it before anything else and waits for nobody to make it.
 __device__ __forceinline__ void part_await(const KvParts& parts, int i, KvWait& wait) {
     uint32_t there = 0;
     const long long t0 = clock64();
@@ -162,6 +165,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 // sequence; the caller splits a sequence's units into its heads and tiles. The host has checked that all units together
 // are fewer than 2^31.
 struct KvShare {
+    int me;    // which share; none from `ctas` on
     int b;     // sequence of the next unit
     int off;   // unit within it
     int left;  // units of this CTA that are not taken yet
@@ -171,9 +175,9 @@ struct KvShare {
     __device__ __forceinline__ int first(int cta) const { return each * cta + min(cta, more); }
     // CTAs that hold the next `rest` units after this CTA's share
     __device__ __forceinline__ int followers(int rest) const {
-        const int me = blockIdx.x + 1, end = first(me) + rest;
+        const int next = me + 1, end = first(next) + rest;
         int n = 0;
-        while (me + n < ctas && first(me + n) < end) ++n;
+        while (next + n < ctas && first(next + n) < end) ++n;
         return n;
     }
 };
@@ -183,12 +187,14 @@ constexpr int KV_SHARE_SCRATCH = 40;
 // every m units takes m of a unit's time and L / m of a part's: least with m = sqrt(L part / unit), which is the least that
 // a CTA gets (part_cost: part / unit), except where all units together are fewer.
 template <int THREADS, class Count>
-__device__ __forceinline__ KvShare kv_share(const KvPages& c, const KvBatch& bt, int* scratch, float part_cost,
-                                            Count&& count) {
+__device__ __forceinline__ KvShare kv_share(const KvPages& c, const KvBatch& bt, const KvParts& parts, int* scratch,
+                                            float part_cost, Count&& count) {
     // scratch: KV_SHARE_SCRATCH values of shared memory. Thread t sums a contiguous range of the sequences. No CTA without a
     // share lies between others: the parts of a cut segment belong to consecutive CTAs.
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    constexpr int WARPS = THREADS / 32;
+    constexpr int WARPS = THREADS / 32, PLACE = KV_SHARE_SCRATCH - 1;
+    static_assert(2 * WARPS + 2 <= PLACE, "scratch");
+    if (t == THREADS - 1) scratch[PLACE] = (int)atomicInc(parts.started, gridDim.x - 1);  // beside the others' loads
     const int span = (bt.batch + THREADS - 1) / THREADS;
     const int b0 = min(bt.batch, t * span), b1 = min(bt.batch, b0 + span);
     int sum = 0, longest = 0;
@@ -215,11 +221,13 @@ __device__ __forceinline__ KvShare kv_share(const KvPages& c, const KvBatch& bt,
     const int least = max(1, (int)(sqrtf(longest * part_cost) + 0.5f));
     KvShare s;
     s.ctas = min((int)gridDim.x, (total + least - 1) / least);
-    const uint32_t parts = max(s.ctas, 1);
-    s.each = (int)((uint32_t)total / parts);
-    s.more = total - s.each * (int)parts;
-    const int me = min((int)blockIdx.x, s.ctas), first = s.first(me);
-    s.left = me < s.ctas ? s.first(me + 1) - first : 0;
+    const uint32_t shares = max(s.ctas, 1);
+    s.each = (int)((uint32_t)total / shares);
+    s.more = total - s.each * (int)shares;
+    const int place = scratch[PLACE];
+    s.me = place < s.ctas ? s.ctas - 1 - place : s.ctas;
+    const int first = s.first(s.me);
+    s.left = s.me < s.ctas ? s.first(s.me + 1) - first : 0;
     before += incl - sum;
     if (first >= before && first < before + sum) {
         int off = first - before, b = b0;
@@ -288,7 +296,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
         *longest = max(*longest, tiles_of(s));
         return tiles_of(s) * c.heads;
     };
-    KvShare share = kv_share<STEP_THREADS>(c, bt, scratch, STEP_PART_COST, units_of);
+    KvShare share = kv_share<STEP_THREADS>(c, bt, parts, scratch, STEP_PART_COST, units_of);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     KvWait wait{c.status};
     int stage = 0;
@@ -439,7 +447,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
             // Join the four warps, eight rows at a time.
             const bool leaves = t0 > 0;                                             // a part for an earlier CTA
             const int follow = leaves ? 0 : share.followers(tiles - count);  // CTAs with the rest of this one
-            for (int i = threadIdx.x; i < follow; i += 32 * STEP_WARPS) part_await(parts, blockIdx.x + 1 + i, wait);
+            for (int i = threadIdx.x; i < follow; i += 32 * STEP_WARPS) part_await(parts, share.me + 1 + i, wait);
 #pragma unroll
             for (int u = 0; u < R / 8; ++u) {
                 l[u] += __shfl_xor_sync(FULL, l[u], 1);
@@ -477,7 +485,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
             if (works && leaves) {
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    const int64_t p = (int64_t)blockIdx.x * STEP_ROWS + 8 * u + r8;
+                    const int64_t p = (int64_t)share.me * STEP_ROWS + 8 * u + r8;
                     float4* po = reinterpret_cast<float4*>(parts.o + p * DP + d);
                     po[0] = make_float4(v[u][0], v[u][1], v[u][2], v[u][3]);
                     po[1] = make_float4(v[u][4], v[u][5], v[u][6], v[u][7]);
@@ -492,7 +500,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
                     for (int k = 0; k < FLY; ++k)
 #pragma unroll
                         for (int u = 0; u < U; ++u) {
-                            const int64_t p = (int64_t)(blockIdx.x + 1 + min(k0 + k, follow - 1)) * STEP_ROWS + 8 * u + r8;
+                            const int64_t p = (int64_t)(share.me + 1 + min(k0 + k, follow - 1)) * STEP_ROWS + 8 * u + r8;
                             const float4* po = reinterpret_cast<const float4*>(parts.o + p * DP + d);
                             ml[k][u] = __ldcg(parts.ml + p);
                             x[k][u] = __ldcg(po);
@@ -534,8 +542,8 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
                 }
             }
             if (leaves || follow) asm volatile("bar.sync 1, 128;" ::: "memory");
-            if (leaves && threadIdx.x == 0) part_publish(parts, blockIdx.x);
-            for (int i = threadIdx.x; i < follow; i += 32 * STEP_WARPS) parts.ready[blockIdx.x + 1 + i] = 0;
+            if (leaves && threadIdx.x == 0) part_publish(parts, share.me);
+            for (int i = threadIdx.x; i < follow; i += 32 * STEP_WARPS) parts.ready[share.me + 1 + i] = 0;
         }
     }
     // A wait that ran out may have left copies in flight into this CTA's memory: see them land before it ends.

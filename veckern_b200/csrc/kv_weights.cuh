@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(WEIGHTS_THREADS, 1)
     tmem_fence_before();
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const WeightsShape shape{a, a.tokens};
-    KvShare share = kv_share<WEIGHTS_THREADS>(c, bt, scratch, WEIGHTS_PART_COST, [&](const KvSeq& s, int* longest) {
+    KvShare share = kv_share<WEIGHTS_THREADS>(c, bt, parts, scratch, WEIGHTS_PART_COST, [&](const KvSeq& s, int* longest) {
         if (!shape.takes(s)) return 0;
         *longest = max(*longest, shape.row_tiles(s));
         return shape.before(s, shape.pairs(s)) * c.heads;
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(WEIGHTS_THREADS, 1)
             asm volatile("bar.sync %0, 256;" ::"r"(5 + i) : "memory");
             if (half == 1) continue;
             total += *other;
-            const int part = 2 * blockIdx.x + i;
+            const int part = 2 * walk.share.me + i;
             if (g.leaves) {
                 parts.o[(int64_t)part * CHUNK_SLOTS + r] = total;
                 asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");
