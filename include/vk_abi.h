@@ -351,7 +351,8 @@ typedef struct {
 typedef struct vk_kv vk_kv_t;
 int vk_kv_create(const vk_kv_desc_t* desc, vk_kv_t** out);
 int vk_kv_destroy(vk_kv_t* kv);
-/* Waits for the cache's work on `stream` and reports any kernel-side error (and clears it). */
+/* Waits for the cache's work on `stream` and reports any kernel-side error (and clears it). A cache has one status word:
+ * with calls on several streams, an error may be reported by the first vk_kv_sync of any of them. */
 int vk_kv_sync(vk_kv_t* kv, void* stream);
 
 /* New token t of sequence b, of T, goes to slot lens[b] - T + t. Element (token, head, i) of the new keys is
@@ -385,7 +386,10 @@ typedef struct {
     void* workspace; /* DEVICE, 256-byte aligned, at least vk_kv_attend_workspace bytes, for one call at a time (the
                         calls of one stream may share it, of several caches too, if one host thread issues them at a
                         time: a call may be two launches). Its first VK_KV_WORKSPACE_ZEROED
-                        bytes have to be zero; a call leaves them zero, unless vk_kv_sync reports VK_ERR_DEVICE */
+                        bytes have to be zero; a call leaves them zero. After VK_ERR_DEVICE from vk_kv_sync every
+                        workspace that the cache's calls have used since the last vk_kv_sync, on whatever stream, is
+                        cleared before it is used again (vk_kv_workspace_clear): until then each call with one that a wait
+                        has left unfinished is void, and its cache's vk_kv_sync says so */
     size_t workspace_bytes;
 } vk_kv_attend_t;
 #define VK_KV_WORKSPACE_ZEROED 8192
@@ -397,6 +401,8 @@ int vk_kv_attend_workspace(const vk_kv_t* kv, const vk_kv_batch_t* batch, const 
  * outlive the graphs that hold its address. */
 int vk_kv_workspace_create(int device, size_t bytes, void** out);
 int vk_kv_workspace_destroy(int device, void* workspace);
+/* Clears a workspace's start; done when the call returns. No call may be using it. */
+int vk_kv_workspace_clear(int device, void* workspace);
 int vk_kv_attend(vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_attend_t* args, void* stream);
 
 /* For every sequence of n slots and every kv head: k = min(n, keep) slots are kept, the last r = min(recent, k) and, of

@@ -120,6 +120,10 @@ class Fake(types.ModuleType):
         self.cleared.append(out[0])
         return N.VK_OK
 
+    def vk_kv_workspace_clear(self, device, at):
+        self.calls.append(("clear", at))
+        return N.VK_OK
+
     def vk_kv_attend_workspace(self, h, batch, args, size):
         C.cast(size, C.POINTER(C.c_size_t))[0] = self.need
         return N.VK_OK
@@ -160,6 +164,7 @@ def fake(monkeypatch):
     monkeypatch.setitem(sys.modules, "torch", f)
     monkeypatch.setattr(kvcache, "lib", lambda: f)
     monkeypatch.setattr(kvcache, "_WORK", {})
+    monkeypatch.setattr(kvcache, "_OUTGROWN", [])
     return f
 
 
@@ -272,6 +277,37 @@ def test_calls_that_share_working_memory_are_issued_one_at_a_time(fake):
     assert order == ["another stream", "first", "same stream"]
 
 
+@pytest.mark.parametrize("code", [N.VK_OK, N.VK_ERR_INVALID, N.VK_ERR_DEVICE])
+def test_sync_clears_all_working_memory_after_a_wait_ran_out(fake, code):
+    """The status word is the cache's, working memory the stream's: the call that gave up may have been any of the cache's
+    streams', and a graph may hold what was outgrown."""
+    cache, q, offsets, table, lens, _ = make(fake)
+    cache.attend(q, offsets, table, lens)
+    cache.attend(q, offsets, table, lens, stream=9)
+    fake.need = 5000
+    cache.attend(Tensor(fake, (3, 4, 64), dtype=torch.bfloat16), offsets, table, lens, stream=9)
+    used = {c[2].workspace for c in fake.calls}
+    assert len(used) == 3
+    fake.calls.clear()
+    fake.sync_code = code
+    if code == N.VK_OK:
+        cache.sync()
+    else:
+        with pytest.raises(N.VkError) as e:
+            cache.sync()
+        assert e.value.code == code
+    if code != N.VK_ERR_DEVICE:
+        assert not fake.calls
+        return
+    assert {c[1] for c in fake.calls if c[0] == "clear"} == used, "memory whose flags may be anything stays in use"
+    for i, c in enumerate(fake.calls):  # no call that is under way may still use it
+        assert c[0] != "clear" or fake.calls[i - 1][0] == "synchronize"
+    fake.calls.clear()
+    cache.attend(q, offsets, table, lens, stream=9)
+    assert fake.calls[0][2].workspace in used
+
+
 def test_workspace_entries_refuse_null():
+    assert N.lib().vk_kv_workspace_clear(0, None) == N.VK_ERR_INVALID and "workspace" in N.last_error()
     assert N.lib().vk_kv_workspace_create(0, 1 << 20, None) == N.VK_ERR_INVALID and "out" in N.last_error()
     assert N.lib().vk_kv_workspace_destroy(0, None) == N.VK_OK

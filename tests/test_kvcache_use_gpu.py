@@ -176,3 +176,42 @@ def test_threads_with_a_stream_each():
         t.join()
     c.cache.sync()
     assert not wrong
+
+
+def test_working_memory_that_a_wait_has_left_unfinished():
+    """A call whose wait ran out leaves its mark and any flags in the stream's working memory (both are set here by hand).
+    Later calls with it report that they are void, of another cache too; sync clears it, and nothing sticks."""
+    import torch
+
+    from veckern_b200 import _native as N
+    from veckern_b200 import kvcache
+
+    a, b = (Cache([9000, 5000, 700], 32, 2, 128, seed=21 + i) for i in range(2))
+    st = torch.cuda.Stream()
+    for c in (a, b):
+        c.made = call(c, CHUNK)
+        c.want = c.cache.attend(*c.made[:2], c.table, c.lens)
+        c.cache.sync()
+    st.wait_stream(torch.cuda.current_stream())
+    a.cache.attend(*a.made[:2], a.table, a.lens, stream=st)
+    a.cache.sync(st)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        captured = a.cache.attend(*a.made[:2], a.table, a.lens)
+    flags = kvcache._WORK[(0, st.cuda_stream)]._memory[:kvcache._ZEROED].view(torch.int32)
+    assert not flags.any()
+    flags[:16] = 1
+    flags[-2] = 1
+    torch.cuda.synchronize()
+    a.cache.sync(st)  # of cache a nothing is void yet
+    b.cache.attend(*b.made[:2], b.table, b.lens, stream=st)
+    with pytest.raises(N.VkError, match="workspace") as e:
+        b.cache.sync(st)
+    assert e.value.code == N.VK_ERR_DEVICE and not flags.any()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(captured, a.want))
+    for c in (a, b):
+        got = c.cache.attend(*c.made[:2], c.table, c.lens, stream=st)
+        c.cache.sync(st)
+        assert all(torch.equal(x, y) for x, y in zip(got, c.want))

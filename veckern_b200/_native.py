@@ -137,6 +137,7 @@ ABI = {
     "vk_kv_attend": (C.c_int, [_vp, _vp, _vp, _vp]),
     "vk_kv_attend_workspace": (C.c_int, [_vp, _vp, _vp, C.POINTER(C.c_size_t)]),
     "vk_kv_workspace_create": (C.c_int, [C.c_int, C.c_size_t, C.POINTER(_vp)]),
+    "vk_kv_workspace_clear": (C.c_int, [C.c_int, _vp]),
     "vk_kv_workspace_destroy": (C.c_int, [C.c_int, _vp]),
     "vk_kv_evict": (C.c_int, [_vp, _vp, _vp, _vp]),
     "vk_ivf_create": (C.c_int, [C.c_int, _vp, C.c_int, C.c_int, _vp, _i64, _vp, C.c_int, _vp, C.POINTER(_vp)]),

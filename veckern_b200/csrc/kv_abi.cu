@@ -83,7 +83,7 @@ struct AttendPlan {
     bool step;
     int rows, s_rows;  // of the step path, rounded up to 8 or 16; to 4, 8 or 16
     int ctas;
-    size_t ready, started, o, ml, s, bytes;  // offsets
+    size_t ready, started, bad, o, ml, s, bytes;  // offsets
 };
 
 AttendPlan plan_attend(const vk_kv* kv, const vk::KvBatch& bt, int group, int max_q, bool scores) {
@@ -98,6 +98,7 @@ AttendPlan plan_attend(const vk_kv* kv, const vk::KvBatch& bt, int group, int ma
     // What has to be zero before a call lies at the start, whatever the sizes.
     const size_t rows_of_parts = (size_t)p.ctas * (p.step ? vk::STEP_ROWS : 2 * vk::CHUNK_ROWS);
     p.started = VK_KV_WORKSPACE_ZEROED - sizeof(uint32_t);
+    p.bad = p.started - sizeof(uint32_t);
     p.o = VK_KV_WORKSPACE_ZEROED;
     p.ml = p.o + align256(rows_of_parts * dp * sizeof(float));
     p.s = p.ml + align256(rows_of_parts * sizeof(float2));
@@ -257,6 +258,7 @@ int launch_attend(const vk_kv* kv, const vk::KvBatch& bt, const vk::KvAttend& a,
     vk::KvParts parts{};
     parts.ready = reinterpret_cast<uint32_t*>(w + p.ready);
     parts.started = reinterpret_cast<uint32_t*>(w + p.started);
+    parts.bad = reinterpret_cast<uint32_t*>(w + p.bad);
     parts.o = reinterpret_cast<float*>(w + p.o);
     parts.ml = reinterpret_cast<float2*>(w + p.ml);
     parts.s = reinterpret_cast<float*>(w + p.s);
@@ -355,15 +357,19 @@ int vk_kv_destroy(vk_kv_t* kv) {
 int vk_kv_sync(vk_kv_t* kv, void* stream) {
     if (!kv) return fail(VK_ERR_INVALID, "cache must not be NULL");
     DeviceGuard guard(kv->desc.device);
+    if (guard.err != cudaSuccess) return fail(VK_ERR_CUDA, "cudaSetDevice: %s", cudaGetErrorString(guard.err));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     int status = 0;
     VK_TRY_CUDA(cudaMemcpyAsync(&status, kv->status, sizeof(int), cudaMemcpyDeviceToHost, st));
     VK_TRY_CUDA(cudaStreamSynchronize(st));
     if (!status) return VK_OK;
-    VK_TRY_CUDA(cudaMemsetAsync(kv->status, 0, sizeof(int), st));
+    vk::kv_reported_kernel<<<1, 1, 0, st>>>(kv->status, status);
+    VK_TRY_CUDA(cudaGetLastError());
     VK_TRY_CUDA(cudaStreamSynchronize(st));
     if (status & (vk::ERR_WAIT_TIMEOUT | vk::ERR_DRAIN_TIMEOUT))
         return fail(VK_ERR_DEVICE, "a bounded wait ran out in a cache kernel (status %d)", status);
+    if (status & vk::ERR_WORKSPACE)
+        return fail(VK_ERR_DEVICE, "a call's workspace was not cleared after a bounded wait had run out in another call");
     return fail(VK_ERR_INVALID, "a page number, length or offset was out of range; the slots it names were left out");
 }
 
@@ -459,6 +465,14 @@ int vk_kv_workspace_create(int device, size_t bytes, void** out) {
     }
     *out = p;
     return VK_OK;
+}
+
+int vk_kv_workspace_clear(int device, void* workspace) {
+    if (!workspace) return fail(VK_ERR_INVALID, "workspace must not be NULL");
+    DeviceGuard guard(device);
+    if (guard.err != cudaSuccess) return fail(VK_ERR_CUDA, "cudaSetDevice: %s", cudaGetErrorString(guard.err));
+    BesideCapture beside;
+    return clear_workspace(workspace);
 }
 
 int vk_kv_workspace_destroy(int device, void* workspace) {

@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     tmem_fence_after();
     const uint32_t tm = __shfl_sync(FULL, *tmem_at, 0);
-    KvWait wait{c.status};
+    KvWait wait{c.status, parts.bad};
     ChunkWalk walk{c, bt, shape, share, 0, 0, 0, false};
     ChunkSegment g;
     // 384 threads start with 168 registers: 2 x 128 x 200 + 128 x 104 is the same sum

@@ -11,6 +11,8 @@
 
 namespace vk {
 
+enum : int { ERR_WORKSPACE = 8 };  // status bit: the call's workspace is one that a wait that ran out has left as it was
+
 struct KvPages {
     uint16_t* k;  // elements of the cache's 16-bit type
     uint16_t* v;

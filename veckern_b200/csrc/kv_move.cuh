@@ -6,6 +6,9 @@
 
 namespace vk {
 
+// Takes the reported bits out of the status word and no others: a kernel of another stream may set some meanwhile.
+__global__ void kv_reported_kernel(int* status, int bits) { atomicAnd(status, ~bits); }
+
 // One thread per 16 bytes of a new token's head. Every byte is read and written once: bound by memory (9 prompts of up to
 // 2,011 tokens, 8 kv heads of 128, 104 MB: 18.5 us, 5.6 TB/s), by the launch for a step's few tokens (2.4 us).
 __global__ void __launch_bounds__(256) kv_append_kernel(KvPages c, KvBatch bt, const uint16_t* k, const uint16_t* v,

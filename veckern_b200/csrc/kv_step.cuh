@@ -39,6 +39,7 @@ constexpr long long KV_WAIT_BUDGET = 4000000000LL;  // cycles: about two seconds
 struct KvParts {
     uint32_t* ready;
     uint32_t* started;  // CTAs of the running kernel that have begun; the last one makes it zero again
+    uint32_t* bad;      // not zero: a wait ran out in a call with this workspace, so that the flags may be anything
     float* o;    // [part]: unnormalised sums
     float2* ml;  // [part][row]: maximum (base 2) and sum
     float* s;    // [sequence][kv head][slot][s_rows]: scaled scores (base 2) of the step path, for the weights
@@ -94,16 +95,20 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 }
 
 // Bounded waits of one thread or warp: after the first that runs out, the later ones return at once, so that the CTA
-// unwinds; what it computes then is void and the status word says so. Called by whole warps, which leave it together: what
-// follows is often an instruction that all lanes have to execute as one.
+// unwinds; what it computes then is void and the status word says so. The workspace is marked too: later calls with it, of
+// other caches as well, report that theirs is void until it has been cleared. Called by whole warps, which leave it
+// together: what follows is often an instruction that all lanes have to execute as one.
 struct KvWait {
     int* status;
+    uint32_t* bad;
     bool dead = false;
+    __device__ __forceinline__ void ran_out() {
+        dead = true;
+        atomicOr(status, ERR_WAIT_TIMEOUT);
+        *reinterpret_cast<volatile uint32_t*>(bad) = 1u;
+    }
     __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t parity) {
-        if (!mbar_try_wait(bar, parity) && !dead && !mbar_wait_bounded(bar, parity, KV_WAIT_BUDGET)) {
-            dead = true;
-            atomicOr(status, ERR_WAIT_TIMEOUT);
-        }
+        if (!mbar_try_wait(bar, parity) && !dead && !mbar_wait_bounded(bar, parity, KV_WAIT_BUDGET)) ran_out();
         __syncwarp();
     }
 };
@@ -119,10 +124,7 @@ __device__ __forceinline__ void part_await(const KvParts& parts, int i, KvWait& 
     while (!wait.dead) {
         asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(there) : "l"(parts.ready + i) : "memory");
         if (there) break;
-        if (clock64() - t0 > KV_WAIT_BUDGET) {
-            wait.dead = true;
-            atomicOr(wait.status, ERR_WAIT_TIMEOUT);
-        }
+        if (clock64() - t0 > KV_WAIT_BUDGET) wait.ran_out();
     }
 }
 __device__ __forceinline__ float part_factor(float m, float top) { return m == -INFINITY ? 0.f : ex2(m - top); }
@@ -194,7 +196,10 @@ __device__ __forceinline__ KvShare kv_share(const KvPages& c, const KvBatch& bt,
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     constexpr int WARPS = THREADS / 32, PLACE = KV_SHARE_SCRATCH - 1;
     static_assert(2 * WARPS + 2 <= PLACE, "scratch");
-    if (t == THREADS - 1) scratch[PLACE] = (int)atomicInc(parts.started, gridDim.x - 1);  // beside the others' loads
+    if (t == THREADS - 1) {  // beside the others' loads
+        scratch[PLACE] = (int)atomicInc(parts.started, gridDim.x - 1);
+        if (*reinterpret_cast<const volatile uint32_t*>(parts.bad)) atomicOr(c.status, ERR_WORKSPACE);
+    }
     const int span = (bt.batch + THREADS - 1) / THREADS;
     const int b0 = min(bt.batch, t * span), b1 = min(bt.batch, b0 + span);
     int sum = 0, longest = 0;
@@ -298,7 +303,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
     };
     KvShare share = kv_share<STEP_THREADS>(c, bt, parts, scratch, STEP_PART_COST, units_of);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    KvWait wait{c.status};
+    KvWait wait{c.status, parts.bad};
     int stage = 0;
     uint32_t phase = 0;
     const int box_shift = min(c.page_shift, 6), boxes = STEP_TILE >> box_shift;

@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(WEIGHTS_THREADS, 1)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     tmem_fence_after();
     const uint32_t tm = __shfl_sync(FULL, *tmem_at, 0);
-    KvWait wait{c.status};
+    KvWait wait{c.status, parts.bad};
     WeightsWalk walk{c, bt, shape, share, 0, 0, 0, false};
     WeightsSegment g;
     if (warp == 17) {

@@ -33,7 +33,7 @@ assert [x.size for x in (_BATCH, _ATTEND, _EVICT)] == [C.sizeof(x) for x in (N.K
 # Attention's working memory by (device, stream): the calls of a stream share it, one at a time; it grows, and its start is
 # zero between calls. What was outgrown is kept: a captured graph may hold its address.
 _WORK: dict = {}
-_OUTGROWN: list = []
+_OUTGROWN: list = []  # (device, working memory)
 _GROWING = threading.Lock()
 _ZEROED = 8192  # VK_KV_WORKSPACE_ZEROED
 
@@ -66,10 +66,22 @@ def _workspace(torch, device, stream: int, need: int) -> _Work:
         if work is not None:
             if work.size >= need:  # another thread was here first
                 return work
-            _OUTGROWN.append(work)
+            _OUTGROWN.append((device.index, work))
             need = max(need, work.size * 3 // 2)
         work = _WORK[key] = _Work(torch, device, stream, need)
     return work
+
+
+def _clear_all(torch, device) -> None:
+    """Clears the device's working memory after a wait ran out: the call may have been on any stream, and captured graphs
+    hold what was outgrown."""
+    with _GROWING:
+        works = [(key[0], work) for key, work in _WORK.items()] + _OUTGROWN
+        for index, work in works:
+            if index == device.index:
+                with work.lock:
+                    torch.cuda.synchronize(device)
+                    check(lib().vk_kv_workspace_clear(index, work.at), "sync (clearing working memory)")
 
 
 _DTYPES = {"torch.float16": N.VK_KV_F16, "torch.bfloat16": N.VK_KV_BF16}
@@ -263,13 +275,15 @@ class PagedCache:
         return seq, head
 
     def sync(self, stream=None) -> None:
-        """Waits for the cache's work on the stream and raises VkError for anything its kernels found wrong."""
-        s = self._stream(stream)
+        """Waits for the cache's work on the stream and raises VkError for anything its kernels found wrong, on other streams
+        too. With the code VK_ERR_DEVICE a bounded wait ran out: what attend gave since the last sync is void, and so is
+        what other caches' calls on the stream gave (their sync says so). The device's working memory is then cleared; no
+        graph with a captured attend may be running."""
         try:
-            check(lib().vk_kv_sync(self._h, s), "sync")
+            check(lib().vk_kv_sync(self._h, self._stream(stream)), "sync")
         except VkError as e:
-            if e.code == N.VK_ERR_DEVICE:  # an aborted call may have left the working memory's start in any state
-                _WORK.pop((self.device.index, s), None)
+            if e.code == N.VK_ERR_DEVICE:
+                _clear_all(self._torch, self.device)
             raise
 
     def close(self) -> None:
