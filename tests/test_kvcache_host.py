@@ -311,3 +311,15 @@ def test_workspace_entries_refuse_null():
     assert N.lib().vk_kv_workspace_clear(0, None) == N.VK_ERR_INVALID and "workspace" in N.last_error()
     assert N.lib().vk_kv_workspace_create(0, 1 << 20, None) == N.VK_ERR_INVALID and "out" in N.last_error()
     assert N.lib().vk_kv_workspace_destroy(0, None) == N.VK_OK
+
+
+def test_kernels_do_not_read_through_the_read_only_path():
+    """They start while the kernel before them runs; that path, and hoisting its loads over the wait, is for memory that
+    nobody writes while a kernel lives."""
+    from pathlib import Path
+
+    found = {}
+    for f in (Path(kvcache.__file__).parent / "csrc").glob("kv_*.cu*"):
+        lines = [x.split("//")[0] for x in f.read_text().splitlines()]
+        found[f.name] = [x for x in lines if "__ldg" in x or "ld.global.nc" in x or "__restrict__" in x]
+    assert found and not any(found.values()), found

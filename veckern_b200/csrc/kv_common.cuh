@@ -3,6 +3,11 @@
 //
 // What a call reads from device memory (offsets, lengths, page numbers) is never trusted: a sequence's bounds are
 // clamped to the call's sizes and a page number outside the cache is not followed. Both set ERR_LAYOUT.
+//
+// These kernels start while the kernel before them on the stream still runs, and wait for its results inside. What that one
+// may have written (anything: lengths from an eviction, rows from an attention, scores, lse) must not be read through the
+// read-only path, which is for memory that nobody writes while the kernel lives: __ldca, which stays behind the wait, and no
+// __ldg.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -39,34 +44,43 @@ struct KvSeq {
     int len;        // slots, new tokens included
 };
 
-__device__ __forceinline__ int kv_len(const KvPages& c, const KvBatch& bt, int b) {
+// The checks come behind all loads, which then wait for one another's latency only.
+__device__ __forceinline__ int kv_len_checked(const KvPages& c, const KvBatch& bt, int len) {
     const int64_t most = (int64_t)bt.width << c.page_shift;
-    int len = __ldg(bt.lens + b);
     if (len < 0 || len > most) {
         atomicOr(c.status, ERR_LAYOUT);
         len = len < 0 ? 0 : (int)most;
     }
     return len;
 }
+__device__ __forceinline__ int kv_len(const KvPages& c, const KvBatch& bt, int b) {
+    return kv_len_checked(c, bt, __ldca(bt.lens + b));
+}
 
 __device__ __forceinline__ KvSeq kv_seq(const KvPages& c, const KvBatch& bt, int b) {
-    int64_t lo = __ldg(bt.offsets + b), hi = __ldg(bt.offsets + b + 1);
+    int64_t lo = __ldca(bt.offsets + b), hi = __ldca(bt.offsets + b + 1);
+    const int len = __ldca(bt.lens + b);
     if (lo < 0 || hi < lo || hi > bt.tokens) {
         atomicOr(c.status, ERR_LAYOUT);
         lo = min(max(lo, int64_t(0)), bt.tokens);
         hi = min(max(hi, lo), bt.tokens);
     }
-    return {lo, (int)(hi - lo), kv_len(c, bt, b)};
+    return {lo, (int)(hi - lo), kv_len_checked(c, bt, len)};
 }
 
-// The page of a slot of sequence b (slot < its length), or -1.
-__device__ __forceinline__ int64_t kv_page(const KvPages& c, const int32_t* table, int slot) {
-    const int page = __ldg(table + (slot >> c.page_shift));
+// The table's entry for a slot (slot < the sequence's length), and the page that it names, or -1.
+__device__ __forceinline__ int kv_entry(const KvPages& c, const int32_t* table, int slot) {
+    return __ldca(table + (slot >> c.page_shift));
+}
+__device__ __forceinline__ int64_t kv_page_checked(const KvPages& c, int page) {
     if ((uint64_t)(int64_t)page >= (uint64_t)c.pages) {
         atomicOr(c.status, ERR_LAYOUT);
         return -1;
     }
     return page;
+}
+__device__ __forceinline__ int64_t kv_page(const KvPages& c, const int32_t* table, int slot) {
+    return kv_page_checked(c, kv_entry(c, table, slot));
 }
 
 template <typename T>
@@ -85,7 +99,7 @@ __device__ __forceinline__ int kv_find(const KvBatch& bt, int64_t row) {
     int lo = 0, hi = bt.batch - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (__ldg(bt.offsets + mid) <= row) lo = mid;
+        if (__ldca(bt.offsets + mid) <= row) lo = mid;
         else hi = mid - 1;
     }
     return lo;

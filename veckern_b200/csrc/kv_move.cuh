@@ -33,8 +33,8 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvPages c, KvBatch bt, c
         const int64_t page = kv_page(c, bt.table + b * bt.table_stride, slot);
         if (page < 0) continue;
         const int in = slot & ((1 << c.page_shift) - 1);
-        const uint4 kk = __ldg(reinterpret_cast<const uint4*>(k + tok * k_tok + head * k_head) + part);
-        const uint4 vv = __ldg(reinterpret_cast<const uint4*>(v + tok * v_tok + head * v_head) + part);
+        const uint4 kk = __ldca(reinterpret_cast<const uint4*>(k + tok * k_tok + head * k_head) + part);
+        const uint4 vv = __ldca(reinterpret_cast<const uint4*>(v + tok * v_tok + head * v_head) + part);
         reinterpret_cast<uint4*>(c.k + page * c.ks[0] + in * c.ks[1] + head * c.ks[2])[part] = kk;
         reinterpret_cast<uint4*>(c.v + page * c.vs[0] + in * c.vs[1] + head * c.vs[2])[part] = vv;
     }
@@ -102,20 +102,28 @@ __global__ void __launch_bounds__(SELECT_THREADS, 2) kv_select_kernel(KvPages c,
     const float* sc = e.scores + b * e.ss[0] + head * e.ss[1];
     int32_t* kept = e.kept + ((int64_t)b * c.heads + head) * e.keep;
     float* ns = e.new_scores + ((int64_t)b * c.heads + head) * e.width;
-    auto score = [&](int64_t slot) { return slot < e.width ? __ldg(sc + slot) : 0.0f; };
+    auto score = [&](int64_t slot) { return slot < e.width ? __ldca(sc + slot) : 0.0f; };
     if (head == 0 && rank == 0 && tid == 0) e.new_lens[b] = k;
     const int slice = (cand + C - 1) / C, from = min(cand, rank * slice), size = min(cand, from + slice) - from;
     const bool fits = slice <= SELECT_HELD;
     for (int i = tid; i < 3 * SELECT_BINS; i += SELECT_THREADS) hist[i] = 0;
-    if (fits)
+    if (fits) {
+        // of the slice, slots that have a score; the loads behind them are of the last one again, so that none of a batch
+        // waits for a branch
+        const int have = (int)min((int64_t)size, max(e.width - from, int64_t(0)));
+        const float* mine = sc + from;
         for (int i0 = tid; i0 < size; i0 += 8 * SELECT_THREADS) {
-            float x[8];
+            float x[8] = {};
+            if (have > 0)
 #pragma unroll
-            for (int u = 0; u < 8; ++u) x[u] = score((int64_t)from + i0 + u * SELECT_THREADS);
+                for (int u = 0; u < 8; ++u) x[u] = __ldca(mine + min(i0 + u * SELECT_THREADS, have - 1));
 #pragma unroll
-            for (int u = 0; u < 8; ++u)
-                if (i0 + u * SELECT_THREADS < size) held[i0 + u * SELECT_THREADS] = kv_rank(x[u]);
+            for (int u = 0; u < 8; ++u) {
+                const int i = i0 + u * SELECT_THREADS;
+                if (i < size) held[i] = kv_rank(i < have ? x[u] : 0.0f);
+            }
         }
+    }
     __syncthreads();
     auto cluster_sync = [&] {
         if constexpr (C > 1) cluster.sync();
@@ -291,12 +299,14 @@ __global__ void __launch_bounds__(256) kv_compact_kernel(KvPages c, KvBatch bt, 
             atomicOr(c.status, ERR_LAYOUT);
             continue;
         }
-        const int from = kept[to];
-        const int64_t p0 = kv_page(c, bt.table + b * bt.table_stride, from);
-        const int64_t p1 = kv_page(c, e.new_table + b * e.new_stride, to);
+        const int from = __ldca(kept + to), entry1 = kv_entry(c, e.new_table + b * e.new_stride, to);
+        const int entry0 = kv_entry(c, bt.table + b * bt.table_stride, from);
+        const int64_t p0 = kv_page_checked(c, entry0), p1 = kv_page_checked(c, entry1);
         if (p0 < 0 || p1 < 0) continue;
-        const uint4 kk = reinterpret_cast<const uint4*>(c.k + p0 * c.ks[0] + (from & in) * c.ks[1] + head * c.ks[2])[part];
-        const uint4 vv = reinterpret_cast<const uint4*>(c.v + p0 * c.vs[0] + (from & in) * c.vs[1] + head * c.vs[2])[part];
+        const uint4 kk =
+            __ldca(reinterpret_cast<const uint4*>(c.k + p0 * c.ks[0] + (from & in) * c.ks[1] + head * c.ks[2]) + part);
+        const uint4 vv =
+            __ldca(reinterpret_cast<const uint4*>(c.v + p0 * c.vs[0] + (from & in) * c.vs[1] + head * c.vs[2]) + part);
         reinterpret_cast<uint4*>(c.k + p1 * c.ks[0] + (to & in) * c.ks[1] + head * c.ks[2])[part] = kk;
         reinterpret_cast<uint4*>(c.v + p1 * c.vs[0] + (to & in) * c.vs[1] + head * c.vs[2])[part] = vv;
     }

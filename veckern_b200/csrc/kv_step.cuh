@@ -356,7 +356,8 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const int d = 16 * k + 8 * e + q2;
-                        q[k][u + 2 * e] = live && d < c.dim ? __ldg(reinterpret_cast<const unsigned int*>(row + d)) : 0u;
+                        const uint32_t x = __ldca(reinterpret_cast<const unsigned int*>(row + (d < c.dim ? d : 0)));
+                        q[k][u + 2 * e] = live && d < c.dim ? x : 0u;
                     }
             }
             const float scale = a.scale * 1.4426950408889634f;
@@ -594,7 +595,7 @@ __global__ void __launch_bounds__(256) kv_step_weights_kernel(KvPages c, KvBatch
             const int64_t j = min(j0 + u * 256, end - 1);
             before[u] = out[j];
 #pragma unroll
-            for (int i = 0; i < R / 4; ++i) x[u][i] = __ldg(sp + j * (R / 4) + i);
+            for (int i = 0; i < R / 4; ++i) x[u][i] = __ldca(sp + j * (R / 4) + i);
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u) {

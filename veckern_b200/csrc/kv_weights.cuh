@@ -261,7 +261,7 @@ __global__ void __launch_bounds__(WEIGHTS_THREADS, 1)
             auto minus_lse = [&](int q) {
                 const int token = q * shape.tokens + row_token;
                 if (row >= shape.tokens * a.group || token >= g.s.count) return -INFINITY;
-                const float v = __ldg(a.lse + (g.s.first + token) * a.heads + g.head * a.group + row - row_token * a.group);
+                const float v = __ldca(a.lse + (g.s.first + token) * a.heads + g.head * a.group + row - row_token * a.group);
                 return v == -INFINITY ? -INFINITY : -v * 1.4426950408889634f;
             };
             Pair sum[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
