@@ -354,6 +354,9 @@ int vk_kv_destroy(vk_kv_t* kv);
 /* Waits for the cache's work on `stream` and reports any kernel-side error (and clears it). A cache has one status word:
  * with calls on several streams, an error may be reported by the first vk_kv_sync of any of them. */
 int vk_kv_sync(vk_kv_t* kv, void* stream);
+/* The limit of a wait inside the kernels of vk_kv_attend calls from here on, in SM cycles, 4e9 (about two seconds) at most;
+ * 0 is that again. One that runs out ends the call early: its results are void, and vk_kv_sync returns VK_ERR_DEVICE. */
+int vk_kv_wait_limit(vk_kv_t* kv, int64_t cycles);
 
 /* New token t of sequence b, of T, goes to slot lens[b] - T + t. Element (token, head, i) of the new keys is
  * k[token * k_stride[0] + head * k_stride[1] + i] (strides in elements, multiples of 8; bases 16-byte aligned). */

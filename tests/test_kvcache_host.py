@@ -311,6 +311,7 @@ def test_workspace_entries_refuse_null():
     assert N.lib().vk_kv_workspace_clear(0, None) == N.VK_ERR_INVALID and "workspace" in N.last_error()
     assert N.lib().vk_kv_workspace_create(0, 1 << 20, None) == N.VK_ERR_INVALID and "out" in N.last_error()
     assert N.lib().vk_kv_workspace_destroy(0, None) == N.VK_OK
+    assert N.lib().vk_kv_wait_limit(None, 5) == N.VK_ERR_INVALID and "cache" in N.last_error()
 
 
 def test_kernels_do_not_read_through_the_read_only_path():

@@ -215,3 +215,30 @@ def test_working_memory_that_a_wait_has_left_unfinished():
         got = c.cache.attend(*c.made[:2], c.table, c.lens, stream=st)
         c.cache.sync(st)
         assert all(torch.equal(x, y) for x, y in zip(got, c.want))
+
+
+@pytest.mark.parametrize("counts", [STEP, CHUNK])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_waits_that_run_out(counts, dim):
+    """With a limit of one cycle the first wait for a copy runs out: the call ends at once, what it had in flight has landed
+    when it does, sync says so, and the next call with the usual limit is right."""
+    import torch
+
+    from veckern_b200 import _native as N
+
+    c = Cache([9000, 5000, 700], 32, 2, dim, seed=31)
+    q, off, s0 = call(c, counts)
+    want, want_lse = c.cache.attend(q, off, c.table, c.lens, scores=s0, max_q=max(counts))
+    c.cache.sync()
+    for _ in range(3):
+        assert N.lib().vk_kv_wait_limit(c.cache._h, 1) == N.VK_OK
+        c.cache.attend(q, off, c.table, c.lens, scores=torch.zeros_like(s0), max_q=max(counts))
+        with pytest.raises(N.VkError, match=r"wait ran out.*status (1|9)\)") as e:
+            c.cache.sync()
+        assert e.value.code == N.VK_ERR_DEVICE
+        assert N.lib().vk_kv_wait_limit(c.cache._h, 0) == N.VK_OK
+        s = torch.zeros_like(s0)
+        out, lse = c.cache.attend(q, off, c.table, c.lens, scores=s, max_q=max(counts))
+        c.cache.sync()
+        assert torch.equal(out, want) and torch.equal(lse, want_lse) and torch.equal(s, s0)
+    assert N.lib().vk_kv_wait_limit(c.cache._h, -1) == N.VK_ERR_INVALID

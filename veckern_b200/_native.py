@@ -133,6 +133,7 @@ ABI = {
     "vk_kv_create": (C.c_int, [C.POINTER(KvDesc), C.POINTER(_vp)]),
     "vk_kv_destroy": (C.c_int, [_vp]),
     "vk_kv_sync": (C.c_int, [_vp, _vp]),
+    "vk_kv_wait_limit": (C.c_int, [_vp, _i64]),
     "vk_kv_append": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "vk_kv_attend": (C.c_int, [_vp, _vp, _vp, _vp]),
     "vk_kv_attend_workspace": (C.c_int, [_vp, _vp, _vp, C.POINTER(C.c_size_t)]),

@@ -14,6 +14,7 @@ struct vk_kv {
     int page_shift = 0;
     int sm_count = 0;
     int* status = nullptr;
+    std::atomic<int64_t> wait_limit{vk::KV_WAIT_LIMIT};
     CUtensorMap map_k, map_v;
     ~vk_kv() {
         if (status) cudaFree(status);
@@ -373,6 +374,13 @@ int vk_kv_sync(vk_kv_t* kv, void* stream) {
     return fail(VK_ERR_INVALID, "a page number, length or offset was out of range; the slots it names were left out");
 }
 
+int vk_kv_wait_limit(vk_kv_t* kv, int64_t cycles) {
+    if (!kv) return fail(VK_ERR_INVALID, "cache must not be NULL");
+    if (cycles < 0) return fail(VK_ERR_INVALID, "cycles must be >= 0");
+    kv->wait_limit.store(cycles ? std::min<int64_t>(cycles, vk::KV_WAIT_LIMIT) : vk::KV_WAIT_LIMIT, std::memory_order_relaxed);
+    return VK_OK;
+}
+
 int vk_kv_append(vk_kv_t* kv, const vk_kv_batch_t* batch, const void* k, const int64_t* k_stride, const void* v,
                  const int64_t* v_stride, void* stream) {
     vk::KvBatch bt{};
@@ -424,6 +432,7 @@ int vk_kv_attend(vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_attend_t* 
     a.max_q = max_q_of(args, bt.tokens);
     a.causal = args->causal != 0;
     a.scale = args->scale;
+    a.wait_limit = kv->wait_limit.load(std::memory_order_relaxed);
     // The kernels count their units of work (tiles and pairs of tiles, of every kv head) in 32 bits.
     const int64_t tiles = ceil_div((int64_t)bt.width << kv->page_shift, vk::STEP_TILE) + 1;
     if (tiles * g * ((double)bt.tokens * a.group / vk::CHUNK_ROWS + 2.0 * bt.batch) >= 2147483648.0)

@@ -273,7 +273,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     uint64_t* s_full = q_empty + 1;  // [tile]
     uint64_t* p_full = s_full + 2;
     uint64_t* o_full = p_full + 2;
-    int* scratch = reinterpret_cast<int*>(o_full + 2);
+    uint64_t* mma_done = o_full + 2;
+    int* scratch = reinterpret_cast<int*>(mma_done + 1);
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(scratch + KV_SHARE_SCRATCH);
     const int warp = __shfl_sync(FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -286,6 +287,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         }
         mbar_init(q_full, 1);
         mbar_init(q_empty, 1);
+        mbar_init(mma_done, 1);
         for (int i = 0; i < 2; ++i) {
             mbar_init(s_full + i, 1);
             mbar_init(p_full + i, 4);
@@ -315,7 +317,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     tmem_fence_after();
     const uint32_t tm = __shfl_sync(FULL, *tmem_at, 0);
-    KvWait wait{c.status, parts.bad};
+    KvWait wait{c.status, parts.bad, scratch + KV_SHARE_OVER, a.wait_limit};
     ChunkWalk walk{c, bt, shape, share, 0, 0, 0, false};
     ChunkSegment g;
     // 384 threads start with 168 registers: 2 x 128 x 200 + 128 x 104 is the same sum
@@ -326,13 +328,16 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         auto at = [&](int n) { return n % RING; };
         auto parity = [&](int n) -> uint32_t { return n / RING & 1; };
         if (warp == 9) {
-            uint32_t q_phase = 0;
+            int q_fills = 0;
+            bool over = false;
             const int box_shift = min(c.page_shift, 6);
             const int boxes = CHUNK_SLOTS >> box_shift;
             const uint32_t me = elect_lane();
-            while (walk.next(&g)) {
-                wait(q_empty, q_phase ^ 1);
-                q_phase ^= 1;
+            while (!over && walk.next(&g)) {
+                wait(q_empty, (q_fills & 1) ^ 1);
+                over = wait.given_up();
+                if (over) break;
+                ++q_fills;
                 if (lane == 0) {
                     const int n = g.lone ? 1 : 2;
                     mbar_arrive_expect_tx(q_full, n * HALVES * shape.tokens * a.group * 128);
@@ -343,13 +348,15 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                 }
                 const int32_t* table = bt.table + g.b * bt.table_stride;
                 const int per = g.lone ? 2 : 1;
-                for (int t = g.t0 * per; t < (g.t0 + g.count) * per; ++t) {
+                for (int t = g.t0 * per; t < (g.t0 + g.count) * per && !over; ++t) {
                     const TilePages tp = tile_pages(c, table, t * CHUNK_SLOTS, boxes, box_shift, g.s.len);
                     // rolled: this warp's registers are few, and what it spills the other one waits for
 #pragma unroll 1
                     for (int side = 0; side < 2; ++side, ++fill) {
                         const int slot = at(fill);
                         wait(kv_empty + slot, parity(fill) ^ 1);
+                        over = wait.given_up();
+                        if (over) break;
                         if (lane == 0) mbar_arrive_expect_tx(kv_full + slot, tp.count * HALVES * (128 << box_shift));
                         __syncwarp();
                         uint8_t* dst = ring + slot * SLOT;
@@ -365,11 +372,10 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                     }
                 }
             }
-            // A wait that ran out may have left copies in flight into this CTA's memory: see them land before it ends.
-            if (wait.dead && lane == 0)
-                for (int k = max(0, fill - RING); k < fill; ++k)
-                    if (!mbar_wait_bounded(kv_full + at(k), parity(k), 2 * KV_WAIT_BUDGET))
-                        atomicOr(c.status, ERR_DRAIN_TIMEOUT);
+            if (lane == 0) {
+                wait.drain(q_full, q_fills);
+                for (int i = 0; i < RING; ++i) wait.drain(kv_full + i, fill / RING + (i < fill % RING));
+            }
         } else if (warp == 8) {
             uint32_t q_phase = 0, p_phase = 0;  // p_phase: bit per tile
             const uint32_t me = elect_lane();
@@ -447,6 +453,8 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                 }
                 fill += count * step;
             }
+            umma_commit(mma_done, me);
+            if (lane == 0) wait.drain(mma_done, 1);
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");

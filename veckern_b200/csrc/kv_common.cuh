@@ -140,6 +140,7 @@ struct KvAttend {
     int max_q;
     int causal;
     float scale;
+    long long wait_limit;  // cycles
 };
 
 }  // namespace vk

@@ -31,7 +31,8 @@ constexpr int STEP_ROWS = 16;  // most rows of a sequence's kv head
 constexpr int STEP_WARPS = 4;  // consumers; one more warp loads
 constexpr int STEP_THREADS = 32 * (STEP_WARPS + 1);
 constexpr int STEP_RING = 96 * 1024;  // bytes in flight per CTA; two CTAs share an SM
-constexpr long long KV_WAIT_BUDGET = 4000000000LL;  // cycles: about two seconds
+constexpr long long KV_WAIT_LIMIT = 4000000000LL;         // cycles: about two seconds
+constexpr long long KV_DRAIN_LIMIT = 2 * KV_WAIT_LIMIT;  // of a wait for what is in flight when a CTA gives up
 
 // What a call keeps in its workspace. A CTA leaves at most one part of each of its row tiles: of its first segment, when
 // that does not begin its (sequence, kv head, rows); ready[part] tells the CTA that waits for it and is zero again when
@@ -98,18 +99,32 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 // unwinds; what it computes then is void and the status word says so. The workspace is marked too: later calls with it, of
 // other caches as well, report that theirs is void until it has been cleared. Called by whole warps, which leave it
 // together: what follows is often an instruction that all lanes have to execute as one.
+//
+// A CTA that gives up starts no more copies, so that a barrier has one fill in flight at most. The warp that starts copies or
+// products waits for its last ones before it ends, whatever the others do: none outlives the CTA.
 struct KvWait {
     int* status;
     uint32_t* bad;
+    int* over;  // shared memory: not zero when a thread of the CTA gave up
+    long long limit;
     bool dead = false;
     __device__ __forceinline__ void ran_out() {
         dead = true;
+        *reinterpret_cast<volatile int*>(over) = 1;
         atomicOr(status, ERR_WAIT_TIMEOUT);
         *reinterpret_cast<volatile uint32_t*>(bad) = 1u;
     }
     __device__ __forceinline__ void operator()(uint64_t* bar, uint32_t parity) {
-        if (!mbar_try_wait(bar, parity) && !dead && !mbar_wait_bounded(bar, parity, KV_WAIT_BUDGET)) ran_out();
+        if (!mbar_try_wait(bar, parity) && !dead && !mbar_wait_bounded(bar, parity, limit)) ran_out();
         __syncwarp();
+    }
+    // Whether a thread of the CTA gave up, the same for the whole warp; who gave up said so before it arrived anywhere.
+    __device__ __forceinline__ bool given_up() const {
+        return __any_sync(FULL, *reinterpret_cast<volatile int*>(over));
+    }
+    // Waits for the last fill of a barrier that has had `fills` of them.
+    __device__ __forceinline__ void drain(uint64_t* bar, int fills) const {
+        if (fills && !mbar_wait_bounded(bar, (fills - 1) & 1, KV_DRAIN_LIMIT)) atomicOr(status, ERR_DRAIN_TIMEOUT);
     }
 };
 
@@ -124,7 +139,7 @@ __device__ __forceinline__ void part_await(const KvParts& parts, int i, KvWait& 
     while (!wait.dead) {
         asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(there) : "l"(parts.ready + i) : "memory");
         if (there) break;
-        if (clock64() - t0 > KV_WAIT_BUDGET) wait.ran_out();
+        if (clock64() - t0 > wait.limit) wait.ran_out();
     }
 }
 __device__ __forceinline__ float part_factor(float m, float top) { return m == -INFINITY ? 0.f : ex2(m - top); }
@@ -184,7 +199,7 @@ struct KvShare {
     }
 };
 
-constexpr int KV_SHARE_SCRATCH = 40;
+constexpr int KV_SHARE_SCRATCH = 40, KV_SHARE_OVER = KV_SHARE_SCRATCH - 1;
 // Count(s, &longest) also raises `longest` to the units of the sequence's longest segment. A segment of L units that is cut
 // every m units takes m of a unit's time and L / m of a part's: least with m = sqrt(L part / unit), which is the least that
 // a CTA gets (part_cost: part / unit), except where all units together are fewer.
@@ -194,8 +209,9 @@ __device__ __forceinline__ KvShare kv_share(const KvPages& c, const KvBatch& bt,
     // scratch: KV_SHARE_SCRATCH values of shared memory. Thread t sums a contiguous range of the sequences. No CTA without a
     // share lies between others: the parts of a cut segment belong to consecutive CTAs.
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    constexpr int WARPS = THREADS / 32, PLACE = KV_SHARE_SCRATCH - 1;
+    constexpr int WARPS = THREADS / 32, PLACE = KV_SHARE_SCRATCH - 2;
     static_assert(2 * WARPS + 2 <= PLACE, "scratch");
+    if (t == 0) scratch[KV_SHARE_OVER] = 0;
     if (t == THREADS - 1) {  // beside the others' loads
         scratch[PLACE] = (int)atomicInc(parts.started, gridDim.x - 1);
         if (*reinterpret_cast<const volatile uint32_t*>(parts.bad)) atomicOr(c.status, ERR_WORKSPACE);
@@ -303,7 +319,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
     };
     KvShare share = kv_share<STEP_THREADS>(c, bt, parts, scratch, STEP_PART_COST, units_of);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    KvWait wait{c.status, parts.bad};
+    KvWait wait{c.status, parts.bad, scratch + KV_SHARE_OVER, a.wait_limit};
     int stage = 0;
     uint32_t phase = 0;
     const int box_shift = min(c.page_shift, 6), boxes = STEP_TILE >> box_shift;
@@ -326,6 +342,10 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
             for (int t = t0; t < t0 + count; ++t) {
                 const TilePages tp = tile_pages(c, table, t * STEP_TILE, boxes, box_shift, s.len);
                 wait(empty + stage, phase ^ 1);
+                if (wait.given_up()) {
+                    share.left = 0;
+                    break;
+                }
                 if (lane == 0) mbar_arrive_expect_tx(full + stage, tp.count * 2 * HALVES * (128 << box_shift));
                 __syncwarp();
                 uint8_t* dst = ring + stage * STAGE;
@@ -552,13 +572,8 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
             for (int i = threadIdx.x; i < follow; i += 32 * STEP_WARPS) parts.ready[share.me + 1 + i] = 0;
         }
     }
-    // A wait that ran out may have left copies in flight into this CTA's memory: see them land before it ends.
-    if (warp == STEP_WARPS && wait.dead && lane == 0)
-        for (int i = 0; i < STAGES; ++i) {
-            const int fills = loaded / STAGES + (i < loaded % STAGES);
-            if (fills && !mbar_wait_bounded(full + i, (fills - 1) & 1, 2 * KV_WAIT_BUDGET))
-                atomicOr(c.status, ERR_DRAIN_TIMEOUT);
-        }
+    if (warp == STEP_WARPS && lane == 0)
+        for (int i = 0; i < STAGES; ++i) wait.drain(full + i, loaded / STAGES + (i < loaded % STAGES));
 }
 
 // Weights that the rows of the step path gave each slot, from the scores that the step kernel left: R of them per slot,

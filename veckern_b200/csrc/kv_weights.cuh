@@ -121,7 +121,8 @@ __global__ void __launch_bounds__(WEIGHTS_THREADS, 1)
     uint64_t* k_empty = k_full + 1;
     uint64_t* s_full = k_empty + 1;  // [slot tile][2]
     uint64_t* s_empty = s_full + 4;
-    int* scratch = reinterpret_cast<int*>(s_empty + 4);
+    uint64_t* mma_done = s_empty + 4;
+    int* scratch = reinterpret_cast<int*>(mma_done + 1);
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(scratch + KV_SHARE_SCRATCH);
     const int warp = __shfl_sync(FULL, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -133,6 +134,7 @@ __global__ void __launch_bounds__(WEIGHTS_THREADS, 1)
         }
         mbar_init(k_full, 1);
         mbar_init(k_empty, 1);
+        mbar_init(mma_done, 1);
         for (int i = 0; i < 4; ++i) {
             mbar_init(s_full + i, 1);
             mbar_init(s_empty + i, 8);
@@ -160,17 +162,21 @@ __global__ void __launch_bounds__(WEIGHTS_THREADS, 1)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     tmem_fence_after();
     const uint32_t tm = __shfl_sync(FULL, *tmem_at, 0);
-    KvWait wait{c.status, parts.bad};
+    KvWait wait{c.status, parts.bad, scratch + KV_SHARE_OVER, a.wait_limit};
     WeightsWalk walk{c, bt, shape, share, 0, 0, 0, false};
     WeightsSegment g;
     if (warp == 17) {
-        int slot = 0, loaded = 0;
-        uint32_t phase = 0, k_phase = 0;
+        int slot = 0, loaded = 0, k_fills = 0;
+        uint32_t phase = 0;
+        bool over = false;
         const int box_shift = min(c.page_shift, 6), boxes = CHUNK_SLOTS >> box_shift;
         const uint32_t me = elect_lane();
-        while (walk.next(&g)) {
+        while (!over && walk.next(&g)) {
             const int32_t* table = bt.table + g.b * bt.table_stride;
-            wait(k_empty, k_phase ^ 1);
+            wait(k_empty, (k_fills & 1) ^ 1);
+            over = wait.given_up();
+            if (over) break;
+            ++k_fills;
             TilePages tp[2];
 #pragma unroll
             for (int u = 0; u < 2; ++u)
@@ -188,9 +194,10 @@ __global__ void __launch_bounds__(WEIGHTS_THREADS, 1)
                         tma_page(smem_k + u * SLOT + half * (CHUNK_SLOTS * 128) + from * 128, &map_k, half * 64, in, g.head,
                                  page, k_full, me);
                 }
-            k_phase ^= 1;
             for (int q = g.q0; q < g.q0 + g.count; ++q) {
                 wait(q_empty + slot, phase ^ 1);
+                over = wait.given_up();
+                if (over) break;
                 if (lane == 0) {
                     mbar_arrive_expect_tx(q_full + slot, HALVES * shape.tokens * a.group * 128);
                     for (int h = 0; h < HALVES; ++h)
@@ -202,14 +209,9 @@ __global__ void __launch_bounds__(WEIGHTS_THREADS, 1)
                 if (++slot == RING) slot = 0, phase ^= 1;
             }
         }
-        // A wait that ran out may have left copies in flight into this CTA's memory: see them land before it ends.
-        if (wait.dead && lane == 0) {
-            for (int i = 0; i < RING; ++i) {
-                const int fills = loaded / RING + (i < loaded % RING);
-                if (fills && !mbar_wait_bounded(q_full + i, (fills - 1) & 1, 2 * KV_WAIT_BUDGET))
-                    atomicOr(c.status, ERR_DRAIN_TIMEOUT);
-            }
-            if (loaded && !mbar_wait_bounded(k_full, k_phase ^ 1, 2 * KV_WAIT_BUDGET)) atomicOr(c.status, ERR_DRAIN_TIMEOUT);
+        if (lane == 0) {
+            wait.drain(k_full, k_fills);
+            for (int i = 0; i < RING; ++i) wait.drain(q_full + i, loaded / RING + (i < loaded % RING));
         }
     } else if (warp == 16) {
         const uint32_t idesc = umma_idesc<T>(CHUNK_ROWS, false, a.scale < 0.f);
@@ -246,6 +248,8 @@ __global__ void __launch_bounds__(WEIGHTS_THREADS, 1)
             }
             umma_commit(k_empty, me);
         }
+        umma_commit(mma_done, me);
+        if (lane == 0) wait.drain(mma_done, 1);
     } else {
         const int wg = warp >> 2, i = wg & 1, half = wg >> 1, r = (warp & 3) * 32 + lane;
         const int row = half * 64 + (r & 63), row_token = (int)a.by_group(row);  // whose lse this thread fetches
