@@ -242,3 +242,29 @@ def test_waits_that_run_out(counts, dim):
         c.cache.sync()
         assert torch.equal(out, want) and torch.equal(lse, want_lse) and torch.equal(s, s0)
     assert N.lib().vk_kv_wait_limit(c.cache._h, -1) == N.VK_ERR_INVALID
+
+
+def test_offsets_that_count_the_tokens_again_and_again():
+    """Offsets that do not ascend give many sequences the same tokens: 2,200 x 131,072 x 8 units, more than 32 bits count.
+    The call is reported and does nothing."""
+    import torch
+
+    from veckern_b200 import PagedCache
+    from veckern_b200 import _native as N
+
+    tokens, batch = 2048, 4400
+    pages = torch.zeros((2, 1024, 8, 64), dtype=torch.bfloat16, device="cuda")
+    table = torch.zeros((1, 128), dtype=torch.int32, device="cuda").expand(batch, -1)
+    lens = torch.full((batch,), 128 * 1024, dtype=torch.int32, device="cuda")
+    offsets = torch.tensor([0, tokens], dtype=torch.int32, device="cuda").repeat(batch // 2 + 1)[:batch + 1].contiguous()
+    out = torch.full((tokens, 128, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    with PagedCache(pages, pages) as cache:
+        cache.attend(torch.zeros_like(out), offsets, table, lens, causal=False, out=out)
+        with pytest.raises(N.VkError, match="out of range"):
+            cache.sync()
+        assert (out == 7).all()
+        ascending = torch.full((batch + 1,), 5, dtype=torch.int32, device="cuda")
+        ascending[0] = 0
+        cache.attend(torch.zeros_like(out), ascending, table, lens // 1024, causal=False, out=out)
+        cache.sync()
+        assert (out[:5] == 0).all() and (out[5:] == 7).all()

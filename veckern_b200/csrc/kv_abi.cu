@@ -435,7 +435,7 @@ int vk_kv_attend(vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_attend_t* 
     a.wait_limit = kv->wait_limit.load(std::memory_order_relaxed);
     // The kernels count their units of work (tiles and pairs of tiles, of every kv head) in 32 bits.
     const int64_t tiles = ceil_div((int64_t)bt.width << kv->page_shift, vk::STEP_TILE) + 1;
-    if (tiles * g * ((double)bt.tokens * a.group / vk::CHUNK_ROWS + 2.0 * bt.batch) >= 2147483648.0)
+    if (tiles * g * ((double)bt.tokens * a.group / vk::CHUNK_ROWS + 2.0 * bt.batch) >= 2147483647.0)
         return fail(VK_ERR_UNSUPPORTED, "too many tiles (tables of %d pages, %lld tokens); use fewer sequences per call",
                     bt.width, (long long)bt.tokens);
     const AttendPlan plan = plan_attend(kv, bt, a.group, a.max_q, a.scores != nullptr);

@@ -179,8 +179,9 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 }
 
 // The share of one CTA: a walk over units laid end to end, sequence by sequence. Count(s) is the number of units of a
-// sequence; the caller splits a sequence's units into its heads and tiles. The host has checked that all units together
-// are fewer than 2^31.
+// sequence; the caller splits a sequence's units into its heads and tiles. The host has checked that the units of sequences
+// whose tokens are the call's, each once, are fewer than 2^31 - 1 together. Offsets that do not ascend can make them more:
+// sums stop there, and such a call is reported and does nothing.
 struct KvShare {
     int me;    // which share; none from `ctas` on
     int b;     // sequence of the next unit
@@ -218,27 +219,31 @@ __device__ __forceinline__ KvShare kv_share(const KvPages& c, const KvBatch& bt,
     }
     const int span = (bt.batch + THREADS - 1) / THREADS;
     const int b0 = min(bt.batch, t * span), b1 = min(bt.batch, b0 + span);
-    int sum = 0, longest = 0;
-    for (int b = b0; b < b1; ++b) sum += count(kv_seq(c, bt, b), &longest);
+    constexpr uint32_t MOST = 0x7fffffff;
+    uint32_t sum = 0;
+    int longest = 0;
+    for (int b = b0; b < b1; ++b) sum = min(sum + (uint32_t)count(kv_seq(c, bt, b), &longest), MOST);
     longest = __reduce_max_sync(FULL, longest);
-    int incl = sum;
+    uint32_t incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(FULL, incl, o);
-        if (lane >= o) incl += x;
+        const uint32_t x = __shfl_up_sync(FULL, incl, o);
+        if (lane >= o) incl = min(incl + x, MOST);
     }
     if (lane == 31) {
-        scratch[warp] = incl;
+        scratch[warp] = (int)incl;
         scratch[WARPS + warp] = longest;
     }
     __syncthreads();
-    int before = 0, total = 0;
+    uint32_t before = 0, all = 0;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
-        if (w < warp) before += scratch[w];
-        total += scratch[w];
+        if (w < warp) before += (uint32_t)scratch[w];
+        all = min(all + (uint32_t)scratch[w], MOST);
         longest = max(longest, scratch[WARPS + w]);
     }
+    if (all == MOST && t == 0) atomicOr(c.status, ERR_LAYOUT);
+    const int total = all == MOST ? 0 : (int)all;
     const int least = max(1, (int)(sqrtf(longest * part_cost) + 0.5f));
     KvShare s;
     s.ctas = min((int)gridDim.x, (total + least - 1) / least);
@@ -249,9 +254,9 @@ __device__ __forceinline__ KvShare kv_share(const KvPages& c, const KvBatch& bt,
     s.me = place < s.ctas ? s.ctas - 1 - place : s.ctas;
     const int first = s.first(s.me);
     s.left = s.me < s.ctas ? s.first(s.me + 1) - first : 0;
-    before += incl - sum;
-    if (first >= before && first < before + sum) {
-        int off = first - before, b = b0;
+    before += incl - sum;  // exact where there are shares
+    if (s.left > 0 && (uint32_t)first >= before && (uint32_t)first < before + sum) {
+        int off = first - (int)before, b = b0;
         if (b1 - b0 > 1)
             for (;; ++b) {
                 const int n = count(kv_seq(c, bt, b), &longest);
