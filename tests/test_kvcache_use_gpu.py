@@ -268,3 +268,36 @@ def test_offsets_that_count_the_tokens_again_and_again():
         cache.attend(torch.zeros_like(out), ascending, table, lens // 1024, causal=False, out=out)
         cache.sync()
         assert (out[:5] == 0).all() and (out[5:] == 7).all()
+
+
+@pytest.mark.parametrize("counts", [[1, 1], [40, 33]])
+def test_results_whose_rows_overlap_are_refused(counts):
+    """Scores that sequences or heads share would be added to by several threads without an order; the same of out."""
+    import torch
+
+    from veckern_b200 import _native as N
+
+    c = Cache([300, 200], 16, 2, 64, seed=5)
+    q, off, _ = call(c, counts, heads=4)
+    room = torch.zeros((2, 2, 400), device="cuda")
+    for s in (room[:1].expand(2, -1, -1), room[:, :1].expand(-1, 2, -1), room.as_strided((2, 2, 300), (600, 299, 1)),
+              room.as_strided((2, 2, 300), (300, 300, 1))):
+        with pytest.raises(N.VkError, match="scores: rows overlap"):
+            c.cache.attend(q, off, c.table, c.lens, scores=s)
+    n = sum(counts)
+    for out in (torch.zeros((1, 4, 64), dtype=c.dtype, device="cuda").expand(n, -1, -1),
+                torch.zeros((n, 1, 64), dtype=c.dtype, device="cuda").expand(-1, 4, -1)):
+        with pytest.raises(N.VkError, match="out: rows overlap"):
+            c.cache.attend(q, off, c.table, c.lens, out=out)
+    want, want_lse = c.cache.attend(q, off, c.table, c.lens)
+    for s in (room[:, :, :300], room[:, :, 50:350].transpose(0, 1), torch.zeros((2, 9, 300), device="cuda")[:, ::5]):
+        before = s.clone()
+        head_major = torch.empty((4, n, 64), dtype=c.dtype, device="cuda").transpose(0, 1)
+        out, lse = c.cache.attend(q, off, c.table, c.lens, scores=s, out=head_major)
+        c.cache.sync()
+        check_attend(c, q, counts, out, lse, True, None, s, before)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    one = Cache([300], 16, 1, 64, seed=6)  # one row: its strides say nothing
+    q, off, _ = call(one, [5])
+    one.cache.attend(q, off, one.table, one.lens, scores=torch.zeros((1, 1, 300), device="cuda").as_strided((1, 1, 300), (0, 0, 1)))
+    one.cache.sync()

@@ -2,6 +2,7 @@
 #include <atomic>
 #include <new>
 #include <type_traits>
+#include <utility>
 
 #include <cudaTypedefs.h>
 
@@ -69,6 +70,16 @@ int check_rows(const char* what, const void* p, const int64_t* stride) {
     if (!stride || stride[0] < 0 || stride[1] < 0 || stride[0] % 8 || stride[1] % 8)
         return fail(VK_ERR_INVALID, "%s: strides must be multiples of 8 elements", what);
     return VK_OK;
+}
+
+// Whether rows of `len` elements at i * s0 + j * s1, i < n0, j < n1, may share elements. (Rows that two strides interleave
+// without a common element count as sharing some: nobody lays out results like that.)
+bool rows_overlap(int64_t n0, int64_t s0, int64_t n1, int64_t s1, int64_t len) {
+    if (n0 <= 1) n0 = n1, s0 = s1, n1 = 1;
+    if (n0 <= 1 || len == 0) return false;
+    if (n1 <= 1) return s0 < len;
+    if (s0 > s1) std::swap(s0, s1), std::swap(n0, n1);
+    return s0 < len || s1 < (__int128)s0 * (n0 - 1) + len;
 }
 
 size_t align256(size_t x) { return (x + 255) / 256 * 256; }
@@ -410,6 +421,11 @@ int vk_kv_attend(vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_attend_t* 
     VK_TRY(check_rows("q", args->q, args->q_stride));
     VK_TRY(check_rows("out", args->out, args->out_stride));
     if (!args->lse) return fail(VK_ERR_INVALID, "lse must not be NULL");
+    if (rows_overlap(bt.tokens, args->out_stride[0], args->heads, args->out_stride[1], kv->desc.head_dim))
+        return fail(VK_ERR_INVALID, "out: rows overlap");
+    if (args->scores &&
+        rows_overlap(bt.batch, args->scores_stride[0], g, args->scores_stride[1], args->scores_width))
+        return fail(VK_ERR_INVALID, "scores: rows overlap; each sequence and kv head is added to its own");
     DeviceGuard guard(kv->desc.device);
     if (guard.err != cudaSuccess) return fail(VK_ERR_CUDA, "cudaSetDevice: %s", cudaGetErrorString(guard.err));
     vk::KvAttend a{};
