@@ -301,3 +301,27 @@ def test_results_whose_rows_overlap_are_refused(counts):
     q, off, _ = call(one, [5])
     one.cache.attend(q, off, one.table, one.lens, scores=torch.zeros((1, 1, 300), device="cuda").as_strided((1, 1, 300), (0, 0, 1)))
     one.cache.sync()
+
+
+def test_a_new_cache_reports_what_its_first_call_finds():
+    """The status word is clear when the cache is made, not when the default stream comes to it: work that is pending there
+    must not clear what a call on another stream has found meanwhile."""
+    import torch
+
+    from veckern_b200 import PagedCache
+    from veckern_b200 import _native as N
+
+    c = Cache([300, 200], 16, 2, 64, seed=5)
+    q, off, _ = call(c, [1, 1])
+    st = torch.cuda.Stream()
+    bad = c.table.clone()
+    bad[0, 1] = -1
+    c.cache.attend(q, off, c.table, c.lens, stream=st)
+    torch.cuda.synchronize()
+    wait_on_current(100)
+    with PagedCache(c.k, c.v) as cache:
+        cache.attend(q, off, bad, c.lens, stream=st)
+        torch.cuda.synchronize()
+        with pytest.raises(N.VkError, match="out of range"):
+            cache.sync(st)
+        cache.sync(st)

@@ -301,14 +301,15 @@ struct BesideCapture {
     ~BesideCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
 };
 
-// Clears a workspace's start, on a stream that nothing else uses, and waits for it.
-int clear_workspace(void* workspace) {
+// Clears memory that is not in use, on a stream that nothing else uses, and waits for it: the default stream, on which
+// cudaMemset runs, is not ordered with streams that do not block on it.
+int clear_now(void* p, size_t bytes) {
     cudaStream_t st;
     VK_TRY_CUDA(cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking));
-    cudaError_t e = cudaMemsetAsync(workspace, 0, VK_KV_WORKSPACE_ZEROED, st);
+    cudaError_t e = cudaMemsetAsync(p, 0, bytes, st);
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
     cudaStreamDestroy(st);
-    return e == cudaSuccess ? VK_OK : fail(VK_ERR_CUDA, "clearing a workspace: %s", cudaGetErrorString(e));
+    return e == cudaSuccess ? VK_OK : fail(VK_ERR_CUDA, "clearing device memory: %s", cudaGetErrorString(e));
 }
 
 }  // namespace
@@ -343,13 +344,13 @@ int vk_kv_create(const vk_kv_desc_t* d, vk_kv_t** out) {
     while ((1 << kv->page_shift) < d->page_size) ++kv->page_shift;
     cudaError_t e = cudaDeviceGetAttribute(&kv->sm_count, cudaDevAttrMultiProcessorCount, d->device);
     if (e == cudaSuccess) e = cudaMalloc(&kv->status, sizeof(int));
-    if (e == cudaSuccess) e = cudaMemset(kv->status, 0, sizeof(int));
     if (e != cudaSuccess) {
         delete kv;
         return fail(e == cudaErrorMemoryAllocation ? VK_ERR_NOMEM : VK_ERR_CUDA, "vk_kv_create: %s",
                     cudaGetErrorString(e));
     }
-    int r = encode_map(*d, d->k, d->k_stride, &kv->map_k);
+    int r = clear_now(kv->status, sizeof(int));
+    if (r == VK_OK) r = encode_map(*d, d->k, d->k_stride, &kv->map_k);
     if (r == VK_OK) r = encode_map(*d, d->v, d->v_stride, &kv->map_v);
     if (r != VK_OK) {
         delete kv;
@@ -483,7 +484,7 @@ int vk_kv_workspace_create(int device, size_t bytes, void** out) {
     BesideCapture beside;
     void* p = nullptr;
     VK_TRY_CUDA(cudaMalloc(&p, std::max<size_t>(bytes, VK_KV_WORKSPACE_ZEROED)));
-    const int r = clear_workspace(p);
+    const int r = clear_now(p, VK_KV_WORKSPACE_ZEROED);
     if (r != VK_OK) {
         cudaFree(p);
         return r;
@@ -497,7 +498,7 @@ int vk_kv_workspace_clear(int device, void* workspace) {
     DeviceGuard guard(device);
     if (guard.err != cudaSuccess) return fail(VK_ERR_CUDA, "cudaSetDevice: %s", cudaGetErrorString(guard.err));
     BesideCapture beside;
-    return clear_workspace(workspace);
+    return clear_now(workspace, VK_KV_WORKSPACE_ZEROED);
 }
 
 int vk_kv_workspace_destroy(int device, void* workspace) {
