@@ -299,7 +299,8 @@ def test_results_whose_rows_overlap_are_refused(counts):
         assert torch.equal(out, want) and torch.equal(lse, want_lse)
     one = Cache([300], 16, 1, 64, seed=6)  # one row: its strides say nothing
     q, off, _ = call(one, [5])
-    one.cache.attend(q, off, one.table, one.lens, scores=torch.zeros((1, 1, 300), device="cuda").as_strided((1, 1, 300), (0, 0, 1)))
+    s = torch.zeros((1, 1, 300), device="cuda").as_strided((1, 1, 300), (0, 0, 1))
+    one.cache.attend(q, off, one.table, one.lens, scores=s)
     one.cache.sync()
 
 
@@ -325,3 +326,87 @@ def test_a_new_cache_reports_what_its_first_call_finds():
         with pytest.raises(N.VkError, match="out of range"):
             cache.sync(st)
         cache.sync(st)
+
+
+def same(x, y):
+    """Bit for bit (NaN included)."""
+    import torch
+
+    return torch.equal(x.contiguous().view(torch.int16), y.contiguous().view(torch.int16))
+
+
+def refused(c, what="attention read .* as zeros"):
+    from veckern_b200 import _native as N
+
+    with pytest.raises(N.VkError, match=f"out of range: {what}"):
+        c.cache.sync()
+
+
+@pytest.mark.parametrize("counts", [[1, 1, 1], [20, 1, 30]])
+def test_what_is_refused_changes_nothing_else(counts):
+    """Page numbers, lengths and offsets out of range: an attention gives the other sequences what it gave before, and reads a
+    page that is not there as zeros; an append writes the slots that it can and no others."""
+    import torch
+
+    c = Cache([100, 60, 90], 16, 2, 64, seed=6, extra=3)
+    q, off, _ = call(c, counts, heads=4)
+    good, good_lse = c.cache.attend(q, off, c.table, c.lens, causal=False)
+    c.cache.sync()
+    check_attend(c, q, counts, good, good_lse, False)
+    k0, v0 = c.k.clone(), c.v.clone()
+    at = [0, counts[0], sum(counts[:2]), sum(counts)]
+    others = [i for i in range(at[3]) if not at[1] <= i < at[2]]
+    for wrong in (-5, -1, c.k.shape[0], 2 ** 31 - 1):
+        t = c.table.clone()
+        t[1, 2] = wrong
+        out, lse = c.cache.attend(q, off, t, c.lens, causal=False)
+        refused(c)
+        assert torch.equal(out[others], good[others]) and torch.equal(lse[others], good_lse[others])
+        zeros = Cache.__new__(Cache)
+        zeros.__dict__.update(c.__dict__)
+        zeros.k, zeros.v = torch.cat([c.k, torch.zeros_like(c.k[:1])]), torch.cat([c.v, torch.zeros_like(c.v[:1])])
+        zeros.table = torch.where(t == wrong, c.k.shape[0], t).to(torch.int32)
+        zeros.table[c.table == 2 ** 31 - 1] = 2 ** 31 - 1
+        check_attend(zeros, q, counts, out, lse, False)
+        # the last of sequence 1's slots 60 - count .. 59 lie in the page that is not there (slots 32 .. 47) or behind it
+        t = c.table.clone()
+        t[1, 3] = wrong
+        ones = torch.ones((at[3], 2, 64), dtype=c.dtype, device="cuda")
+        c.cache.append(ones, ones, off, t, c.lens)
+        refused(c, ".* nothing was written")
+        own = torch.zeros(c.k.shape[:2], dtype=torch.bool, device="cuda")
+        for b, (n, cnt) in enumerate(zip(c.lens_list, counts)):
+            j = torch.arange(n - cnt, n, device="cuda")
+            if b == 1:
+                j = j[j < 48]
+            own[c.table[b].long()[j // 16], j % 16] = True
+        for x, x0 in ((c.k, k0), (c.v, v0)):
+            assert (x[own] == 1).all() and same(x[~own], x0[~own])
+            x.copy_(x0)
+    # lengths: below zero none, past the table all of its slots (their page numbers lie past the sequence's)
+    for length in (-1, 10 ** 9):
+        lens = c.lens.clone()
+        lens[1] = length
+        out, lse = c.cache.attend(q, off, c.table, lens, causal=False)
+        refused(c)
+        assert torch.equal(out[others], good[others]) and torch.equal(lse[others], good_lse[others])
+        if length < 0:
+            assert (out[at[1]:at[2]] == 0).all() and (lse[at[1]:at[2]] == -torch.inf).all()
+    # offsets: sequences whose own pair is in range and ascends keep their results
+    for bad, kept in (([0, at[1], at[2], 10 ** 6], [0, 1]), ([-3, at[1], at[2], at[3]], [1, 2]), ([0, at[2], at[1], at[1]], [])):
+        o = torch.tensor(bad, dtype=torch.int32, device="cuda")
+        out, lse = c.cache.attend(q, o, c.table, c.lens, causal=False)
+        refused(c)
+        for b in kept:
+            assert torch.equal(out[at[b]:at[b + 1]], good[at[b]:at[b + 1]])
+    # more new tokens than slots: the last ones are written
+    new = torch.arange(9, device="cuda", dtype=c.dtype)[:, None, None].expand(-1, 2, 64).contiguous()
+    c.cache.append(new, new, c.offsets([9]), c.table[:1], torch.tensor([5], dtype=torch.int32, device="cuda"))
+    refused(c, ".* nothing was written")
+    first = int(c.table[0, 0])
+    assert torch.equal(c.k[first, :5], new[4:]) and torch.equal(c.v[first, :5], new[4:])
+    c.k[first, :5], c.v[first, :5] = k0[first, :5], v0[first, :5]
+    assert same(c.k, k0) and same(c.v, v0)
+    again, again_lse = c.cache.attend(q, off, c.table, c.lens, causal=False)
+    c.cache.sync()
+    assert torch.equal(again, good) and torch.equal(again_lse, good_lse)

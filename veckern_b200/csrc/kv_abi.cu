@@ -383,7 +383,9 @@ int vk_kv_sync(vk_kv_t* kv, void* stream) {
         return fail(VK_ERR_DEVICE, "a bounded wait ran out in a cache kernel (status %d)", status);
     if (status & vk::ERR_WORKSPACE)
         return fail(VK_ERR_DEVICE, "a call's workspace was not cleared after a bounded wait had run out in another call");
-    return fail(VK_ERR_INVALID, "a page number, length or offset was out of range; the slots it names were left out");
+    return fail(VK_ERR_INVALID,
+                "a page number, length or offset was out of range: attention read the slots of such a page as zeros, nothing "
+                "was written to them, and rows of such offsets may be missing");
 }
 
 int vk_kv_wait_limit(vk_kv_t* kv, int64_t cycles) {
