@@ -555,7 +555,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                 const float mine = top;
                 lone_ml[i * CHUNK_ROWS + r] = make_float2(top, total);
                 tmem_fence_before();
-                asm volatile("bar.sync 3, 256;" ::: "memory");
+                bar_sync(3, 256);
                 tmem_fence_after();
                 const float2 ml = lone_ml[(i ^ 1) * CHUNK_ROWS + r];
                 top = fmaxf(top, ml.x);
@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
             auto part_of = [&](int k) -> int64_t { return 2 * (int64_t)(walk.share.me + k) + i; };
             if (follow) {
                 for (int k = r; k < follow; k += 128) part_await(parts, (int)part_of(1 + k), wait);
-                asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+                bar_sync(1 + i, 128);
                 float f = 1.f;
                 for (int k0 = 0; k0 < follow; k0 += 8) {  // eight in flight; the last ones again, for nothing
                     float2 ml[8];
@@ -652,15 +652,15 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                 }
             }
             tmem_fence_before();
-            if (g.lone) asm volatile("bar.sync 3, 256;" ::: "memory");  // both have read the two sums
+            if (g.lone) bar_sync(3, 256);  // both have read the two sums
             if (leaves) {
                 parts.ml[part_of(0) * CHUNK_ROWS + r] = make_float2(top, total);
-                asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+                bar_sync(1 + i, 128);
                 if (r == 0) part_publish(parts, (int)part_of(0));
             } else {
                 if (live && !(g.lone && i == 1)) a.lse[tok * a.heads + h] = (top + log2f(total)) * 0.6931471805599453f;
                 if (follow) {
-                    asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+                    bar_sync(1 + i, 128);
                     for (int k = r; k < follow; k += 128) parts.ready[part_of(1 + k)] = 0;
                 }
             }

@@ -128,6 +128,13 @@ struct KvWait {
     }
 };
 
+// A barrier of `threads` threads, whole warps. Their lanes meet first: what comes before is often a loop or a branch that they
+// leave one by one, and all lanes of a warp have to execute the barrier as one.
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+    __syncwarp();
+    asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
 // Part `i` is written (by threads that a barrier has joined since): tell the CTA that adds it up.
 __device__ __forceinline__ void part_publish(const KvParts& parts, int i) {
     asm volatile("st.release.gpu.global.u32 [%0], %1;" ::"l"(parts.ready + i), "r"(1u) : "memory");
@@ -496,7 +503,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
                 for (int i = 0; i < DP / 8; ++i)
                     *reinterpret_cast<float2*>(sum_o + (warp * 8 + g) * DP + 8 * i + q2) =
                         make_float2(o[i][2 * u], o[i][2 * u + 1]);
-                asm volatile("bar.sync 1, 128;" ::: "memory");
+                bar_sync(1, 32 * STEP_WARPS);
                 top[u] = -INFINITY;
                 if (works) {
                     const int r = 8 * u + r8;
@@ -511,7 +518,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
                         for (int e = 0; e < 8; ++e) v[u][e] += f * sum_o[(w * 8 + r8) * DP + d + e];
                     }
                 }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
+                bar_sync(1, 32 * STEP_WARPS);
             }
             if (works && leaves) {
 #pragma unroll
@@ -572,7 +579,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
                     if (d == 0) a.lse[tok * a.heads + h] = (top[u] + log2f(total[u])) * 0.6931471805599453f;
                 }
             }
-            if (leaves || follow) asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (leaves || follow) bar_sync(1, 32 * STEP_WARPS);
             if (leaves && threadIdx.x == 0) part_publish(parts, share.me);
             for (int i = threadIdx.x; i < follow; i += 32 * STEP_WARPS) parts.ready[share.me + 1 + i] = 0;
         }

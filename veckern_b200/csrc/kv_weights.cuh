@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(WEIGHTS_THREADS, 1)
                 const int buf = used & 1;
                 if (r < 64) lse[buf * 64 + r] = next;
                 if (q + 1 < g.q0 + g.count) next = minus_lse(q + 1);
-                asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");
+                bar_sync(1 + wg, 128);
                 wait(s_full + 2 * i + buf, used >> 1 & 1);
                 ++used;
                 tmem_fence_after();
@@ -314,19 +314,19 @@ __global__ void __launch_bounds__(WEIGHTS_THREADS, 1)
             float* other = s_sum + (turn & 1) * 256 + i * 128 + r;
             turn ^= 1;
             if (half == 1) *other = total;
-            asm volatile("bar.sync %0, 256;" ::"r"(5 + i) : "memory");
+            bar_sync(5 + i, 256);
             if (half == 1) continue;
             total += *other;
             const int part = 2 * walk.share.me + i;
             if (g.leaves) {
                 parts.o[(int64_t)part * CHUNK_SLOTS + r] = total;
-                asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");
+                bar_sync(1 + wg, 128);
                 if (r == 0) part_publish(parts, part);
             } else {
                 const int follow = walk.share.followers(g.rest);
                 if (follow) {
                     for (int k = r; k < follow; k += 128) part_await(parts, part + 2 + 2 * k, wait);
-                    asm volatile("bar.sync %0, 128;" ::"r"(1 + wg) : "memory");
+                    bar_sync(1 + wg, 128);
                     for (int k0 = 0; k0 < follow; k0 += 8) {  // eight in flight; the last ones again, for nothing
                         float x[8];
 #pragma unroll
