@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     tmem_fence_after();
     const uint32_t tm = __shfl_sync(FULL, *tmem_at, 0);
-    KvWait wait{c.status, parts.bad, scratch + KV_SHARE_OVER, a.wait_limit};
+    KvWait wait{c.status, parts.bad, a.wait_limit};
     ChunkWalk walk{c, bt, shape, share, 0, 0, 0, false};
     ChunkSegment g;
     // 384 threads start with 168 registers: 2 x 128 x 200 + 128 x 104 is the same sum
@@ -328,15 +328,15 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
         auto at = [&](int n) { return n % RING; };
         auto parity = [&](int n) -> uint32_t { return n / RING & 1; };
         if (warp == 9) {
+            uint32_t q_phase = 0;
             int q_fills = 0;
-            bool over = false;
             const int box_shift = min(c.page_shift, 6);
             const int boxes = CHUNK_SLOTS >> box_shift;
             const uint32_t me = elect_lane();
-            while (!over && walk.next(&g)) {
-                wait(q_empty, (q_fills & 1) ^ 1);
-                over = wait.given_up();
-                if (over) break;
+            while (!wait.dead && walk.next(&g)) {
+                wait.together(q_empty, q_phase ^ 1);
+                if (wait.dead) break;
+                q_phase ^= 1;
                 ++q_fills;
                 if (lane == 0) {
                     const int n = g.lone ? 1 : 2;
@@ -348,15 +348,14 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                 }
                 const int32_t* table = bt.table + g.b * bt.table_stride;
                 const int per = g.lone ? 2 : 1;
-                for (int t = g.t0 * per; t < (g.t0 + g.count) * per && !over; ++t) {
+                for (int t = g.t0 * per; t < (g.t0 + g.count) * per && !wait.dead; ++t) {
                     const TilePages tp = tile_pages(c, table, t * CHUNK_SLOTS, boxes, box_shift, g.s.len);
                     // rolled: this warp's registers are few, and what it spills the other one waits for
 #pragma unroll 1
                     for (int side = 0; side < 2; ++side, ++fill) {
                         const int slot = at(fill);
-                        wait(kv_empty + slot, parity(fill) ^ 1);
-                        over = wait.given_up();
-                        if (over) break;
+                        wait.together(kv_empty + slot, parity(fill) ^ 1);
+                        if (wait.dead) break;
                         if (lane == 0) mbar_arrive_expect_tx(kv_full + slot, tp.count * HALVES * (128 << box_shift));
                         __syncwarp();
                         uint8_t* dst = ring + slot * SLOT;
@@ -408,13 +407,13 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                         }
                     }
                     umma_commit(s_full + i, me);
-                    if (lone || i == 1) umma_commit(kv_empty + slot, me);
+                    if (lone || i == 1) umma_commit(kv_empty + slot, wait.live(me));
                 };
                 wait(q_full, q_phase);
                 q_phase ^= 1;
                 scores(0, 0);
                 scores(0, 1);
-                if (count == 1) umma_commit(q_empty, me);
+                if (count == 1) umma_commit(q_empty, wait.live(me));
                 for (int u = 0; u < count; ++u) {
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
@@ -445,11 +444,11 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                                 umma_ts(o, p + e * 8, v + e * 128, idesc_o, u > 0 || e > 0, me);
                         }
                         p_phase ^= 1u << i;
-                        if (lone || i == 1) umma_commit(kv_empty + slot, me);
+                        if (lone || i == 1) umma_commit(kv_empty + slot, wait.live(me));
                         if (u + 1 < count) scores(u + 1, i);
                         else umma_commit(o_full + i, me);
                     }
-                    if (u + 2 == count) umma_commit(q_empty, me);
+                    if (u + 2 == count) umma_commit(q_empty, wait.live(me));
                 }
                 fill += count * step;
             }

@@ -100,17 +100,16 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 // other caches as well, report that theirs is void until it has been cleared. Called by whole warps, which leave it
 // together: what follows is often an instruction that all lanes have to execute as one.
 //
-// A CTA that gives up starts no more copies, so that a barrier has one fill in flight at most. The warp that starts copies or
-// products waits for its last ones before it ends, whatever the others do: none outlives the CTA.
+// A thread that gave up hands no memory back to be filled again and fills none, so that a barrier has one fill in flight at
+// most, which its phase tells. The warp that starts copies or products waits for its last ones before it ends, whatever the
+// others do: none outlives the CTA.
 struct KvWait {
     int* status;
     uint32_t* bad;
-    int* over;  // shared memory: not zero when a thread of the CTA gave up
     long long limit;
     bool dead = false;
     __device__ __forceinline__ void ran_out() {
         dead = true;
-        *reinterpret_cast<volatile int*>(over) = 1;
         atomicOr(status, ERR_WAIT_TIMEOUT);
         *reinterpret_cast<volatile uint32_t*>(bad) = 1u;
     }
@@ -118,10 +117,15 @@ struct KvWait {
         if (!mbar_try_wait(bar, parity) && !dead && !mbar_wait_bounded(bar, parity, limit)) ran_out();
         __syncwarp();
     }
-    // Whether a thread of the CTA gave up, the same for the whole warp; who gave up said so before it arrived anywhere.
-    __device__ __forceinline__ bool given_up() const {
-        return __any_sync(FULL, *reinterpret_cast<volatile int*>(over));
+    // The same, and all lanes of the warp give up if one does. For warps that fill memory: they copy with the elected lane's
+    // predicate as it is (one computed from it made every copy slower: 8 x 5 tokens over 4,001 slots 20.6 us where this takes
+    // 19.1), under a branch of the whole warp.
+    __device__ __forceinline__ void together(uint64_t* bar, uint32_t parity) {
+        if (__all_sync(FULL, mbar_try_wait(bar, parity)) || dead) return;
+        if (!__all_sync(FULL, mbar_wait_bounded(bar, parity, limit))) ran_out();
     }
+    // `me` (whether this lane acts for its warp), unless the lane gave up.
+    __device__ __forceinline__ uint32_t live(uint32_t me) const { return dead ? 0u : me; }
     // Waits for the last fill of a barrier that has had `fills` of them.
     __device__ __forceinline__ void drain(uint64_t* bar, int fills) const {
         if (fills && !mbar_wait_bounded(bar, (fills - 1) & 1, KV_DRAIN_LIMIT)) atomicOr(status, ERR_DRAIN_TIMEOUT);
@@ -207,7 +211,7 @@ struct KvShare {
     }
 };
 
-constexpr int KV_SHARE_SCRATCH = 40, KV_SHARE_OVER = KV_SHARE_SCRATCH - 1;
+constexpr int KV_SHARE_SCRATCH = 40;
 // Count(s, &longest) also raises `longest` to the units of the sequence's longest segment. A segment of L units that is cut
 // every m units takes m of a unit's time and L / m of a part's: least with m = sqrt(L part / unit), which is the least that
 // a CTA gets (part_cost: part / unit), except where all units together are fewer.
@@ -217,9 +221,8 @@ __device__ __forceinline__ KvShare kv_share(const KvPages& c, const KvBatch& bt,
     // scratch: KV_SHARE_SCRATCH values of shared memory. Thread t sums a contiguous range of the sequences. No CTA without a
     // share lies between others: the parts of a cut segment belong to consecutive CTAs.
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    constexpr int WARPS = THREADS / 32, PLACE = KV_SHARE_SCRATCH - 2;
+    constexpr int WARPS = THREADS / 32, PLACE = KV_SHARE_SCRATCH - 1;
     static_assert(2 * WARPS + 2 <= PLACE, "scratch");
-    if (t == 0) scratch[KV_SHARE_OVER] = 0;
     if (t == THREADS - 1) {  // beside the others' loads
         scratch[PLACE] = (int)atomicInc(parts.started, gridDim.x - 1);
         if (*reinterpret_cast<const volatile uint32_t*>(parts.bad)) atomicOr(c.status, ERR_WORKSPACE);
@@ -331,7 +334,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
     };
     KvShare share = kv_share<STEP_THREADS>(c, bt, parts, scratch, STEP_PART_COST, units_of);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    KvWait wait{c.status, parts.bad, scratch + KV_SHARE_OVER, a.wait_limit};
+    KvWait wait{c.status, parts.bad, a.wait_limit};
     int stage = 0;
     uint32_t phase = 0;
     const int box_shift = min(c.page_shift, 6), boxes = STEP_TILE >> box_shift;
@@ -353,8 +356,8 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
             const uint32_t me = elect_lane();
             for (int t = t0; t < t0 + count; ++t) {
                 const TilePages tp = tile_pages(c, table, t * STEP_TILE, boxes, box_shift, s.len);
-                wait(empty + stage, phase ^ 1);
-                if (wait.given_up()) {
+                wait.together(empty + stage, phase ^ 1);
+                if (wait.dead) {
                     share.left = 0;
                     break;
                 }
@@ -479,7 +482,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
                     if (ends) fence_proxy_async_smem();
                 }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(empty + stage);
+                if (lane == 0 && !wait.dead) mbar_arrive(empty + stage);
                 if (++stage == STAGES) stage = 0, phase ^= 1;
             }
             // Join the four warps, eight rows at a time.

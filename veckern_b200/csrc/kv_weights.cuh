@@ -162,20 +162,19 @@ __global__ void __launch_bounds__(WEIGHTS_THREADS, 1)
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     tmem_fence_after();
     const uint32_t tm = __shfl_sync(FULL, *tmem_at, 0);
-    KvWait wait{c.status, parts.bad, scratch + KV_SHARE_OVER, a.wait_limit};
+    KvWait wait{c.status, parts.bad, a.wait_limit};
     WeightsWalk walk{c, bt, shape, share, 0, 0, 0, false};
     WeightsSegment g;
     if (warp == 17) {
         int slot = 0, loaded = 0, k_fills = 0;
-        uint32_t phase = 0;
-        bool over = false;
+        uint32_t phase = 0, k_phase = 0;
         const int box_shift = min(c.page_shift, 6), boxes = CHUNK_SLOTS >> box_shift;
         const uint32_t me = elect_lane();
-        while (!over && walk.next(&g)) {
+        while (!wait.dead && walk.next(&g)) {
             const int32_t* table = bt.table + g.b * bt.table_stride;
-            wait(k_empty, (k_fills & 1) ^ 1);
-            over = wait.given_up();
-            if (over) break;
+            wait.together(k_empty, k_phase ^ 1);
+            if (wait.dead) break;
+            k_phase ^= 1;
             ++k_fills;
             TilePages tp[2];
 #pragma unroll
@@ -195,9 +194,9 @@ __global__ void __launch_bounds__(WEIGHTS_THREADS, 1)
                                  page, k_full, me);
                 }
             for (int q = g.q0; q < g.q0 + g.count; ++q) {
-                wait(q_empty + slot, phase ^ 1);
-                over = wait.given_up();
-                if (over) break;
+                wait.together(q_empty + slot, phase ^ 1);
+                if (wait.dead) break;
+                ++loaded;
                 if (lane == 0) {
                     mbar_arrive_expect_tx(q_full + slot, HALVES * shape.tokens * a.group * 128);
                     for (int h = 0; h < HALVES; ++h)
@@ -205,7 +204,6 @@ __global__ void __launch_bounds__(WEIGHTS_THREADS, 1)
                                  (int)g.s.first + q * shape.tokens, q_full + slot);
                 }
                 __syncwarp();
-                ++loaded;
                 if (++slot == RING) slot = 0, phase ^= 1;
             }
         }
@@ -243,10 +241,10 @@ __global__ void __launch_bounds__(WEIGHTS_THREADS, 1)
                     }
                     umma_commit(s_full + 2 * i + buf, me);
                 }
-                umma_commit(q_empty + slot, me);
+                umma_commit(q_empty + slot, wait.live(me));
                 if (++slot == RING) slot = 0, phase ^= 1;
             }
-            umma_commit(k_empty, me);
+            umma_commit(k_empty, wait.live(me));
         }
         umma_commit(mma_done, me);
         if (lane == 0) wait.drain(mma_done, 1);
