@@ -304,7 +304,8 @@ int vk_ivf_assign_device(int device, const float* d_x, int64_t n, int d, const f
 /* Paged key/value cache (no counterpart in the reference): the step of a retrieval user after the search. The keys
  * and values of retrieved passages and of a model's own tokens live in fixed-size pages in DEVICE memory; a page
  * table per sequence, made e.g. from a search's ids, lists the pages it reads (several sequences may list the same
- * page). A sequence of length n occupies slots 0 .. n-1; slot s is entry s % page_size of page table[s / page_size].
+ * page). A sequence of length n occupies slots 0 .. n-1; slot s is entry s % page_size of page table[s / page_size]: every
+ * page but the last is full, so that passages whose pages several sequences list have to fill whole pages.
  *   vk_kv_append   writes new tokens' keys and values behind a sequence
  *   vk_kv_attend   attention of a sequence's new tokens (one, a few or a chunk) over its slots and, on request, the
  *                  attention weight that every slot gathered
@@ -374,16 +375,17 @@ int vk_kv_append(vk_kv_t* kv, const vk_kv_batch_t* batch, const void* k, const i
 typedef struct {
     const void* q; /* [tokens][heads][head_dim], the cache's type */
     int64_t q_stride[2];
-    void* out; /* the same shape and type */
+    void* out; /* the same shape and type; its rows must not overlap */
     int64_t out_stride[2];
     float* lse;    /* [tokens][heads], contiguous */
     float* scores; /* element (b, kv head, slot) at scores[b * scores_stride[0] + head * scores_stride[1] + slot],
-                      slots < scores_width; NULL: not gathered */
+                      slots < scores_width, rows that do not overlap; NULL: not gathered */
     int64_t scores_stride[2];
     int64_t scores_width;
     int heads; /* a multiple of kv_heads, at most 128 times it */
-    int max_q; /* at least the largest number of new tokens of a sequence; 0 = unknown (`tokens` is assumed). A sequence
-                  that has more may be left out, which vk_kv_sync reports */
+    int max_q; /* at least the largest number of new tokens of a sequence; 0 = unknown (`tokens` is assumed). Up to 16 rows
+                  (max_q x heads / kv_heads) the kernel for few rows takes the call, above that the one for chunks. A
+                  sequence that has more than max_q may be left out, which vk_kv_sync reports */
     int causal;
     float scale;
     void* workspace; /* DEVICE, 256-byte aligned, at least vk_kv_attend_workspace bytes, for one call at a time (the
@@ -397,7 +399,8 @@ typedef struct {
 } vk_kv_attend_t;
 #define VK_KV_WORKSPACE_ZEROED 8192
 /* Bytes of working memory that vk_kv_attend needs for these sizes (pointers in batch and args are not read, except
- * whether args->scores is NULL). */
+ * whether args->scores is NULL). On 148 SMs at most 20 MB for chunks and 3 MB for few rows; for few rows with scores, 16 to
+ * 64 bytes more for each of them (batch x kv_heads x scores_width, or the tables' slots where those are fewer). */
 int vk_kv_attend_workspace(const vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_attend_t* args, size_t* bytes);
 /* Working memory of `bytes` bytes whose start is zero when the call returns. Also while streams are being captured: nothing
  * of it is recorded, so that every graph, and calls outside of graphs, may use it in any order, one at a time. It has to

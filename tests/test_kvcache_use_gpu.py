@@ -410,3 +410,25 @@ def test_what_is_refused_changes_nothing_else(counts):
     again, again_lse = c.cache.attend(q, off, c.table, c.lens, causal=False)
     c.cache.sync()
     assert torch.equal(again, good) and torch.equal(again_lse, good_lse)
+
+
+def test_working_memory_goes_by_the_scores():
+    """Tables are often as wide as the longest sequence that may ever come: kept scores take memory for the slots that have a
+    score, not for all of the table's."""
+    import torch
+
+    from veckern_b200 import kvcache
+
+    c = Cache([300, 200], 16, 2, 64, seed=5)
+    q, off, s = call(c, [1, 1])
+    wide = torch.full((2, 1 << 16), 2 ** 31 - 1, dtype=torch.int32, device="cuda")  # a million slots
+    wide[:, :c.table.shape[1]] = c.table
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    out, lse = c.cache.attend(q, off, wide, c.lens, scores=s, max_q=1, stream=st)
+    c.cache.sync(st)
+    check_attend(c, q, [1, 1], out, lse, True, None, s, torch.zeros_like(s))
+    small = kvcache._WORK[(0, st.cuda_stream)].size
+    c.cache.attend(q, off, c.table, c.lens, scores=s, max_q=1, stream=st)
+    c.cache.sync(st)
+    assert kvcache._WORK[(0, st.cuda_stream)].size == small < 16 << 20

@@ -88,17 +88,20 @@ size_t align256(size_t x) { return (x + 255) / 256 * 256; }
 //
 // Where every sequence has at most 16 rows (tokens x query heads of a kv head) the step kernel reads the cache at the
 // memory's rate on mma.sync; with a longer sequence in the call the chunk kernel takes them all. Its tile of 128 rows is
-// mostly empty for a short sequence, but it reads 2 x 128 slots per 3,300 cycles and SM, which is the memory's rate too
-// (a step of 32 sequences of up to 8,192 slots: 132 us, the step kernel 119), so that a launch for the short ones of a
-// mixed call would cost more than it saves.
+// mostly empty for a short sequence, but it reads 2 x 128 slots per 3,300 cycles and SM, which is the memory's rate too, so
+// that a launch for the short ones of a mixed call would cost more than it saves. Both sides, the same call with the bound
+// and without it (32 heads over 8 of 128): 32 sequences of up to 8,192 slots 120 and 132 us, 4 of up to 50,021 102 and 105;
+// 8 x 5 tokens over up to 4,001 slots (24 heads over 8 of 64) 17.2 and 24.1. With weights a chunk's products are computed
+// twice, where the step kernel keeps them: 141 and 291, 122 and 150, 28 and 50.
 struct AttendPlan {
     bool step;
     int rows, s_rows;  // of the step path, rounded up to 8 or 16; to 4, 8 or 16
     int ctas;
+    int64_t s_slots;
     size_t ready, started, bad, o, ml, s, bytes;  // offsets
 };
 
-AttendPlan plan_attend(const vk_kv* kv, const vk::KvBatch& bt, int group, int max_q, bool scores) {
+AttendPlan plan_attend(const vk_kv* kv, const vk::KvBatch& bt, int group, int max_q, int64_t scores_width) {
     AttendPlan p{};
     const int64_t rows = (int64_t)max_q * group;
     p.step = rows <= vk::STEP_ROWS;
@@ -106,7 +109,8 @@ AttendPlan plan_attend(const vk_kv* kv, const vk::KvBatch& bt, int group, int ma
     p.s_rows = rows <= 4 ? 4 : p.rows;
     p.ctas = p.step ? 2 * kv->sm_count : kv->sm_count;
     const int dp = kv->desc.head_dim <= 64 ? 64 : 128;
-    const int64_t slots = (int64_t)bt.width << kv->page_shift;
+    // of the step path's kept scores: a table may be far wider than its sequences and their scores
+    p.s_slots = std::min((int64_t)bt.width << kv->page_shift, scores_width);
     // What has to be zero before a call lies at the start, whatever the sizes.
     const size_t rows_of_parts = (size_t)p.ctas * (p.step ? vk::STEP_ROWS : 2 * vk::CHUNK_ROWS);
     p.started = VK_KV_WORKSPACE_ZEROED - sizeof(uint32_t);
@@ -114,7 +118,8 @@ AttendPlan plan_attend(const vk_kv* kv, const vk::KvBatch& bt, int group, int ma
     p.o = VK_KV_WORKSPACE_ZEROED;
     p.ml = p.o + align256(rows_of_parts * dp * sizeof(float));
     p.s = p.ml + align256(rows_of_parts * sizeof(float2));
-    p.bytes = p.s + (scores && p.step ? align256((size_t)bt.batch * kv->desc.kv_heads * slots * p.s_rows * sizeof(float)) : 0);
+    p.bytes = p.s;
+    if (p.step) p.bytes += align256((size_t)bt.batch * kv->desc.kv_heads * p.s_slots * p.s_rows * sizeof(float));
     return p;
 }
 
@@ -155,12 +160,11 @@ int launch_step_as(const vk_kv* kv, const vk::KvPages& c, const vk::KvBatch& bt,
     VK_TRY(prepare_kernel<fn>(kv->desc.device, smem));
     VK_TRY(launch_behind(fn, dim3(ctas), vk::STEP_THREADS, smem, st, kv->map_k, kv->map_v, c, bt, a, parts));
     if constexpr (SCORES) {
-        const int64_t width = std::min(parts.s_slots, a.scores_width);
-        if (width > 0) {
+        if (parts.s_slots > 0) {
             const auto weights = parts.s_rows == 4   ? &vk::kv_step_weights_kernel<4>
                                  : parts.s_rows == 8 ? &vk::kv_step_weights_kernel<8>
                                                      : &vk::kv_step_weights_kernel<16>;
-            const int64_t blocks = std::min<int64_t>(ceil_div(width, vk::STEP_WEIGHTS_SLOTS), 4096);
+            const int64_t blocks = std::min<int64_t>(ceil_div(parts.s_slots, vk::STEP_WEIGHTS_SLOTS), 4096);
             VK_TRY(launch_behind(weights, dim3((unsigned)blocks, c.heads, bt.batch), 256, 0, st, c, bt, a, parts));
         }
     }
@@ -274,7 +278,7 @@ int launch_attend(const vk_kv* kv, const vk::KvBatch& bt, const vk::KvAttend& a,
     parts.o = reinterpret_cast<float*>(w + p.o);
     parts.ml = reinterpret_cast<float2*>(w + p.ml);
     parts.s = reinterpret_cast<float*>(w + p.s);
-    parts.s_slots = (int64_t)bt.width << kv->page_shift;
+    parts.s_slots = p.s_slots;
     parts.s_rows = p.s_rows;
     if (p.step)
         return c.dim <= 64 ? launch_step<T, 64>(kv, c, bt, a, parts, p, st) : launch_step<T, 128>(kv, c, bt, a, parts, p, st);
@@ -457,7 +461,7 @@ int vk_kv_attend(vk_kv_t* kv, const vk_kv_batch_t* batch, const vk_kv_attend_t* 
     if (tiles * g * ((double)bt.tokens * a.group / vk::CHUNK_ROWS + 2.0 * bt.batch) >= 2147483647.0)
         return fail(VK_ERR_UNSUPPORTED, "too many tiles (tables of %d pages, %lld tokens); use fewer sequences per call",
                     bt.width, (long long)bt.tokens);
-    const AttendPlan plan = plan_attend(kv, bt, a.group, a.max_q, a.scores != nullptr);
+    const AttendPlan plan = plan_attend(kv, bt, a.group, a.max_q, a.scores ? a.scores_width : 0);
     if (args->workspace_bytes < plan.bytes || !args->workspace || reinterpret_cast<uintptr_t>(args->workspace) % 256)
         return fail(VK_ERR_INVALID, "workspace must be 256-byte aligned and hold %zu bytes (vk_kv_attend_workspace)",
                     plan.bytes);
@@ -474,7 +478,10 @@ int vk_kv_attend_workspace(const vk_kv_t* kv, const vk_kv_batch_t* batch, const 
     sizes.offsets = sizes.table = sizes.lens = &none;
     VK_TRY(check_batch(kv, &sizes, true, &bt));
     VK_TRY(check_attend(kv, args));
-    *bytes = plan_attend(kv, bt, args->heads / kv->desc.kv_heads, max_q_of(args, bt.tokens), args->scores != nullptr).bytes;
+    if (args->scores && args->scores_width < 0) return fail(VK_ERR_INVALID, "scores: width must be >= 0");
+    *bytes = plan_attend(kv, bt, args->heads / kv->desc.kv_heads, max_q_of(args, bt.tokens),
+                         args->scores ? args->scores_width : 0)
+                 .bytes;
     return VK_OK;
 }
 

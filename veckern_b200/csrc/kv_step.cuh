@@ -44,7 +44,7 @@ struct KvParts {
     float* o;    // [part]: unnormalised sums
     float2* ml;  // [part][row]: maximum (base 2) and sum
     float* s;    // [sequence][kv head][slot][s_rows]: scaled scores (base 2) of the step path, for the weights
-    int64_t s_slots;
+    int64_t s_slots;  // slots that have a score and may be a sequence's
     int s_rows;  // rows rounded up to 4, 8 or 16
 };
 
@@ -397,6 +397,7 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
             }
             const float scale = a.scale * 1.4426950408889634f;
             const int open = min(s.len, row_limit(s, a.causal, 0));  // slots that every row sees
+            const int kept = SCORES ? (int)min((int64_t)s.len, parts.s_slots) : 0;
             float o[DP / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < DP / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
@@ -439,11 +440,11 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
                         if constexpr (SCORES) {
                             const int64_t first = ((int64_t)share.b * c.heads + head) * parts.s_slots + slot0 + q2;
                             float* sp = parts.s + first * parts.s_rows + g + 8 * u;
-                            // a slot past the sequence may lie past the workspace's last slot: only its own are written
+                            // kept where the sequence and the workspace have the slot
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 const int j = (e >> 1) * 8 + (e & 1);
-                                if (slot0 + q2 + j < s.len && g + 8 * u < parts.s_rows)
+                                if (slot0 + q2 + j < kept && g + 8 * u < parts.s_rows)
                                     sp[j * parts.s_rows] = x[e >> 1][2 * u + (e & 1)];
                             }
                         }
