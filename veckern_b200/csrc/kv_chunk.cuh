@@ -348,8 +348,11 @@ __global__ void __launch_bounds__(CHUNK_THREADS, 1)
                 }
                 const int32_t* table = bt.table + g.b * bt.table_stride;
                 const int per = g.lone ? 2 : 1;
-                for (int t = g.t0 * per; t < (g.t0 + g.count) * per && !wait.dead; ++t) {
-                    const TilePages tp = tile_pages(c, table, t * CHUNK_SLOTS, boxes, box_shift, g.s.len);
+                const int end = (g.t0 + g.count) * per;
+                int entry = tile_entries(c, table, g.t0 * per * CHUNK_SLOTS, boxes, box_shift, g.s.len);
+                for (int t = g.t0 * per; t < end && !wait.dead; ++t) {
+                    const TilePages tp = tile_pages(c, entry, t * CHUNK_SLOTS, boxes, box_shift, g.s.len);
+                    if (t + 1 < end) entry = tile_entries(c, table, (t + 1) * CHUNK_SLOTS, boxes, box_shift, g.s.len);
                     // rolled: this warp's registers are few, and what it spills the other one waits for
 #pragma unroll 1
                     for (int side = 0; side < 2; ++side, ++fill) {

@@ -74,18 +74,24 @@ __device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int 
         "l"(map), "r"(d), "r"(slot), "r"(head), "r"(page), "r"(smem_u32(bar)), "r"(me)
         : "memory");
 }
-// The pages of a tile's boxes, lane i the i-th box's (a page that does not exist lies past the map: it reads as zero), and
-// the number of boxes that the sequence reaches.
+// The table's entries for a tile's boxes, lane i the i-th box's; loaded a tile ahead, since a load does not move over the waits
+// and copies in between.
+__device__ __forceinline__ int tile_entries(const KvPages& c, const int32_t* table, int first, int boxes, int box_shift,
+                                            int len) {
+    const int lane = threadIdx.x & 31, slot = first + (lane << box_shift);
+    return lane < boxes && slot < len ? kv_entry(c, table, slot) : 0;
+}
+// The pages of these boxes (a page that does not exist lies past the map: it reads as zero), and the number of boxes that the
+// sequence reaches.
 struct TilePages {
     int page, count;
 };
-__device__ __forceinline__ TilePages tile_pages(const KvPages& c, const int32_t* table, int first, int boxes, int box_shift,
-                                                int len) {
+__device__ __forceinline__ TilePages tile_pages(const KvPages& c, int entry, int first, int boxes, int box_shift, int len) {
     const int lane = threadIdx.x & 31, slot = first + (lane << box_shift);
     const bool live = lane < boxes && slot < len;
     int page = 0;
     if (live) {
-        page = (int)kv_page(c, table, slot);
+        page = (int)kv_page_checked(c, entry);
         if (page < 0) page = (int)c.pages;
     }
     return {page, __popc(__ballot_sync(FULL, live))};
@@ -224,8 +230,9 @@ __device__ __forceinline__ KvShare kv_share(const KvPages& c, const KvBatch& bt,
     constexpr int WARPS = THREADS / 32, PLACE = KV_SHARE_SCRATCH - 1;
     static_assert(2 * WARPS + 2 <= PLACE, "scratch");
     if (t == THREADS - 1) {  // beside the others' loads
+        const uint32_t bad = *reinterpret_cast<const volatile uint32_t*>(parts.bad);
         scratch[PLACE] = (int)atomicInc(parts.started, gridDim.x - 1);
-        if (*reinterpret_cast<const volatile uint32_t*>(parts.bad)) atomicOr(c.status, ERR_WORKSPACE);
+        if (bad) atomicOr(c.status, ERR_WORKSPACE);
     }
     const int span = (bt.batch + THREADS - 1) / THREADS;
     const int b0 = min(bt.batch, t * span), b1 = min(bt.batch, b0 + span);
@@ -354,8 +361,10 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
         const int32_t* table = bt.table + share.b * bt.table_stride;
         if (warp == STEP_WARPS) {
             const uint32_t me = elect_lane();
+            int entry = tile_entries(c, table, t0 * STEP_TILE, boxes, box_shift, s.len);
             for (int t = t0; t < t0 + count; ++t) {
-                const TilePages tp = tile_pages(c, table, t * STEP_TILE, boxes, box_shift, s.len);
+                const TilePages tp = tile_pages(c, entry, t * STEP_TILE, boxes, box_shift, s.len);
+                if (t + 1 < t0 + count) entry = tile_entries(c, table, (t + 1) * STEP_TILE, boxes, box_shift, s.len);
                 wait.together(empty + stage, phase ^ 1);
                 if (wait.dead) {
                     share.left = 0;

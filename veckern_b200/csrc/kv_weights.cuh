@@ -178,9 +178,10 @@ __global__ void __launch_bounds__(WEIGHTS_THREADS, 1)
             ++k_fills;
             TilePages tp[2];
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-                tp[u] = tile_pages(c, table, g.pair * WEIGHTS_PAIR + u * CHUNK_SLOTS, u == 0 || g.both ? boxes : 0, box_shift,
-                                   g.s.len);
+            for (int u = 0; u < 2; ++u) {
+                const int first = g.pair * WEIGHTS_PAIR + u * CHUNK_SLOTS, n = u == 0 || g.both ? boxes : 0;
+                tp[u] = tile_pages(c, tile_entries(c, table, first, n, box_shift, g.s.len), first, n, box_shift, g.s.len);
+            }
             if (lane == 0) mbar_arrive_expect_tx(k_full, (tp[0].count + tp[1].count) * HALVES * (128 << box_shift));
             __syncwarp();
 #pragma unroll
