@@ -375,7 +375,7 @@ int vk_kv_append(vk_kv_t* kv, const vk_kv_batch_t* batch, const void* k, const i
 typedef struct {
     const void* q; /* [tokens][heads][head_dim], the cache's type */
     int64_t q_stride[2];
-    void* out; /* the same shape and type; its rows must not overlap */
+    void* out; /* the same shape and type; its rows must not overlap, nor lie in q */
     int64_t out_stride[2];
     float* lse;    /* [tokens][heads], contiguous */
     float* scores; /* element (b, kv head, slot) at scores[b * scores_stride[0] + head * scores_stride[1] + slot],

@@ -16,9 +16,15 @@
 // and 128 x 128 exponentials on the special function units (1,024 cycles as well). Tensor memory holds S and O of two
 // tiles and no more, so a tile's products wait for its weights and the other way round: a unit takes as long as one tile's
 // weights (1,400 cycles), its products (1,200) and the hand-overs between them (800), while the other tile fills the gaps.
-// Measured (4,096 tokens over 16,384 slots, 32 heads over 8, head size 128): 752 us, 1,280 TFLOP/s, in a short run at
-// 1.8 GHz. What did not pay: a part of the exponentials by a polynomial (1 in 8: 758 us, 2 in 8: 777), the weights handed
-// over in two halves (770), a warp of its own for each tile's products (920; taking turns 781).
+// Measured (4,096 tokens over 16,384 slots, 32 heads over 8, head size 128): 860-873 us, 1,100-1,120 TFLOP/s, in a run of
+// many, where power holds the clock down; 738 us, 1,300 TFLOP/s, for eight calls from rest. Tensor pipe and special function
+// units are each busy for 64 % of it. What did not pay, measured from rest against the 752 us of the time: a part of the
+// exponentials by a polynomial (1 in 8: 758 us, 2 in 8: 777), the weights handed over in two halves (770), a warp of its own
+// for each tile's products (920; taking turns 781).
+//
+// The weights are rounded to the cache's 16-bit type, as in the step kernel; scores, references, sums and O are 32-bit. Which
+// rows of a warp move their reference together depends on the tile's rows, so that a row's last bit may depend on its
+// neighbours; equal calls give equal bits.
 #pragma once
 #include "kv_step.cuh"
 
@@ -58,7 +64,8 @@ static_assert(2 * chunk_smem<64>() > 233472 && 2 * chunk_smem<128>() > 233472, "
 // The instructions below are reached by a whole warp and take effect for the lane that `me` is nonzero in. Issued inside
 // a branch of that lane instead, every operand was moved from the lane's to the warp's registers anew, about 100 cycles
 // per product: the warp that issues them was the kernel's bound (4,096 tokens over 16,384 slots, 32 heads over 8:
-// 1,105 us then, 770 now).
+// 1,105 us then, 770 when this came). `me` is what elect.sync gave: with the first lane's, computed, the case took 982 us in
+// a run of many, 860 with this.
 constexpr uint32_t UMMA_HIGH = 1024u >> 4 | 1u << 14 | 2u << 29;
 __device__ __forceinline__ uint32_t umma_low(uint32_t addr, uint32_t lead) { return addr >> 4 | (lead >> 4) << 16; }
 template <typename T>
@@ -148,8 +155,10 @@ __device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
     return p;
 }
 // ---- the order of units
-// sum of floor((a i + b) / m) over 0 <= i < n, by Euclid's steps on (m, a). The sum is below 2^31 (the host has checked
-// the units), so that arithmetic modulo 2^32 gives it; a n + b after the first reduction is below m (n + 1).
+// sum of floor((a i + b) / m) over 0 <= i < n, by Euclid's steps on (m, a): taking out the whole parts of a / m and b / m
+// leaves a sum of the same kind with a and m exchanged (such sums: Graham, Knuth and Patashnik, "Concrete Mathematics",
+// section 3.5). The sum is below 2^31 (the host has checked the units), so that arithmetic modulo 2^32 gives it; a n + b after
+// the first reduction is below m (n + 1).
 __device__ __forceinline__ uint32_t floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
     uint32_t sum = 0;
     while (n > 0) {

@@ -10,7 +10,8 @@ namespace vk {
 __global__ void kv_reported_kernel(int* status, int bits) { atomicAnd(status, ~bits); }
 
 // One thread per 16 bytes of a new token's head. Every byte is read and written once: bound by memory (9 prompts of up to
-// 2,011 tokens, 8 kv heads of 128, 104 MB: 18.5 us, 5.6 TB/s), by the launch for a step's few tokens (2.4 us).
+// 2,011 tokens, 8 kv heads of 128, 104 MB: 20.9 us, 5.0 TB/s among calls on other data, 18.9 when one call is repeated), by
+// the launch for a step's few tokens (2.5 us in a graph).
 __global__ void __launch_bounds__(256) kv_append_kernel(KvPages c, KvBatch bt, const uint16_t* k, const uint16_t* v,
                                                         int64_t k_tok, int64_t k_head, int64_t v_tok, int64_t v_head) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -70,8 +71,8 @@ __device__ __forceinline__ uint32_t kv_rank(float x) {
 // first ones; where a CTA's kept slots go follows from the counts of the CTAs before it.
 //
 // Bound by latency: up to eight cluster-wide steps, and a slice's passes through shared memory. Up to 16 CTAs per
-// (sequence, kv head), so that a long sequence's passes are short. Measured, 8 kv heads: 1,087 slots 9 us, 131,072 slots 25
-// us (one block of 1,024 threads per head: 29 and 265).
+// (sequence, kv head), so that a long sequence's passes are short. Measured, 8 kv heads, cold caches: 1,087 slots 11 us, 131,072
+// slots 28 us (one block of 1,024 threads per head: 29 and 265).
 constexpr int SELECT_THREADS = 512;
 constexpr int SELECT_BINS = 2048;
 constexpr int SELECT_HELD = 16384;  // ranks that a CTA keeps in shared memory; a larger slice is read again instead

@@ -15,9 +15,13 @@
 // and sum, on mma.sync m16n8k16: at 16 rows the tensor work is under a fifth of its rate while memory is saturated, and
 // the operands stay in registers from the scores to the values, which tcgen05's 128-row tiles would not allow.
 //
-// Measured: 32 sequences of up to 8,192 slots, 32 heads over 8 of 128: 117-121 us, 6.0-6.2 TB/s; one token over 1,000
-// slots: 9.4 us in a graph, of which reading is one. Two CTAs share an SM (at a head size of 64, 8 x 5 tokens over 4,001
-// slots: three make no difference, four take 25.8 us where two take 17.5).
+// The weights are rounded to the cache's 16-bit type before they meet the values, since the products take operands of one
+// type; sums, maxima, totals and kept scores stay in 32 bits. Their error, 2^-9 of a weight at most, lies under the result's
+// own rounding to that type.
+//
+// Measured: 32 sequences of up to 8,192 slots, 32 heads over 8 of 128: 118-121 us, 6.0-6.2 TB/s; one token over 1,000
+// slots: 10.9 us in a graph, of which reading is one and the atomic that orders the shares 0.7. Two CTAs share an SM (at a
+// head size of 64, 8 x 5 tokens over 4,001 slots: three make no difference, four take 25.8 us where two take 17.4).
 #pragma once
 #include <cuda.h>
 
@@ -64,7 +68,8 @@ __device__ __forceinline__ uint32_t elect_lane() {
 }
 // A 2-d box of a page (box slots x 64 elements of one head) into shared memory. Reached by a whole warp with equal
 // arguments, copied once, by the lane whose `me` is nonzero: from lanes with arguments of their own a copy takes over 100
-// cycles each (2,048 tokens over 8,192 slots, 32 heads over 8 of 128, pages of 8 slots: 271 us then, 197 now).
+// cycles each (2,048 tokens over 8,192 slots, 32 heads over 8 of 128, pages of 8 slots: 271 us then, 197 when this came, 207
+// now).
 __device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* map, int d, int slot, int head, int page,
                                          uint64_t* bar, uint32_t me) {
     asm volatile(

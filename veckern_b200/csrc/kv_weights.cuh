@@ -10,9 +10,10 @@
 // row tile within a pair, the pair's keys stay in shared memory and the rows stream; the units of all (sequence, kv head,
 // pair)s are laid end to end and shared out equally, and cut pairs are finished from parts, as in the step kernel.
 //
-// Bound: one exponential per (row, slot), 16 a clock and SM on the special function units (1,024 cycles per 128 x 128
-// tile against 512 for its product at a head size of 128). Measured: 2,048 tokens over 16,384 slots, 16 heads over 8 of 128:
-// 173 us, 63 % of that rate; without the exponentials 122 us, without the products 159.
+// The least it could take: one exponential per (row, slot), 16 a clock and SM on the special function units (1,024 cycles per
+// 128 x 128 tile against 512 for its product at a head size of 128). Measured: 2,048 tokens over 16,384 slots, 16 heads over 8
+// of 128: 180 us, 61 % of that rate. What holds it back is the rest of a tile: of 173 us then, 122 were left without the
+// exponentials (loads from tensor memory, additions, a barrier per row tile for the rows' lse), 159 without the products.
 #pragma once
 #include "kv_chunk.cuh"
 

@@ -191,7 +191,7 @@ class PagedCache:
                max_q: int = 0, out=None, lse=None, stream=None):
         """Attention of new tokens q [tokens, heads, head_dim] over their sequences' slots: (out like q, lse [tokens,
         heads] float32). Token t of T sees slots up to lens[b] - T + t when causal, all lens[b] otherwise; a row that
-        sees none gets zeros and -inf. scale defaults to head_dim ** -0.5. scores, [batch, kv_heads, width] float32
+        sees none gets zeros and -inf. out, if given, is not q itself. scale defaults to head_dim ** -0.5. scores, [batch, kv_heads, width] float32
         with the last dimension contiguous: the attention weights of a sequence's tokens and of a kv head's query
         heads are added to its slots. max_q: an upper bound of a sequence's new tokens, where the caller knows it (a
         decoding step: 1). Where it says that no sequence has more than 16 rows (new tokens x query heads of a kv head) the
