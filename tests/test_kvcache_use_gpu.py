@@ -432,3 +432,20 @@ def test_working_memory_goes_by_the_scores():
     c.cache.attend(q, off, c.table, c.lens, scores=s, max_q=1, stream=st)
     c.cache.sync(st)
     assert kvcache._WORK[(0, st.cuda_stream)].size == small < 16 << 20
+
+
+def test_more_tokens_than_32_bits_count_are_refused():
+    """A sequence's tokens are rounded up to pairs of row tiles (up to 256 tokens) in 32 bits."""
+    import ctypes as C
+
+    from veckern_b200 import _native as N
+
+    c = Cache([30], 8, 1, 64)
+    at = c.table.data_ptr()
+    strides = (C.c_int64 * 2)(0, 0)
+    for tokens, code in ((2 ** 31 - 1, N.VK_ERR_INVALID), (2 ** 31 - 1023, N.VK_ERR_INVALID), (-1, N.VK_ERR_INVALID),
+                         (0, N.VK_OK)):
+        b = N.KvBatch(batch=1, table_width=4, table_stride=4, tokens=tokens, offsets=at, table=at, lens=at)
+        assert N.lib().vk_kv_append(c.cache._h, C.byref(b), at, strides, at, strides, None) == code
+        if code:
+            assert "tokens" in N.last_error()

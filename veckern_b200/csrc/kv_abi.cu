@@ -48,7 +48,8 @@ int check_batch(const vk_kv* kv, const vk_kv_batch_t* bt, bool offsets, vk::KvBa
     if (!kv) return fail(VK_ERR_INVALID, "cache must not be NULL");
     if (!bt) return fail(VK_ERR_INVALID, "batch must not be NULL");
     if (bt->batch < 0 || bt->batch > 65535) return fail(VK_ERR_INVALID, "batch must be in [0, 65535]");
-    if (bt->tokens < 0 || bt->tokens > INT32_MAX) return fail(VK_ERR_INVALID, "tokens must be in [0, 2^31)");
+    // the kernels round counts of tokens up to pairs of row tiles in 32 bits
+    if (bt->tokens < 0 || bt->tokens > INT32_MAX - 1024) return fail(VK_ERR_INVALID, "tokens must be in [0, 2^31 - 1024)");
     if (bt->table_width < 0 || bt->table_stride < 0 ||
         ((int64_t)bt->table_width << kv->page_shift) > INT32_MAX - 1024)
         return fail(VK_ERR_INVALID, "table_width must be >= 0 and cover less than 2^31 slots");
