@@ -405,7 +405,8 @@ __global__ void __launch_bounds__(STEP_THREADS, 2)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const int d = 16 * k + 8 * e + q2;
-                        const uint32_t x = __ldca(reinterpret_cast<const unsigned int*>(row + (d < c.dim ? d : 0)));
+                        uint32_t x = 0u;
+                        if (u == 0 || R == 16) x = __ldca(reinterpret_cast<const unsigned int*>(row + (d < c.dim ? d : 0)));
                         q[k][u + 2 * e] = live && d < c.dim ? x : 0u;
                     }
             }

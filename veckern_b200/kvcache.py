@@ -15,9 +15,9 @@ All tensors are torch tensors on the cache's device. Sequence b of a call has th
 (int32, [batch + 1]), lens[b] slots with the new tokens included (int32, [batch]) and the pages table[b] (int32,
 [batch, width]; entries past its last slot are not read). Calls are asynchronous on `stream` (a torch.cuda.Stream or raw
 handle; default: the current stream), which the results they make belong to as well: another stream waits before it reads
-them. sync() waits and raises what the kernels found wrong. The calls of one stream share
-their working memory, those captured into CUDA graphs on it too: such graphs are replayed in any order, one after the
-other, and not while eager calls of that stream run. No derivatives: a cache is for inference.
+them. sync() waits and raises what the kernels found wrong. The calls of one stream share their working memory, those captured
+into CUDA graphs on it too: such graphs are replayed in any order, one after the other, and not while eager calls of that
+stream run. No derivatives: a cache is for inference.
 """
 from __future__ import annotations
 
@@ -191,13 +191,13 @@ class PagedCache:
                max_q: int = 0, out=None, lse=None, stream=None):
         """Attention of new tokens q [tokens, heads, head_dim] over their sequences' slots: (out like q, lse [tokens,
         heads] float32). Token t of T sees slots up to lens[b] - T + t when causal, all lens[b] otherwise; a row that
-        sees none gets zeros and -inf. out, if given, is not q itself. scale defaults to head_dim ** -0.5. scores, [batch, kv_heads, width] float32
-        with the last dimension contiguous: the attention weights of a sequence's tokens and of a kv head's query
-        heads are added to its slots. max_q: an upper bound of a sequence's new tokens, where the caller knows it (a
-        decoding step: 1). Where it says that no sequence has more than 16 rows (new tokens x query heads of a kv head) the
-        kernel for few rows takes the call; without it (0) any sequence may have all of the tokens, and the kernel for
-        chunks takes it (a decoding batch of 32 over up to 8,192 slots: 132 us where it takes 120, with weights 291 where it
-        takes 141)."""
+        sees none gets zeros and -inf. out, if given, is not q itself. scale defaults to head_dim ** -0.5. scores,
+        [batch, kv_heads, width] float32 with the last dimension contiguous: the attention weights of a sequence's
+        tokens and of a kv head's query heads are added to its slots. max_q: an upper bound of a sequence's new tokens,
+        where the caller knows it (a decoding step: 1). Where it says that no sequence has more than 16 rows (new
+        tokens x query heads of a kv head) the kernel for few rows takes the call; without it (0) any sequence may have
+        all of the tokens, and the kernel for chunks takes it (a decoding batch of 32 over up to 8,192 slots: 132 us
+        where it takes 120, with weights 291 where it takes 141)."""
         torch = self._torch
         if q.dim() != 3:
             raise ValueError("q must be [tokens, heads, head_dim]")
